@@ -372,6 +372,102 @@ int32_t lf_pack_ints(const int32_t* codes, int64_t rows, int32_t n, int32_t bits
 int32_t lf_unpack_ints(const int32_t* words, int64_t rows, int32_t n_words, int32_t count, int32_t bits,
                        int32_t* codes, void* stream);
 
+/*
+ * The 4-bit row cache: one layer's Keys and Values of ``batch`` sequences, quantised to 4 bits as they
+ * are written (no residual page, no tier table; no reference counterpart).  A row -- one token's Key or
+ * Value of one kv head -- is kept per group of ``group`` channels as 4-bit codes, an fp16 scale and an
+ * fp16 minimum, by the rule of lf_asymmetric_codes at 4 bits: lo = min, s = clamp((max - lo) / 15, 1e-5,
+ * 1e5), code = clamp(rint((x - lo) / s), 0, 15) in IEEE float32; the value read back is the float32
+ * code * fp16(s) + fp16(lo).
+ *
+ * Storage: ``blocks``, one record per 32 tokens of a (sequence, kv head):
+ *   [batch][n_kv][cap_tokens / 32][LF_INT4_BLOCK_BYTES(head_dim, group)], each record
+ *     Key codes      u32 [32][head_dim / 8]   a row's word w (channels 8 w ..) at (w % 4) * (head_dim / 32) + w / 4
+ *     Value codes    u32 [4][16][head_dim / 16]   word (q, c, t): channel 16 t + c of tokens 4 q .. 4 q + 3
+ *                                             (its lower nibbles) and 16 + 4 q .. 16 + 4 q + 3
+ *     Key scale, min fp16 [32][head_dim / group][2]
+ *     Value scale, min fp16 [32][head_dim / group][2]
+ *   A code word's nibble e is in bits (4 e + 3) % 32 .. of the word: the word rotated left by 3.
+ * ``bounds``: bf16 [batch][n_kv][cap_tokens / page_size][2][head_dim], every full page's smallest and
+ * largest Key per channel (of the values read back), rounded outward.  ``lens``: DEVICE int32 [batch],
+ * the sequences' tokens; the write position never leaves the device.
+ *
+ * head_dim 64, 128 or 256; group 32, 64 or 128, at most head_dim; page_size a multiple of 32 up to 1024;
+ * cap_tokens a multiple of page_size; blocks and bounds 16-byte aligned (others: LF_E_UNSUPPORTED or
+ * LF_E_SHAPE).  Lengths outside 0 .. cap_tokens are taken as the nearer end.
+ */
+typedef struct lf_int4_layer {
+    uint8_t* blocks;
+    uint16_t* bounds;
+    int32_t* lens;
+    int32_t batch, n_kv, head_dim;
+    int32_t cap_tokens, page_size, group;
+} lf_int4_layer;
+
+#define LF_INT4_BLOCK_BYTES(head_dim, group) (32 * ((head_dim) + 8 * ((head_dim) / (group))))
+
+/*
+ * Append rows: sequence b gets rows 0 .. counts[b] - 1 of k_src / v_src (``tokens`` rows each; counts, a
+ * DEVICE int32 [batch] of 0 .. tokens, NULL: all of them) behind its lens[b], which then advances.  Rows past
+ * cap_tokens are not written.  Element strides per sequence, head and token, unit channel stride.  Pages that
+ * a sequence completes get their bounds.  Rows that are not finite leave codes, scales and minima without a
+ * meaning for their own groups only.
+ */
+int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void* v_src, int32_t dtype,
+                       const int64_t* k_strides, const int64_t* v_strides, const int32_t* counts, int32_t tokens,
+                       void* stream);
+
+/*
+ * Read rows back: k_out / v_out [batch][n_kv][tokens][head_dim], contiguous, rounded to ``dtype`` (either may
+ * be NULL).  Row t of sequence b is the cache's row starts[b] + t (``starts``: DEVICE int32 [batch], NULL: 0);
+ * rows outside 0 .. lens[b] - 1 are zeros.
+ */
+int32_t lf_int4_read(const lf_int4_layer* layer, const int32_t* starts, int32_t tokens, void* k_out, void* v_out,
+                     int32_t dtype, void* stream);
+
+/* Arguments of lf_int4_attention and lf_int4_select. */
+typedef struct lf_int4_args {
+    const void* query; int32_t dtype;         /* [batch][n_q][q_len][head_dim] by strides   */
+    int32_t n_q, q_len;
+    int64_t q_strides[3];                     /* elements per sequence, head and token; unit channel stride */
+    const int32_t* q_lens;                    /* DEVICE int32 [batch] of 0 .. q_len: query tokens of every
+                                                 sequence (NULL: q_len); out rows behind them are zeros */
+    void* out;                                /* [batch][n_q][q_len][head_dim] contiguous, of ``dtype`` */
+    float scaling;
+    int32_t n_pages;                          /* pages per query token (select; attention: 0 = all) */
+    int32_t* pages;                           /* DEVICE int32 [batch][n_kv][q_len][n_pages]   */
+    int32_t splits;                           /* workgroups that share a sequence's tokens, 1 .. 1024 */
+    int32_t split_tokens;                     /* tokens of each (a multiple of 32); the last split takes
+                                                 what is behind them too; with pages: unused  */
+    void* workspace; int64_t workspace_bytes; /* 16-byte aligned, no initialisation           */
+} lf_int4_args;
+
+/*
+ * Attention over the 4-bit rows: out[b, i, j] = softmax(scaling q[b, i, j] . K_b^T) V_b over rows
+ * 0 .. lens[b] - n + j of sequence b (n its query tokens: they are the sequence's last n, already
+ * appended), query head i reading kv head i / (n_q / n_kv).  A query that sees no row gives zeros.
+ *
+ * With ``pages`` (n_pages > 0): query token j of kv head h attends its own page -- the one its position is in
+ * -- up to itself, and those pages of pages[b][h][j] that lie before it, in ascending order; an entry that
+ * is negative, not before the own page or not greater than the entry in front of it is not attended.
+ *
+ * Scores and sums in fp32.  Split over the tokens into ``splits`` workgroups per (sequence, kv head, row
+ * tile), merged by a second launch when there are more than one.  Workspace: lf_int4_workspace_bytes().
+ */
+int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, void* stream);
+int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t q_len, int32_t splits);
+
+/*
+ * Page selection: for every query token j (at position lens[b] - n + j) and kv head, the n_pages pages of
+ * highest score among those before its own page: score = max over the kv head's query heads of
+ * sum_c max(q_c lo_c, q_c hi_c) with the page's bounds, an upper bound of the page's q . k, summed in
+ * float64 so that the choice does not depend on the order of the sum.  Equal scores: the lower page first;
+ * NaN scores come last.  Writes ``pages`` in ascending order, -1 behind the last one.  n_pages <= 1024.
+ * Workspace: lf_int4_select_workspace_bytes().
+ */
+int32_t lf_int4_select(const lf_int4_layer* layer, const lf_int4_args* args, void* stream);
+int64_t lf_int4_select_workspace_bytes(const lf_int4_layer* layer, int32_t q_len);
+
 #ifdef __cplusplus
 }
 #endif

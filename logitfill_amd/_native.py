@@ -95,6 +95,33 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+class Int4Layer(ctypes.Structure):
+    """``lf_int4_layer``."""
+
+    _fields_ = [
+        ("blocks", c_void_p), ("bounds", c_void_p), ("lens", c_void_p),
+        ("batch", c_int32), ("n_kv", c_int32), ("head_dim", c_int32),
+        ("cap_tokens", c_int32), ("page_size", c_int32), ("group", c_int32),
+    ]
+
+
+class Int4Args(ctypes.Structure):
+    """``lf_int4_args``."""
+
+    _fields_ = [
+        ("query", c_void_p), ("dtype", c_int32),
+        ("n_q", c_int32), ("q_len", c_int32),
+        ("q_strides", c_int64 * 3),
+        ("q_lens", c_void_p),
+        ("out", c_void_p),
+        ("scaling", c_float),
+        ("n_pages", c_int32),
+        ("pages", c_void_p),
+        ("splits", c_int32), ("split_tokens", c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 _SIGNATURES = {
     "lf_abi_version": (c_int32, []),
     "lf_build_info": (c_char_p, []),
@@ -123,6 +150,13 @@ _SIGNATURES = {
     "lf_fill_tail": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p,
                                c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p]),
     "lf_noalloc_scratch_bytes": (c_int64, []),
+    "lf_int4_append": (c_int32, [POINTER(Int4Layer), c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+                                 c_int32, c_void_p]),
+    "lf_int4_read": (c_int32, [POINTER(Int4Layer), c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
+    "lf_int4_attention": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
+    "lf_int4_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32, c_int32, c_int32]),
+    "lf_int4_select": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
+    "lf_int4_select_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32]),
 }
 
 ABI_VERSION = 8

@@ -1,0 +1,410 @@
+// Attention over the 4-bit row cache, on the matrix cores.
+//
+// Scores of 16 tokens and 16 query rows: S^T = Codes . Q^T on v_mfma_f32_16x16x32_bf16, per group g of channels
+//     s_t = sum_g scale_t,g (q_g . code_t,g) + min_t,g sum(q_g),
+// and the Value product O^T = Codes_V^T . P'^T with P'_t,g = p_t scale_t,g,
+//     o_c = sum_t P'_t,g code_t,c + p_t min_t,g.
+// A score's lane holds the tokens of exactly the P' operand its lane of the second product needs (Value words hold
+// eight tokens of a channel in that order), so nothing is exchanged between the two products.
+//
+// Codes enter as bf16 16 + code (one and-or per pair); the 16 is taken out of the scores by the accumulator's start
+// value, -16 sum(q_g), and out of the output by a product of P' with a constant.  Queries are split into bf16 parts
+// that add up to them exactly (bf16 one, fp16 two, fp32 three).  P' is rounded to as many parts as the output's
+// type asks for; the codes count from their middle, 7.5, there (sum p (min + 7.5 scale) is kept in fp32), so that a
+// rounding of P' weighs as the code's distance from it.
+//
+// A workgroup's four waves take the records of its split in turn, each with its own running reference point and
+// sums, merged through LDS at the end; several splits of a sequence are merged by int4_merge_kernel.  The
+// reference point of a row moves only when a score passes it by 2^8: p stays below 2^8 and the sums are rescaled
+// rarely.
+#include "int4_common.hpp"
+
+namespace lf {
+namespace {
+
+constexpr int kWaves = 4, kTile = 16;
+
+struct AttentionArgs {
+    lf_int4_layer L;
+    const void* q;
+    int64_t qb, qh, qt;
+    int vec;  // query rows start on 16 bytes
+    const int32_t* q_lens;
+    void* out;
+    int n_q, g, q_len;
+    float qscale;  // scaling * log2(e)
+    const int32_t* pages;
+    int n_pages;
+    int splits, split_tokens;  // with pages: split_tokens is in records of the page list
+    float* part_o;             // [batch * n_q * q_len][splits][D]
+    float* part_ml;            // [batch * n_q * q_len][splits][2]
+};
+
+template <int NT>
+struct Parts {
+    bf16x8 t[NT];
+};
+
+__device__ __forceinline__ uint32_t upper_pair(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+}
+__device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+
+// Element pairs (a[i], b[i]) in NT bf16 parts; the last part is rounded to nearest, those before it are cut off.
+template <int NT>
+__device__ __forceinline__ Parts<NT> split(const float (&a)[4], const float (&b)[4]) {
+    Parts<NT> r;
+    float x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = a[i]; y[i] = b[i]; }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = n + 1 < NT ? upper_pair(x[i], y[i]) : pack_bf16(x[i], y[i]);
+            if (n + 1 < NT) { x[i] -= upper(x[i]); y[i] -= upper(y[i]); }
+        }
+        r.t[n] = __builtin_bit_cast(bf16x8, w);
+    }
+    return r;
+}
+
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+template <int Dt>
+__device__ __forceinline__ void query8(const AttentionArgs& a, int64_t at, float (&x)[8]) {
+    if (a.vec) {
+        if constexpr (Dt == LF_FP32) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at);
+            const f32x4 u = p[0], v = p[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[e] = u[e]; x[4 + e] = v[e]; }
+        } else {
+            const u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint16_t h = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+                x[e] = Dt == LF_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = load_as_f32(a.q, at + e, Dt);
+    }
+}
+
+template <int D, int GROUP, int Dt>
+__global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(AttentionArgs a) {
+    using R = Int4Rec<D, GROUP>;
+    constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
+    constexpr int NT = Dt == LF_BF16 ? 1 : Dt == LF_FP16 ? 2 : 3;
+    constexpr int kPad = D + 4;
+    __shared__ __attribute__((aligned(16))) float lds_o[(kWaves - 1) * kTile * kPad];
+    __shared__ float lds_ml[kWaves][kTile][2];
+    const int b = blockIdx.z, lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    const int col = lane & 15, quad = lane >> 4;
+    // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
+    const int tiles = gridDim.y / a.L.n_kv, h = blockIdx.y / tiles, tile = blockIdx.y % tiles;
+    int i, j;
+    if (a.n_pages) {
+        j = tile % a.q_len;
+        i = tile / a.q_len * kTile + col;
+    } else {
+        const int r = tile * kTile + col;
+        i = r / a.q_len;
+        j = r % a.q_len;
+    }
+    const bool real = i < a.g;
+    const int len = int4_len(a.L, b);
+    const int n = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+    const int lim = real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
+    int all = real ? lim : 0x7fffffff, top = lim;                 // rows every query of the tile sees, and any
+#pragma unroll
+    for (int m = 1; m < 16; m <<= 1) {
+        all = min(all, __shfl_xor(all, m, kWave));
+        top = max(top, __shfl_xor(top, m, kWave));
+    }
+    all = in_sgpr(all);
+    top = in_sgpr(top);
+
+    // records of this split
+    const int per_page = a.L.page_size / kBlock;
+    const int part = blockIdx.x, own = top > 0 ? (top - 1) / a.L.page_size : 0;
+    int first, last;
+    if (a.n_pages) {
+        first = part * a.split_tokens;
+        last = min(first + a.split_tokens, per_page * (a.n_pages + 1));
+        if (top == 0) last = first;
+    } else {
+        const int blocks = (top + kBlock - 1) / kBlock, per = a.split_tokens / kBlock;
+        first = static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
+        last = part + 1 == a.splits ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
+    }
+    const int32_t* list = a.n_pages ? a.pages + ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * a.n_pages : nullptr;
+
+    Parts<NT> q[CH];
+    float qsum[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) qsum[g] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        float x[8] = {};
+        if (real) query8<Dt>(a, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 32 * c + 8 * quad, x);
+        const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
+        q[c] = split<NT>(lo, hi);
+        qsum[c / CG] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) qsum[g] = rows_sum(qsum[g]);
+
+    constexpr uint32_t kMiddle = 0xC1BCC1BCu;  // bf16 -23.5: the bias of the codes and their middle
+    const bf16x8 middle = __builtin_bit_cast(bf16x8, u32x4{kMiddle, kMiddle, kMiddle, kMiddle});
+    f32x4 o[VT], fix[G];
+    float pm[G], l = 0.f, ref = 0.f, limit = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < VT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < G; ++g) { fix[g] = f32x4{0.f, 0.f, 0.f, 0.f}; pm[g] = 0.f; }
+
+    for (int k = first + wave; k < last; k += kWaves) {
+        int block = k;
+        bool masked;
+        if (a.n_pages) {
+            const int e = k / per_page;
+            int page = own;
+            if (e > 0) {
+                page = list[e - 1];
+                const int before = e > 1 ? list[e - 2] : -1;
+                if (page <= before || page >= own) continue;  // (a negative page is not above the one before)
+                if (page < 0) continue;
+            }
+            block = page * per_page + k % per_page;
+            if (block * kBlock >= top) continue;
+            masked = block * kBlock + kBlock > all;
+        } else {
+            masked = block * kBlock + kBlock > all;
+        }
+        const uint8_t* rec = int4_block(a.L, b, h, block, R::bytes);
+        uint32_t kw[2][CH], vw[VT], ks[2][4][G], vs[2][4][G];
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(rec);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int c = 0; c < CH; ++c) kw[t][c] = words[(16 * t + col) * (D / 8) + CH * quad + c];
+#pragma unroll
+        for (int t = 0; t < VT; ++t) vw[t] = words[R::v / 4 + lane * VT + t];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    ks[t][r][g] = words[R::ksm / 4 + (16 * t + 4 * quad + r) * G + g];
+                    vs[t][r][g] = words[R::vsm / 4 + (16 * t + 4 * quad + r) * G + g];
+                }
+        float y[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const float start = -kCodeBias * qsum[g];
+                f32x4 acc = {start, start, start, start};
+#pragma unroll
+                for (int c = g * CG; c < (g + 1) * CG; ++c) {
+                    const bf16x8 codes = codes8(kw[t][c]);
+#pragma unroll
+                    for (int m = NT - 1; m >= 0; --m) acc = mfma(codes, q[c].t[m], acc);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float x = fmaf(pair_scale(ks[t][r][g]), acc[r], pair_min(ks[t][r][g]) * qsum[g]);
+                    y[t][r] = g == 0 ? x : y[t][r] + x;
+                }
+            }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[t][r] *= a.qscale;
+        if (masked) {
+            // rows a query does not see: no score, and neither scale nor minimum (what stands there need not be finite)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool seen = block * kBlock + 16 * t + 4 * quad + r < lim;
+                    y[t][r] = seen ? y[t][r] : -__builtin_inff();
+#pragma unroll
+                    for (int g = 0; g < G; ++g) vs[t][r][g] = seen ? vs[t][r][g] : 0u;
+                }
+        }
+        float most = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
+                           fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
+        if (__any(most > limit)) {
+            most = rows_max(most);
+            const bool moves = most > limit;
+            const float scale = !moves ? 1.f : limit == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - most);
+            if (moves) { ref = most; limit = most + 8.f; }
+            l *= scale;
+#pragma unroll
+            for (int g = 0; g < G; ++g) { pm[g] *= scale; fix[g] *= scale; }
+#pragma unroll
+            for (int t = 0; t < VT; ++t) o[t] *= scale;
+        }
+        float p[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                p[t][r] = __builtin_amdgcn_exp2f(y[t][r] - ref);
+                l += p[t][r];
+            }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            float lo[4], hi[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                lo[r] = p[0][r] * pair_scale(vs[0][r][g]);
+                hi[r] = p[1][r] * pair_scale(vs[1][r][g]);
+                pm[g] = fmaf(p[0][r], pair_min(vs[0][r][g]), pm[g]);
+                pm[g] = fmaf(p[1][r], pair_min(vs[1][r][g]), pm[g]);
+                pm[g] = fmaf(7.5f, lo[r], pm[g]);
+                pm[g] = fmaf(7.5f, hi[r], pm[g]);
+            }
+            const Parts<NT> w = split<NT>(lo, hi);
+#pragma unroll
+            for (int m = NT - 1; m >= 0; --m) {
+                fix[g] = mfma(middle, w.t[m], fix[g]);
+#pragma unroll
+                for (int t = g * TG; t < (g + 1) * TG; ++t) o[t] = mfma(codes8(vw[t]), w.t[m], o[t]);
+            }
+        }
+    }
+
+    // the waves' sums at one reference point
+    l = rows_sum(l);
+    const float m_wave = limit == -__builtin_inff() ? limit : ref;
+    if (quad == 0) { lds_ml[wave][col][0] = m_wave; lds_ml[wave][col][1] = l; }
+#pragma unroll
+    for (int g = 0; g < G; ++g) pm[g] = rows_sum(pm[g]);
+    __syncthreads();
+    float m_all = lds_ml[0][col][0];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, lds_ml[w][col][0]);
+    const float mine = m_wave == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_wave - m_all);
+#pragma unroll
+    for (int t = 0; t < VT; ++t) {
+        o[t] = (o[t] + fix[t / TG] + pm[t / TG]) * mine;
+        if (wave > 0) *reinterpret_cast<f32x4*>(lds_o + ((wave - 1) * kTile + col) * kPad + 16 * t + 4 * quad) = o[t];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float l_all = l * mine;
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) {
+        const float m = lds_ml[w][col][0];
+        l_all += m == -__builtin_inff() ? 0.f : lds_ml[w][col][1] * __builtin_amdgcn_exp2f(m - m_all);
+#pragma unroll
+        for (int t = 0; t < VT; ++t) o[t] += *reinterpret_cast<const f32x4*>(lds_o + ((w - 1) * kTile + col) * kPad + 16 * t + 4 * quad);
+    }
+    if (!real) return;
+    const int64_t row = (static_cast<int64_t>(b) * a.n_q + h * a.g + i) * a.q_len + j;
+    if (a.splits == 1) {
+        const float inv = l_all > 0.f ? 1.f / l_all : l_all == 0.f ? 0.f : l_all;
+#pragma unroll
+        for (int t = 0; t < VT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) store_from_f32(a.out, row * D + 16 * t + 4 * quad + r, Dt, inv == 0.f && l_all == 0.f ? 0.f : o[t][r] * inv);
+        return;
+    }
+    float* dst = a.part_o + (row * a.splits + part) * D;
+#pragma unroll
+    for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t + 4 * quad) = o[t];
+    if (quad == 0) {
+        float* ml = a.part_ml + (row * a.splits + part) * 2;
+        ml[0] = m_all;
+        ml[1] = l_all;
+    }
+}
+
+// One wave per output row: the splits' sums at their largest reference point.
+template <int D>
+__global__ __launch_bounds__(256) void int4_merge_kernel(AttentionArgs a, int64_t rows, int dtype) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kWave) + threadIdx.x / kWave;
+    if (row >= rows) return;
+    const int lane = threadIdx.x % kWave;
+    const float* ml = a.part_ml + row * a.splits * 2;
+    const float* part = a.part_o + row * a.splits * D;
+    float m = -__builtin_inff();
+    for (int s = lane; s < a.splits; s += kWave) m = fmaxf(m, ml[2 * s]);
+    m = wave_max(m);
+    float o[D / kWave] = {}, l = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+        if (ml[2 * s] == -__builtin_inff()) continue;  // saw no row
+        const float w = __builtin_amdgcn_exp2f(ml[2 * s] - m);
+        l = fmaf(w, ml[2 * s + 1], l);
+#pragma unroll
+        for (int c = 0; c < D / kWave; ++c) o[c] = fmaf(w, part[s * D + c * kWave + lane], o[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < D / kWave; ++c) store_from_f32(a.out, row * D + c * kWave + lane, dtype, l == 0.f ? 0.f : o[c] / l);
+}
+
+template <int D, int GROUP, int Dt>
+void launch_typed(const AttentionArgs& a, int tiles, hipStream_t stream) {
+    hipLaunchKernelGGL((int4_attention_kernel<D, GROUP, Dt>), dim3(a.splits, a.L.n_kv * tiles, a.L.batch),
+                       dim3(kWaves * kWave), 0, stream, a);
+    if (a.splits > 1) {
+        const int64_t rows = static_cast<int64_t>(a.L.batch) * a.n_q * a.q_len;
+        hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, a, rows, Dt);
+    }
+}
+
+}  // namespace
+
+int64_t int4_part_bytes(const lf_int4_layer& L, int n_q, int q_len, int splits) {
+    return splits <= 1 ? 0 : static_cast<int64_t>(L.batch) * n_q * q_len * splits * (L.head_dim + 2) * 4;
+}
+
+int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream) {
+    AttentionArgs a{};
+    a.L = L;
+    a.q = A.query;
+    a.qb = A.q_strides[0]; a.qh = A.q_strides[1]; a.qt = A.q_strides[2];
+    const int esize = A.dtype == LF_FP32 ? 4 : 2;
+    a.vec = reinterpret_cast<uintptr_t>(A.query) % 16 == 0;
+    for (int i = 0; i < 3; ++i) a.vec = a.vec && A.q_strides[i] * esize % 16 == 0;
+    a.q_lens = A.q_lens;
+    a.out = A.out;
+    a.n_q = A.n_q; a.g = A.n_q / L.n_kv; a.q_len = A.q_len;
+    a.qscale = A.scaling * kLog2e;
+    a.pages = A.pages; a.n_pages = A.n_pages;
+    a.splits = A.splits;
+    a.split_tokens = A.split_tokens;
+    const int64_t rows = static_cast<int64_t>(L.batch) * A.n_q * A.q_len;
+    a.part_o = static_cast<float*>(A.workspace);
+    a.part_ml = a.part_o + rows * A.splits * L.head_dim;
+    int tiles = (a.g * A.q_len + kTile - 1) / kTile;
+    if (A.n_pages) {
+        tiles = (a.g + kTile - 1) / kTile * A.q_len;
+        const int records = L.page_size / kBlock * (A.n_pages + 1);
+        a.split_tokens = (records + A.splits - 1) / A.splits;
+    }
+    return int4_dispatch(L, [&](auto shape) {
+        constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
+        if (A.dtype == LF_BF16) launch_typed<D, GROUP, LF_BF16>(a, tiles, stream);
+        else if (A.dtype == LF_FP16) launch_typed<D, GROUP, LF_FP16>(a, tiles, stream);
+        else launch_typed<D, GROUP, LF_FP32>(a, tiles, stream);
+        const hipError_t err = hipGetLastError();
+        return err == hipSuccess ? LF_OK : static_cast<int>(err);
+    });
+}
+
+}  // namespace lf

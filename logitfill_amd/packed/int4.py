@@ -1,0 +1,479 @@
+"""A KV cache held in 4 bits, quantised as it is written, and the attention that reads it.
+
+It stands beside ``PackedKVManager`` for the cases that need no tier table: every token's Key and
+Value row is kept as 4-bit codes with a float16 scale and minimum per ``group_size`` channels (the
+rule of ``layout.asymmetric_codes`` at 4 bits), written the moment it is committed.  There is no
+residual page and nothing to flush, the cache can be truncated (rejected draft tokens), and every
+write position lives on the device, so a step that commits and attends can be captured in a HIP
+graph and replayed until the capacity is reached.
+
+* ``Int4KVManager``  -- the cache of a model's layers (``commit``, ``truncate``, ``reset``; a layer's
+  ``read`` / ``dequantize``).
+* ``int4_attention`` -- commits the new tokens, then attends over the cached rows; with ``pages``
+  over those pages and the query's own one only.
+* ``select_pages``   -- the pages whose Keys' bounds admit the largest ``q . k``, per query token and
+  kv head.
+
+No reference counterpart: the reference's packed backend keeps Values at 2 bits in its kernel and
+falls back to the dense path for other widths (``src/logitfill/packed/reference.py:62-68``).
+Nothing here runs on the CPU.
+"""
+from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import Optional
+
+import torch
+
+from logitfill_amd import _native
+from logitfill_amd.packed.cache import _check_device
+from logitfill_amd.packed.reference import _cu_count
+
+BLOCK = 32  # tokens of a storage record
+MAX_SPLITS = 1024
+MAX_PAGES = 1024
+
+
+def _block_bytes(head_dim: int, group: int) -> int:
+    """``LF_INT4_BLOCK_BYTES``."""
+    return BLOCK * (head_dim + 8 * (head_dim // group))
+
+
+def check_layout(head_dim: int, page_size: int, group_size: int) -> None:
+    """The layouts the kernels serve; ``ValueError`` for any other."""
+    if head_dim not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256, got {head_dim}")
+    if group_size not in (32, 64, 128) or group_size > head_dim:
+        raise ValueError(f"group_size must be 32, 64 or 128 and at most head_dim {head_dim}, got {group_size}")
+    if page_size <= 0 or page_size % BLOCK or page_size > 1024:
+        raise ValueError(f"page_size must be a multiple of {BLOCK} up to 1024, got {page_size}")
+
+
+def _on(device: torch.device):
+    """``device`` made current for a launch (the default stream names no device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _check_rows(t: torch.Tensor, device: torch.device, name: str) -> torch.Tensor:
+    """``t`` as the kernels read it: on this device, a row type they take, unit channel stride."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}; logitfill_amd runs on ROCm devices only")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+    _native.dtype_code(t.dtype)
+    t = t.detach()
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides(t: torch.Tensor):
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+class _Int4Store:
+    """One layer's 4-bit rows for ``batch`` sequences."""
+
+    def __init__(self, n_kv: int, head_dim: int, page_size: int, group_size: int, *, device="cuda", batch: int = 1,
+                 capacity_tokens: int = 0):
+        self.device = _check_device(device)
+        self.n_kv, self.head_dim = int(n_kv), int(head_dim)
+        self.page_size, self.group_size = int(page_size), int(group_size)
+        check_layout(self.head_dim, self.page_size, self.group_size)
+        if self.n_kv <= 0 or int(batch) <= 0:
+            raise ValueError("n_kv and batch must be positive")
+        self.batch = int(batch)
+        self.lengths = [0] * self.batch
+        self._cap = 0
+        self._blocks: Optional[torch.Tensor] = None
+        self._bounds: Optional[torch.Tensor] = None
+        self._struct: Optional[_native.Int4Layer] = None
+        with torch.inference_mode(False):
+            self._lens = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
+        self._dirty = False  # the device's lengths are behind the host's
+        if capacity_tokens:
+            self.reserve(capacity_tokens)
+
+    @property
+    def length(self) -> int:
+        """Tokens of sequence 0."""
+        return self.lengths[0]
+
+    @property
+    def capacity(self) -> int:
+        return self._cap
+
+    # ---- storage -------------------------------------------------------------
+    def reserve(self, tokens: int) -> None:
+        """Grow the capacity to at least ``tokens`` per sequence (doubling, page aligned).  The new arrays have
+        other addresses: a captured graph keeps the old ones, so reserve before the capture."""
+        P = self.page_size
+        need = -(-int(tokens) // P) * P
+        if need <= self._cap:
+            return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"the cache holds {self._cap} tokens and the captured step needs {tokens}: "
+                               "reserve the capacity before the capture")
+        cap = max(need, 2 * self._cap)
+        if cap > 1 << 30:
+            cap = need
+        if cap > 1 << 30:
+            raise ValueError(f"{tokens} tokens per sequence (at most {1 << 30})")
+        B, H, D = self.batch, self.n_kv, self.head_dim
+        with torch.inference_mode(False), torch.no_grad():
+            blocks = torch.zeros(B, H, cap // BLOCK, _block_bytes(D, self.group_size), dtype=torch.uint8,
+                                 device=self.device)
+            bounds = torch.zeros(B, H, cap // P, 2, D, dtype=torch.bfloat16, device=self.device)
+            if self._cap:
+                blocks[:, :, : self._cap // BLOCK].copy_(self._blocks)
+                bounds[:, :, : self._cap // P].copy_(self._bounds)
+        self._blocks, self._bounds, self._cap, self._struct = blocks, bounds, cap, None
+
+    def layer_struct(self) -> _native.Int4Layer:
+        """The ``lf_int4_layer`` describing this store, its device lengths up to date on the current stream."""
+        if self._cap == 0:
+            self.reserve(self.page_size)
+        if self._dirty:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the cache was truncated or reset since its last launch: "
+                                   "call manager.sync_lengths() before the capture")
+            if min(self.lengths) == max(self.lengths):
+                self._lens.fill_(self.lengths[0])
+            else:
+                self._lens.copy_(_native.upload(self.lengths, torch.int32, self.device))
+            self._dirty = False
+        if self._struct is None:
+            s = _native.Int4Layer()
+            s.blocks, s.bounds, s.lens = self._blocks.data_ptr(), self._bounds.data_ptr(), self._lens.data_ptr()
+            s.batch, s.n_kv, s.head_dim = self.batch, self.n_kv, self.head_dim
+            s.cap_tokens, s.page_size, s.group = self._cap, self.page_size, self.group_size
+            self._struct = s
+        return self._struct
+
+    def set_lengths(self, lengths) -> None:
+        """Host lengths; the device's follow before the next launch."""
+        lengths = [int(n) for n in lengths]
+        if lengths != self.lengths:
+            self.lengths = lengths
+            self._dirty = True
+
+    def page_bounds(self) -> torch.Tensor:
+        """bf16 ``[batch, n_kv, capacity / page_size, 2, head_dim]``: every full page's smallest and largest Key per
+        channel (the values read back, rounded outward); what stands behind a sequence's full pages has no meaning."""
+        if self._cap == 0:
+            self.reserve(self.page_size)
+        return self._bounds
+
+    # ---- rows ------------------------------------------------------------------
+    def check_append(self, key: torch.Tensor, value: torch.Tensor, lengths):
+        """Checked ``(key, value, per-sequence counts or None)`` of an append."""
+        if key.dim() != 4 or key.shape != value.shape:
+            raise ValueError(f"Key and Value rows must be of one shape [batch, n_kv, T, head_dim], got "
+                             f"{tuple(key.shape)} and {tuple(value.shape)}")
+        B, H, T, D = (int(x) for x in key.shape)
+        if B != self.batch or H != self.n_kv or D != self.head_dim:
+            raise ValueError(f"expected [{self.batch}, {self.n_kv}, T, {self.head_dim}], got {tuple(key.shape)}")
+        if key.dtype != value.dtype:
+            raise TypeError("key and value must share a dtype")
+        key, value = _check_rows(key, self.device, "key"), _check_rows(value, self.device, "value")
+        if lengths is not None:
+            lengths = [int(n) for n in lengths]
+            if len(lengths) != B or min(lengths) < 0 or max(lengths) > T:
+                raise ValueError("lengths must give 0 <= length <= T for every sequence")
+            if min(lengths) == T:
+                lengths = None
+        return key, value, lengths
+
+    def append_batch(self, key: torch.Tensor, value: torch.Tensor, lengths=None,
+                     counts: Optional[torch.Tensor] = None) -> None:
+        """Append ``key/value [batch, n_kv, T, head_dim]`` (sequence b its first ``lengths[b]`` tokens; ``counts``:
+        the same on the device, if the caller has them there)."""
+        key, value, lengths = self.check_append(key, value, lengths)
+        T = int(key.shape[2])
+        if T == 0 or (lengths is not None and max(lengths) == 0):
+            return
+        new = [n + (T if lengths is None else lengths[b]) for b, n in enumerate(self.lengths)]
+        with _on(self.device):
+            self.reserve(max(new))
+            struct = self.layer_struct()
+            if lengths is not None and counts is None:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a commit of ragged lengths uploads them and cannot be captured")
+                counts = _native.upload(lengths, torch.int32, self.device)
+            st = _native.load().lf_int4_append(
+                struct, key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key), _strides(value),
+                0 if lengths is None else counts.data_ptr(), T, _native.current_stream_ptr(self.device))
+        _native.check(st, "lf_int4_append")
+        self.lengths = new
+
+    def read(self, starts, tokens: int, dtype=torch.float32):
+        """``tokens`` rows of every sequence read back: ``(K, V) [batch, n_kv, tokens, head_dim]``, row t of sequence b
+        the cache's row ``starts[b] + t`` (an int for all; rows outside the sequence are zeros)."""
+        starts = [int(starts)] * self.batch if isinstance(starts, int) else [int(x) for x in starts]
+        tokens = int(tokens)
+        if len(starts) != self.batch or min(starts) < 0 or max(starts) > 1 << 30 or not 0 <= tokens <= 1 << 30:
+            raise ValueError("read takes one start per sequence and a number of tokens, none negative")
+        code = _native.dtype_code(dtype)
+        k = torch.empty(self.batch, self.n_kv, tokens, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
+        if tokens:
+            with _on(self.device):
+                struct = self.layer_struct()
+                at = None if max(starts) == 0 else _native.upload(starts, torch.int32, self.device)
+                st = _native.load().lf_int4_read(struct, 0 if at is None else at.data_ptr(), tokens, k.data_ptr(),
+                                                 v.data_ptr(), code, _native.current_stream_ptr(self.device))
+            _native.check(st, "lf_int4_read")
+        return k, v
+
+    def dequantize(self, b: int = 0):
+        """Dense float32 ``(K, V) [n_kv, length, head_dim]`` of sequence ``b`` (as ``_LayerStore.dequantize``)."""
+        if not 0 <= b < self.batch:
+            raise IndexError(f"sequence {b} of a batch of {self.batch}")
+        k, v = self.read(0, self.lengths[b])
+        return k[b], v[b]
+
+
+class Int4KVManager:
+    """The 4-bit cache of ``n_layers`` layers for ``batch_size`` sequences.
+
+    ``head_dim`` 64, 128 or 256; ``group_size`` 32, 64 or 128 channels per scale and minimum;
+    ``page_size`` (a multiple of 32 up to 1024) is the unit of ``select_pages``.  ``top_pages``: the
+    model integration attends that many selected pages per query and kv head (0: every row).
+    """
+
+    commits_new_tokens = True  # the attention writes the new tokens before it reads
+
+    def __init__(self, n_layers: int, n_q: int, n_kv: int, head_dim: int, page_size: int = 128, group_size: int = 64,
+                 device="cuda", *, batch_size: int = 1, capacity_tokens: int = 0, top_pages: int = 0):
+        self.n_q, self.n_kv, self.head_dim = int(n_q), int(n_kv), int(head_dim)
+        self.page_size, self.group_size = int(page_size), int(group_size)
+        self.batch_size, self.top_pages = int(batch_size), int(top_pages)
+        if self.n_kv <= 0 or self.n_q <= 0 or self.n_q % self.n_kv:
+            raise ValueError("query heads must divide into KV heads")
+        if not 0 <= self.top_pages <= MAX_PAGES:
+            raise ValueError(f"top_pages must lie in 0 .. {MAX_PAGES}, got {top_pages}")
+        check_layout(self.head_dim, self.page_size, self.group_size)
+        self.device = _check_device(device)
+        self.seq_len = 0
+        self.layers = [_Int4Store(self.n_kv, self.head_dim, self.page_size, self.group_size, device=self.device,
+                                  batch=self.batch_size, capacity_tokens=capacity_tokens) for _ in range(int(n_layers))]
+        self._workspaces: dict = {}
+
+    def commit(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor, lengths=None) -> None:
+        """Append ``key/value [batch, n_kv, T, head_dim]`` to layer ``layer_idx``, quantised as they are written.
+        ``lengths``: per-sequence token counts for ragged batches."""
+        self._append(layer_idx, key, value, lengths)
+
+    def _append(self, layer_idx: int, key, value, lengths, counts=None) -> None:
+        if key.shape[0] != self.batch_size:
+            raise NotImplementedError(
+                f"this manager holds {self.batch_size} sequence(s); got a batch of {key.shape[0]}")
+        self.layers[layer_idx].append_batch(key, value, lengths, counts)
+        self._note(layer_idx)
+
+    def _note(self, layer_idx: int) -> None:
+        if self.layers[layer_idx] is self.layers[-1]:
+            self.seq_len = self.layers[-1].length
+
+    def layer_length(self, layer_idx: int) -> int:
+        return self.layers[layer_idx].length
+
+    def truncate(self, lengths) -> None:
+        """Forget every layer's tokens past ``lengths[b]`` (an int for all; rejected draft tokens, a prompt's common
+        start).  The device's lengths follow with the next call; before a capture, call ``sync_lengths``."""
+        lengths = [int(lengths)] * self.batch_size if isinstance(lengths, int) else [int(n) for n in lengths]
+        if len(lengths) != self.batch_size:
+            raise ValueError("truncate takes one length per sequence")
+        for layer in self.layers:
+            if any(n < 0 or n > have for n, have in zip(lengths, layer.lengths)):
+                raise ValueError(f"truncate to {lengths}: the cache holds {layer.lengths}")
+        for layer in self.layers:
+            layer.set_lengths(lengths)
+        self.seq_len = self.layers[-1].length if self.layers else 0
+
+    def advance(self, tokens) -> None:
+        """Tell the host of tokens that replays of a captured step committed on the device (per sequence, or an int for
+        all): graph replays move the device's lengths only."""
+        tokens = [int(tokens)] * self.batch_size if isinstance(tokens, int) else [int(n) for n in tokens]
+        if len(tokens) != self.batch_size or min(tokens) < 0:
+            raise ValueError("advance takes one count of tokens per sequence, none negative")
+        for layer in self.layers:
+            if any(n + t > layer.capacity for n, t in zip(layer.lengths, tokens)):
+                raise ValueError("more tokens than the cache's capacity")
+        for layer in self.layers:
+            layer.lengths = [n + t for n, t in zip(layer.lengths, tokens)]
+        self.seq_len = self.layers[-1].length if self.layers else 0
+
+    def sync_lengths(self) -> None:
+        """Bring the device's lengths up to the host's on the current stream (before a capture)."""
+        for layer in self.layers:
+            with _on(layer.device):
+                layer.layer_struct()
+
+    def reset(self) -> None:
+        """Forget every token (storage is kept for reuse)."""
+        for layer in self.layers:
+            layer.set_lengths([0] * self.batch_size)
+        self.seq_len = 0
+
+    def workspace(self, nbytes: int) -> torch.Tensor:
+        """Scratch for one launch (needs no clearing).  One per stream, grown on demand: calls on a stream follow one
+        another.  A capture takes memory of its own, which the graph keeps: two graphs share none."""
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=self.device)
+        stream = _native.current_stream_ptr(self.device)
+        ws = self._workspaces.get(stream)
+        if ws is None or ws.numel() < nbytes:
+            with torch.inference_mode(False):
+                ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=self.device)
+            self._workspaces[stream] = ws
+        return ws
+
+
+def _check_query(manager, query: torch.Tensor) -> torch.Tensor:
+    if query.dim() != 4 or query.shape[0] != manager.batch_size or query.shape[1] != manager.n_q \
+            or query.shape[3] != manager.head_dim:
+        raise ValueError(f"query must be [{manager.batch_size}, {manager.n_q}, q_len, {manager.head_dim}], "
+                         f"got {tuple(query.shape)}")
+    if query.shape[2] < 1:
+        raise ValueError("query holds no token")
+    return _check_rows(query, manager.device, "query")
+
+
+def _query_lengths(manager, q_len: int, lengths):
+    """Per-sequence query tokens as a device tensor, or None when every sequence has ``q_len``."""
+    if lengths is None:
+        return None
+    lengths = [int(n) for n in lengths]
+    if len(lengths) != manager.batch_size or min(lengths) < 0 or max(lengths) > q_len:
+        raise ValueError("lengths must give 0 <= length <= q_len for every sequence")
+    if min(lengths) == q_len:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a call of ragged lengths uploads them and cannot be captured")
+    return _native.upload(lengths, torch.int32, manager.device)
+
+
+def _args(manager, query: torch.Tensor, counts, scaling: float) -> _native.Int4Args:
+    a = _native.Int4Args()
+    a.query, a.dtype = query.data_ptr(), _native.dtype_code(query.dtype)
+    a.n_q, a.q_len = manager.n_q, int(query.shape[2])
+    a.q_strides = _strides(query)
+    a.q_lens = 0 if counts is None else counts.data_ptr()
+    a.scaling = float(scaling)
+    return a
+
+
+# A launch of about this many workgroups per CU, none of less than MIN_SPLIT tokens.
+WORKGROUPS_PER_CU = 4
+MIN_SPLIT = 128
+
+
+def plan_splits(tokens: int, rows: int, cus: int) -> tuple[int, int]:
+    """``(splits, tokens of each)`` for sequences of up to ``tokens`` rows, ``rows`` workgroups per split."""
+    want = max(1, WORKGROUPS_PER_CU * cus // max(rows, 1))
+    size = max(MIN_SPLIT, -(-tokens // want))
+    size = -(-size // MIN_SPLIT) * MIN_SPLIT
+    splits = max(1, -(-tokens // size))
+    if splits > MAX_SPLITS:
+        size = -(-(-(-tokens // MAX_SPLITS)) // MIN_SPLIT) * MIN_SPLIT
+        splits = -(-tokens // size)
+    return splits, size
+
+
+def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, key_new: Optional[torch.Tensor],
+                   value_new: Optional[torch.Tensor], scaling: float, *, lengths=None,
+                   pages: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Commit the new tokens, then attend: ``query [B, n_q, q_len, D]`` -> ``[B, n_q, q_len, D]``.
+
+    ``key_new / value_new [B, n_kv, q_len, D]`` (None: they are in the cache already) are appended to
+    the layer as ``manager.commit`` does; the queries are the sequence's last ``q_len`` tokens, each
+    of which sees the cached rows up to its own.  ``lengths``: per-sequence token counts of a ragged
+    batch; rows of the output behind them, and rows of queries that see no token, are zeros.
+
+    ``pages`` (int32 ``[B, n_kv, q_len, n]``, from ``select_pages``): each query token attends its own
+    page up to itself and the listed pages before it.  Entries ascend; a negative one, one that is
+    not before the own page or not above its predecessor is not attended.  Without it a manager of
+    ``top_pages`` selects that many itself.
+
+    Everything is enqueued on the current stream.
+    """
+    layer = manager.layers[layer_idx]
+    query = _check_query(manager, query)
+    q_len = int(query.shape[2])
+    B, D = manager.batch_size, manager.head_dim
+    if (key_new is None) != (value_new is None):
+        raise ValueError("key_new and value_new come together")
+    if key_new is not None:
+        key_new, value_new, _ = layer.check_append(key_new, value_new, lengths)
+        if key_new.shape[2] != q_len:
+            raise ValueError(f"{key_new.shape[2]} new tokens and {q_len} query tokens")
+    if pages is not None:
+        if pages.dim() != 4 or tuple(pages.shape[:3]) != (B, manager.n_kv, q_len) or not 1 <= pages.shape[3] <= MAX_PAGES:
+            raise ValueError(f"pages must be [{B}, {manager.n_kv}, {q_len}, 1 .. {MAX_PAGES}], got {tuple(pages.shape)}")
+        if pages.dtype != torch.int32:
+            raise TypeError(f"pages must be int32, got {pages.dtype}")
+        if pages.device != manager.device:
+            raise ValueError(f"pages are on {pages.device}, the cache on {manager.device}")
+        pages = pages.contiguous()
+    with _on(manager.device):
+        counts = _query_lengths(manager, q_len, lengths)
+        if key_new is not None:
+            manager._append(layer_idx, key_new, value_new, lengths, counts)
+        if pages is None and manager.top_pages:
+            pages = _select(manager, layer, query, manager.top_pages, counts)
+        out = torch.empty(B, manager.n_q, q_len, D, dtype=query.dtype, device=manager.device)
+        a = _args(manager, query, counts, scaling)
+        a.out = out.data_ptr()
+        group = manager.n_q // manager.n_kv
+        cus = _cu_count(manager.device)
+        if pages is None:
+            tiles = -(-group * q_len // 16)
+            a.splits, a.split_tokens = plan_splits(max(max(layer.lengths), 1), B * manager.n_kv * tiles, cus)
+        else:
+            a.pages, a.n_pages = pages.data_ptr(), int(pages.shape[3])
+            tiles = -(-group // 16) * q_len
+            seen = min(a.n_pages + 1, -(-max(max(layer.lengths), 1) // layer.page_size)) * layer.page_size
+            a.splits, _ = plan_splits(seen, B * manager.n_kv * tiles, cus)
+        lib = _native.load()
+        struct = layer.layer_struct()
+        if a.splits > 1:
+            a.workspace_bytes = lib.lf_int4_workspace_bytes(struct, a.n_q, a.q_len, a.splits)
+            ws = manager.workspace(a.workspace_bytes)
+            a.workspace = ws.data_ptr()
+        st = lib.lf_int4_attention(struct, a, _native.current_stream_ptr(manager.device))
+    _native.check(st, "lf_int4_attention")
+    return out
+
+
+def _select(manager, layer, query: torch.Tensor, top_pages: int, counts) -> torch.Tensor:
+    q_len = int(query.shape[2])
+    lib = _native.load()
+    struct = layer.layer_struct()
+    pages = torch.empty(manager.batch_size, manager.n_kv, q_len, top_pages, dtype=torch.int32, device=manager.device)
+    a = _args(manager, query, counts, 1.0)
+    a.pages, a.n_pages = pages.data_ptr(), top_pages
+    a.workspace_bytes = lib.lf_int4_select_workspace_bytes(struct, q_len)
+    ws = manager.workspace(a.workspace_bytes)
+    a.workspace = ws.data_ptr()
+    st = lib.lf_int4_select(struct, a, _native.current_stream_ptr(manager.device))
+    _native.check(st, "lf_int4_select")
+    return pages
+
+
+def select_pages(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, top_pages: int, *,
+                 lengths=None) -> torch.Tensor:
+    """The pages that each query token's kv head attends: int32 ``[B, n_kv, q_len, top_pages]``, ascending, -1
+    behind the last one.
+
+    ``query [B, n_q, q_len, D]``: the sequence's last ``q_len`` tokens, already committed.  Candidates
+    are the pages before the query's own one (which ``int4_attention`` attends by itself); a page's
+    score is the largest, over the kv head's query heads, of ``sum_c max(q_c lo_c, q_c hi_c)`` with the
+    page's ``page_bounds``, formed in float64.  Equal scores: the lower page first.
+    """
+    query = _check_query(manager, query)
+    top_pages = int(top_pages)
+    if not 1 <= top_pages <= MAX_PAGES:
+        raise ValueError(f"top_pages must lie in 1 .. {MAX_PAGES}, got {top_pages}")
+    with _on(manager.device):
+        counts = _query_lengths(manager, int(query.shape[2]), lengths)
+        return _select(manager, manager.layers[layer_idx], query, top_pages, counts)
