@@ -101,14 +101,42 @@ __device__ __forceinline__ void query8(const AttentionArgs& a, int64_t at, float
     }
 }
 
+// A wave's ring of records in LDS, filled by DMA: ``kRing`` - 1 of them are on their way while one is worked on.
+constexpr int kRing = 3;
+template <int D, int GROUP>
+struct Ring {
+    using R = Int4Rec<D, GROUP>;
+    static constexpr int loads = (R::bytes + 1023) / 1024;  // DMA instructions a record takes
+    static constexpr int bytes = kWaves * kRing * R::bytes;
+    static constexpr int pad = D + 4;                       // floats between rows of the waves' merge
+    static constexpr int merge = (kWaves - 1) * kTile * pad * 4;
+    static constexpr int lds = bytes > merge ? bytes : merge;
+
+    static __device__ __forceinline__ void load(const uint8_t* rec, uint32_t slot, int lane) {
+        const unsigned char* g = rec + 16 * lane;
+#pragma unroll
+        for (int k = 0; k < R::bytes / 1024; ++k) dma16(g + 1024 * k, slot + 1024 * k);
+        constexpr int rest = R::bytes % 1024 / 16;
+        if constexpr (rest > 0)
+            if (lane < rest) dma16(g + R::bytes / 1024 * 1024, slot + R::bytes / 1024 * 1024);
+    }
+};
+
+// This wave's DMA so far is done, except the newest N instructions, and so are its LDS reads.
+template <int N>
+__device__ __forceinline__ void wait_ring() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
 template <int D, int GROUP, int Dt>
 __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(AttentionArgs a) {
     using R = Int4Rec<D, GROUP>;
+    using S = Ring<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
     constexpr int NT = Dt == LF_BF16 ? 1 : Dt == LF_FP16 ? 2 : 3;
-    constexpr int kPad = D + 4;
-    __shared__ __attribute__((aligned(16))) float lds_o[(kWaves - 1) * kTile * kPad];
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float lds_ml[kWaves][kTile][2];
+    int32_t* lds_pages = reinterpret_cast<int32_t*>(smem + S::lds);  // with pages only
     const int b = blockIdx.z, lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
     // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
@@ -143,21 +171,55 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
         first = part * a.split_tokens;
         last = min(first + a.split_tokens, per_page * (a.n_pages + 1));
         if (top == 0) last = first;
+        // the pages of the list that the split takes, -1 for an entry that is none in front of the own page
+        const int32_t* list = a.pages + ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * a.n_pages;
+        const int e0 = first / per_page, e1 = (last + per_page - 1) / per_page;
+        for (int e = e0 + threadIdx.x; e < e1; e += kWaves * kWave) {
+            int page = own;
+            if (e > 0) {
+                page = list[e - 1];
+                if (page < 0 || page >= own || (e > 1 && page <= list[e - 2])) page = -1;
+            }
+            lds_pages[e - e0] = page;
+        }
+        __syncthreads();
     } else {
         const int blocks = (top + kBlock - 1) / kBlock, per = a.split_tokens / kBlock;
         first = static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
         last = part + 1 == a.splits ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
     }
-    const int32_t* list = a.n_pages ? a.pages + ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * a.n_pages : nullptr;
+    const int count = last > first + wave ? (last - first - wave + kWaves - 1) / kWaves : 0;  // this wave's records
+    // The k-th of them, or -1 for one that is not attended (its place in the ring is filled with another).
+    const auto block_of = [&](int k) {
+        const int at = first + wave + k * kWaves;
+        if (!a.n_pages) return at;
+        const int e = at / per_page, page = in_sgpr(lds_pages[e - first / per_page]);
+        const int block = page * per_page + (at - e * per_page);
+        return page < 0 || block * kBlock >= top ? -1 : block;
+    };
+    const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
+    const uint32_t ring = lds_addr(smem) + wave * kRing * R::bytes;
+    const auto fill = [&](int k, int slot) {
+        const int block = block_of(k);
+        S::load(base + static_cast<int64_t>(block < 0 ? own * per_page : block) * R::bytes, ring + slot * R::bytes, lane);
+    };
+#pragma unroll
+    for (int k = 0; k < kRing - 1; ++k)
+        if (k < count) fill(k, k);
 
     Parts<NT> q[CH];
     float qsum[G];
+    const bool flip = a.qscale < 0.f;  // a negative scale goes into the queries: scores are then compared unscaled
+    const float qscale = fmaxf(fabsf(a.qscale), 1e-37f);
 #pragma unroll
     for (int g = 0; g < G; ++g) qsum[g] = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         float x[8] = {};
         if (real) query8<Dt>(a, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 32 * c + 8 * quad, x);
+        if (flip)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = -x[e];
         const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
         q[c] = split<NT>(lo, hi);
         qsum[c / CG] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
@@ -174,66 +236,51 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
 #pragma unroll
     for (int g = 0; g < G; ++g) { fix[g] = f32x4{0.f, 0.f, 0.f, 0.f}; pm[g] = 0.f; }
 
-    for (int k = first + wave; k < last; k += kWaves) {
-        int block = k;
-        bool masked;
-        if (a.n_pages) {
-            const int e = k / per_page;
-            int page = own;
-            if (e > 0) {
-                page = list[e - 1];
-                const int before = e > 1 ? list[e - 2] : -1;
-                if (page <= before || page >= own) continue;  // (a negative page is not above the one before)
-                if (page < 0) continue;
-            }
-            block = page * per_page + k % per_page;
-            if (block * kBlock >= top) continue;
-            masked = block * kBlock + kBlock > all;
-        } else {
-            masked = block * kBlock + kBlock > all;
-        }
-        const uint8_t* rec = int4_block(a.L, b, h, block, R::bytes);
-        uint32_t kw[2][CH], vw[VT], ks[2][4][G], vs[2][4][G];
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(rec);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int c = 0; c < CH; ++c) kw[t][c] = words[(16 * t + col) * (D / 8) + CH * quad + c];
-#pragma unroll
-        for (int t = 0; t < VT; ++t) vw[t] = words[R::v / 4 + lane * VT + t];
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int g = 0; g < G; ++g) {
-                    ks[t][r][g] = words[R::ksm / 4 + (16 * t + 4 * quad + r) * G + g];
-                    vs[t][r][g] = words[R::vsm / 4 + (16 * t + 4 * quad + r) * G + g];
-                }
+    int slot = 0;
+    for (int k = 0; k < count; ++k) {
+        if (k + kRing - 1 <= count) wait_ring<(kRing - 2) * S::loads>();
+        else wait_ring<0>();
+        if (k + kRing - 1 < count) fill(k + kRing - 1, slot == 0 ? kRing - 1 : slot - 1);
+        const unsigned char* rec = smem + (wave * kRing + slot) * R::bytes;
+        slot = slot + 1 == kRing ? 0 : slot + 1;
+        const int block = block_of(k);
+        if (block < 0) continue;
+
         float y[2][4];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            uint32_t kw[CH];
+            __builtin_memcpy(kw, __builtin_assume_aligned(rec + (16 * t + col) * (D / 2) + CH * 4 * quad, CH == 2 ? 8 : 16), CH * 4);
+            u32x4 ks[G];
+            const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::ksm + (16 * t + 4 * quad) * 4 * G);
+#pragma unroll
+            for (int g = 0; g < G; ++g) ks[g] = sm[g];
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const float start = -kCodeBias * qsum[g];
                 f32x4 acc = {start, start, start, start};
 #pragma unroll
                 for (int c = g * CG; c < (g + 1) * CG; ++c) {
-                    const bf16x8 codes = codes8(kw[t][c]);
+                    const bf16x8 codes = codes8(kw[c]);
 #pragma unroll
                     for (int m = NT - 1; m >= 0; --m) acc = mfma(codes, q[c].t[m], acc);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float x = fmaf(pair_scale(ks[t][r][g]), acc[r], pair_min(ks[t][r][g]) * qsum[g]);
-                    y[t][r] = g == 0 ? x : y[t][r] + x;
+                    const uint32_t pair = ks[(r * G + g) >> 2][(r * G + g) & 3];
+                    const float m = g == 0 ? pair_min(pair) * qsum[g] : fmaf(pair_min(pair), qsum[g], y[t][r]);
+                    y[t][r] = fmaf(pair_scale(pair), acc[r], m);
                 }
             }
+        }
+        u32x4 vs[2][G];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t) {
+            const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::vsm + (16 * t + 4 * quad) * 4 * G);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[t][r] *= a.qscale;
-        if (masked) {
+            for (int g = 0; g < G; ++g) vs[t][g] = sm[g];
+        }
+        if (block * kBlock + kBlock > all) {
             // rows a query does not see: no score, and neither scale nor minimum (what stands there need not be finite)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -242,11 +289,15 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
                     const bool seen = block * kBlock + 16 * t + 4 * quad + r < lim;
                     y[t][r] = seen ? y[t][r] : -__builtin_inff();
 #pragma unroll
-                    for (int g = 0; g < G; ++g) vs[t][r][g] = seen ? vs[t][r][g] : 0u;
+                    for (int g = 0; g < G; ++g) {
+                        uint32_t pair = vs[t][(r * G + g) >> 2][(r * G + g) & 3];
+                        vs[t][(r * G + g) >> 2][(r * G + g) & 3] = seen ? pair : 0u;
+                    }
                 }
         }
         float most = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
                            fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
+        most *= qscale;
         if (__any(most > limit)) {
             most = rows_max(most);
             const bool moves = most > limit;
@@ -263,27 +314,31 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
         for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                p[t][r] = __builtin_amdgcn_exp2f(y[t][r] - ref);
+                p[t][r] = __builtin_amdgcn_exp2f(fmaf(y[t][r], qscale, -ref));
                 l += p[t][r];
             }
+        const u32x4* vw = reinterpret_cast<const u32x4*>(rec + R::v) + lane;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             float lo[4], hi[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                lo[r] = p[0][r] * pair_scale(vs[0][r][g]);
-                hi[r] = p[1][r] * pair_scale(vs[1][r][g]);
-                pm[g] = fmaf(p[0][r], pair_min(vs[0][r][g]), pm[g]);
-                pm[g] = fmaf(p[1][r], pair_min(vs[1][r][g]), pm[g]);
+                const uint32_t a0 = vs[0][(r * G + g) >> 2][(r * G + g) & 3], a1 = vs[1][(r * G + g) >> 2][(r * G + g) & 3];
+                lo[r] = p[0][r] * pair_scale(a0);
+                hi[r] = p[1][r] * pair_scale(a1);
+                pm[g] = fmaf(p[0][r], pair_min(a0), pm[g]);
+                pm[g] = fmaf(p[1][r], pair_min(a1), pm[g]);
                 pm[g] = fmaf(7.5f, lo[r], pm[g]);
                 pm[g] = fmaf(7.5f, hi[r], pm[g]);
             }
             const Parts<NT> w = split<NT>(lo, hi);
 #pragma unroll
-            for (int m = NT - 1; m >= 0; --m) {
-                fix[g] = mfma(middle, w.t[m], fix[g]);
+            for (int m = NT - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
 #pragma unroll
-                for (int t = g * TG; t < (g + 1) * TG; ++t) o[t] = mfma(codes8(vw[t]), w.t[m], o[t]);
+            for (int t = g * TG; t < (g + 1) * TG; ++t) {
+                const bf16x8 codes = codes8(vw[(t >> 2) * kWave][t & 3]);
+#pragma unroll
+                for (int m = NT - 1; m >= 0; --m) o[t] = mfma(codes, w.t[m], o[t]);
             }
         }
     }
@@ -294,7 +349,8 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
     if (quad == 0) { lds_ml[wave][col][0] = m_wave; lds_ml[wave][col][1] = l; }
 #pragma unroll
     for (int g = 0; g < G; ++g) pm[g] = rows_sum(pm[g]);
-    __syncthreads();
+    __syncthreads();  // every wave is done with its ring, too
+    float* lds_o = reinterpret_cast<float*>(smem);
     float m_all = lds_ml[0][col][0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) m_all = fmaxf(m_all, lds_ml[w][col][0]);
@@ -302,7 +358,7 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
         o[t] = (o[t] + fix[t / TG] + pm[t / TG]) * mine;
-        if (wave > 0) *reinterpret_cast<f32x4*>(lds_o + ((wave - 1) * kTile + col) * kPad + 16 * t + 4 * quad) = o[t];
+        if (wave > 0) *reinterpret_cast<f32x4*>(lds_o + ((wave - 1) * kTile + col) * S::pad + 16 * t + 4 * quad) = o[t];
     }
     __syncthreads();
     if (wave > 0) return;
@@ -312,16 +368,16 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
         const float m = lds_ml[w][col][0];
         l_all += m == -__builtin_inff() ? 0.f : lds_ml[w][col][1] * __builtin_amdgcn_exp2f(m - m_all);
 #pragma unroll
-        for (int t = 0; t < VT; ++t) o[t] += *reinterpret_cast<const f32x4*>(lds_o + ((w - 1) * kTile + col) * kPad + 16 * t + 4 * quad);
+        for (int t = 0; t < VT; ++t) o[t] += *reinterpret_cast<const f32x4*>(lds_o + ((w - 1) * kTile + col) * S::pad + 16 * t + 4 * quad);
     }
     if (!real) return;
     const int64_t row = (static_cast<int64_t>(b) * a.n_q + h * a.g + i) * a.q_len + j;
     if (a.splits == 1) {
-        const float inv = l_all > 0.f ? 1.f / l_all : l_all == 0.f ? 0.f : l_all;
+        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;  // (no row seen: zeros)
 #pragma unroll
         for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) store_from_f32(a.out, row * D + 16 * t + 4 * quad + r, Dt, inv == 0.f && l_all == 0.f ? 0.f : o[t][r] * inv);
+            for (int r = 0; r < 4; ++r) store_from_f32(a.out, row * D + 16 * t + 4 * quad + r, Dt, o[t][r] * inv);
         return;
     }
     float* dst = a.part_o + (row * a.splits + part) * D;
@@ -334,37 +390,70 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
     }
 }
 
-// One wave per output row: the splits' sums at their largest reference point.
+// The splits' sums at their largest reference point: a workgroup per output row, whose waves take the splits in
+// turn (sixteen of every 64, all loads on their way at once) and add up through LDS.
 template <int D>
-__global__ __launch_bounds__(256) void int4_merge_kernel(AttentionArgs a, int64_t rows, int dtype) {
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kWave) + threadIdx.x / kWave;
-    if (row >= rows) return;
-    const int lane = threadIdx.x % kWave;
+__global__ __launch_bounds__(256) void int4_merge_kernel(AttentionArgs a, int dtype) {
+    constexpr int C = D / kWave, kTake = 16;
+    __shared__ float lds[4][D];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave)), waves = blockDim.x / kWave;
     const float* ml = a.part_ml + row * a.splits * 2;
-    const float* part = a.part_o + row * a.splits * D;
+    const float* parts = a.part_o + row * a.splits * D + lane * C;
     float m = -__builtin_inff();
     for (int s = lane; s < a.splits; s += kWave) m = fmaxf(m, ml[2 * s]);
     m = wave_max(m);
-    float o[D / kWave] = {}, l = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-        if (ml[2 * s] == -__builtin_inff()) continue;  // saw no row
-        const float w = __builtin_amdgcn_exp2f(ml[2 * s] - m);
-        l = fmaf(w, ml[2 * s + 1], l);
+    float o[C] = {}, l = 0.f;
+    for (int s0 = 0; s0 < a.splits; s0 += kWave) {
+        float w = 0.f;
+        if (s0 + lane < a.splits) {
+            const float ms = ml[2 * (s0 + lane)];
+            w = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+            l = w == 0.f ? l : fmaf(w, ml[2 * (s0 + lane) + 1], l);
+        }
+        for (int k0 = wave * kTake; k0 < kWave && s0 + k0 < a.splits; k0 += waves * kTake) {
+            float x[kTake][C];
 #pragma unroll
-        for (int c = 0; c < D / kWave; ++c) o[c] = fmaf(w, part[s * D + c * kWave + lane], o[c]);
+            for (int k = 0; k < kTake; ++k)
+#pragma unroll
+                for (int c = 0; c < C; ++c) x[k][c] = s0 + k0 + k < a.splits ? parts[(s0 + k0 + k) * D + c] : 0.f;
+#pragma unroll
+            for (int k = 0; k < kTake; ++k) {
+                // (a split that saw no row weighs nothing, whatever stands in its place)
+                const float wk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), k0 + k));
+#pragma unroll
+                for (int c = 0; c < C; ++c) o[c] = wk == 0.f ? o[c] : fmaf(wk, x[k][c], o[c]);
+            }
+        }
+    }
+    l = wave_sum(l);
+    if (waves > 1) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) lds[wave][lane * C + c] = o[c];
+        __syncthreads();
+        if (wave > 0) return;
+        for (int v = 1; v < waves; ++v)
+#pragma unroll
+            for (int c = 0; c < C; ++c) o[c] += lds[v][lane * C + c];
     }
 #pragma unroll
-    for (int c = 0; c < D / kWave; ++c) store_from_f32(a.out, row * D + c * kWave + lane, dtype, l == 0.f ? 0.f : o[c] / l);
+    for (int c = 0; c < C; ++c) store_from_f32(a.out, row * D + lane * C + c, dtype, l == 0.f ? 0.f : o[c] / l);
 }
 
 template <int D, int GROUP, int Dt>
-void launch_typed(const AttentionArgs& a, int tiles, hipStream_t stream) {
-    hipLaunchKernelGGL((int4_attention_kernel<D, GROUP, Dt>), dim3(a.splits, a.L.n_kv * tiles, a.L.batch),
-                       dim3(kWaves * kWave), 0, stream, a);
+int launch_typed(const AttentionArgs& a, int tiles, hipStream_t stream) {
+    const auto fn = int4_attention_kernel<D, GROUP, Dt>;
+    int lds = Ring<D, GROUP>::lds;
+    if (a.n_pages) lds += 4 * (a.split_tokens / (a.L.page_size / kBlock) + 2);  // the split's entries of the page list
+    const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
+    if (st != LF_OK) return st;
+    hipLaunchKernelGGL(fn, dim3(a.splits, a.L.n_kv * tiles, a.L.batch), dim3(kWaves * kWave), lds, stream, a);
     if (a.splits > 1) {
-        const int64_t rows = static_cast<int64_t>(a.L.batch) * a.n_q * a.q_len;
-        hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, stream, a, rows, Dt);
+        const uint32_t rows = static_cast<uint32_t>(a.L.batch) * a.n_q * a.q_len;
+        hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.splits > 16 ? 256 : 64), 0, stream, a, Dt);
     }
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }
 
 }  // namespace
@@ -399,11 +488,9 @@ int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStre
     }
     return int4_dispatch(L, [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
-        if (A.dtype == LF_BF16) launch_typed<D, GROUP, LF_BF16>(a, tiles, stream);
-        else if (A.dtype == LF_FP16) launch_typed<D, GROUP, LF_FP16>(a, tiles, stream);
-        else launch_typed<D, GROUP, LF_FP32>(a, tiles, stream);
-        const hipError_t err = hipGetLastError();
-        return err == hipSuccess ? LF_OK : static_cast<int>(err);
+        return A.dtype == LF_BF16 ? launch_typed<D, GROUP, LF_BF16>(a, tiles, stream)
+               : A.dtype == LF_FP16 ? launch_typed<D, GROUP, LF_FP16>(a, tiles, stream)
+                                    : launch_typed<D, GROUP, LF_FP32>(a, tiles, stream);
     });
 }
 

@@ -44,8 +44,8 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t w) {
 
 // A Key row's word w (channels 8 w .. 8 w + 7) and a Value block's word of (token, channel), in words.
 __host__ __device__ constexpr int key_word(int D, int w) { return (w & 3) * (D / 32) + (w >> 2); }
-__host__ __device__ constexpr int value_word(int D, int tok, int c) {
-    return (((tok & 15) >> 2) * 16 + (c & 15)) * (D / 16) + (c >> 4);
+__host__ __device__ constexpr int value_word(int tok, int c) {
+    return (((c >> 6) * 64 + ((tok & 15) >> 2) * 16 + (c & 15)) << 2) + ((c >> 4) & 3);
 }
 __host__ __device__ constexpr int value_nibble(int tok) { return (tok & 3) + 4 * (tok >> 4); }
 

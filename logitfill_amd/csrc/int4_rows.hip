@@ -107,15 +107,17 @@ __device__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int s
         const int tok = 4 * quad + (e & 3) + 16 * (e >> 2);
         if (tok >= t0 && tok < t1) fresh |= nibble_bits(15u, e);
     }
-    uint32_t* vw = reinterpret_cast<uint32_t*>(rec + R::v) + lane * (D / 16);
+    u32x4* vw = reinterpret_cast<u32x4*>(rec + R::v) + lane;
 #pragma unroll
-    for (int t = 0; t < D / 16; ++t) {
-        uint32_t word = 0;
+    for (int u = 0; u < D / 64; ++u) {
+        u32x4 word = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-            word |= nibble_bits(codes[(4 * quad + (e & 3) + 16 * (e >> 2)) * D + 16 * t + c0] & 15u, e);
-        if (whole) vw[t] = word;
-        else if (fresh) vw[t] = (vw[t] & ~fresh) | (word & fresh);
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                word[t] |= nibble_bits(codes[(4 * quad + (e & 3) + 16 * (e >> 2)) * D + 64 * u + 16 * t + c0] & 15u, e);
+        if (whole) vw[u * kWave] = word;
+        else if (fresh) vw[u * kWave] = (vw[u * kWave] & ~fresh) | (word & fresh);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -280,7 +282,7 @@ __global__ __launch_bounds__(256) void int4_read_kernel(ReadArgs a) {
                 const uint32_t* v = reinterpret_cast<const uint32_t*>(rec + R::v);
                 const int e = value_nibble(row);
 #pragma unroll
-                for (int c = 0; c < 8; ++c) code[c] = turn(v[value_word(D, row, 8 * w + c)], (4 * e + 3) & 31) & 15u;
+                for (int c = 0; c < 8; ++c) code[c] = turn(v[value_word(row, 8 * w + c)], (4 * e + 3) & 31) & 15u;
             }
         }
 #pragma unroll
