@@ -385,8 +385,8 @@ int32_t lf_unpack_ints(const int32_t* words, int64_t rows, int32_t n_words, int3
  *     Key codes      u32 [32][head_dim / 8]   a row's word w (channels 8 w ..) at (w % 4) * (head_dim / 32) + w / 4
  *     Value codes    u32 [head_dim / 64][4][16][4]   word (s, q, c, t): channel 64 s + 16 t + c of tokens
  *                                             4 q .. 4 q + 3 (lower nibbles) and 16 + 4 q .. 16 + 4 q + 3
- *     Key scale, min fp16 [32][head_dim / group][2]
- *     Value scale, min fp16 [32][head_dim / group][2]
+ *     Key scale, min fp16 [head_dim / group][32][2]
+ *     Value scale, min fp16 [head_dim / group][32][2]
  *   A code word's nibble e is in bits (4 e + 3) % 32 .. of the word: the word rotated left by 3.
  * ``bounds``: bf16 [batch][n_kv][cap_tokens / page_size][2][head_dim], every full page's smallest and
  * largest Key per channel (of the values read back), rounded outward.  ``lens``: DEVICE int32 [batch],

@@ -79,6 +79,10 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// LDS reads stay behind this point: hoisted all to a record's start they take more registers than three waves a
+// SIMD leave.
+__device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
+
 template <int Dt>
 __device__ __forceinline__ void query8(const AttentionArgs& a, int64_t at, float (&x)[8]) {
     if (a.vec) {
@@ -102,7 +106,7 @@ __device__ __forceinline__ void query8(const AttentionArgs& a, int64_t at, float
 }
 
 // A wave's ring of records in LDS, filled by DMA: ``kRing`` - 1 of them are on their way while one is worked on.
-constexpr int kRing = 3;
+constexpr int kRing = 2;
 template <int D, int GROUP>
 struct Ring {
     using R = Int4Rec<D, GROUP>;
@@ -129,7 +133,7 @@ __device__ __forceinline__ void wait_ring() {
 }
 
 template <int D, int GROUP, int Dt>
-__global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(AttentionArgs a) {
     using R = Int4Rec<D, GROUP>;
     using S = Ring<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
@@ -137,10 +141,14 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float lds_ml[kWaves][kTile][2];
     int32_t* lds_pages = reinterpret_cast<int32_t*>(smem + S::lds);  // with pages only
-    const int b = blockIdx.z, lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    // Workgroups are dispatched x fastest, one XCD after the other: kv heads first, so that the XCDs get equal shares
+    // of sequences of unlike lengths (splits first: 32 ragged contexts of 4K-64K tokens in 4 splits 545 us, against 429: 2 of 8 XCDs
+    // had the last, mostly empty split) and the row tiles of a head, which read the same records, few of them; the
+    // splits last, so that a long sequence's later ones follow everyone's first.
+    const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
+    const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
     // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
-    const int tiles = gridDim.y / a.L.n_kv, h = blockIdx.y / tiles, tile = blockIdx.y % tiles;
     int i, j;
     if (a.n_pages) {
         j = tile % a.q_len;
@@ -165,7 +173,7 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
 
     // records of this split
     const int per_page = a.L.page_size / kBlock;
-    const int part = blockIdx.x, own = top > 0 ? (top - 1) / a.L.page_size : 0;
+    const int own = top > 0 ? (top - 1) / a.L.page_size : 0;
     int first, last;
     if (a.n_pages) {
         first = part * a.split_tokens;
@@ -236,28 +244,23 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
 #pragma unroll
     for (int g = 0; g < G; ++g) { fix[g] = f32x4{0.f, 0.f, 0.f, 0.f}; pm[g] = 0.f; }
 
-    int slot = 0;
-    for (int k = 0; k < count; ++k) {
-        if (k + kRing - 1 <= count) wait_ring<(kRing - 2) * S::loads>();
-        else wait_ring<0>();
-        if (k + kRing - 1 < count) fill(k + kRing - 1, slot == 0 ? kRing - 1 : slot - 1);
-        const unsigned char* rec = smem + (wave * kRing + slot) * R::bytes;
-        slot = slot + 1 == kRing ? 0 : slot + 1;
-        const int block = block_of(k);
-        if (block < 0) continue;
-
+    // One record, of tokens from t0.  Masked: rows a query does not see get no score, and neither scale nor minimum (what
+    // stands there need not be finite).  (Branches around the selects alone: two copies of the body, one without them,
+    // took 40 registers more.)
+    const auto attend = [&](const unsigned char* rec, bool masked, int t0) {
+        const auto seen = [&](int t, int r) { return t0 + 16 * t + 4 * quad + r < lim; };
         float y[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             uint32_t kw[CH];
             __builtin_memcpy(kw, __builtin_assume_aligned(rec + (16 * t + col) * (D / 2) + CH * 4 * quad, CH == 2 ? 8 : 16), CH * 4);
-            u32x4 ks[G];
-            const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::ksm + (16 * t + 4 * quad) * 4 * G);
-#pragma unroll
-            for (int g = 0; g < G; ++g) ks[g] = sm[g];
+            const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::ksm) + 4 * t + quad;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const float start = -kCodeBias * qsum[g];
+                const u32x4 pair = sm[8 * g];
+                float start = -kCodeBias * qsum[g];
+                // (formed anew per record: kept, the G accumulator starts take the registers of a third wave)
+                if constexpr (G > 2) asm volatile("" : "+v"(start));
                 f32x4 acc = {start, start, start, start};
 #pragma unroll
                 for (int c = g * CG; c < (g + 1) * CG; ++c) {
@@ -267,33 +270,14 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const uint32_t pair = ks[(r * G + g) >> 2][(r * G + g) & 3];
-                    const float m = g == 0 ? pair_min(pair) * qsum[g] : fmaf(pair_min(pair), qsum[g], y[t][r]);
-                    y[t][r] = fmaf(pair_scale(pair), acc[r], m);
+                    const float m = g == 0 ? pair_min(pair[r]) * qsum[g] : fmaf(pair_min(pair[r]), qsum[g], y[t][r]);
+                    y[t][r] = fmaf(pair_scale(pair[r]), acc[r], m);
                 }
             }
-        }
-        u32x4 vs[2][G];
+            phase();
+            if (masked)
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::vsm + (16 * t + 4 * quad) * 4 * G);
-#pragma unroll
-            for (int g = 0; g < G; ++g) vs[t][g] = sm[g];
-        }
-        if (block * kBlock + kBlock > all) {
-            // rows a query does not see: no score, and neither scale nor minimum (what stands there need not be finite)
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool seen = block * kBlock + 16 * t + 4 * quad + r < lim;
-                    y[t][r] = seen ? y[t][r] : -__builtin_inff();
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        uint32_t pair = vs[t][(r * G + g) >> 2][(r * G + g) & 3];
-                        vs[t][(r * G + g) >> 2][(r * G + g) & 3] = seen ? pair : 0u;
-                    }
-                }
+                for (int r = 0; r < 4; ++r) y[t][r] = seen(t, r) ? y[t][r] : -__builtin_inff();
         }
         float most = fmaxf(fmaxf(fmaxf(y[0][0], y[0][1]), fmaxf(y[0][2], y[0][3])),
                            fmaxf(fmaxf(y[1][0], y[1][1]), fmaxf(y[1][2], y[1][3])));
@@ -317,21 +301,27 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
                 p[t][r] = __builtin_amdgcn_exp2f(fmaf(y[t][r], qscale, -ref));
                 l += p[t][r];
             }
+        phase();
         const u32x4* vw = reinterpret_cast<const u32x4*>(rec + R::v) + lane;
+        const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::vsm) + quad;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            float lo[4], hi[4];
+            u32x4 pair[2] = {sm[8 * g], sm[8 * g + 4]};
+            if (masked)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t a0 = vs[0][(r * G + g) >> 2][(r * G + g) & 3], a1 = vs[1][(r * G + g) >> 2][(r * G + g) & 3];
-                lo[r] = p[0][r] * pair_scale(a0);
-                hi[r] = p[1][r] * pair_scale(a1);
-                pm[g] = fmaf(p[0][r], pair_min(a0), pm[g]);
-                pm[g] = fmaf(p[1][r], pair_min(a1), pm[g]);
-                pm[g] = fmaf(7.5f, lo[r], pm[g]);
-                pm[g] = fmaf(7.5f, hi[r], pm[g]);
-            }
-            const Parts<NT> w = split<NT>(lo, hi);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) pair[t][r] = seen(t, r) ? pair[t][r] : 0u;
+            float x[2][4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    x[t][r] = p[t][r] * pair_scale(pair[t][r]);
+                    pm[g] = fmaf(p[t][r], pair_min(pair[t][r]), pm[g]);
+                    pm[g] = fmaf(7.5f, x[t][r], pm[g]);
+                }
+            const Parts<NT> w = split<NT>(x[0], x[1]);
 #pragma unroll
             for (int m = NT - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
 #pragma unroll
@@ -340,7 +330,21 @@ __global__ __launch_bounds__(kWaves * kWave) void int4_attention_kernel(Attentio
 #pragma unroll
                 for (int m = NT - 1; m >= 0; --m) o[t] = mfma(codes, w.t[m], o[t]);
             }
+            phase();
         }
+    };
+
+    int slot = 0;
+    for (int k = 0; k < count; ++k) {
+        if (k + kRing - 1 <= count) wait_ring<(kRing - 2) * S::loads>();
+        else wait_ring<0>();
+        if (k + kRing - 1 < count) fill(k + kRing - 1, slot == 0 ? kRing - 1 : slot - 1);
+        const unsigned char* rec = smem + (wave * kRing + slot) * R::bytes;
+        slot = slot + 1 == kRing ? 0 : slot + 1;
+        const int block = block_of(k);
+        if (block < 0) continue;
+
+        attend(rec, block * kBlock + kBlock > all, block * kBlock);
     }
 
     // the waves' sums at one reference point
@@ -447,7 +451,7 @@ int launch_typed(const AttentionArgs& a, int tiles, hipStream_t stream) {
     if (a.n_pages) lds += 4 * (a.split_tokens / (a.L.page_size / kBlock) + 2);  // the split's entries of the page list
     const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
     if (st != LF_OK) return st;
-    hipLaunchKernelGGL(fn, dim3(a.splits, a.L.n_kv * tiles, a.L.batch), dim3(kWaves * kWave), lds, stream, a);
+    hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, a);
     if (a.splits > 1) {
         const uint32_t rows = static_cast<uint32_t>(a.L.batch) * a.n_q * a.q_len;
         hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.splits > 16 ? 256 : 64), 0, stream, a, Dt);

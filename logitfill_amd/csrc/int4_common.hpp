@@ -20,7 +20,7 @@ struct Int4Rec {
     static constexpr int chunks = D / 32;       // words of a Key row that one lane of a product takes
     static constexpr int v = 16 * D;            // Key codes: 32 rows of D / 2 bytes
     static constexpr int ksm = 32 * D;
-    static constexpr int vsm = ksm + 128 * G;   // 32 rows of G (scale, min) pairs
+    static constexpr int vsm = ksm + 128 * G;   // G times 32 rows' (scale, min) pairs
     static constexpr int bytes = vsm + 128 * G;
     static_assert(bytes == LF_INT4_BLOCK_BYTES(D, GROUP), "record size");
 };

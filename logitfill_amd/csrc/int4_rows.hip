@@ -83,7 +83,7 @@ __device__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int s
             quantise8<GROUP>(x, code, s, lo);
             if (row >= t1) continue;
             if (w % (GROUP / 8) == 0)
-                sm[row * R::G + w / (GROUP / 8)] = f32_to_f16(s) | static_cast<uint32_t>(f32_to_f16(lo)) << 16;
+                sm[w / (GROUP / 8) * kBlock + row] = f32_to_f16(s) | static_cast<uint32_t>(f32_to_f16(lo)) << 16;
             if (kv == 0) {
                 uint32_t word = 0;
 #pragma unroll
@@ -145,7 +145,7 @@ __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int 
         const uint8_t* rec = rec0 + (t / kBlock) * R::bytes;
         const int row = t % kBlock;
         const uint32_t word = reinterpret_cast<const uint32_t*>(rec)[row * LR + key_word(D, w)];
-        const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + R::ksm)[row * R::G + w / (GROUP / 8)];
+        const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + R::ksm)[w / (GROUP / 8) * kBlock + row];
         const float s = pair_scale(sm), m = pair_min(sm);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void int4_read_kernel(ReadArgs a) {
         uint32_t code[8] = {};
         float s = 0.f, m = 0.f;
         if (there) {
-            const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + (kv ? R::vsm : R::ksm))[row * R::G + g];
+            const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + (kv ? R::vsm : R::ksm))[g * kBlock + row];
             s = pair_scale(sm);
             m = pair_min(sm);
             if (kv == 0) {

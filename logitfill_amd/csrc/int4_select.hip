@@ -14,6 +14,7 @@ struct SelectArgs {
     int64_t qb, qh, qt;
     const int32_t* q_lens;
     int g, q_len, dtype;
+    int vec;  // 2-byte query rows that start on 16 bytes
     int n_pages;
     int32_t* pages;
     uint64_t* keys;  // [batch][n_kv][q_len][cap_tokens / page_size]
@@ -35,11 +36,17 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 }
 
 
-// D / 8 lanes take a page, eight channels each; a workgroup takes kScorePages pages of one (query token, kv head).
-constexpr int kScorePages = 64;
+// D / 8 lanes take a page, eight channels each; a workgroup takes kScorePages pages of one (query token, kv head),
+// eight heads at a time: their elements stay in registers, their sums are exchanged so that each step of the
+// butterfly halves the heads a lane still adds up.
+constexpr int kScorePages = 32, kHeads = 8;
+
+__device__ __forceinline__ double other(double x, int mask) { return __shfl_xor(x, mask, kWave); }
+
 template <int D>
 __global__ __launch_bounds__(256) void int4_score_kernel(SelectArgs a) {
-    constexpr int LR = D / 8, RP = 256 / LR;
+    constexpr int LR = D / 8, RP = 256 / LR, Steps = kScorePages / RP > 0 ? kScorePages / RP : 1;
+    static_assert(LR >= kHeads, "a lane per head");
     const int b = blockIdx.z, h = blockIdx.y / a.q_len, j = blockIdx.y % a.q_len;
     const int count = candidates(a, b, j);
     const int p0 = blockIdx.x * kScorePages;
@@ -49,94 +56,185 @@ __global__ __launch_bounds__(256) void int4_score_kernel(SelectArgs a) {
     const uint16_t* bounds = a.L.bounds + (static_cast<int64_t>(b) * a.L.n_kv + h) * pages * 2 * D + 8 * w;
     uint64_t* keys = a.keys + ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * pages;
     const int p1 = min(p0 + kScorePages, count);
-    for (int base = p0; base < p1; base += RP) {
-        const int page = base + threadIdx.x / LR, from = min(page, p1 - 1);
-        const u32x4 lo = *reinterpret_cast<const u32x4*>(bounds + static_cast<int64_t>(from) * 2 * D);
-        const u32x4 hi = *reinterpret_cast<const u32x4*>(bounds + static_cast<int64_t>(from) * 2 * D + D);
-        double best = -__builtin_inf();
-        bool bad = false;
-        for (int i = 0; i < a.g; ++i) {
-            double sum = 0.;
+    u32x4 lo[Steps], hi[Steps];
+#pragma unroll
+    for (int s = 0; s < Steps; ++s) {
+        const int64_t at = static_cast<int64_t>(min(p0 + s * RP + static_cast<int>(threadIdx.x) / LR, p1 - 1)) * 2 * D;
+        lo[s] = *reinterpret_cast<const u32x4*>(bounds + at);
+        hi[s] = *reinterpret_cast<const u32x4*>(bounds + at + D);
+    }
+    double best[Steps];
+    bool bad[Steps];
+#pragma unroll
+    for (int s = 0; s < Steps; ++s) { best[s] = -__builtin_inf(); bad[s] = false; }
+    for (int i0 = 0; i0 < a.g; i0 += kHeads) {
+        float q[kHeads][8];
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k) {
+            // (heads past the group repeat its last one)
+            const int64_t at = b * a.qb + static_cast<int64_t>(h * a.g + min(i0 + k, a.g - 1)) * a.qh + j * a.qt + 8 * w;
+            if (a.vec) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const uint16_t u = static_cast<uint16_t>(x[e >> 1] >> (16 * (e & 1)));
+                    q[k][e] = a.dtype == LF_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) q[k][e] = load_as_f32(a.q, at + e, a.dtype);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < Steps; ++s) {
+            double sum[kHeads];
+#pragma unroll
+            for (int k = 0; k < kHeads; ++k) sum[k] = 0.;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float q = load_as_f32(a.q, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 8 * w + e, a.dtype);
-                const uint32_t l = e & 1 ? lo[e >> 1] & 0xffff0000u : lo[e >> 1] << 16, u = e & 1 ? hi[e >> 1] & 0xffff0000u : hi[e >> 1] << 16;
-                const float k = __uint_as_float(q < 0.f ? l : u);
-                sum = fma(static_cast<double>(q), static_cast<double>(k), sum);
-            }
+                const uint32_t l = e & 1 ? lo[s][e >> 1] & 0xffff0000u : lo[s][e >> 1] << 16, u = e & 1 ? hi[s][e >> 1] & 0xffff0000u : hi[s][e >> 1] << 16;
 #pragma unroll
-            for (int m = 1; m < LR; m <<= 1) sum += __shfl_xor(sum, m, kWave);
-            bad |= sum != sum;
-            best = sum > best ? sum : best;
+                for (int k = 0; k < kHeads; ++k)
+                    sum[k] = fma(static_cast<double>(q[k][e]), static_cast<double>(__uint_as_float(q[k][e] < 0.f ? l : u)), sum[k]);
+            }
+            // lanes w and w ^ m split the heads that are left, then the lanes of one head add up
+            bool nan = false;
+#pragma unroll
+            for (int m = 1, left = kHeads / 2; left > 0; m <<= 1, left >>= 1)
+#pragma unroll
+                for (int k = 0; k < left; ++k) {
+                    const bool upper = w & m;
+                    const double keep = upper ? sum[k + left] : sum[k], give = upper ? sum[k] : sum[k + left];
+                    sum[k] = keep + other(give, m);
+                }
+#pragma unroll
+            for (int m = kHeads; m < LR; m <<= 1) sum[0] += other(sum[0], m);
+            nan = sum[0] != sum[0];
+            double top = sum[0];
+            int any = nan;
+#pragma unroll
+            for (int m = 1; m < kHeads; m <<= 1) {
+                const double o = other(top, m);
+                top = o > top ? o : top;
+                any |= __shfl_xor(any, m, kWave);
+            }
+            bad[s] |= any != 0;
+            best[s] = top > best[s] ? top : best[s];
         }
-        if (page < p1 && w == 0) keys[page] = bad ? 0 : score_key(best);
+    }
+#pragma unroll
+    for (int s = 0; s < Steps; ++s) {
+        const int page = p0 + s * RP + threadIdx.x / LR;
+        if (page < p1 && w == 0) keys[page] = bad[s] ? 0 : score_key(best[s]);
     }
 }
 
-// A workgroup per (query token, kv head): the n_pages-th largest key, eight bits at a time, then the pages above it
-// and the first of those at it, in order.
-__global__ __launch_bounds__(256) void int4_top_kernel(SelectArgs a) {
+// A workgroup per (query token, kv head): the n_pages-th largest key, eight bits at a time (as far as the pages at
+// the prefix are more than are needed), then the pages above it and the first of those at it, in order.  Thread t
+// holds keys t, t + T, .. in registers (``Hold`` of them, 0: any number, read anew).
+template <int T, int Hold>
+__global__ __launch_bounds__(T) void int4_top_kernel(SelectArgs a) {
+    constexpr int W = T / kWave;
     __shared__ int hist[256];
-    __shared__ int found[2];      // bucket, keys above it
-    __shared__ int wave_sum[2][4];
+    __shared__ int found[3];  // bucket, keys above it, keys in it
+    __shared__ int sums[2][2][W];
     const int b = blockIdx.z, h = blockIdx.y / a.q_len, j = blockIdx.y % a.q_len, tid = threadIdx.x;
+    const int lane = tid % kWave, wave = tid / kWave;
     const int count = candidates(a, b, j), top = a.n_pages;
     const int pages = a.L.cap_tokens / a.L.page_size;
     const int64_t slot = (static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j;
     int32_t* out = a.pages + slot * top;
     if (count <= top) {
-        for (int k = tid; k < top; k += 256) out[k] = k < count ? k : -1;
+        for (int k = tid; k < top; k += T) out[k] = k < count ? k : -1;
         return;
     }
     const uint64_t* keys = a.keys + slot * pages;
+    uint64_t held[Hold ? Hold : 1];
+    if constexpr (Hold > 0)
+#pragma unroll
+        for (int s = 0; s < Hold; ++s) held[s] = s * T + tid < count ? keys[s * T + tid] : 0;
+    const auto each = [&](auto&& fn) {
+        if constexpr (Hold > 0) {
+#pragma unroll
+            for (int s = 0; s < Hold; ++s)
+                if (s * T < count) fn(s * T + tid, held[s]);
+        } else {
+            for (int k0 = 0; k0 < count; k0 += T) fn(k0 + tid, k0 + tid < count ? keys[k0 + tid] : 0);
+        }
+    };
     uint64_t prefix = 0;
-    int need = top;  // keys still to find at the prefix
-    for (int shift = 56; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
+    int need = top, shift = 56;  // keys still to find among those whose upper bits are the prefix
+    for (;; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
         __syncthreads();
-        for (int k = tid; k < count; k += 256)
-            if (shift == 56 || keys[k] >> (shift + 8) == prefix) atomicAdd(&hist[(keys[k] >> shift) & 255], 1);
+        each([&](int k, uint64_t key) {
+            const bool in = k < count && (shift == 56 || key >> (shift + 8) == prefix);
+            const int digit = static_cast<int>(key >> shift) & 255;
+            // a wave whose keys share the digit (the first ones: sign and exponent) counts them at once
+            const uint64_t mask = __ballot(in);
+            if (mask == 0) return;
+            const int lead = __builtin_amdgcn_readlane(digit, __builtin_ctzll(mask));
+            const uint64_t same = __ballot(in && digit == lead);
+            if (lane == 0) atomicAdd(&hist[lead], __popcll(same));
+            if (in && digit != lead) atomicAdd(&hist[digit], 1);
+        });
         __syncthreads();
-        if (tid == 0) {
-            int above = 0, bucket = 255;
-            while (bucket > 0 && above + hist[bucket] < need) above += hist[bucket--];
-            found[0] = bucket;
-            found[1] = above;
+        if (wave == 0) {
+            // lane i: buckets 255 - 4 i down to 252 - 4 i
+            int n[4], mine = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) { n[c] = hist[255 - 4 * lane - c]; mine += n[c]; }
+            int upto = mine;
+#pragma unroll
+            for (int m = 1; m < kWave; m <<= 1) {
+                const int o = __shfl_up(upto, m, kWave);
+                upto += lane >= m ? o : 0;
+            }
+            int above = upto - mine;
+            if (above < need && need <= upto) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    if (above < need && need <= above + n[c]) {
+                        found[0] = 255 - 4 * lane - c;
+                        found[1] = above;
+                        found[2] = n[c];
+                    }
+                    above += n[c];
+                }
+            }
         }
         __syncthreads();
         prefix = prefix << 8 | static_cast<uint64_t>(found[0]);
         need -= found[1];
-        __syncthreads();
+        if (found[2] == need || shift == 0) break;  // (uniform: all threads read the same)
     }
-    // keys above the prefix are in, and the first ``need`` equal to it
-    int placed = 0, equal = 0;
-    for (int k0 = 0; k0 < count; k0 += 256) {
-        const int k = k0 + tid;
-        const uint64_t key = k < count ? keys[k] : 0;
-        const bool is_equal = k < count && key == prefix;
-        const uint64_t eq = __ballot(is_equal);
-        const int lane = tid % kWave, wave = tid / kWave;
-        const uint64_t below = (1ull << lane) - 1;
-        if (lane == 0) wave_sum[0][wave] = __popcll(eq);
-        __syncthreads();
-        int eq_before = equal + __popcll(eq & below), eq_all = equal;
-        for (int v = 0; v < 4; ++v) {
-            if (v < wave) eq_before += wave_sum[0][v];
-            eq_all += wave_sum[0][v];
+    int placed = 0, equal = 0, turn = 0;
+    each([&](int k, uint64_t key) {
+        const uint64_t upper = key >> shift;
+        const bool at = k < count && upper == prefix, over = k < count && upper > prefix;
+        const uint64_t at_mask = __ballot(at), over_mask = __ballot(over), below = (1ull << lane) - 1;
+        if (lane == 0) {
+            sums[turn][0][wave] = __popcll(at_mask);
+            sums[turn][1][wave] = __popcll(over_mask);
         }
-        const bool in = k < count && (key > prefix || (is_equal && eq_before < need));
-        const uint64_t take = __ballot(in);
-        if (lane == 0) wave_sum[1][wave] = __popcll(take);
-        __syncthreads();
-        int at = placed + __popcll(take & below);
-        for (int v = 0; v < 4; ++v) {
-            if (v < wave) at += wave_sum[1][v];
-            placed += wave_sum[1][v];
+        __syncthreads();  // (one per round: the next one writes the other half)
+        int at_before = equal + __popcll(at_mask & below), over_before = placed + __popcll(over_mask & below);
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            if (v < wave) { at_before += sums[turn][0][v]; over_before += sums[turn][1][v]; }
+            equal += sums[turn][0][v];
+            placed += sums[turn][1][v];
         }
-        equal = eq_all;
-        if (in && at < top) out[at] = k;
-        __syncthreads();
-    }
+        // in front of this one: all above the prefix, and of those at it as many as are needed
+        const int place = over_before + min(at_before, need);
+        if ((over || (at && at_before < need)) && place < top) out[place] = k;
+        turn ^= 1;
+    });
+}
+
+template <int T, int Hold>
+void launch_top(const SelectArgs& a, hipStream_t stream) {
+    hipLaunchKernelGGL((int4_top_kernel<T, Hold>), dim3(1, a.L.n_kv * a.q_len, a.L.batch), dim3(T), 0, stream, a);
 }
 
 }  // namespace
@@ -152,6 +250,8 @@ int launch_int4_select(const lf_int4_layer& L, const lf_int4_args& A, hipStream_
     a.qb = A.q_strides[0]; a.qh = A.q_strides[1]; a.qt = A.q_strides[2];
     a.q_lens = A.q_lens;
     a.g = A.n_q / L.n_kv; a.q_len = A.q_len; a.dtype = A.dtype;
+    a.vec = A.dtype != LF_FP32 && reinterpret_cast<uintptr_t>(A.query) % 16 == 0;
+    for (int i = 0; i < 3; ++i) a.vec = a.vec && A.q_strides[i] % 8 == 0;
     a.n_pages = A.n_pages;
     a.pages = A.pages;
     a.keys = static_cast<uint64_t*>(A.workspace);
@@ -162,7 +262,10 @@ int launch_int4_select(const lf_int4_layer& L, const lf_int4_args& A, hipStream_
         return LF_OK;
     });
     if (st != LF_OK) return st;
-    hipLaunchKernelGGL(int4_top_kernel, dim3(1, L.n_kv * A.q_len, L.batch), dim3(256), 0, stream, a);
+    if (pages <= 256) launch_top<256, 1>(a, stream);
+    else if (pages <= 1024) launch_top<256, 4>(a, stream);
+    else if (pages <= 16384) launch_top<1024, 16>(a, stream);
+    else launch_top<1024, 0>(a, stream);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }

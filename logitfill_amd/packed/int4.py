@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -363,21 +364,50 @@ def _args(manager, query: torch.Tensor, counts, scaling: float) -> _native.Int4A
     return a
 
 
-# A launch of about this many workgroups per CU, none of less than MIN_SPLIT tokens.
-WORKGROUPS_PER_CU = 4
-MIN_SPLIT = 128
+# Tokens a split is a multiple of (a record for each of a workgroup's four waves).
+SPLIT_UNIT = 128
+# A workgroup's fixed cost (its queries, the first records' way, the waves' merge, its share of the splits') in
+# units of its work: about 3 us against 2 us a unit.
+SPLIT_OVERHEAD = 1.5
 
 
-def plan_splits(tokens: int, rows: int, cus: int) -> tuple[int, int]:
-    """``(splits, tokens of each)`` for sequences of up to ``tokens`` rows, ``rows`` workgroups per split."""
-    want = max(1, WORKGROUPS_PER_CU * cus // max(rows, 1))
-    size = max(MIN_SPLIT, -(-tokens // want))
-    size = -(-size // MIN_SPLIT) * MIN_SPLIT
-    splits = max(1, -(-tokens // size))
-    if splits > MAX_SPLITS:
-        size = -(-(-(-tokens // MAX_SPLITS)) // MIN_SPLIT) * MIN_SPLIT
-        splits = -(-tokens // size)
-    return splits, size
+def workgroups_per_cu(head_dim: int, group: int) -> int:
+    """Attention workgroups that a CU holds: by registers 4, 3 and 2 at head_dim 64, 128 and 256, and by the record
+    rings' LDS 1 at head_dim 256 with groups of 32."""
+    return {64: 4, 128: 3, 256: 2 if group > 32 else 1}[head_dim]
+
+
+@functools.lru_cache(maxsize=512)
+def _plan(units: tuple, rows: int, slots: int) -> int:
+    """Units a split takes, of sequences of ``units`` (their work, ``rows`` workgroups a split): the size of least
+    estimated time -- all work and every split's fixed cost over the slots, and half a split's for the last round,
+    or one split's where all are there at once."""
+    total, longest = sum(units) * rows, max(units)
+    least = -(-longest // MAX_SPLITS)
+    best, choice = None, longest
+    for k in (1, 1.25, 1.5, 2, 3, 4, 6, 8, 12):
+        for size in {max(least, int(total / (slots * k))), max(least, -int(-total // (slots * k)))}:
+            size = min(max(size, 1), longest)
+            items = rows * sum(-(-u // size) for u in units)
+            if items <= slots:
+                cost = size + SPLIT_OVERHEAD
+            else:
+                cost = (total + SPLIT_OVERHEAD * items) / slots + 0.5 * size
+            if best is None or cost < best:
+                best, choice = cost, size
+    # the next sizes up may make one round of sequences that the even share leaves just above it
+    for size in range(choice, min(longest, 2 * choice) + 1):
+        if rows * sum(-(-u // size) for u in units) <= slots:
+            return size if size + SPLIT_OVERHEAD < best else choice
+    return choice
+
+
+def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3) -> tuple[int, int]:
+    """``(splits, tokens of each)`` for sequences of ``tokens`` rows (an int, or one per sequence), ``rows``
+    workgroups per sequence and split."""
+    tokens = (tokens,) if isinstance(tokens, int) else tokens
+    size = _plan(tuple([-(-n // SPLIT_UNIT) or 1 for n in tokens]), rows, per_cu * cus) * SPLIT_UNIT
+    return -(-max(max(tokens), 1) // size), size
 
 
 def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, key_new: Optional[torch.Tensor],
@@ -425,15 +455,13 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
         a = _args(manager, query, counts, scaling)
         a.out = out.data_ptr()
         group = manager.n_q // manager.n_kv
-        cus = _cu_count(manager.device)
-        if pages is None:
-            tiles = -(-group * q_len // 16)
-            a.splits, a.split_tokens = plan_splits(max(max(layer.lengths), 1), B * manager.n_kv * tiles, cus)
-        else:
+        tokens, tiles = layer.lengths, -(-group * q_len // 16)
+        if pages is not None:
             a.pages, a.n_pages = pages.data_ptr(), int(pages.shape[3])
-            tiles = -(-group // 16) * q_len
-            seen = min(a.n_pages + 1, -(-max(max(layer.lengths), 1) // layer.page_size)) * layer.page_size
-            a.splits, _ = plan_splits(seen, B * manager.n_kv * tiles, cus)
+            # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
+            tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
+        a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, _cu_count(manager.device),
+                                               workgroups_per_cu(D, manager.group_size))
         lib = _native.load()
         struct = layer.layer_struct()
         if a.splits > 1:
