@@ -383,8 +383,9 @@ int32_t lf_unpack_ints(const int32_t* words, int64_t rows, int32_t n_words, int3
  * Storage: ``blocks``, one record per 32 tokens of a (sequence, kv head):
  *   [batch][n_kv][cap_tokens / 32][LF_INT4_BLOCK_BYTES(head_dim, group)], each record
  *     Key codes      u32 [32][head_dim / 8]   a row's word w (channels 8 w ..) at (w % 4) * (head_dim / 32) + w / 4
- *     Value codes    u32 [head_dim / 64][4][16][4]   word (s, q, c, t): channel 64 s + 16 t + c of tokens
- *                                             4 q .. 4 q + 3 (lower nibbles) and 16 + 4 q .. 16 + 4 q + 3
+ *     Value codes    u32 [head_dim / 64][4][16][4]   word (s, q, c, t): one channel of tokens 4 q .. 4 q + 3
+ *                                             (lower nibbles) and 16 + 4 q .. 16 + 4 q + 3; the channel is
+ *                                             64 s + 4 c + t, with groups of 32 64 s + 32 (t / 2) + 2 c + t % 2
  *     Key scale, min fp16 [head_dim / group][32][2]
  *     Value scale, min fp16 [head_dim / group][32][2]
  *   A code word's nibble e is in bits (4 e + 3) % 32 .. of the word: the word rotated left by 3.
@@ -406,9 +407,12 @@ typedef struct lf_int4_layer {
 
 #define LF_INT4_BLOCK_BYTES(head_dim, group) (32 * ((head_dim) + 8 * ((head_dim) / (group))))
 
+/* Set the sequences' lengths (``lens``: HOST int32 [batch], read during the call). */
+int32_t lf_int4_set_lens(const lf_int4_layer* layer, const int32_t* lens, void* stream);
+
 /*
  * Append rows: sequence b gets rows 0 .. counts[b] - 1 of k_src / v_src (``tokens`` rows each; counts, a
- * DEVICE int32 [batch] of 0 .. tokens, NULL: all of them) behind its lens[b], which then advances.  Rows past
+ * HOST int32 [batch] of 0 .. tokens read during the call, NULL: all of them) behind its lens[b], which then advances.  Rows past
  * cap_tokens are not written.  Element strides per sequence, head and token, unit channel stride.  Pages that
  * a sequence completes get their bounds.  Rows that are not finite leave codes, scales and minima without a
  * meaning for their own groups only.
@@ -419,8 +423,8 @@ int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void
 
 /*
  * Read rows back: k_out / v_out [batch][n_kv][tokens][head_dim], contiguous, rounded to ``dtype`` (either may
- * be NULL).  Row t of sequence b is the cache's row starts[b] + t (``starts``: DEVICE int32 [batch], NULL: 0);
- * rows outside 0 .. lens[b] - 1 are zeros.
+ * be NULL, both 16-byte aligned).  Row t of sequence b is the cache's row starts[b] + t (``starts``: HOST int32
+ * [batch] read during the call, NULL: 0); rows outside 0 .. lens[b] - 1 are zeros.
  */
 int32_t lf_int4_read(const lf_int4_layer* layer, const int32_t* starts, int32_t tokens, void* k_out, void* v_out,
                      int32_t dtype, void* stream);

@@ -2,6 +2,7 @@
 #include "int4_common.hpp"
 
 namespace lf {
+int launch_int4_set_lens(const lf_int4_layer& L, const int32_t* lens, hipStream_t stream);
 int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_src, int dtype, const int64_t* k_strides,
                        const int64_t* v_strides, const int32_t* counts, int tokens, hipStream_t stream);
 int launch_int4_read(const lf_int4_layer& L, const int32_t* starts, int tokens, void* k_out, void* v_out, int dtype,
@@ -51,6 +52,15 @@ int32_t check_query(const lf_int4_layer* L, const lf_int4_args* A) {
 
 extern "C" {
 
+int32_t lf_int4_set_lens(const lf_int4_layer* layer, const int32_t* lens, void* stream) {
+    const int32_t st = check_int4(layer);
+    if (st != LF_OK) return st;
+    if (!lens) return LF_E_NULL;
+    for (int32_t b = 0; b < layer->batch; ++b)
+        if (lens[b] < 0 || lens[b] > layer->cap_tokens) return LF_E_SHAPE;
+    return lf::launch_int4_set_lens(*layer, lens, static_cast<hipStream_t>(stream));
+}
+
 int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void* v_src, int32_t dtype,
                        const int64_t* k_strides, const int64_t* v_strides, const int32_t* counts, int32_t tokens,
                        void* stream) {
@@ -60,6 +70,8 @@ int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void
     if (tokens < 0 || tokens > (1 << 30)) return LF_E_SHAPE;
     if (tokens == 0) return LF_OK;
     if (!k_src || !v_src || !k_strides || !v_strides) return LF_E_NULL;
+    for (int32_t b = 0; counts && b < layer->batch; ++b)
+        if (counts[b] < 0 || counts[b] > tokens) return LF_E_SHAPE;
     return lf::launch_int4_append(*layer, k_src, v_src, dtype, k_strides, v_strides, counts, tokens,
                                   static_cast<hipStream_t>(stream));
 }
@@ -71,6 +83,9 @@ int32_t lf_int4_read(const lf_int4_layer* layer, const int32_t* starts, int32_t 
     if (!valid_dtype(dtype)) return LF_E_DTYPE;
     if (tokens < 0 || tokens > (1 << 30)) return LF_E_SHAPE;
     if (!k_out && !v_out) return LF_E_NULL;
+    if (!aligned16(k_out) || !aligned16(v_out)) return LF_E_SHAPE;
+    for (int32_t b = 0; starts && b < layer->batch; ++b)
+        if (starts[b] < 0 || starts[b] > (1 << 30)) return LF_E_SHAPE;
     if (tokens == 0) return LF_OK;
     return lf::launch_int4_read(*layer, starts, tokens, k_out, v_out, dtype, static_cast<hipStream_t>(stream));
 }

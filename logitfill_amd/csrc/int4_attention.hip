@@ -49,12 +49,6 @@ __device__ __forceinline__ uint32_t upper_pair(float a, float b) {
     return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
 }
 __device__ __forceinline__ float upper(float x) { return __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
-}
-
 // Element pairs (a[i], b[i]) in NT bf16 parts; the last part is rounded to nearest, those before it are cut off.
 template <int NT>
 __device__ __forceinline__ Parts<NT> split(const float (&a)[4], const float (&b)[4]) {
@@ -103,6 +97,21 @@ __device__ __forceinline__ void query8(const AttentionArgs& a, int64_t at, float
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = load_as_f32(a.q, at + e, Dt);
     }
+}
+
+// fn(channel, values) for every four consecutive channels that a lane of the transposed output holds.
+template <int D, int GROUP, class Fn>
+__device__ __forceinline__ void each_run(const f32x4 (&o)[D / 16], int quad, Fn&& fn) {
+    constexpr int N = GROUP == 32 ? 2 : 4;  // tiles whose rows' channels are neighbours
+#pragma unroll
+    for (int t = 0; t < D / 16; t += N)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[t + e % N][(4 * k + e) / N];
+            fn(value_channel<GROUP>(4 * quad + 4 * k / N, t), x);
+        }
 }
 
 // A wave's ring of records in LDS, filled by DMA: ``kRing`` - 1 of them are on their way while one is worked on.
@@ -379,14 +388,12 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     if (a.splits == 1) {
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;  // (no row seen: zeros)
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) store_from_f32(a.out, row * D + 16 * t + 4 * quad + r, Dt, o[t][r] * inv);
+        for (int t = 0; t < VT; ++t) o[t] *= inv;
+        each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<Dt>(a.out, row * D + c, x); });
         return;
     }
     float* dst = a.part_o + (row * a.splits + part) * D;
-#pragma unroll
-    for (int t = 0; t < VT; ++t) *reinterpret_cast<f32x4*>(dst + 16 * t + 4 * quad) = o[t];
+    each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<LF_FP32>(dst, c, x); });
     if (quad == 0) {
         float* ml = a.part_ml + (row * a.splits + part) * 2;
         ml[0] = m_all;

@@ -31,9 +31,6 @@ struct Int4Rec {
 __device__ __forceinline__ uint32_t turn(uint32_t w, int bits) { return __builtin_amdgcn_alignbit(w, w, bits); }
 __device__ __forceinline__ uint32_t code_at(uint32_t w, int e) { return turn(w, (4 * e + 3) & 31) & 15u; }
 
-// Bits of nibble e of a word.
-__device__ __forceinline__ uint32_t nibble_bits(uint32_t code, int e) { return turn(code, (32 - (4 * e + 3)) & 31); }
-
 // A word's eight codes as bf16 16 + code; element 2 i is nibble i, element 2 i + 1 nibble i + 4.
 constexpr float kCodeBias = 16.f;
 __device__ __forceinline__ bf16x8 codes8(uint32_t w) {
@@ -42,12 +39,46 @@ __device__ __forceinline__ bf16x8 codes8(uint32_t w) {
                                             (turn(w, 12) & mask) | base});
 }
 
-// A Key row's word w (channels 8 w .. 8 w + 7) and a Value block's word of (token, channel), in words.
+// Where a Key row's word w (channels 8 w .. 8 w + 7) stands in it.
 __host__ __device__ constexpr int key_word(int D, int w) { return (w & 3) * (D / 32) + (w >> 2); }
-__host__ __device__ constexpr int value_word(int tok, int c) {
-    return (((c >> 6) * 64 + ((tok & 15) >> 2) * 16 + (c & 15)) << 2) + ((c >> 4) & 3);
+
+// Four consecutive Value words belong to lane (quad, c): of channels 64 s + 4 c + t, or with groups of 32, where a
+// product's sixteen channels have to be of one group, 64 s + 32 (t / 2) + 2 c + t % 2.  A row r of tile t of the
+// transposed output is then channel value_channel(r, t).
+template <int GROUP>
+__host__ __device__ constexpr int value_channel(int c, int t) {
+    return GROUP == 32 ? 64 * (t >> 2) + 32 * ((t >> 1) & 1) + 2 * c + (t & 1) : 64 * (t >> 2) + 4 * c + (t & 3);
 }
-__host__ __device__ constexpr int value_nibble(int tok) { return (tok & 3) + 4 * (tok >> 4); }
+
+constexpr int kInlineSeqs = 64;  // sequences whose numbers travel in one launch's arguments
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    return f32_to_f16(a) | static_cast<uint32_t>(f32_to_f16(b)) << 16;
+}
+
+// N (2, 4 or 8) floats to consecutive elements, rounded to nearest.
+template <int Dt, int N>
+__device__ __forceinline__ void store_row(void* p, int64_t at, const float (&x)[N]) {
+    if constexpr (Dt == LF_FP32 && N == 2) {
+        *reinterpret_cast<u32x2*>(static_cast<float*>(p) + at) = u32x2{__float_as_uint(x[0]), __float_as_uint(x[1])};
+    } else if constexpr (Dt == LF_FP32) {
+#pragma unroll
+        for (int e = 0; e < N; e += 4) *reinterpret_cast<f32x4*>(static_cast<float*>(p) + at + e) = f32x4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+    } else {
+        uint32_t w[N / 2];
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e) w[e] = Dt == LF_BF16 ? pack_bf16(x[2 * e], x[2 * e + 1]) : pack_f16(x[2 * e], x[2 * e + 1]);
+        uint16_t* dst = static_cast<uint16_t*>(p) + at;
+        if constexpr (N == 8) *reinterpret_cast<u32x4*>(dst) = u32x4{w[0], w[1], w[2], w[3]};
+        else if constexpr (N == 2) *reinterpret_cast<uint32_t*>(dst) = w[0];
+        else *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
+    }
+}
 
 // Record ``block`` of (sequence b, kv head h).
 __device__ __forceinline__ uint8_t* int4_block(const lf_int4_layer& L, int b, int h, int block, int bytes) {

@@ -18,35 +18,55 @@ struct RowsArgs {
     lf_int4_layer L;
     const void* src[2];
     int64_t sb[2], sh[2], st[2];
-    const int32_t* counts;
     int tokens;
-    int vec;  // every source row starts on 16 bytes
+    int vec;       // every source row starts on 16 bytes
+    int b0;        // the launch's first sequence
+    int counted;   // 1: counts holds the tokens of sequences b0 ..
+    int32_t counts[kInlineSeqs];
 };
 
-// Eight consecutive elements of a row as float32.
+// Eight consecutive elements of a row, as they are and as float32.
 template <int Dt>
-__device__ __forceinline__ void load8(const void* p, int64_t at, int vec, float (&x)[8]) {
-    if (vec) {
-        if constexpr (Dt == LF_FP32) {
-            const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
-            const f32x4 a = q[0], b = q[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
+struct Raw8 {
+    u32x4 w[Dt == LF_FP32 ? 2 : 1];
+};
+template <int Dt>
+__device__ __forceinline__ Raw8<Dt> load8(const void* p, int64_t at, int vec) {
+    Raw8<Dt> r;
+    if constexpr (Dt == LF_FP32) {
+        const uint32_t* q = static_cast<const uint32_t*>(p) + at;
+        if (vec) {
+            r.w[0] = *reinterpret_cast<const u32x4*>(q);
+            r.w[1] = *reinterpret_cast<const u32x4*>(q + 4);
         } else {
-            const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint16_t u = static_cast<uint16_t>(a[e >> 1] >> (16 * (e & 1)));
-                x[e] = Dt == LF_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
-            }
+            for (int e = 0; e < 8; ++e) r.w[e >> 2][e & 3] = q[e];
         }
     } else {
+        const uint16_t* q = static_cast<const uint16_t*>(p) + at;
+        if (vec) {
+            r.w[0] = *reinterpret_cast<const u32x4*>(q);
+        } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = load_as_f32(p, at + e, Dt);
+            for (int e = 0; e < 4; ++e) r.w[0][e] = q[2 * e] | static_cast<uint32_t>(q[2 * e + 1]) << 16;
+        }
+    }
+    return r;
+}
+template <int Dt>
+__device__ __forceinline__ void widen8(const Raw8<Dt>& r, float (&x)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if constexpr (Dt == LF_FP32) x[e] = __uint_as_float(r.w[e >> 2][e & 3]);
+        else if constexpr (Dt == LF_BF16) x[e] = __uint_as_float(e & 1 ? r.w[0][e >> 1] & 0xffff0000u : r.w[0][e >> 1] << 16);
+        else x[e] = f16_to_f32(static_cast<uint16_t>(r.w[0][e >> 1] >> (16 * (e & 1))));
     }
 }
 
-// Codes of a lane's eight channels; scale and minimum of their group in every lane.
+// Codes of a lane's eight channels; scale and minimum of their group in every lane.  The quotient is formed from the
+// correctly rounded reciprocal of the scale, which the group's codes share, and one correction by the exact residual
+// (Markstein): the correctly rounded quotient, as the division gives it.  A range beyond float32's is cut to its
+// largest number, whose quotient clamps to 15 as the infinite one does.  Adding 2^23 rounds to an integer, half to even.
 template <int GROUP>
 __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&code)[8], float& s, float& lo) {
     lo = x[0];
@@ -59,64 +79,105 @@ __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&code)[
         hi = fmaxf(hi, __shfl_xor(hi, m, kWave));
     }
     s = fminf(fmaxf((hi - lo) / 15.f, 1e-5f), 1e5f);
+    const float y = 1.f / s;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) code[e] = static_cast<uint32_t>(fminf(fmaxf(rintf((x[e] - lo) / s), 0.f), 15.f));
+    for (int e = 0; e < 8; ++e) {
+        const float d = fminf(x[e] - lo, 3.40282347e38f), q0 = d * y, q = fmaf(fmaf(-q0, s, d), y, q0);
+        code[e] = __float_as_uint(__builtin_amdgcn_fmed3f(q, 0.f, 15.f) + 8388608.f) & 15u;
+    }
+}
+
+// Four Value words from eight tokens' codes of four channels, a byte each: word c's nibble e is byte c of tok[e].
+__device__ __forceinline__ u32x4 value_words(const uint32_t (&tok)[8]) {
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = tok[2 * k] | tok[2 * k + 1] << 4;
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), b = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+    const u32x4 w = {__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u),
+                     __builtin_amdgcn_perm(d, c, 0x05040100u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
+    return u32x4{turn(w[0], 29), turn(w[1], 29), turn(w[2], 29), turn(w[3], 29)};
 }
 
 // Tokens t0 .. t1 - 1 of a record, from source rows src0 .. of (b, h); one wave.  ``codes``: its 32 x D bytes of LDS.
-template <int D, int GROUP, int Dt>
-__device__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int src0, int t0, int t1, uint8_t* codes) {
+// Whole: all 32, every row's load on its way before the first is used.
+template <int D, int GROUP, int Dt, bool Whole>
+__device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int src0, int t0, int t1, uint8_t* codes) {
     using R = Int4Rec<D, GROUP>;
-    constexpr int LR = D / 8, RP = kWave / LR;  // lanes per row, rows per pass
+    constexpr int LR = D / 8, RP = kWave / LR, Passes = kBlock / RP;  // lanes per row, rows per pass
     const int lane = threadIdx.x & (kWave - 1), w = lane % LR;
     uint32_t* words = reinterpret_cast<uint32_t*>(rec);
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        const int64_t base = b * a.sb[kv] + h * a.sh[kv] + 8 * w;
+    const auto load = [&](int kv, int row) {
+        return load8<Dt>(a.src[kv], b * a.sb[kv] + h * a.sh[kv] + 8 * w + (src0 + static_cast<int64_t>(row) - t0) * a.st[kv], a.vec);
+    };
+    const auto take = [&](int kv, int row, const Raw8<Dt>& raw, bool real) {
+        float x[8], s, lo;
+        widen8<Dt>(raw, x);
+        uint32_t code[8];
+        quantise8<GROUP>(x, code, s, lo);
+        if (!real) return;
         uint32_t* sm = reinterpret_cast<uint32_t*>(rec + (kv ? R::vsm : R::ksm));
-        for (int r0 = t0; r0 < t1; r0 += RP) {
-            const int row = r0 + lane / LR;
-            const int from = src0 + min(row, t1 - 1) - t0;
-            float x[8], s, lo;
-            load8<Dt>(a.src[kv], base + from * a.st[kv], a.vec, x);
-            uint32_t code[8];
-            quantise8<GROUP>(x, code, s, lo);
-            if (row >= t1) continue;
-            if (w % (GROUP / 8) == 0)
-                sm[w / (GROUP / 8) * kBlock + row] = f32_to_f16(s) | static_cast<uint32_t>(f32_to_f16(lo)) << 16;
-            if (kv == 0) {
-                uint32_t word = 0;
+        if (w % (GROUP / 8) == 0)
+            sm[w / (GROUP / 8) * kBlock + row] = f32_to_f16(s) | static_cast<uint32_t>(f32_to_f16(lo)) << 16;
+        if (kv == 0) {
+            uint32_t word = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) word |= nibble_bits(code[e], e);
-                words[row * LR + key_word(D, w)] = word;
-            } else {
-                u32x2 packed = {0, 0};
+            for (int e = 0; e < 8; ++e) word |= code[e] << (4 * e);
+            words[row * LR + key_word(D, w)] = turn(word, 29);
+        } else {
+            u32x2 packed = {0, 0};
 #pragma unroll
-                for (int e = 0; e < 8; ++e) packed[e >> 2] |= code[e] << (8 * (e & 3));
-                *reinterpret_cast<u32x2*>(codes + row * D + 8 * w) = packed;
+            for (int e = 0; e < 8; ++e) packed[e >> 2] |= code[e] << (8 * (e & 3));
+            *reinterpret_cast<u32x2*>(codes + row * D + 8 * w) = packed;
+        }
+    };
+    if constexpr (Whole) {
+        constexpr int Ahead = Dt == LF_FP32 || Passes > 8 ? 4 : 8;  // rows on their way
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int p0 = 0; p0 < Passes; p0 += Ahead) {
+                Raw8<Dt> raw[Ahead];
+#pragma unroll
+                for (int p = 0; p < Ahead && p0 + p < Passes; ++p) raw[p] = load(kv, (p0 + p) * RP + lane / LR);
+#pragma unroll
+                for (int p = 0; p < Ahead && p0 + p < Passes; ++p) take(kv, (p0 + p) * RP + lane / LR, raw[p], true);
             }
+    } else {
+        for (int r0 = t0; r0 < t1; r0 += RP) {
+            const int row = r0 + lane / LR, from = min(row, t1 - 1);
+            const Raw8<Dt> k = load(0, from), v = load(1, from);
+            take(0, row, k, row < t1);
+            take(1, row, v, row < t1);
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const bool whole = t0 == 0 && t1 == kBlock;
     const int quad = lane >> 4, c0 = lane & 15;
     uint32_t fresh = 0;  // the nibbles this write replaces
+    if constexpr (!Whole)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int tok = 4 * quad + (e & 3) + 16 * (e >> 2);
-        if (tok >= t0 && tok < t1) fresh |= nibble_bits(15u, e);
-    }
+        for (int e = 0; e < 8; ++e) {
+            const int tok = 4 * quad + (e & 3) + 16 * (e >> 2);
+            if (tok >= t0 && tok < t1) fresh |= turn(15u << (4 * e), 29);
+        }
     u32x4* vw = reinterpret_cast<u32x4*>(rec + R::v) + lane;
 #pragma unroll
     for (int u = 0; u < D / 64; ++u) {
-        u32x4 word = {0, 0, 0, 0};
+        uint32_t tok[8];
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                word[t] |= nibble_bits(codes[(4 * quad + (e & 3) + 16 * (e >> 2)) * D + 64 * u + 16 * t + c0] & 15u, e);
-        if (whole) vw[u * kWave] = word;
+        for (int e = 0; e < 8; ++e) {
+            // (rows this write does not bring: whatever the LDS holds, and replaced below)
+            const uint8_t* at = codes + (4 * quad + (e & 3) + 16 * (e >> 2)) * D + 64 * u;
+            if constexpr (GROUP == 32) {
+                tok[e] = *reinterpret_cast<const uint16_t*>(at + 2 * c0) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(at + 32 + 2 * c0)) << 16;
+            } else {
+                tok[e] = *reinterpret_cast<const uint32_t*>(at + 4 * c0);
+            }
+            if constexpr (!Whole) tok[e] &= 0x0f0f0f0fu;
+        }
+        const u32x4 word = value_words(tok);
+        if constexpr (Whole) vw[u * kWave] = word;
         else if (fresh) vw[u * kWave] = (vw[u * kWave] & ~fresh) | (word & fresh);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -130,8 +191,8 @@ __device__ __forceinline__ uint16_t bf16_up(float x) {
 }
 __device__ __forceinline__ uint16_t bf16_down(float x) { return static_cast<uint16_t>(bf16_up(-x) ^ 0x8000u); }
 
-// Per-channel bounds of full page ``page``'s Keys, from the records: ``n`` threads (whole waves) of index tid.
-// One wave alone (n == 64), or all of a workgroup's with ``red`` [n / 64][2][D] and barriers.
+// Per-channel bounds of full page ``page``'s Keys, from the records, by the whole workgroup (``n`` threads, barriers);
+// ``red`` [n / 64][2][D].
 template <int D, int GROUP>
 __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int tid, int n, float* red) {
     using R = Int4Rec<D, GROUP>;
@@ -141,6 +202,7 @@ __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int 
     float lo[8], hi[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) { lo[e] = __builtin_inff(); hi[e] = -__builtin_inff(); }
+#pragma unroll 4
     for (int t = tid / LR; t < P; t += n / LR) {
         const uint8_t* rec = rec0 + (t / kBlock) * R::bytes;
         const int row = t % kBlock;
@@ -162,15 +224,6 @@ __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int 
             hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], m, kWave));
         }
     uint16_t* out = L.bounds + ((static_cast<int64_t>(b) * L.n_kv + h) * (L.cap_tokens / P) + page) * 2 * D;
-    if (n == kWave) {
-        if (lane < LR)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                out[8 * w + e] = bf16_down(lo[e]);
-                out[D + 8 * w + e] = bf16_up(hi[e]);
-            }
-        return;
-    }
     if (lane < LR)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -185,27 +238,28 @@ __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int 
     }
 }
 
-__device__ __forceinline__ int append_count(const RowsArgs& a, int b) {
-    return a.counts ? min(max(a.counts[b], 0), a.tokens) : a.tokens;
+__device__ __forceinline__ int append_count(const RowsArgs& a, int i) { return a.counted ? a.counts[i] : a.tokens; }
+__device__ __forceinline__ int append_end(const RowsArgs& a, int i, int start) {
+    return static_cast<int>(min(static_cast<int64_t>(start) + append_count(a, i), static_cast<int64_t>(a.L.cap_tokens)));
 }
 
 // Many tokens: a workgroup per (page, kv head, sequence), a wave per record.
 template <int D, int GROUP, int Dt>
 __global__ __launch_bounds__(256) void int4_append_pages_kernel(RowsArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kBlock * D];
-    const int b = blockIdx.z, h = blockIdx.y, P = a.L.page_size;
-    const int start = int4_len(a.L, b);
-    const int end = static_cast<int>(min(static_cast<int64_t>(start) + append_count(a, b), static_cast<int64_t>(a.L.cap_tokens)));
+    const int b = a.b0 + blockIdx.z, h = blockIdx.y, P = a.L.page_size;
+    const int start = int4_len(a.L, b), end = append_end(a, blockIdx.z, start);
     const int page = start / P + blockIdx.x;
     if (static_cast<int64_t>(page) * P >= end) return;
     const int p0 = page * P, lo = max(start, p0), hi = min(end, p0 + P);
-    const int wave = threadIdx.x / kWave;
+    const int wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     for (int k = wave; k < P / kBlock; k += blockDim.x / kWave) {
         const int k0 = p0 + k * kBlock;
         const int t0 = max(lo - k0, 0), t1 = min(hi - k0, kBlock);
-        if (t0 < t1)
-            write_block<D, GROUP, Dt>(a, int4_block(a.L, b, h, k0 / kBlock, Int4Rec<D, GROUP>::bytes), b, h,
-                                      k0 + t0 - start, t0, t1, lds + wave * kBlock * D);
+        if (t0 >= t1) continue;
+        uint8_t* rec = int4_block(a.L, b, h, k0 / kBlock, Int4Rec<D, GROUP>::bytes);
+        if (t1 - t0 == kBlock) write_block<D, GROUP, Dt, true>(a, rec, b, h, k0 - start, 0, kBlock, lds + wave * kBlock * D);
+        else write_block<D, GROUP, Dt, false>(a, rec, b, h, k0 + t0 - start, t0, t1, lds + wave * kBlock * D);
     }
     if (hi < p0 + P) return;
     __threadfence_block();
@@ -214,9 +268,8 @@ __global__ __launch_bounds__(256) void int4_append_pages_kernel(RowsArgs a) {
 }
 
 __global__ void int4_advance_kernel(RowsArgs a) {
-    const int b = blockIdx.x * blockDim.x + threadIdx.x;
-    if (b < a.L.batch)
-        a.L.lens[b] = static_cast<int>(min(static_cast<int64_t>(int4_len(a.L, b)) + append_count(a, b), static_cast<int64_t>(a.L.cap_tokens)));
+    const int i = threadIdx.x, b = a.b0 + i;
+    if (i < kInlineSeqs && b < a.L.batch) a.L.lens[b] = append_end(a, i, int4_len(a.L, b));
 }
 
 // A few tokens (at most a record's): a workgroup per sequence, a wave per kv head; the workgroup advances the length.
@@ -225,97 +278,139 @@ template <int D, int GROUP, int Dt>
 __global__ __launch_bounds__(512) void int4_append_few_kernel(RowsArgs a) {
     constexpr int kWaves = D > 128 ? 4 : 8;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * kBlock * D];
-    const int b = blockIdx.x, P = a.L.page_size, wave = threadIdx.x / kWave;
-    const int start = int4_len(a.L, b);
-    const int end = static_cast<int>(min(static_cast<int64_t>(start) + append_count(a, b), static_cast<int64_t>(a.L.cap_tokens)));
-    for (int h = wave; h < a.L.n_kv && start < end; h += blockDim.x / kWave) {
+    const int b = a.b0 + blockIdx.x, P = a.L.page_size, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    const int start = int4_len(a.L, b), end = append_end(a, blockIdx.x, start);
+    for (int h = wave; h < a.L.n_kv && start < end; h += kWaves)
         for (int k = start / kBlock; k * kBlock < end; ++k) {
             const int t0 = max(start - k * kBlock, 0), t1 = min(end - k * kBlock, kBlock);
-            write_block<D, GROUP, Dt>(a, int4_block(a.L, b, h, k, Int4Rec<D, GROUP>::bytes), b, h, k * kBlock + t0 - start,
-                                      t0, t1, lds + wave * kBlock * D);
+            write_block<D, GROUP, Dt, false>(a, int4_block(a.L, b, h, k, Int4Rec<D, GROUP>::bytes), b, h,
+                                             k * kBlock + t0 - start, t0, t1, lds + wave * kBlock * D);
         }
-        for (int page = start / P; page < end / P; ++page) {
-            __threadfence_block();
-            page_bounds<D, GROUP>(a.L, b, h, page, threadIdx.x % kWave, kWave, nullptr);
-        }
-    }
-    __syncthreads();  // every wave has read the length
+    __threadfence_block();
+    __syncthreads();  // every wave has read the length, and its rows are there
     if (threadIdx.x == 0) a.L.lens[b] = end;
+    for (int page = start / P; page < end / P; ++page)
+        for (int h = 0; h < a.L.n_kv; ++h) {
+            page_bounds<D, GROUP>(a.L, b, h, page, threadIdx.x, kWaves * kWave, reinterpret_cast<float*>(lds));
+            __syncthreads();
+        }
+}
+
+struct LensArgs {
+    int32_t* lens;
+    int b0, n;
+    int32_t value[kInlineSeqs];
+};
+__global__ void int4_set_lens_kernel(LensArgs a) {
+    if (static_cast<int>(threadIdx.x) < a.n) a.lens[a.b0 + threadIdx.x] = a.value[threadIdx.x];
 }
 
 struct ReadArgs {
     lf_int4_layer L;
-    const int32_t* starts;
     int tokens;
+    int b0;
     void* out[2];
-    int dtype;
+    int32_t starts[kInlineSeqs];
 };
 
-// A thread per (token, eight channels): one Key word, and one nibble of eight Value words.
-template <int D, int GROUP>
+// A wave per record: a Key word and row segment of eight channels per lane, then Values of four (two and two) channels
+// and eight tokens.
+template <int D, int GROUP, int Dt>
 __global__ __launch_bounds__(256) void int4_read_kernel(ReadArgs a) {
     using R = Int4Rec<D, GROUP>;
-    constexpr int LR = D / 8;
-    const int b = blockIdx.z, h = blockIdx.y;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int t = static_cast<int>(i / LR), w = static_cast<int>(i % LR);
-    if (t >= a.tokens) return;
-    const int64_t pos = static_cast<int64_t>(a.starts ? a.starts[b] : 0) + t;
-    const bool there = pos >= 0 && pos < int4_len(a.L, b);
-    const int64_t dst = ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.tokens + t) * D + 8 * w;
-    const uint8_t* rec = int4_block(a.L, b, h, there ? static_cast<int>(pos / kBlock) : 0, R::bytes);
-    const int row = there ? static_cast<int>(pos % kBlock) : 0, g = w / (GROUP / 8);
+    constexpr int LR = D / 8, RP = kWave / LR;
+    const int b = a.b0 + blockIdx.z, h = blockIdx.y, lane = threadIdx.x % kWave;
+    const int start = a.starts[blockIdx.z], len = int4_len(a.L, b);
+    const int block = start / kBlock + static_cast<int>(blockIdx.x) * 4 + in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    const int64_t pos0 = static_cast<int64_t>(block) * kBlock, end = static_cast<int64_t>(start) + a.tokens;
+    if (pos0 >= end) return;
+    const bool there = pos0 < len;
+    const uint8_t* rec = int4_block(a.L, b, h, there ? block : 0, R::bytes);
+    // element 0 of the row of the record's token 0, which may lie in front of the first
+    const int64_t dst = ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.tokens + (pos0 - start)) * D;
+    if (a.out[0]) {
+        const int w = lane % LR;
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-        if (!a.out[kv]) continue;
-        uint32_t code[8] = {};
-        float s = 0.f, m = 0.f;
-        if (there) {
-            const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + (kv ? R::vsm : R::ksm))[g * kBlock + row];
-            s = pair_scale(sm);
-            m = pair_min(sm);
-            if (kv == 0) {
-                const uint32_t word = reinterpret_cast<const uint32_t*>(rec)[row * LR + key_word(D, w)];
+        for (int p = 0; p < kBlock / RP; ++p) {
+            const int row = p * RP + lane / LR;
+            const uint32_t word = reinterpret_cast<const uint32_t*>(rec)[row * LR + key_word(D, w)];
+            const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + R::ksm)[w / (GROUP / 8) * kBlock + row];
+            float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) code[e] = code_at(word, e);
-            } else {
-                const uint32_t* v = reinterpret_cast<const uint32_t*>(rec + R::v);
-                const int e = value_nibble(row);
+            for (int e = 0; e < 8; ++e) x[e] = pos0 + row < len ? fmaf(static_cast<float>(code_at(word, e)), pair_scale(sm), pair_min(sm)) : 0.f;
+            if (pos0 + row >= start && pos0 + row < end) store_row<Dt>(a.out[0], dst + row * D + 8 * w, x);
+        }
+    }
+    if (a.out[1]) {
+        const int quad = lane >> 4, c0 = lane & 15;
 #pragma unroll
-                for (int c = 0; c < 8; ++c) code[c] = turn(v[value_word(row, 8 * w + c)], (4 * e + 3) & 31) & 15u;
+        for (int u = 0; u < D / 64; ++u) {
+            const u32x4 word = reinterpret_cast<const u32x4*>(rec + R::v)[u * kWave + lane];
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                u32x4 sm[2];  // of the four channels, or of the lower and the upper two
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int g = GROUP == 32 ? 2 * u + k : 64 * u / GROUP;
+                    sm[k] = reinterpret_cast<const u32x4*>(rec + R::vsm)[g * (kBlock / 4) + 4 * v + quad];
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * v + 4 * quad + r;
+                    float x[4];
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        x[t] = pos0 + row < len ? fmaf(static_cast<float>(code_at(word[t], r + 4 * v)), pair_scale(sm[t >> 1][r]), pair_min(sm[t >> 1][r])) : 0.f;
+                    if (pos0 + row < start || pos0 + row >= end) continue;
+                    if constexpr (GROUP == 32) {
+                        const float a0[2] = {x[0], x[1]}, a1[2] = {x[2], x[3]};
+                        store_row<Dt>(a.out[1], dst + row * D + 64 * u + 2 * c0, a0);
+                        store_row<Dt>(a.out[1], dst + row * D + 64 * u + 32 + 2 * c0, a1);
+                    } else {
+                        store_row<Dt>(a.out[1], dst + row * D + 64 * u + 4 * c0, x);
+                    }
+                }
             }
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) store_from_f32(a.out[kv], dst + e, a.dtype, fmaf(static_cast<float>(code[e]), s, m));
     }
 }
 
 template <int D, int GROUP, int Dt>
-int append_typed(const RowsArgs& a, hipStream_t stream) {
+void append_typed(const RowsArgs& a, int batch, hipStream_t stream) {
     const lf_int4_layer& L = a.L;
     if (a.tokens <= kFewTokens) {
-        const int waves = min(L.n_kv, D > 128 ? 4 : 8);
-        hipLaunchKernelGGL((int4_append_few_kernel<D, GROUP, Dt>), dim3(L.batch), dim3(waves * kWave), 0, stream, a);
-    } else {
-        const int P = L.page_size, waves = min(4, P / kBlock);
-        const int64_t pages = (static_cast<int64_t>(a.tokens) + 2 * P - 2) / P;  // that a run of tokens can touch
-        const int64_t here = min(pages, static_cast<int64_t>(L.cap_tokens / P) + 1);
-        hipLaunchKernelGGL((int4_append_pages_kernel<D, GROUP, Dt>), dim3(static_cast<uint32_t>(here), L.n_kv, L.batch),
-                           dim3(waves * kWave), 0, stream, a);
-        hipLaunchKernelGGL(int4_advance_kernel, dim3((L.batch + 255) / 256), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((int4_append_few_kernel<D, GROUP, Dt>), dim3(batch), dim3((D > 128 ? 4 : 8) * kWave), 0, stream, a);
+        return;
     }
+    const int P = L.page_size, waves = min(4, P / kBlock);
+    const int64_t pages = (static_cast<int64_t>(a.tokens) + 2 * P - 2) / P;  // that a run of tokens can touch
+    const int64_t here = min(pages, static_cast<int64_t>(L.cap_tokens / P) + 1);
+    hipLaunchKernelGGL((int4_append_pages_kernel<D, GROUP, Dt>), dim3(static_cast<uint32_t>(here), L.n_kv, batch),
+                       dim3(waves * kWave), 0, stream, a);
+    hipLaunchKernelGGL(int4_advance_kernel, dim3(1), dim3(kInlineSeqs), 0, stream, a);
+}
+
+int last_error() {
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }
 
 }  // namespace
 
+int launch_int4_set_lens(const lf_int4_layer& L, const int32_t* lens, hipStream_t stream) {
+    for (int b0 = 0; b0 < L.batch; b0 += kInlineSeqs) {
+        LensArgs a{L.lens, b0, min(kInlineSeqs, L.batch - b0), {}};
+        for (int i = 0; i < a.n; ++i) a.value[i] = lens[b0 + i];
+        hipLaunchKernelGGL(int4_set_lens_kernel, dim3(1), dim3(kInlineSeqs), 0, stream, a);
+    }
+    return last_error();
+}
+
 int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_src, int dtype, const int64_t* k_strides,
                        const int64_t* v_strides, const int32_t* counts, int tokens, hipStream_t stream) {
     RowsArgs a{};
     a.L = L;
     a.src[0] = k_src; a.src[1] = v_src;
-    a.counts = counts;
     a.tokens = tokens;
     const int esize = dtype == LF_FP32 ? 4 : 2;
     bool vec = true;
@@ -326,23 +421,38 @@ int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_
         for (int i = 0; i < 3; ++i) vec = vec && s[i] * esize % 16 == 0;
     }
     a.vec = vec;
+    a.counted = counts != nullptr;
     return int4_dispatch(L, [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
-        return dtype == LF_BF16 ? append_typed<D, GROUP, LF_BF16>(a, stream)
-               : dtype == LF_FP16 ? append_typed<D, GROUP, LF_FP16>(a, stream) : append_typed<D, GROUP, LF_FP32>(a, stream);
+        for (a.b0 = 0; a.b0 < L.batch; a.b0 += kInlineSeqs) {
+            const int n = min(kInlineSeqs, L.batch - a.b0);
+            for (int i = 0; i < n && counts; ++i) a.counts[i] = counts[a.b0 + i];
+            if (dtype == LF_BF16) append_typed<D, GROUP, LF_BF16>(a, n, stream);
+            else if (dtype == LF_FP16) append_typed<D, GROUP, LF_FP16>(a, n, stream);
+            else append_typed<D, GROUP, LF_FP32>(a, n, stream);
+        }
+        return last_error();
     });
 }
 
 int launch_int4_read(const lf_int4_layer& L, const int32_t* starts, int tokens, void* k_out, void* v_out, int dtype,
                      hipStream_t stream) {
-    ReadArgs a{L, starts, tokens, {k_out, v_out}, dtype};
+    ReadArgs a{};
+    a.L = L;
+    a.tokens = tokens;
+    a.out[0] = k_out; a.out[1] = v_out;
     return int4_dispatch(L, [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
-        const int64_t threads = static_cast<int64_t>(tokens) * (D / 8);
-        hipLaunchKernelGGL((int4_read_kernel<D, GROUP>), dim3(static_cast<uint32_t>((threads + 255) / 256), L.n_kv, L.batch),
-                           dim3(256), 0, stream, a);
-        const hipError_t err = hipGetLastError();
-        return err == hipSuccess ? LF_OK : static_cast<int>(err);
+        const int64_t records = (static_cast<int64_t>(tokens) + 2 * kBlock - 2) / kBlock;  // that a run of tokens can touch
+        for (a.b0 = 0; a.b0 < L.batch; a.b0 += kInlineSeqs) {
+            const int n = min(kInlineSeqs, L.batch - a.b0);
+            for (int i = 0; i < n; ++i) a.starts[i] = starts ? starts[a.b0 + i] : 0;
+            const dim3 grid(static_cast<uint32_t>((records + 3) / 4), L.n_kv, n);
+            if (dtype == LF_BF16) hipLaunchKernelGGL((int4_read_kernel<D, GROUP, LF_BF16>), grid, dim3(256), 0, stream, a);
+            else if (dtype == LF_FP16) hipLaunchKernelGGL((int4_read_kernel<D, GROUP, LF_FP16>), grid, dim3(256), 0, stream, a);
+            else hipLaunchKernelGGL((int4_read_kernel<D, GROUP, LF_FP32>), grid, dim3(256), 0, stream, a);
+        }
+        return last_error();
     });
 }
 

@@ -67,8 +67,17 @@ def _check_rows(t: torch.Tensor, device: torch.device, name: str) -> torch.Tenso
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=256)
+def _stride_array(strides: tuple):
+    return (ctypes.c_int64 * 3)(*strides[:3])
+
+
 def _strides(t: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+    return _stride_array(t.stride())
+
+
+def _ints(values):
+    return (ctypes.c_int32 * len(values))(*values)
 
 
 class _Int4Store:
@@ -133,21 +142,19 @@ class _Int4Store:
         """The ``lf_int4_layer`` describing this store, its device lengths up to date on the current stream."""
         if self._cap == 0:
             self.reserve(self.page_size)
-        if self._dirty:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("the cache was truncated or reset since its last launch: "
-                                   "call manager.sync_lengths() before the capture")
-            if min(self.lengths) == max(self.lengths):
-                self._lens.fill_(self.lengths[0])
-            else:
-                self._lens.copy_(_native.upload(self.lengths, torch.int32, self.device))
-            self._dirty = False
         if self._struct is None:
             s = _native.Int4Layer()
             s.blocks, s.bounds, s.lens = self._blocks.data_ptr(), self._bounds.data_ptr(), self._lens.data_ptr()
             s.batch, s.n_kv, s.head_dim = self.batch, self.n_kv, self.head_dim
             s.cap_tokens, s.page_size, s.group = self._cap, self.page_size, self.group_size
             self._struct = s
+        if self._dirty:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the cache was truncated or reset since its last launch: "
+                                   "call manager.sync_lengths() before the capture")
+            _native.check(_native.load().lf_int4_set_lens(self._struct, _ints(self.lengths),
+                                                          _native.current_stream_ptr(self.device)), "lf_int4_set_lens")
+            self._dirty = False
         return self._struct
 
     def set_lengths(self, lengths) -> None:
@@ -184,25 +191,21 @@ class _Int4Store:
                 lengths = None
         return key, value, lengths
 
-    def append_batch(self, key: torch.Tensor, value: torch.Tensor, lengths=None,
-                     counts: Optional[torch.Tensor] = None) -> None:
-        """Append ``key/value [batch, n_kv, T, head_dim]`` (sequence b its first ``lengths[b]`` tokens; ``counts``:
-        the same on the device, if the caller has them there)."""
-        key, value, lengths = self.check_append(key, value, lengths)
+    def append_batch(self, key: torch.Tensor, value: torch.Tensor, lengths=None) -> None:
+        """Append ``key/value [batch, n_kv, T, head_dim]`` (sequence b its first ``lengths[b]`` tokens)."""
+        self._append(*self.check_append(key, value, lengths))
+
+    def _append(self, key: torch.Tensor, value: torch.Tensor, lengths) -> None:
         T = int(key.shape[2])
         if T == 0 or (lengths is not None and max(lengths) == 0):
             return
-        new = [n + (T if lengths is None else lengths[b]) for b, n in enumerate(self.lengths)]
+        new = [n + T for n in self.lengths] if lengths is None else [n + t for n, t in zip(self.lengths, lengths)]
         with _on(self.device):
-            self.reserve(max(new))
-            struct = self.layer_struct()
-            if lengths is not None and counts is None:
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("a commit of ragged lengths uploads them and cannot be captured")
-                counts = _native.upload(lengths, torch.int32, self.device)
+            if max(new) > self._cap:
+                self.reserve(max(new))
             st = _native.load().lf_int4_append(
-                struct, key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key), _strides(value),
-                0 if lengths is None else counts.data_ptr(), T, _native.current_stream_ptr(self.device))
+                self.layer_struct(), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
+                _strides(value), None if lengths is None else _ints(lengths), T, _native.current_stream_ptr(self.device))
         _native.check(st, "lf_int4_append")
         self.lengths = new
 
@@ -219,9 +222,8 @@ class _Int4Store:
         if tokens:
             with _on(self.device):
                 struct = self.layer_struct()
-                at = None if max(starts) == 0 else _native.upload(starts, torch.int32, self.device)
-                st = _native.load().lf_int4_read(struct, 0 if at is None else at.data_ptr(), tokens, k.data_ptr(),
-                                                 v.data_ptr(), code, _native.current_stream_ptr(self.device))
+                st = _native.load().lf_int4_read(struct, _ints(starts), tokens, k.data_ptr(), v.data_ptr(), code,
+                                                 _native.current_stream_ptr(self.device))
             _native.check(st, "lf_int4_read")
         return k, v
 
@@ -257,18 +259,15 @@ class Int4KVManager:
         self.seq_len = 0
         self.layers = [_Int4Store(self.n_kv, self.head_dim, self.page_size, self.group_size, device=self.device,
                                   batch=self.batch_size, capacity_tokens=capacity_tokens) for _ in range(int(n_layers))]
-        self._workspaces: dict = {}
+        self._args: dict = {}
 
     def commit(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor, lengths=None) -> None:
         """Append ``key/value [batch, n_kv, T, head_dim]`` to layer ``layer_idx``, quantised as they are written.
         ``lengths``: per-sequence token counts for ragged batches."""
-        self._append(layer_idx, key, value, lengths)
-
-    def _append(self, layer_idx: int, key, value, lengths, counts=None) -> None:
         if key.shape[0] != self.batch_size:
             raise NotImplementedError(
                 f"this manager holds {self.batch_size} sequence(s); got a batch of {key.shape[0]}")
-        self.layers[layer_idx].append_batch(key, value, lengths, counts)
+        self.layers[layer_idx].append_batch(key, value, lengths)
         self._note(layer_idx)
 
     def _note(self, layer_idx: int) -> None:
@@ -316,19 +315,6 @@ class Int4KVManager:
             layer.set_lengths([0] * self.batch_size)
         self.seq_len = 0
 
-    def workspace(self, nbytes: int) -> torch.Tensor:
-        """Scratch for one launch (needs no clearing).  One per stream, grown on demand: calls on a stream follow one
-        another.  A capture takes memory of its own, which the graph keeps: two graphs share none."""
-        if torch.cuda.is_current_stream_capturing():
-            return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=self.device)
-        stream = _native.current_stream_ptr(self.device)
-        ws = self._workspaces.get(stream)
-        if ws is None or ws.numel() < nbytes:
-            with torch.inference_mode(False):
-                ws = torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=self.device)
-            self._workspaces[stream] = ws
-        return ws
-
 
 def _check_query(manager, query: torch.Tensor) -> torch.Tensor:
     if query.dim() != 4 or query.shape[0] != manager.batch_size or query.shape[1] != manager.n_q \
@@ -354,13 +340,29 @@ def _query_lengths(manager, q_len: int, lengths):
     return _native.upload(lengths, torch.int32, manager.device)
 
 
+def _workspace(manager, nbytes: int) -> torch.Tensor:
+    """Scratch of one call, of the current stream's memory (in a capture the graph's own): calls on other streams or
+    from other threads, and other graphs, have another."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=manager.device)
+
+
 def _args(manager, query: torch.Tensor, counts, scaling: float) -> _native.Int4Args:
-    a = _native.Int4Args()
-    a.query, a.dtype = query.data_ptr(), _native.dtype_code(query.dtype)
-    a.n_q, a.q_len = manager.n_q, int(query.shape[2])
-    a.q_strides = _strides(query)
-    a.q_lens = 0 if counts is None else counts.data_ptr()
-    a.scaling = float(scaling)
+    """The call's argument block: a copy of the one kept for the query's form, with this call's tensors."""
+    key = (query.shape[2], query.dtype, query.stride(), scaling)
+    kept = manager._args.get(key)
+    if kept is None:
+        if len(manager._args) >= 64:
+            manager._args.clear()
+        kept = a = _native.Int4Args()
+        a.dtype = _native.dtype_code(query.dtype)
+        a.n_q, a.q_len = manager.n_q, int(query.shape[2])
+        a.q_strides = _strides(query)
+        a.scaling = float(scaling)
+        manager._args[key] = kept
+    a = _native.Int4Args.from_buffer_copy(kept)
+    a.query = query.data_ptr()
+    if counts is not None:
+        a.q_lens = counts.data_ptr()
     return a
 
 
@@ -406,7 +408,7 @@ def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3) -> tuple[int, int]
     """``(splits, tokens of each)`` for sequences of ``tokens`` rows (an int, or one per sequence), ``rows``
     workgroups per sequence and split."""
     tokens = (tokens,) if isinstance(tokens, int) else tokens
-    size = _plan(tuple([-(-n // SPLIT_UNIT) or 1 for n in tokens]), rows, per_cu * cus) * SPLIT_UNIT
+    size = _plan(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), rows, per_cu * cus) * SPLIT_UNIT
     return -(-max(max(tokens), 1) // size), size
 
 
@@ -434,7 +436,7 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     if (key_new is None) != (value_new is None):
         raise ValueError("key_new and value_new come together")
     if key_new is not None:
-        key_new, value_new, _ = layer.check_append(key_new, value_new, lengths)
+        key_new, value_new, new_lengths = layer.check_append(key_new, value_new, lengths)
         if key_new.shape[2] != q_len:
             raise ValueError(f"{key_new.shape[2]} new tokens and {q_len} query tokens")
     if pages is not None:
@@ -448,7 +450,8 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     with _on(manager.device):
         counts = _query_lengths(manager, q_len, lengths)
         if key_new is not None:
-            manager._append(layer_idx, key_new, value_new, lengths, counts)
+            layer._append(key_new, value_new, new_lengths)
+            manager._note(layer_idx)
         if pages is None and manager.top_pages:
             pages = _select(manager, layer, query, manager.top_pages, counts)
         out = torch.empty(B, manager.n_q, q_len, D, dtype=query.dtype, device=manager.device)
@@ -465,8 +468,8 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
         lib = _native.load()
         struct = layer.layer_struct()
         if a.splits > 1:
-            a.workspace_bytes = lib.lf_int4_workspace_bytes(struct, a.n_q, a.q_len, a.splits)
-            ws = manager.workspace(a.workspace_bytes)
+            a.workspace_bytes = 4 * B * a.n_q * a.q_len * a.splits * (D + 2)  # lf_int4_workspace_bytes
+            ws = _workspace(manager, a.workspace_bytes)
             a.workspace = ws.data_ptr()
         st = lib.lf_int4_attention(struct, a, _native.current_stream_ptr(manager.device))
     _native.check(st, "lf_int4_attention")
@@ -481,7 +484,7 @@ def _select(manager, layer, query: torch.Tensor, top_pages: int, counts) -> torc
     a = _args(manager, query, counts, 1.0)
     a.pages, a.n_pages = pages.data_ptr(), top_pages
     a.workspace_bytes = lib.lf_int4_select_workspace_bytes(struct, q_len)
-    ws = manager.workspace(a.workspace_bytes)
+    ws = _workspace(manager, a.workspace_bytes)
     a.workspace = ws.data_ptr()
     st = lib.lf_int4_select(struct, a, _native.current_stream_ptr(manager.device))
     _native.check(st, "lf_int4_select")
