@@ -443,6 +443,10 @@ typedef struct lf_int4_args {
     int32_t splits;                           /* workgroups that share a sequence's tokens, 1 .. 1024 */
     int32_t split_tokens;                     /* tokens of each (a multiple of 32); the last split takes
                                                  what is behind them too; with pages: unused  */
+    int32_t prefix_splits;                    /* > 0: the rows that every query of a 128-row tile sees go to the
+                                                 many-row kernel, in that many workgroups per tile (1 .. 1024, of
+                                                 2-byte queries, head_dim 64 or 128, no pages; else
+                                                 LF_E_UNSUPPORTED), and splits is 1 for what is behind them  */
     void* workspace; int64_t workspace_bytes; /* 16-byte aligned, no initialisation           */
 } lf_int4_args;
 
@@ -456,7 +460,8 @@ typedef struct lf_int4_args {
  * is negative, not before the own page or not greater than the entry in front of it is not attended.
  *
  * Scores and sums in fp32.  Split over the tokens into ``splits`` workgroups per (sequence, kv head, row
- * tile), merged by a second launch when there are more than one.  Workspace: lf_int4_workspace_bytes().
+ * tile), merged by a second launch when there are more than one.  The many-row kernel (prefix_splits) holds
+ * Keys, Values and weights in fp16.  Workspace: lf_int4_workspace_bytes() of splits + prefix_splits.
  */
 int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, void* stream);
 int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t q_len, int32_t splits);

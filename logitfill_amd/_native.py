@@ -117,7 +117,7 @@ class Int4Args(ctypes.Structure):
         ("scaling", c_float),
         ("n_pages", c_int32),
         ("pages", c_void_p),
-        ("splits", c_int32), ("split_tokens", c_int32),
+        ("splits", c_int32), ("split_tokens", c_int32), ("prefix_splits", c_int32),
         ("workspace", c_void_p), ("workspace_bytes", c_int64),
     ]
 

@@ -91,7 +91,7 @@ int32_t lf_int4_read(const lf_int4_layer* layer, const int32_t* starts, int32_t 
 }
 
 int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t q_len, int32_t splits) {
-    if (!layer || layer->batch <= 0 || layer->head_dim <= 0 || n_q <= 0 || q_len <= 0 || splits <= 0 || splits > kMaxSplits)
+    if (!layer || layer->batch <= 0 || layer->head_dim <= 0 || n_q <= 0 || q_len <= 0 || splits <= 0 || splits > kMaxSplits + 1)
         return LF_E_SHAPE;
     return lf::int4_part_bytes(*layer, n_q, q_len, splits);
 }
@@ -103,10 +103,16 @@ int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, 
     if (!A.out) return LF_E_NULL;
     if (A.splits <= 0 || A.splits > kMaxSplits) return LF_E_SHAPE;
     if (A.n_pages == 0 && A.splits > 1 && (A.split_tokens <= 0 || A.split_tokens % 32 != 0)) return LF_E_SHAPE;
-    if (A.splits > 1) {
+    if (A.prefix_splits < 0 || A.prefix_splits > kMaxSplits) return LF_E_SHAPE;
+    if (A.prefix_splits > 0) {
+        if (A.splits != 1) return LF_E_SHAPE;
+        if (A.n_pages > 0 || A.dtype == LF_FP32 || layer->head_dim > 128) return LF_E_UNSUPPORTED;
+    }
+    const int parts = A.splits + A.prefix_splits;
+    if (parts > 1) {
         if (!A.workspace) return LF_E_NULL;
         if (!aligned16(A.workspace)) return LF_E_SHAPE;
-        if (A.workspace_bytes < lf::int4_part_bytes(*layer, A.n_q, A.q_len, A.splits)) return LF_E_WORKSPACE;
+        if (A.workspace_bytes < lf::int4_part_bytes(*layer, A.n_q, A.q_len, parts)) return LF_E_WORKSPACE;
     }
     return lf::launch_int4_attention(*layer, A, static_cast<hipStream_t>(stream));
 }

@@ -20,25 +20,11 @@
 #include "int4_common.hpp"
 
 namespace lf {
+int launch_int4_prefix(const Int4Attention& a, int dtype, hipStream_t stream);
+
 namespace {
 
 constexpr int kWaves = 4, kTile = 16;
-
-struct AttentionArgs {
-    lf_int4_layer L;
-    const void* q;
-    int64_t qb, qh, qt;
-    int vec;  // query rows start on 16 bytes
-    const int32_t* q_lens;
-    void* out;
-    int n_q, g, q_len;
-    float qscale;  // scaling * log2(e)
-    const int32_t* pages;
-    int n_pages;
-    int splits, split_tokens;  // with pages: split_tokens is in records of the page list
-    float* part_o;             // [batch * n_q * q_len][splits][D]
-    float* part_ml;            // [batch * n_q * q_len][splits][2]
-};
 
 template <int NT>
 struct Parts {
@@ -77,43 +63,6 @@ __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
 // SIMD leave.
 __device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
 
-template <int Dt>
-__device__ __forceinline__ void query8(const AttentionArgs& a, int64_t at, float (&x)[8]) {
-    if (a.vec) {
-        if constexpr (Dt == LF_FP32) {
-            const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at);
-            const f32x4 u = p[0], v = p[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { x[e] = u[e]; x[4 + e] = v[e]; }
-        } else {
-            const u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint16_t h = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
-                x[e] = Dt == LF_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = load_as_f32(a.q, at + e, Dt);
-    }
-}
-
-// fn(channel, values) for every four consecutive channels that a lane of the transposed output holds.
-template <int D, int GROUP, class Fn>
-__device__ __forceinline__ void each_run(const f32x4 (&o)[D / 16], int quad, Fn&& fn) {
-    constexpr int N = GROUP == 32 ? 2 : 4;  // tiles whose rows' channels are neighbours
-#pragma unroll
-    for (int t = 0; t < D / 16; t += N)
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = o[t + e % N][(4 * k + e) / N];
-            fn(value_channel<GROUP>(4 * quad + 4 * k / N, t), x);
-        }
-}
-
 // A wave's ring of records in LDS, filled by DMA: ``kRing`` - 1 of them are on their way while one is worked on.
 constexpr int kRing = 2;
 template <int D, int GROUP>
@@ -142,7 +91,7 @@ __device__ __forceinline__ void wait_ring() {
 }
 
 template <int D, int GROUP, int Dt>
-__global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(Int4Attention a) {
     using R = Int4Rec<D, GROUP>;
     using S = Ring<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
@@ -154,7 +103,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     // of sequences of unlike lengths (splits first: 32 ragged contexts of 4K-64K tokens in 4 splits 545 us, against 429: 2 of 8 XCDs
     // had the last, mostly empty split) and the row tiles of a head, which read the same records, few of them; the
     // splits last, so that a long sequence's later ones follow everyone's first.
-    const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
+    const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = a.prefix + blockIdx.z;
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
     // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
@@ -202,8 +151,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         __syncthreads();
     } else {
         const int blocks = (top + kBlock - 1) / kBlock, per = a.split_tokens / kBlock;
-        first = static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
-        last = part + 1 == a.splits ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
+        first = a.prefix ? min(prefix_records(a, len, n, tile / (kManyRows / kTile)), blocks)
+                         : static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
+        last = part + 1 == a.parts ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
     }
     const int count = last > first + wave ? (last - first - wave + kWaves - 1) / kWaves : 0;  // this wave's records
     // The k-th of them, or -1 for one that is not attended (its place in the ring is filled with another).
@@ -358,7 +308,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
 
     // the waves' sums at one reference point
     l = rows_sum(l);
-    const float m_wave = limit == -__builtin_inff() ? limit : ref;
+    const float m_wave = l == 0.f ? -__builtin_inff() : ref;  // (a sum of NaN has a place among the others)
     if (quad == 0) { lds_ml[wave][col][0] = m_wave; lds_ml[wave][col][1] = l; }
 #pragma unroll
     for (int g = 0; g < G; ++g) pm[g] = rows_sum(pm[g]);
@@ -385,17 +335,17 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     }
     if (!real) return;
     const int64_t row = (static_cast<int64_t>(b) * a.n_q + h * a.g + i) * a.q_len + j;
-    if (a.splits == 1) {
+    if (a.parts == 1) {
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;  // (no row seen: zeros)
 #pragma unroll
         for (int t = 0; t < VT; ++t) o[t] *= inv;
         each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<Dt>(a.out, row * D + c, x); });
         return;
     }
-    float* dst = a.part_o + (row * a.splits + part) * D;
+    float* dst = a.part_o + (row * a.parts + part) * D;
     each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<LF_FP32>(dst, c, x); });
     if (quad == 0) {
-        float* ml = a.part_ml + (row * a.splits + part) * 2;
+        float* ml = a.part_ml + (row * a.parts + part) * 2;
         ml[0] = m_all;
         ml[1] = l_all;
     }
@@ -404,36 +354,35 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
 // The splits' sums at their largest reference point: a workgroup per output row, whose waves take the splits in
 // turn (sixteen of every 64, all loads on their way at once) and add up through LDS.
 template <int D>
-__global__ __launch_bounds__(256) void int4_merge_kernel(AttentionArgs a, int dtype) {
+__global__ __launch_bounds__(256) void int4_merge_kernel(Int4Attention a, int dtype) {
     constexpr int C = D / kWave, kTake = 16;
     __shared__ float lds[4][D];
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave)), waves = blockDim.x / kWave;
-    const float* ml = a.part_ml + row * a.splits * 2;
-    const float* parts = a.part_o + row * a.splits * D + lane * C;
+    const float* ml = a.part_ml + row * a.parts * 2;
+    const float* parts = a.part_o + row * a.parts * D + lane * C;
     float m = -__builtin_inff();
-    for (int s = lane; s < a.splits; s += kWave) m = fmaxf(m, ml[2 * s]);
+    for (int s = lane; s < a.parts; s += kWave) m = fmaxf(m, ml[2 * s]);
     m = wave_max(m);
     float o[C] = {}, l = 0.f;
-    for (int s0 = 0; s0 < a.splits; s0 += kWave) {
+    for (int s0 = 0; s0 < a.parts; s0 += kWave) {
         float w = 0.f;
-        if (s0 + lane < a.splits) {
+        if (s0 + lane < a.parts) {
             const float ms = ml[2 * (s0 + lane)];
             w = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-            l = w == 0.f ? l : fmaf(w, ml[2 * (s0 + lane) + 1], l);
+            l = fmaf(w, ml[2 * (s0 + lane) + 1], l);
         }
-        for (int k0 = wave * kTake; k0 < kWave && s0 + k0 < a.splits; k0 += waves * kTake) {
+        for (int k0 = wave * kTake; k0 < kWave && s0 + k0 < a.parts; k0 += waves * kTake) {
             float x[kTake][C];
 #pragma unroll
             for (int k = 0; k < kTake; ++k)
 #pragma unroll
-                for (int c = 0; c < C; ++c) x[k][c] = s0 + k0 + k < a.splits ? parts[(s0 + k0 + k) * D + c] : 0.f;
+                for (int c = 0; c < C; ++c) x[k][c] = s0 + k0 + k < a.parts ? parts[(s0 + k0 + k) * D + c] : 0.f;
 #pragma unroll
             for (int k = 0; k < kTake; ++k) {
-                // (a split that saw no row weighs nothing, whatever stands in its place)
                 const float wk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), k0 + k));
 #pragma unroll
-                for (int c = 0; c < C; ++c) o[c] = wk == 0.f ? o[c] : fmaf(wk, x[k][c], o[c]);
+                for (int c = 0; c < C; ++c) o[c] = fmaf(wk, x[k][c], o[c]);
             }
         }
     }
@@ -452,16 +401,17 @@ __global__ __launch_bounds__(256) void int4_merge_kernel(AttentionArgs a, int dt
 }
 
 template <int D, int GROUP, int Dt>
-int launch_typed(const AttentionArgs& a, int tiles, hipStream_t stream) {
+int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
     const auto fn = int4_attention_kernel<D, GROUP, Dt>;
     int lds = Ring<D, GROUP>::lds;
     if (a.n_pages) lds += 4 * (a.split_tokens / (a.L.page_size / kBlock) + 2);  // the split's entries of the page list
-    const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
+    int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
+    if (st == LF_OK && a.prefix) st = launch_int4_prefix(a, Dt, stream);
     if (st != LF_OK) return st;
     hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, a);
-    if (a.splits > 1) {
+    if (a.parts > 1) {
         const uint32_t rows = static_cast<uint32_t>(a.L.batch) * a.n_q * a.q_len;
-        hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.splits > 16 ? 256 : 64), 0, stream, a, Dt);
+        hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.parts > 16 ? 256 : 64), 0, stream, a, Dt);
     }
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? LF_OK : static_cast<int>(err);
@@ -474,7 +424,7 @@ int64_t int4_part_bytes(const lf_int4_layer& L, int n_q, int q_len, int splits) 
 }
 
 int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream) {
-    AttentionArgs a{};
+    Int4Attention a{};
     a.L = L;
     a.q = A.query;
     a.qb = A.q_strides[0]; a.qh = A.q_strides[1]; a.qt = A.q_strides[2];
@@ -487,10 +437,12 @@ int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStre
     a.qscale = A.scaling * kLog2e;
     a.pages = A.pages; a.n_pages = A.n_pages;
     a.splits = A.splits;
+    a.prefix = A.prefix_splits;
+    a.parts = a.splits + a.prefix;
     a.split_tokens = A.split_tokens;
     const int64_t rows = static_cast<int64_t>(L.batch) * A.n_q * A.q_len;
     a.part_o = static_cast<float*>(A.workspace);
-    a.part_ml = a.part_o + rows * A.splits * L.head_dim;
+    a.part_ml = a.part_o + rows * a.parts * L.head_dim;
     int tiles = (a.g * A.q_len + kTile - 1) / kTile;
     if (A.n_pages) {
         tiles = (a.g + kTile - 1) / kTile * A.q_len;

@@ -92,6 +92,73 @@ __device__ __forceinline__ int int4_len(const lf_int4_layer& L, int b) {
 __device__ __forceinline__ float pair_scale(uint32_t sm) { return f16_to_f32(static_cast<uint16_t>(sm)); }
 __device__ __forceinline__ float pair_min(uint32_t sm) { return f16_to_f32(static_cast<uint16_t>(sm >> 16)); }
 
+// An attention call, as its kernels take it.
+struct Int4Attention {
+    lf_int4_layer L;
+    const void* q;
+    int64_t qb, qh, qt;
+    int vec;  // query rows start on 16 bytes
+    const int32_t* q_lens;
+    void* out;
+    int n_q, g, q_len;
+    float qscale;  // scaling * log2(e)
+    const int32_t* pages;
+    int n_pages;
+    int splits, split_tokens;  // with pages: split_tokens is in records of the page list
+    int prefix;                // splits of the many-row kernel in front of them
+    int parts;                 // prefix + splits
+    float* part_o;             // [batch * n_q * q_len][parts][D]
+    float* part_ml;            // [batch * n_q * q_len][parts][2]
+};
+
+constexpr int kManyRows = 128;  // query rows of a many-row workgroup
+
+// The records in front of everything that some query of many-row tile ``tile`` does not see: rows are (head of the
+// group, token), tokens fastest, and a tile of one head starts at its first token.
+__device__ __forceinline__ int prefix_records(const Int4Attention& a, int len, int n, int tile) {
+    const int r0 = tile * kManyRows, r1 = min(r0 + kManyRows, a.g * a.q_len) - 1;
+    const int j = r0 / a.q_len == r1 / a.q_len ? r0 % a.q_len : 0;
+    return j < n ? max(len - n + j + 1, 0) / kBlock : 0;
+}
+
+// Eight elements of a query row as float32.
+template <int Dt>
+__device__ __forceinline__ void query8(const Int4Attention& a, int64_t at, float (&x)[8]) {
+    if (a.vec) {
+        if constexpr (Dt == LF_FP32) {
+            const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(a.q) + at);
+            const f32x4 u = p[0], v = p[1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { x[e] = u[e]; x[4 + e] = v[e]; }
+        } else {
+            const u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const uint16_t h = static_cast<uint16_t>(u[e >> 1] >> (16 * (e & 1)));
+                x[e] = Dt == LF_BF16 ? bf16_to_f32(h) : f16_to_f32(h);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = load_as_f32(a.q, at + e, Dt);
+    }
+}
+
+// fn(channel, values) for every four consecutive channels that a lane of the transposed output holds.
+template <int D, int GROUP, class Fn>
+__device__ __forceinline__ void each_run(const f32x4 (&o)[D / 16], int quad, Fn&& fn) {
+    constexpr int N = GROUP == 32 ? 2 : 4;  // tiles whose rows' channels are neighbours
+#pragma unroll
+    for (int t = 0; t < D / 16; t += N)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[t + e % N][(4 * k + e) / N];
+            fn(value_channel<GROUP>(4 * quad + 4 * k / N, t), x);
+        }
+}
+
 // Calls fn(Int4Shape<D, GROUP>) for a layer's shape; LF_E_UNSUPPORTED for any other.
 template <int D, int GROUP>
 struct Int4Shape {

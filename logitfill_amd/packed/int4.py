@@ -412,6 +412,12 @@ def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3) -> tuple[int, int]
     return -(-max(max(tokens), 1) // size), size
 
 
+# From this many query rows per kv head up, and this many tokens in front of the queries, the many-row kernel takes
+# what every query sees.
+MANY_ROWS = 64
+MANY_ROWS_HISTORY = 256
+
+
 def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, key_new: Optional[torch.Tensor],
                    value_new: Optional[torch.Tensor], scaling: float, *, lengths=None,
                    pages: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -463,12 +469,19 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
             a.pages, a.n_pages = pages.data_ptr(), int(pages.shape[3])
             # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
             tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
-        a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, _cu_count(manager.device),
-                                               workgroups_per_cu(D, manager.group_size))
+        cus = _cu_count(manager.device)
+        if pages is None and group * q_len >= MANY_ROWS and D <= 128 and query.dtype != torch.float32 \
+                and max(tokens) >= q_len + MANY_ROWS_HISTORY:
+            a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus)
+            a.splits = 1
+        else:
+            a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,
+                                                   workgroups_per_cu(D, manager.group_size))
+        parts = a.splits + a.prefix_splits
         lib = _native.load()
         struct = layer.layer_struct()
-        if a.splits > 1:
-            a.workspace_bytes = 4 * B * a.n_q * a.q_len * a.splits * (D + 2)  # lf_int4_workspace_bytes
+        if parts > 1:
+            a.workspace_bytes = 4 * B * a.n_q * q_len * parts * (D + 2)  # lf_int4_workspace_bytes
             ws = _workspace(manager, a.workspace_bytes)
             a.workspace = ws.data_ptr()
         st = lib.lf_int4_attention(struct, a, _native.current_stream_ptr(manager.device))

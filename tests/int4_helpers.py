@@ -34,6 +34,17 @@ def _size(x, group: int) -> np.ndarray:
     return np.abs(o4.values(x, group)) + 32 * scale
 
 
+def many_rows_bound(q, k, v, scaling):
+    """What the many-row kernel's fp16 steps add: a Key off by 2^-11 of itself (2^-25 at least) and a query by 2^-24
+    of its row's largest element move a score by d; a weight off by 2^-11 and a Value off by 2^-11 (2^-25)."""
+    if k.shape[0] == 0:
+        return 0.0
+    a, qa = np.abs(k), np.abs(q).astype(np.float64)
+    d = abs(scaling) * ((qa @ (a * 2.0 ** -11 + 2.0 ** -25).T).max(-1, keepdims=True)
+                        + 2.0 ** -24 * qa.max(-1, keepdims=True) * a.sum(-1).max())
+    return (2 * d + 3 * 2.0 ** -11) * np.abs(v).max() + 2.0 ** -25
+
+
 def attention_bound(q, k_size, v_size, scaling, ref, dtype: str, smax: float):
     """Largest admitted |out - ref| per element of ``ref [rows, D]``.
 
@@ -86,6 +97,8 @@ def expected(q, key, value, lengths, group: int, scaling: float, dtype: str, *, 
                 r = o4.attend(qn[b, head, j], k, v, scaling, np.broadcast_to(seen, (g, total)))
                 out[b, head, j] = r
                 tol[b, head, j] = attention_bound(qn[b, head, j], k_size[seen], v_size[seen], scaling, r, dtype, smax)
+                if pages is None and g * n >= 64 and k.shape[-1] <= 128 and dtype != "fp32":
+                    tol[b, head, j] += many_rows_bound(qn[b, head, j], k[seen], v[seen], scaling)
     return out, tol
 
 

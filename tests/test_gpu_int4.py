@@ -195,6 +195,71 @@ def test_attention(gpu, D, group, page, n_q, n_kv, lengths, q_len, dtype):
     assert torch.equal(out, int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5))
 
 
+MANY = [
+    # rows of several 128-row tiles, tiles of one head and of several, ragged histories, a history of whole records
+    (128, 128, 128, 28, 4, [1500], 61, "bf16"),
+    (128, 64, 64, 8, 2, [900, 400, 290], 40, "fp16"),
+    (128, 32, 32, 12, 2, [1024, 77], 130, "bf16"),
+    (64, 64, 64, 4, 2, [2000], 300, "bf16"),
+    (64, 32, 32, 16, 1, [640, 0, 5], 9, "fp16"),
+    (128, 64, 128, 64, 1, [1333], 1, "bf16"),
+]
+
+
+@pytest.mark.parametrize("D,group,page,n_q,n_kv,lengths,q_len,dtype", MANY)
+def test_many_query_rows(gpu, D, group, page, n_q, n_kv, lengths, q_len, dtype):
+    """The many-row kernel in front of the general one; the whole output close in the mean, too: independent roundings
+    of weights, Keys and Values (fp16) and of the output."""
+    B = len(lengths)
+    key, value = rows((B, n_kv, max(lengths), D), dtype, sum(lengths) + 1)
+    q = query((B, n_q, q_len, D), dtype, D + q_len)
+    mgr = manager(gpu, D, group, page, n_q, n_kv, B)
+    mgr.commit(0, key.to(gpu), value.to(gpu), lengths)
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5)
+    ref, tol = expected(q, key, value, lengths, group, D ** -0.5, dtype)
+    assert_within(out, ref, tol)
+    rel = np.linalg.norm(f32(out) - ref) / np.linalg.norm(ref)
+    assert rel <= {"bf16": 2.0 ** -8, "fp16": 2.0 ** -10}[dtype], rel
+    assert torch.equal(out, int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5))
+    # queries of unlike counts: zeros behind them, and NaN rows of the cache no query of theirs sees
+    counts = [max(1, min(n, q_len - 7 * b)) if n else 0 for b, n in enumerate(lengths)]
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, -D ** -0.5, lengths=counts)
+    ref, tol = expected(q, key, value, lengths, group, -D ** -0.5, dtype, q_lens=counts)
+    assert_within(out, ref, tol)
+
+
+def test_many_query_rows_of_any_size(gpu):
+    """Rows of 2^-60 to 2^60 (float16's range is passed through the rows' factor), of zeros, and one of NaN."""
+    D, T, n = 128, 700, 70
+    key, value = rows((1, 1, T, D), "bf16", 8)
+    q = query((1, 1, n, D), "bf16", 8).float()
+    size = torch.exp2(torch.linspace(-60, 0, n))
+    q = (q * size[:, None]).to(torch.bfloat16)
+    q[0, 0, 11] = 0
+    mgr = manager(gpu, D, 64, 64, 1, 1)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    ref, tol = expected(q, key, value, [T], 64, D ** -0.5, "bf16")
+    assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol)
+    big = (q.float() * 2.0 ** 60).to(torch.bfloat16)
+    ref, tol = expected(big, key, value, [T], 64, 2.0 ** -60, "bf16")
+    assert_within(int4_attention(mgr, 0, big.to(gpu), None, None, 2.0 ** -60), ref, tol)
+    q[0, 0, 30] = float("nan")
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5)[0, 0]
+    assert out[30].isnan().all() and torch.isfinite(out[:30]).all() and torch.isfinite(out[31:]).all()
+
+
+@pytest.mark.parametrize("n", [1, 64])
+def test_a_nan_key_reaches_every_query_that_sees_it(gpu, n):
+    """In a split of its own, too, far below the others' scores."""
+    D, T = 64, 5000
+    key, value = rows((1, 1, T, D), "bf16", 9)
+    key[0, 0, 3] = float("nan")
+    q = query((1, 2, n, D), "bf16", 9).to(gpu)
+    mgr = manager(gpu, D, 32, 32, 2, 1)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    assert int4_attention(mgr, 0, q, None, None, 1.0).isnan().all()
+
+
 @pytest.mark.parametrize("scaling", [3.0, -0.4, 0.0])
 def test_attention_sharp_and_flat(gpu, scaling):
     """Scores of hundreds (one token takes all), of the other sign, and all equal."""

@@ -97,6 +97,10 @@ def test_append_and_read_refusals():
     ({"workspace": AT + 4}, SHAPE), ({"workspace_bytes": 100}, WORKSPACE), ({"n_pages": 4}, NULL),
     ({"n_pages": 1025, "pages": AT}, SHAPE), ({"n_pages": -1}, SHAPE),
     ({"n_pages": 4, "pages": AT, "q_len": 20000}, SHAPE),
+    ({"prefix_splits": -1}, SHAPE), ({"prefix_splits": 1025}, SHAPE), ({"prefix_splits": 4}, SHAPE),
+    ({"prefix_splits": 4, "splits": 1, "dtype": 2}, UNSUPPORTED),
+    ({"prefix_splits": 4, "splits": 1, "n_pages": 2, "pages": AT}, UNSUPPORTED),
+    ({"prefix_splits": 4, "splits": 1, "workspace_bytes": 5 * 2 * 28 * 130 * 4 - 1}, WORKSPACE),
 ])
 def test_attention_refusals(change, want):
     assert _native.load().lf_int4_attention(_layer(), _args(**change), None) == want
