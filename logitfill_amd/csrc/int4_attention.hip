@@ -194,6 +194,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
 #pragma unroll
     for (int g = 0; g < G; ++g) qsum[g] = rows_sum(qsum[g]);
 
+    const uint32_t code_base = in_vgpr(kCodeBase);
     constexpr uint32_t kMiddle = 0xC1BCC1BCu;  // bf16 -23.5: the bias of the codes and their middle
     const bf16x8 middle = __builtin_bit_cast(bf16x8, u32x4{kMiddle, kMiddle, kMiddle, kMiddle});
     f32x4 o[VT], fix[G];
@@ -223,13 +224,14 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
                 f32x4 acc = {start, start, start, start};
 #pragma unroll
                 for (int c = g * CG; c < (g + 1) * CG; ++c) {
-                    const bf16x8 codes = codes8(kw[c]);
+                    const bf16x8 codes = codes8(kw[c], code_base);
 #pragma unroll
                     for (int m = NT - 1; m >= 0; --m) acc = mfma(codes, q[c].t[m], acc);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float m = g == 0 ? pair_min(pair[r]) * qsum[g] : fmaf(pair_min(pair[r]), qsum[g], y[t][r]);
+                    // (a sum with zero where it is a product: it takes the fp16 factor as it is)
+                    const float m = fmaf(pair_min(pair[r]), qsum[g], g == 0 ? 0.f : y[t][r]);
                     y[t][r] = fmaf(pair_scale(pair[r]), acc[r], m);
                 }
             }
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    x[t][r] = p[t][r] * pair_scale(pair[t][r]);
+                    x[t][r] = fmaf(p[t][r], pair_scale(pair[t][r]), 0.f);
                     pm[g] = fmaf(p[t][r], pair_min(pair[t][r]), pm[g]);
                     pm[g] = fmaf(7.5f, x[t][r], pm[g]);
                 }
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
             for (int m = NT - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
 #pragma unroll
             for (int t = g * TG; t < (g + 1) * TG; ++t) {
-                const bf16x8 codes = codes8(vw[(t >> 2) * kWave][t & 3]);
+                const bf16x8 codes = codes8(vw[(t >> 2) * kWave][t & 3], code_base);
 #pragma unroll
                 for (int m = NT - 1; m >= 0; --m) o[t] = mfma(codes, w.t[m], o[t]);
             }

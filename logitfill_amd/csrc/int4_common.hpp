@@ -31,10 +31,19 @@ struct Int4Rec {
 __device__ __forceinline__ uint32_t turn(uint32_t w, int bits) { return __builtin_amdgcn_alignbit(w, w, bits); }
 __device__ __forceinline__ uint32_t code_at(uint32_t w, int e) { return turn(w, (4 * e + 3) & 31) & 15u; }
 
-// A word's eight codes as bf16 16 + code; element 2 i is nibble i, element 2 i + 1 nibble i + 4.
+// A constant in a vector register: the and-or of a code's pair takes one literal-free scalar and vector operands (with
+// both as literals it is an and, then an or).
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// A word's eight codes as bf16 16 + code; element 2 i is nibble i, element 2 i + 1 nibble i + 4.  ``base``: kCodeBase
+// in a vector register.
 constexpr float kCodeBias = 16.f;
-__device__ __forceinline__ bf16x8 codes8(uint32_t w) {
-    constexpr uint32_t mask = 0x00780078u, base = 0x41804180u;
+constexpr uint32_t kCodeBase = 0x41804180u;
+__device__ __forceinline__ bf16x8 codes8(uint32_t w, uint32_t base) {
+    constexpr uint32_t mask = 0x00780078u;
     return __builtin_bit_cast(bf16x8, u32x4{(w & mask) | base, (turn(w, 4) & mask) | base, (turn(w, 8) & mask) | base,
                                             (turn(w, 12) & mask) | base});
 }

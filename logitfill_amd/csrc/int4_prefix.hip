@@ -28,11 +28,11 @@ __device__ __forceinline__ uint32_t upper_pair(uint32_t a, uint32_t b) { return 
 
 // A word's eight codes times s[i] plus m[i], element pairs (nibble i, nibble i + 4): the fp16 bits 0x5800 | code << 3
 // are 128 + code.
-__device__ __forceinline__ u32x4 dequant8(uint32_t w, const uint32_t (&s)[4], const uint32_t (&m)[4]) {
+__device__ __forceinline__ u32x4 dequant8(uint32_t w, const uint32_t (&s)[4], const uint32_t (&m)[4], uint32_t base) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = ((i ? turn(w, 4 * i) : w) & 0x00780078u) | 0x58005800u;
+        const uint32_t bits = ((i ? turn(w, 4 * i) : w) & 0x00780078u) | base;
         const f16x2 code = __builtin_bit_cast(f16x2, bits) - f16x2{static_cast<_Float16>(128), static_cast<_Float16>(128)};
         r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, m[i])));
     }
@@ -55,56 +55,45 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
 
     // This wave's share of a record: 0, 1: sixteen Key rows; 2, 3: half of a lane's Value words.
     const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
-    constexpr int KG = G, VG = GROUP == 32 ? 2 : 1;  // groups a lane's Key words and Value words lie in
-    constexpr int VW = VT / 2;                       // Value words of a lane: words 2 (wave - 2) .. or super-column wave - 2
+    constexpr int VW = VT / 2;                          // a lane's Value words
+    constexpr int VG = GROUP == 32 ? VW / 2 : 1;        // and the groups they lie in
+    const uint32_t code_base = in_vgpr(0x58005800u);
+    // Every wave loads the same pieces, whichever it stages: with a branch around the loads, what it joins waited for them.
     struct Raw {
         uint32_t w[4];
-        u32x4 sm[2 * VG];  // Values: tokens 4 quad .. and 16 + 4 quad .. of each group; Keys: [0][g] its row's
+        uint32_t key[G];        // scale and minimum of a Key row's groups
+        u32x4 value[2 * VG];    // of tokens 4 quad .. and 16 + 4 quad .. of a Value word's groups
     };
+    const int half = wave & 1;
+    const uint32_t word_at = wave < 2 ? (16 * half + col) * (D / 2) + CH * 4 * quad
+                                      : R::v + 16 * lane + (VW == 4 ? 1024 * half : 8 * half);
+    const uint32_t key_at = R::ksm + 4 * (16 * half + col);
+    // (head_dim 64: words 2 half, 2 half + 1 are of group half with groups of 32)
+    const uint32_t value_at = R::vsm + 16 * quad + 4 * kBlock * (GROUP == 32 ? VG * half : 64 * half * (VW / 4) / GROUP);
     const auto load = [&](int record, Raw& r) {
         const uint8_t* rec = base + static_cast<int64_t>(record) * R::bytes;
-        if (wave < 2) {
-            const uint8_t* at = rec + (16 * wave + col) * (D / 2) + CH * 4 * quad;
-            if constexpr (CH == 4) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(at);
+        if constexpr (CH == 4) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(rec + word_at);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) r.w[c] = x[c];
-            } else {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(at);
-                r.w[0] = x[0];
-                r.w[1] = x[1];
-            }
-#pragma unroll
-            for (int g = 0; g < KG; ++g) r.sm[0][g] = reinterpret_cast<const uint32_t*>(rec + R::ksm)[g * kBlock + 16 * wave + col];
+            for (int c = 0; c < 4; ++c) r.w[c] = x[c];
         } else {
-            const int v = wave - 2;
-            const uint8_t* at = rec + R::v + 16 * lane;
-            if constexpr (VW == 4) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(at + 1024 * v);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) r.w[c] = x[c];
-            } else {
-                const u32x2 x = *reinterpret_cast<const u32x2*>(at + 8 * v);
-                r.w[0] = x[0];
-                r.w[1] = x[1];
-            }
-#pragma unroll
-            for (int k = 0; k < VG; ++k) {
-                // head_dim 64: words 2 v, 2 v + 1 are of group v with groups of 32
-                const int g = GROUP == 32 ? (VW == 4 ? 2 * v + k : v) : 64 * v * (VW / 4) / GROUP;
-                const u32x4* sm = reinterpret_cast<const u32x4*>(rec + R::vsm) + g * (kBlock / 4) + quad;
-                r.sm[2 * k] = sm[0];
-                r.sm[2 * k + 1] = sm[4];
-            }
+            const u32x2 x = *reinterpret_cast<const u32x2*>(rec + word_at);
+            r.w[0] = x[0];
+            r.w[1] = x[1];
         }
+#pragma unroll
+        for (int g = 0; g < G; ++g) r.key[g] = *reinterpret_cast<const uint32_t*>(rec + key_at + 4 * kBlock * g);
+#pragma unroll
+        for (int k = 0; k < 2 * VG; ++k)
+            r.value[k] = *reinterpret_cast<const u32x4*>(rec + value_at + 4 * kBlock * (k >> 1) + 64 * (k & 1));
     };
     const auto stage = [&](const Raw& r, u32x4* to) {
         if (wave < 2) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
-                const uint32_t pair = r.sm[0][c / (CH / G)], s = lower_pair(pair, pair), m = upper_pair(pair, pair);
+                const uint32_t pair = r.key[c / (CH / G)], s = lower_pair(pair, pair), m = upper_pair(pair, pair);
                 const uint32_t ss[4] = {s, s, s, s}, mm[4] = {m, m, m, m};
-                to[(wave * CH + c) * kWave + lane] = dequant8(r.w[c], ss, mm);
+                to[(half * CH + c) * kWave + lane] = dequant8(r.w[c], ss, mm, code_base);
             }
         } else {
 #pragma unroll
@@ -112,19 +101,19 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
                 uint32_t s[4], m[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[i] = lower_pair(r.sm[2 * k][i], r.sm[2 * k + 1][i]);
-                    m[i] = upper_pair(r.sm[2 * k][i], r.sm[2 * k + 1][i]);
+                    s[i] = lower_pair(r.value[2 * k][i], r.value[2 * k + 1][i]);
+                    m[i] = upper_pair(r.value[2 * k][i], r.value[2 * k + 1][i]);
                 }
 #pragma unroll
                 for (int c = k * (VW / VG); c < (k + 1) * (VW / VG); ++c)
-                    to[kK + ((wave - 2) * VW + c) * kWave + lane] = dequant8(r.w[c], s, m);
+                    to[kK + (half * VW + c) * kWave + lane] = dequant8(r.w[c], s, m, code_base);
             }
         }
     };
 
     // rows (head of the group, token), tokens fastest: this lane's, one of each row tile
     f16x8 q[MT][CH];
-    float scale[MT], ref[MT], limit[MT];
+    float scale[MT], ref[MT], limit[MT];  // limit: how far a score may pass ref; -inf until one is seen
     int row[MT];  // head of the group * q_len + token, or -1
     const bool flip = a.qscale < 0.f;
 #pragma unroll
@@ -190,24 +179,34 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
         f16x8 p[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            float most = fmaxf(fmaxf(fmaxf(y[t][0][0], y[t][0][1]), fmaxf(y[t][0][2], y[t][0][3])),
-                               fmaxf(fmaxf(y[t][1][0], y[t][1][1]), fmaxf(y[t][1][2], y[t][1][3])));
-            most *= scale[t];
+            // (scaled before they are compared: the comparisons take a product's sums as they are)
+            float z[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) z[u][i] = fmaf(y[t][u][i], scale[t], -ref[t]);
+            float most = fmaxf(fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[0][2], z[0][3])),
+                               fmaxf(fmaxf(z[1][0], z[1][1]), fmaxf(z[1][2], z[1][3])));
             if (__any(most > limit[t])) {
                 most = rows_max(most);
                 const bool moves = most > limit[t];
-                const float down = !moves ? 1.f : limit[t] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref[t] - most);
-                if (moves) { ref[t] = most; limit[t] = most + 8.f; }
+                const float by = moves ? most : 0.f;
+                const float down = limit[t] < 0.f && moves ? 0.f : __builtin_amdgcn_exp2f(-by);
+                ref[t] += by;
+                limit[t] = moves ? 8.f : limit[t];
                 l[t] *= down;
 #pragma unroll
                 for (int v = 0; v < VT; ++v) o[t][v] *= down;
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[u][i] -= by;
             }
             // element 2 i is token i of the lower sixteen, element 2 i + 1 of the upper
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                    p[t][2 * i + u] = static_cast<_Float16>(__builtin_amdgcn_exp2f(fmaf(y[t][u][i], scale[t], -ref[t])));
+                for (int u = 0; u < 2; ++u) p[t][2 * i + u] = static_cast<_Float16>(__builtin_amdgcn_exp2f(z[u][i]));
             l[t] = mfma(ones, p[t], l[t]);
         }
 #pragma unroll

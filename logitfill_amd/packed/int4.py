@@ -369,8 +369,9 @@ def _args(manager, query: torch.Tensor, counts, scaling: float) -> _native.Int4A
 # Tokens a split is a multiple of (a record for each of a workgroup's four waves).
 SPLIT_UNIT = 128
 # A workgroup's fixed cost (its queries, the first records' way, the waves' merge, its share of the splits') in
-# units of its work: about 3 us against 2 us a unit.
+# units of its work: about 3 us against 2 us a unit.  A many-row workgroup writes eight times the sums.
 SPLIT_OVERHEAD = 1.5
+MANY_ROWS_OVERHEAD = 4.0
 
 
 def workgroups_per_cu(head_dim: int, group: int) -> int:
@@ -380,35 +381,40 @@ def workgroups_per_cu(head_dim: int, group: int) -> int:
 
 
 @functools.lru_cache(maxsize=512)
-def _plan(units: tuple, rows: int, slots: int) -> int:
+def _plan(units: tuple, rows: int, slots: int, overhead: float) -> int:
     """Units a split takes, of sequences of ``units`` (their work, ``rows`` workgroups a split): the size of least
     estimated time -- all work and every split's fixed cost over the slots, and half a split's for the last round,
     or one split's where all are there at once."""
     total, longest = sum(units) * rows, max(units)
     least = -(-longest // MAX_SPLITS)
-    best, choice = None, longest
-    for k in (1, 1.25, 1.5, 2, 3, 4, 6, 8, 12):
-        for size in {max(least, int(total / (slots * k))), max(least, -int(-total // (slots * k)))}:
-            size = min(max(size, 1), longest)
-            items = rows * sum(-(-u // size) for u in units)
-            if items <= slots:
-                cost = size + SPLIT_OVERHEAD
-            else:
-                cost = (total + SPLIT_OVERHEAD * items) / slots + 0.5 * size
-            if best is None or cost < best:
-                best, choice = cost, size
-    # the next sizes up may make one round of sequences that the even share leaves just above it
-    for size in range(choice, min(longest, 2 * choice) + 1):
-        if rows * sum(-(-u // size) for u in units) <= slots:
-            return size if size + SPLIT_OVERHEAD < best else choice
-    return choice
+
+    def items(size):
+        return rows * sum(-(-u // size) for u in units)
+
+    share = max(1, least, -(-total // slots))
+    sizes = {max(least, total // (slots * k), 1) for k in (2, 3, 4, 6, 8, 12, 16)} | {share, longest}
+    # the first size past the even share that makes one round of sequences it does not divide
+    once = next((size for size in range(share, min(longest, 2 * share) + 1) if items(size) <= slots), None)
+    if once:
+        sizes.add(once)
+
+    # (one round of unlike items leaves the compute units unlike loads: 32 contexts of 4K-64K tokens in 6 splits, all
+    # there at once, 322 us, in 10 290, in 24 297; 16 equal ones in 12 56, in 24 62)
+    uneven = 1.0 if min(units) == longest else 1.15
+
+    def cost(size):
+        n = items(size)
+        return uneven * (size + overhead) if n <= slots else (total + overhead * n) / slots + 0.5 * size
+
+    return min((min(size, longest) for size in sorted(sizes, reverse=True)), key=cost)
 
 
-def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3) -> tuple[int, int]:
+def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3, overhead: float = SPLIT_OVERHEAD) -> tuple[int, int]:
     """``(splits, tokens of each)`` for sequences of ``tokens`` rows (an int, or one per sequence), ``rows``
     workgroups per sequence and split."""
     tokens = (tokens,) if isinstance(tokens, int) else tokens
-    size = _plan(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), rows, per_cu * cus) * SPLIT_UNIT
+    size = _plan(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), rows, per_cu * cus,
+                 overhead) * SPLIT_UNIT
     return -(-max(max(tokens), 1) // size), size
 
 
@@ -472,7 +478,8 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
         cus = _cu_count(manager.device)
         if pages is None and group * q_len >= MANY_ROWS and D <= 128 and query.dtype != torch.float32 \
                 and max(tokens) >= q_len + MANY_ROWS_HISTORY:
-            a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus)
+            a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
+                                             overhead=MANY_ROWS_OVERHEAD)
             a.splits = 1
         else:
             a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,
