@@ -390,7 +390,7 @@ int32_t lf_unpack_ints(const int32_t* words, int64_t rows, int32_t n_words, int3
  *     Value scale, min fp16 [head_dim / group][32][2]
  *   A code word's nibble e is in bits (4 e + 3) % 32 .. of the word: the word rotated left by 3.
  * ``bounds``: bf16 [batch][n_kv][cap_tokens / page_size][2][head_dim], every full page's smallest and
- * largest Key per channel (of the values read back), rounded outward.  ``lens``: DEVICE int32 [batch],
+ * largest Key per channel (of the values read back), rounded outward (infinities: bf16's largest number).  ``lens``: DEVICE int32 [batch],
  * the sequences' tokens; the write position never leaves the device.
  *
  * head_dim 64, 128 or 256; group 32, 64 or 128, at most head_dim; page_size a multiple of 32 up to 1024;
@@ -412,14 +412,16 @@ int32_t lf_int4_set_lens(const lf_int4_layer* layer, const int32_t* lens, void* 
 
 /*
  * Append rows: sequence b gets rows 0 .. counts[b] - 1 of k_src / v_src (``tokens`` rows each; counts, a
- * HOST int32 [batch] of 0 .. tokens read during the call, NULL: all of them) behind its lens[b], which then advances.  Rows past
- * cap_tokens are not written.  Element strides per sequence, head and token, unit channel stride.  Pages that
- * a sequence completes get their bounds.  Rows that are not finite leave codes, scales and minima without a
- * meaning for their own groups only.
+ * HOST int32 [batch] of 0 .. tokens read during the call, NULL: all of them) behind its lens[b], which then
+ * advances.  ``starts``: HOST int32 [batch] of 0 .. cap_tokens, read during the call: the rows go behind
+ * starts[b] rows in place of lens[b] (a caller that knows the lengths saves the launch that advances them; rows
+ * from there on are replaced), NULL: lens.  Rows past cap_tokens are not written.  Element strides per sequence,
+ * head and token, unit channel stride.  Pages that a sequence completes get their bounds.  Rows that are not
+ * finite leave codes, scales and minima without a meaning for their own groups only.
  */
 int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void* v_src, int32_t dtype,
-                       const int64_t* k_strides, const int64_t* v_strides, const int32_t* counts, int32_t tokens,
-                       void* stream);
+                       const int64_t* k_strides, const int64_t* v_strides, const int32_t* starts, const int32_t* counts,
+                       int32_t tokens, void* stream);
 
 /*
  * Read rows back: k_out / v_out [batch][n_kv][tokens][head_dim], contiguous, rounded to ``dtype`` (either may

@@ -152,7 +152,7 @@ _SIGNATURES = {
     "lf_noalloc_scratch_bytes": (c_int64, []),
     "lf_int4_set_lens": (c_int32, [POINTER(Int4Layer), c_void_p, c_void_p]),
     "lf_int4_append": (c_int32, [POINTER(Int4Layer), c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
-                                 c_int32, c_void_p]),
+                                 c_void_p, c_int32, c_void_p]),
     "lf_int4_read": (c_int32, [POINTER(Int4Layer), c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
     "lf_int4_attention": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
     "lf_int4_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32, c_int32, c_int32]),

@@ -4,7 +4,8 @@
 namespace lf {
 int launch_int4_set_lens(const lf_int4_layer& L, const int32_t* lens, hipStream_t stream);
 int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_src, int dtype, const int64_t* k_strides,
-                       const int64_t* v_strides, const int32_t* counts, int tokens, hipStream_t stream);
+                       const int64_t* v_strides, const int32_t* starts, const int32_t* counts, int tokens,
+                       hipStream_t stream);
 int launch_int4_read(const lf_int4_layer& L, const int32_t* starts, int tokens, void* k_out, void* v_out, int dtype,
                      hipStream_t stream);
 int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream);
@@ -62,8 +63,8 @@ int32_t lf_int4_set_lens(const lf_int4_layer* layer, const int32_t* lens, void* 
 }
 
 int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void* v_src, int32_t dtype,
-                       const int64_t* k_strides, const int64_t* v_strides, const int32_t* counts, int32_t tokens,
-                       void* stream) {
+                       const int64_t* k_strides, const int64_t* v_strides, const int32_t* starts, const int32_t* counts,
+                       int32_t tokens, void* stream) {
     const int32_t st = check_int4(layer);
     if (st != LF_OK) return st;
     if (!valid_dtype(dtype)) return LF_E_DTYPE;
@@ -72,7 +73,9 @@ int32_t lf_int4_append(const lf_int4_layer* layer, const void* k_src, const void
     if (!k_src || !v_src || !k_strides || !v_strides) return LF_E_NULL;
     for (int32_t b = 0; counts && b < layer->batch; ++b)
         if (counts[b] < 0 || counts[b] > tokens) return LF_E_SHAPE;
-    return lf::launch_int4_append(*layer, k_src, v_src, dtype, k_strides, v_strides, counts, tokens,
+    for (int32_t b = 0; starts && b < layer->batch; ++b)
+        if (starts[b] < 0 || starts[b] > layer->cap_tokens) return LF_E_SHAPE;
+    return lf::launch_int4_append(*layer, k_src, v_src, dtype, k_strides, v_strides, starts, counts, tokens,
                                   static_cast<hipStream_t>(stream));
 }
 

@@ -22,7 +22,8 @@ struct RowsArgs {
     int vec;       // every source row starts on 16 bytes
     int b0;        // the launch's first sequence
     int counted;   // 1: counts holds the tokens of sequences b0 ..
-    int32_t counts[kInlineSeqs];
+    int started;   // 1: starts holds their lengths
+    int32_t counts[kInlineSeqs], starts[kInlineSeqs];
 };
 
 // Eight consecutive elements of a row, as they are and as float32.
@@ -184,9 +185,10 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
     __builtin_amdgcn_wave_barrier();
 }
 
-// float32 rounded outward to bf16 (the pair's lower bound down, its upper bound up).
+// float32 rounded outward to bf16 (the pair's lower bound down, its upper bound up), infinities to the largest number
+// (a selection multiplies bounds by zeros).
 __device__ __forceinline__ uint16_t bf16_up(float x) {
-    const uint32_t u = __float_as_uint(x);
+    const uint32_t u = __float_as_uint(__builtin_amdgcn_fmed3f(x, -3.3895314e38f, 3.3895314e38f));
     return static_cast<uint16_t>((u >> 31 ? u : u + 0xffffu) >> 16);
 }
 __device__ __forceinline__ uint16_t bf16_down(float x) { return static_cast<uint16_t>(bf16_up(-x) ^ 0x8000u); }
@@ -239,6 +241,7 @@ __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int 
 }
 
 __device__ __forceinline__ int append_count(const RowsArgs& a, int i) { return a.counted ? a.counts[i] : a.tokens; }
+__device__ __forceinline__ int append_start(const RowsArgs& a, int i) { return a.started ? a.starts[i] : int4_len(a.L, a.b0 + i); }
 __device__ __forceinline__ int append_end(const RowsArgs& a, int i, int start) {
     return static_cast<int>(min(static_cast<int64_t>(start) + append_count(a, i), static_cast<int64_t>(a.L.cap_tokens)));
 }
@@ -248,7 +251,9 @@ template <int D, int GROUP, int Dt>
 __global__ __launch_bounds__(256) void int4_append_pages_kernel(RowsArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kBlock * D];
     const int b = a.b0 + blockIdx.z, h = blockIdx.y, P = a.L.page_size;
-    const int start = int4_len(a.L, b), end = append_end(a, blockIdx.z, start);
+    const int start = append_start(a, blockIdx.z), end = append_end(a, blockIdx.z, start);
+    // (with the lengths in the arguments nobody reads lens)
+    if (a.started && blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.L.lens[b] = end;
     const int page = start / P + blockIdx.x;
     if (static_cast<int64_t>(page) * P >= end) return;
     const int p0 = page * P, lo = max(start, p0), hi = min(end, p0 + P);
@@ -279,7 +284,7 @@ __global__ __launch_bounds__(512) void int4_append_few_kernel(RowsArgs a) {
     constexpr int kWaves = D > 128 ? 4 : 8;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kWaves * kBlock * D];
     const int b = a.b0 + blockIdx.x, P = a.L.page_size, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
-    const int start = int4_len(a.L, b), end = append_end(a, blockIdx.x, start);
+    const int start = append_start(a, blockIdx.x), end = append_end(a, blockIdx.x, start);
     for (int h = wave; h < a.L.n_kv && start < end; h += kWaves)
         for (int k = start / kBlock; k * kBlock < end; ++k) {
             const int t0 = max(start - k * kBlock, 0), t1 = min(end - k * kBlock, kBlock);
@@ -387,7 +392,7 @@ void append_typed(const RowsArgs& a, int batch, hipStream_t stream) {
     const int64_t here = min(pages, static_cast<int64_t>(L.cap_tokens / P) + 1);
     hipLaunchKernelGGL((int4_append_pages_kernel<D, GROUP, Dt>), dim3(static_cast<uint32_t>(here), L.n_kv, batch),
                        dim3(waves * kWave), 0, stream, a);
-    hipLaunchKernelGGL(int4_advance_kernel, dim3(1), dim3(kInlineSeqs), 0, stream, a);
+    if (!a.started) hipLaunchKernelGGL(int4_advance_kernel, dim3(1), dim3(kInlineSeqs), 0, stream, a);
 }
 
 int last_error() {
@@ -407,7 +412,8 @@ int launch_int4_set_lens(const lf_int4_layer& L, const int32_t* lens, hipStream_
 }
 
 int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_src, int dtype, const int64_t* k_strides,
-                       const int64_t* v_strides, const int32_t* counts, int tokens, hipStream_t stream) {
+                       const int64_t* v_strides, const int32_t* starts, const int32_t* counts, int tokens,
+                       hipStream_t stream) {
     RowsArgs a{};
     a.L = L;
     a.src[0] = k_src; a.src[1] = v_src;
@@ -422,11 +428,13 @@ int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_
     }
     a.vec = vec;
     a.counted = counts != nullptr;
+    a.started = starts != nullptr;
     return int4_dispatch(L, [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
         for (a.b0 = 0; a.b0 < L.batch; a.b0 += kInlineSeqs) {
             const int n = min(kInlineSeqs, L.batch - a.b0);
             for (int i = 0; i < n && counts; ++i) a.counts[i] = counts[a.b0 + i];
+            for (int i = 0; i < n && starts; ++i) a.starts[i] = starts[a.b0 + i];
             if (dtype == LF_BF16) append_typed<D, GROUP, LF_BF16>(a, n, stream);
             else if (dtype == LF_FP16) append_typed<D, GROUP, LF_FP16>(a, n, stream);
             else append_typed<D, GROUP, LF_FP32>(a, n, stream);

@@ -36,97 +36,76 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 }
 
 
-// D / 8 lanes take a page, eight channels each; a workgroup takes kScorePages pages of one (query token, kv head),
-// eight heads at a time: their elements stay in registers, their sums are exchanged so that each step of the
-// butterfly halves the heads a lane still adds up.
-constexpr int kScorePages = 32, kHeads = 8;
+// D / 8 lanes take a page, eight channels each, and eight heads at a time: the heads' elements stay in registers, widened
+// once, and their sums are exchanged so that each step of the butterfly halves the heads a lane still adds up.  (As
+// products of float64 matrix instructions, max(q, 0) hi + min(q, 0) lo with sixteen heads a tile: 9 us where this takes
+// XXX, and 22 in one launch with the choice below; they do four times the products at a sixteenth of the rate of bf16.)
+constexpr int kHeads = 8;
+constexpr int score_pages(int D) { return 256 / (D / 8); }  // of a workgroup
 
 __device__ __forceinline__ double other(double x, int mask) { return __shfl_xor(x, mask, kWave); }
 
 template <int D>
 __global__ __launch_bounds__(256) void int4_score_kernel(SelectArgs a) {
-    constexpr int LR = D / 8, RP = 256 / LR, Steps = kScorePages / RP > 0 ? kScorePages / RP : 1;
+    constexpr int LR = D / 8;
     static_assert(LR >= kHeads, "a lane per head");
     const int b = blockIdx.z, h = blockIdx.y / a.q_len, j = blockIdx.y % a.q_len;
     const int count = candidates(a, b, j);
-    const int p0 = blockIdx.x * kScorePages;
+    const int p0 = blockIdx.x * score_pages(D);
     if (p0 >= count || count <= a.n_pages) return;
-    const int w = threadIdx.x % LR;
+    const int w = threadIdx.x % LR, page = p0 + threadIdx.x / LR;
     const int pages = a.L.cap_tokens / a.L.page_size;
-    const uint16_t* bounds = a.L.bounds + (static_cast<int64_t>(b) * a.L.n_kv + h) * pages * 2 * D + 8 * w;
-    uint64_t* keys = a.keys + ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * pages;
-    const int p1 = min(p0 + kScorePages, count);
-    u32x4 lo[Steps], hi[Steps];
-#pragma unroll
-    for (int s = 0; s < Steps; ++s) {
-        const int64_t at = static_cast<int64_t>(min(p0 + s * RP + static_cast<int>(threadIdx.x) / LR, p1 - 1)) * 2 * D;
-        lo[s] = *reinterpret_cast<const u32x4*>(bounds + at);
-        hi[s] = *reinterpret_cast<const u32x4*>(bounds + at + D);
-    }
-    double best[Steps];
-    bool bad[Steps];
-#pragma unroll
-    for (int s = 0; s < Steps; ++s) { best[s] = -__builtin_inf(); bad[s] = false; }
+    const uint16_t* bounds = a.L.bounds + ((static_cast<int64_t>(b) * a.L.n_kv + h) * pages + min(page, count - 1)) * 2 * D + 8 * w;
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(bounds), hi = *reinterpret_cast<const u32x4*>(bounds + D);
+    double best = -__builtin_inf();
+    int nan = 0;
     for (int i0 = 0; i0 < a.g; i0 += kHeads) {
-        float q[kHeads][8];
+        double sum[kHeads];
 #pragma unroll
         for (int k = 0; k < kHeads; ++k) {
             // (heads past the group repeat its last one)
             const int64_t at = b * a.qb + static_cast<int64_t>(h * a.g + min(i0 + k, a.g - 1)) * a.qh + j * a.qt + 8 * w;
+            float q[8];
             if (a.vec) {
                 const u32x4 x = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(a.q) + at);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const uint16_t u = static_cast<uint16_t>(x[e >> 1] >> (16 * (e & 1)));
-                    q[k][e] = a.dtype == LF_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
+                    q[e] = a.dtype == LF_BF16 ? bf16_to_f32(u) : f16_to_f32(u);
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) q[k][e] = load_as_f32(a.q, at + e, a.dtype);
+                for (int e = 0; e < 8; ++e) q[e] = load_as_f32(a.q, at + e, a.dtype);
             }
-        }
-#pragma unroll
-        for (int s = 0; s < Steps; ++s) {
-            double sum[kHeads];
-#pragma unroll
-            for (int k = 0; k < kHeads; ++k) sum[k] = 0.;
+            sum[k] = 0.;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t l = e & 1 ? lo[s][e >> 1] & 0xffff0000u : lo[s][e >> 1] << 16, u = e & 1 ? hi[s][e >> 1] & 0xffff0000u : hi[s][e >> 1] << 16;
-#pragma unroll
-                for (int k = 0; k < kHeads; ++k)
-                    sum[k] = fma(static_cast<double>(q[k][e]), static_cast<double>(__uint_as_float(q[k][e] < 0.f ? l : u)), sum[k]);
+                const double l = __uint_as_float(e & 1 ? lo[e >> 1] & 0xffff0000u : lo[e >> 1] << 16);
+                const double u = __uint_as_float(e & 1 ? hi[e >> 1] & 0xffff0000u : hi[e >> 1] << 16);
+                sum[k] = fma(static_cast<double>(q[e]), q[e] < 0.f ? l : u, sum[k]);
             }
-            // lanes w and w ^ m split the heads that are left, then the lanes of one head add up
-            bool nan = false;
-#pragma unroll
-            for (int m = 1, left = kHeads / 2; left > 0; m <<= 1, left >>= 1)
-#pragma unroll
-                for (int k = 0; k < left; ++k) {
-                    const bool upper = w & m;
-                    const double keep = upper ? sum[k + left] : sum[k], give = upper ? sum[k] : sum[k + left];
-                    sum[k] = keep + other(give, m);
-                }
-#pragma unroll
-            for (int m = kHeads; m < LR; m <<= 1) sum[0] += other(sum[0], m);
-            nan = sum[0] != sum[0];
-            double top = sum[0];
-            int any = nan;
-#pragma unroll
-            for (int m = 1; m < kHeads; m <<= 1) {
-                const double o = other(top, m);
-                top = o > top ? o : top;
-                any |= __shfl_xor(any, m, kWave);
-            }
-            bad[s] |= any != 0;
-            best[s] = top > best[s] ? top : best[s];
         }
+        // lanes w and w ^ m split the heads that are left, then the lanes of one head add up
+#pragma unroll
+        for (int m = 1, left = kHeads / 2; left > 0; m <<= 1, left >>= 1)
+#pragma unroll
+            for (int k = 0; k < left; ++k) {
+                const bool upper = w & m;
+                const double keep = upper ? sum[k + left] : sum[k], give = upper ? sum[k] : sum[k + left];
+                sum[k] = keep + other(give, m);
+            }
+#pragma unroll
+        for (int m = kHeads; m < LR; m <<= 1) sum[0] += other(sum[0], m);
+        nan |= sum[0] != sum[0];
+        best = sum[0] > best ? sum[0] : best;
     }
 #pragma unroll
-    for (int s = 0; s < Steps; ++s) {
-        const int page = p0 + s * RP + threadIdx.x / LR;
-        if (page < p1 && w == 0) keys[page] = bad[s] ? 0 : score_key(best[s]);
+    for (int m = 1; m < kHeads; m <<= 1) {
+        const double o = other(best, m);
+        best = o > best ? o : best;
+        nan |= __shfl_xor(nan, m, kWave);
     }
+    if (page < count && w == 0) a.keys[((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * pages + page] = nan ? 0 : score_key(best);
 }
 
 // A workgroup per (query token, kv head): the n_pages-th largest key, eight bits at a time (as far as the pages at
@@ -256,7 +235,7 @@ int launch_int4_select(const lf_int4_layer& L, const lf_int4_args& A, hipStream_
     a.pages = A.pages;
     a.keys = static_cast<uint64_t*>(A.workspace);
     const int pages = L.cap_tokens / L.page_size;
-    const dim3 grid((pages + kScorePages - 1) / kScorePages, L.n_kv * A.q_len, L.batch);
+    const dim3 grid((pages + score_pages(L.head_dim) - 1) / score_pages(L.head_dim), L.n_kv * A.q_len, L.batch);
     const int st = int4_dispatch(L, [&](auto shape) {
         hipLaunchKernelGGL((int4_score_kernel<decltype(shape)::d>), grid, dim3(256), 0, stream, a);
         return LF_OK;

@@ -20,7 +20,6 @@ Nothing here runs on the CPU.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from typing import Optional
@@ -51,19 +50,26 @@ def check_layout(head_dim: int, page_size: int, group_size: int) -> None:
         raise ValueError(f"page_size must be a multiple of {BLOCK} up to 1024, got {page_size}")
 
 
-def _on(device: torch.device):
-    """``device`` made current for a launch (the default stream names no device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _here(fn):
+    """``fn(owner, ...)`` with the owner's device current (the default stream names no device)."""
+    @functools.wraps(fn)
+    def call(owner, *args, **kwargs):
+        if torch.cuda.current_device() == owner.device.index:
+            return fn(owner, *args, **kwargs)
+        with torch.cuda.device(owner.device):
+            return fn(owner, *args, **kwargs)
+    return call
 
 
 def _check_rows(t: torch.Tensor, device: torch.device, name: str) -> torch.Tensor:
     """``t`` as the kernels read it: on this device, a row type they take, unit channel stride."""
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} is on {t.device}; logitfill_amd runs on ROCm devices only")
     if t.device != device:
+        if not t.is_cuda:
+            raise RuntimeError(f"{name} is on {t.device}; logitfill_amd runs on ROCm devices only")
         raise ValueError(f"{name} is on {t.device}, the cache on {device}")
     _native.dtype_code(t.dtype)
-    t = t.detach()
+    if t.requires_grad:
+        t = t.detach()
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
@@ -138,8 +144,8 @@ class _Int4Store:
                 bounds[:, :, : self._cap // P].copy_(self._bounds)
         self._blocks, self._bounds, self._cap, self._struct = blocks, bounds, cap, None
 
-    def layer_struct(self) -> _native.Int4Layer:
-        """The ``lf_int4_layer`` describing this store, its device lengths up to date on the current stream."""
+    def layer_struct(self, lengths: bool = True) -> _native.Int4Layer:
+        """The ``lf_int4_layer`` describing this store; ``lengths``: the device's up to date on the current stream."""
         if self._cap == 0:
             self.reserve(self.page_size)
         if self._struct is None:
@@ -148,7 +154,7 @@ class _Int4Store:
             s.batch, s.n_kv, s.head_dim = self.batch, self.n_kv, self.head_dim
             s.cap_tokens, s.page_size, s.group = self._cap, self.page_size, self.group_size
             self._struct = s
-        if self._dirty:
+        if lengths and self._dirty:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the cache was truncated or reset since its last launch: "
                                    "call manager.sync_lengths() before the capture")
@@ -174,12 +180,13 @@ class _Int4Store:
     # ---- rows ------------------------------------------------------------------
     def check_append(self, key: torch.Tensor, value: torch.Tensor, lengths):
         """Checked ``(key, value, per-sequence counts or None)`` of an append."""
-        if key.dim() != 4 or key.shape != value.shape:
+        shape = key.shape
+        if len(shape) != 4 or shape != value.shape:
             raise ValueError(f"Key and Value rows must be of one shape [batch, n_kv, T, head_dim], got "
-                             f"{tuple(key.shape)} and {tuple(value.shape)}")
-        B, H, T, D = (int(x) for x in key.shape)
+                             f"{tuple(shape)} and {tuple(value.shape)}")
+        B, H, T, D = shape
         if B != self.batch or H != self.n_kv or D != self.head_dim:
-            raise ValueError(f"expected [{self.batch}, {self.n_kv}, T, {self.head_dim}], got {tuple(key.shape)}")
+            raise ValueError(f"expected [{self.batch}, {self.n_kv}, T, {self.head_dim}], got {tuple(shape)}")
         if key.dtype != value.dtype:
             raise TypeError("key and value must share a dtype")
         key, value = _check_rows(key, self.device, "key"), _check_rows(value, self.device, "value")
@@ -195,20 +202,27 @@ class _Int4Store:
         """Append ``key/value [batch, n_kv, T, head_dim]`` (sequence b its first ``lengths[b]`` tokens)."""
         self._append(*self.check_append(key, value, lengths))
 
+    @_here
     def _append(self, key: torch.Tensor, value: torch.Tensor, lengths) -> None:
-        T = int(key.shape[2])
+        T = key.shape[2]
         if T == 0 or (lengths is not None and max(lengths) == 0):
             return
-        new = [n + T for n in self.lengths] if lengths is None else [n + t for n, t in zip(self.lengths, lengths)]
-        with _on(self.device):
-            if max(new) > self._cap:
-                self.reserve(max(new))
-            st = _native.load().lf_int4_append(
-                self.layer_struct(), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
-                _strides(value), None if lengths is None else _ints(lengths), T, _native.current_stream_ptr(self.device))
+        old = self.lengths
+        new = [n + T for n in old] if lengths is None else [n + t for n, t in zip(old, lengths)]
+        if max(new) > self._cap:
+            self.reserve(max(new))
+        # the rows go where the host's lengths end and the device's follow; a captured commit moves the device's own
+        captured = torch.cuda.is_current_stream_capturing()
+        st = _native.load().lf_int4_append(
+            self.layer_struct(captured), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
+            _strides(value), None if captured else _ints(old), None if lengths is None else _ints(lengths), T,
+            _native.current_stream_ptr(self.device))
         _native.check(st, "lf_int4_append")
         self.lengths = new
+        if not captured:
+            self._dirty = False
 
+    @_here
     def read(self, starts, tokens: int, dtype=torch.float32):
         """``tokens`` rows of every sequence read back: ``(K, V) [batch, n_kv, tokens, head_dim]``, row t of sequence b
         the cache's row ``starts[b] + t`` (an int for all; rows outside the sequence are zeros)."""
@@ -220,10 +234,8 @@ class _Int4Store:
         k = torch.empty(self.batch, self.n_kv, tokens, self.head_dim, dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         if tokens:
-            with _on(self.device):
-                struct = self.layer_struct()
-                st = _native.load().lf_int4_read(struct, _ints(starts), tokens, k.data_ptr(), v.data_ptr(), code,
-                                                 _native.current_stream_ptr(self.device))
+            st = _native.load().lf_int4_read(self.layer_struct(), _ints(starts), tokens, k.data_ptr(), v.data_ptr(),
+                                             code, _native.current_stream_ptr(self.device))
             _native.check(st, "lf_int4_read")
         return k, v
 
@@ -303,11 +315,11 @@ class Int4KVManager:
             layer.lengths = [n + t for n, t in zip(layer.lengths, tokens)]
         self.seq_len = self.layers[-1].length if self.layers else 0
 
+    @_here
     def sync_lengths(self) -> None:
         """Bring the device's lengths up to the host's on the current stream (before a capture)."""
         for layer in self.layers:
-            with _on(layer.device):
-                layer.layer_struct()
+            layer.layer_struct()
 
     def reset(self) -> None:
         """Forget every token (storage is kept for reuse)."""
@@ -317,11 +329,11 @@ class Int4KVManager:
 
 
 def _check_query(manager, query: torch.Tensor) -> torch.Tensor:
-    if query.dim() != 4 or query.shape[0] != manager.batch_size or query.shape[1] != manager.n_q \
-            or query.shape[3] != manager.head_dim:
+    shape = query.shape
+    if len(shape) != 4 or shape[0] != manager.batch_size or shape[1] != manager.n_q or shape[3] != manager.head_dim:
         raise ValueError(f"query must be [{manager.batch_size}, {manager.n_q}, q_len, {manager.head_dim}], "
-                         f"got {tuple(query.shape)}")
-    if query.shape[2] < 1:
+                         f"got {tuple(shape)}")
+    if shape[2] < 1:
         raise ValueError("query holds no token")
     return _check_rows(query, manager.device, "query")
 
@@ -369,8 +381,8 @@ def _args(manager, query: torch.Tensor, counts, scaling: float) -> _native.Int4A
 # Tokens a split is a multiple of (a record for each of a workgroup's four waves).
 SPLIT_UNIT = 128
 # A workgroup's fixed cost (its queries, the first records' way, the waves' merge, its share of the splits') in
-# units of its work: about 3 us against 2 us a unit.  A many-row workgroup writes eight times the sums.
-SPLIT_OVERHEAD = 1.5
+# units of its work: some 5 us against 2 us a unit.  A many-row workgroup writes eight times the sums.
+SPLIT_OVERHEAD = 3.0
 MANY_ROWS_OVERHEAD = 4.0
 
 
@@ -383,7 +395,7 @@ def workgroups_per_cu(head_dim: int, group: int) -> int:
 @functools.lru_cache(maxsize=512)
 def _plan(units: tuple, rows: int, slots: int, overhead: float) -> int:
     """Units a split takes, of sequences of ``units`` (their work, ``rows`` workgroups a split): the size of least
-    estimated time -- all work and every split's fixed cost over the slots, and half a split's for the last round,
+    estimated time -- all work and every split's fixed cost over the slots, and part of a split's for the last round,
     or one split's where all are there at once."""
     total, longest = sum(units) * rows, max(units)
     least = -(-longest // MAX_SPLITS)
@@ -404,7 +416,7 @@ def _plan(units: tuple, rows: int, slots: int, overhead: float) -> int:
 
     def cost(size):
         n = items(size)
-        return uneven * (size + overhead) if n <= slots else (total + overhead * n) / slots + 0.5 * size
+        return uneven * (size + overhead) if n <= slots else (total + overhead * n) / slots + 0.3 * size
 
     return min((min(size, longest) for size in sorted(sizes, reverse=True)), key=cost)
 
@@ -443,12 +455,13 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     """
     layer = manager.layers[layer_idx]
     query = _check_query(manager, query)
-    q_len = int(query.shape[2])
-    B, D = manager.batch_size, manager.head_dim
+    q_len = query.shape[2]
+    B = manager.batch_size
+    new = None
     if (key_new is None) != (value_new is None):
         raise ValueError("key_new and value_new come together")
     if key_new is not None:
-        key_new, value_new, new_lengths = layer.check_append(key_new, value_new, lengths)
+        new = layer.check_append(key_new, value_new, lengths)
         if key_new.shape[2] != q_len:
             raise ValueError(f"{key_new.shape[2]} new tokens and {q_len} query tokens")
     if pages is not None:
@@ -459,43 +472,47 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
         if pages.device != manager.device:
             raise ValueError(f"pages are on {pages.device}, the cache on {manager.device}")
         pages = pages.contiguous()
-    with _on(manager.device):
-        counts = _query_lengths(manager, q_len, lengths)
-        if key_new is not None:
-            layer._append(key_new, value_new, new_lengths)
-            manager._note(layer_idx)
-        if pages is None and manager.top_pages:
-            pages = _select(manager, layer, query, manager.top_pages, counts)
-        out = torch.empty(B, manager.n_q, q_len, D, dtype=query.dtype, device=manager.device)
-        a = _args(manager, query, counts, scaling)
-        a.out = out.data_ptr()
-        group = manager.n_q // manager.n_kv
-        tokens, tiles = layer.lengths, -(-group * q_len // 16)
-        if pages is not None:
-            a.pages, a.n_pages = pages.data_ptr(), int(pages.shape[3])
-            # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
-            tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
-        cus = _cu_count(manager.device)
-        if pages is None and group * q_len >= MANY_ROWS and D <= 128 and query.dtype != torch.float32 \
-                and max(tokens) >= q_len + MANY_ROWS_HISTORY:
-            a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
-                                             overhead=MANY_ROWS_OVERHEAD)
-            a.splits = 1
-        else:
-            a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,
-                                                   workgroups_per_cu(D, manager.group_size))
-        parts = a.splits + a.prefix_splits
-        lib = _native.load()
-        struct = layer.layer_struct()
-        if parts > 1:
-            a.workspace_bytes = 4 * B * a.n_q * q_len * parts * (D + 2)  # lf_int4_workspace_bytes
-            ws = _workspace(manager, a.workspace_bytes)
-            a.workspace = ws.data_ptr()
-        st = lib.lf_int4_attention(struct, a, _native.current_stream_ptr(manager.device))
+    return _attend(manager, layer_idx, layer, query, new, scaling, lengths, pages)
+
+
+@_here
+def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: float, lengths, pages) -> torch.Tensor:
+    """``int4_attention`` of checked arguments; ``new``: those of the append."""
+    B, n_q, q_len, D = query.shape
+    counts = _query_lengths(manager, q_len, lengths)
+    if new is not None:
+        layer._append(*new)
+        manager._note(layer_idx)
+    if pages is None and manager.top_pages:
+        pages = _select(manager, layer, query, manager.top_pages, counts)
+    out = torch.empty(B, n_q, q_len, D, dtype=query.dtype, device=manager.device)
+    a = _args(manager, query, counts, scaling)
+    a.out = out.data_ptr()
+    group, cus = n_q // manager.n_kv, _cu_count(manager.device)
+    tokens, tiles = layer.lengths, -(-group * q_len // 16)
+    if pages is not None:
+        a.pages, a.n_pages = pages.data_ptr(), pages.shape[3]
+        # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
+        tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
+    if pages is None and group * q_len >= MANY_ROWS and D <= 128 and query.dtype != torch.float32 \
+            and max(tokens) >= q_len + MANY_ROWS_HISTORY:
+        a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
+                                         overhead=MANY_ROWS_OVERHEAD)
+        a.splits = 1
+    else:
+        a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,
+                                               workgroups_per_cu(D, manager.group_size))
+    parts = a.splits + a.prefix_splits
+    if parts > 1:
+        nbytes = 4 * B * n_q * q_len * parts * (D + 2)  # lf_int4_workspace_bytes
+        ws = _workspace(manager, nbytes)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    st = _native.load().lf_int4_attention(layer.layer_struct(), a, _native.current_stream_ptr(manager.device))
     _native.check(st, "lf_int4_attention")
     return out
 
 
+@_here
 def _select(manager, layer, query: torch.Tensor, top_pages: int, counts) -> torch.Tensor:
     q_len = int(query.shape[2])
     lib = _native.load()
@@ -525,6 +542,5 @@ def select_pages(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, to
     top_pages = int(top_pages)
     if not 1 <= top_pages <= MAX_PAGES:
         raise ValueError(f"top_pages must lie in 1 .. {MAX_PAGES}, got {top_pages}")
-    with _on(manager.device):
-        counts = _query_lengths(manager, int(query.shape[2]), lengths)
-        return _select(manager, manager.layers[layer_idx], query, top_pages, counts)
+    counts = _query_lengths(manager, query.shape[2], lengths)
+    return _select(manager, manager.layers[layer_idx], query, top_pages, counts)

@@ -69,7 +69,7 @@ BAD_LAYERS = [
 def test_every_entry_point_checks_the_layer(change, want):
     lib, L = _native.load(), _layer(**change)
     s = (ctypes.c_int64 * 3)(0, 0, 0)
-    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, 4, None) == want
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, None, 4, None) == want
     assert lib.lf_int4_read(L, None, 4, AT, AT, 0, None) == want
     assert lib.lf_int4_attention(L, _args(), None) == want
     assert lib.lf_int4_select(L, _args(n_pages=4, pages=AT), None) == want
@@ -78,12 +78,22 @@ def test_every_entry_point_checks_the_layer(change, want):
 def test_append_and_read_refusals():
     lib, L = _native.load(), _layer()
     s = (ctypes.c_int64 * 3)(0, 0, 0)
-    assert lib.lf_int4_append(None, AT, AT, 0, s, s, None, 4, None) == NULL
-    assert lib.lf_int4_append(L, 0, AT, 0, s, s, None, 4, None) == NULL
-    assert lib.lf_int4_append(L, AT, AT, 0, None, s, None, 4, None) == NULL
-    assert lib.lf_int4_append(L, AT, AT, 3, s, s, None, 4, None) == DTYPE
-    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, -1, None) == SHAPE
-    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, 0, None) == 0
+    assert lib.lf_int4_append(None, AT, AT, 0, s, s, None, None, 4, None) == NULL
+    assert lib.lf_int4_append(L, 0, AT, 0, s, s, None, None, 4, None) == NULL
+    assert lib.lf_int4_append(L, AT, AT, 0, None, s, None, None, 4, None) == NULL
+    assert lib.lf_int4_append(L, AT, AT, 3, s, s, None, None, 4, None) == DTYPE
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, None, -1, None) == SHAPE
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, None, 0, None) == 0
+    bad = [(ctypes.c_int32 * 2)(*x) for x in ((-1, 0), (0, 5), (0, 1025))]
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, bad[0], 4, None) == SHAPE
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, None, bad[1], 4, None) == SHAPE
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, bad[0], None, 4, None) == SHAPE
+    assert lib.lf_int4_append(L, AT, AT, 0, s, s, bad[2], None, 4, None) == SHAPE
+    assert lib.lf_int4_set_lens(L, None, None) == NULL
+    assert lib.lf_int4_set_lens(L, bad[0], None) == SHAPE
+    assert lib.lf_int4_set_lens(L, bad[2], None) == SHAPE
+    assert lib.lf_int4_read(L, bad[0], 4, AT, AT, 0, None) == SHAPE
+    assert lib.lf_int4_read(L, None, 4, AT + 8, AT, 0, None) == SHAPE
     assert lib.lf_int4_read(L, None, 4, 0, 0, 0, None) == NULL
     assert lib.lf_int4_read(L, None, 4, AT, 0, -1, None) == DTYPE
     assert lib.lf_int4_read(L, None, -4, AT, 0, 0, None) == SHAPE
