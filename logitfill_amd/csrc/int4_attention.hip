@@ -117,6 +117,13 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         j = r % a.q_len;
     }
     const bool real = i < a.g;
+    // The first record is on its way before the sequence's length is: where it lies hangs on neither (with pages or
+    // behind a many-row prefix it does).  A wave that finds it has none waits for the load all the same.
+    const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
+    const uint32_t ring = lds_addr(smem) + wave * kRing * R::bytes;
+    const int64_t early = static_cast<int64_t>(part) * (a.split_tokens / kBlock) + wave;
+    const bool ahead = !a.n_pages && !a.prefix && early < a.L.cap_tokens / kBlock;
+    if (ahead) S::load(base + early * R::bytes, ring, lane);
     const int len = int4_len(a.L, b);
     const int n = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
     const int lim = real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
@@ -164,15 +171,14 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         const int block = page * per_page + (at - e * per_page);
         return page < 0 || block * kBlock >= top ? -1 : block;
     };
-    const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
-    const uint32_t ring = lds_addr(smem) + wave * kRing * R::bytes;
     const auto fill = [&](int k, int slot) {
         const int block = block_of(k);
         S::load(base + static_cast<int64_t>(block < 0 ? own * per_page : block) * R::bytes, ring + slot * R::bytes, lane);
     };
 #pragma unroll
-    for (int k = 0; k < kRing - 1; ++k)
+    for (int k = ahead ? 1 : 0; k < kRing - 1; ++k)
         if (k < count) fill(k, k);
+    if (ahead && count == 0) wait_ring<0>();
 
     Parts<NT> q[CH];
     float qsum[G];
@@ -362,7 +368,15 @@ __global__ __launch_bounds__(256) void int4_merge_kernel(Int4Attention a, int dt
     const int64_t row = blockIdx.x;
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave)), waves = blockDim.x / kWave;
     const float* ml = a.part_ml + row * a.parts * 2;
-    const float* parts = a.part_o + row * a.parts * D + lane * C;
+    const float* sums = a.part_o + row * a.parts * D + lane * C;
+    float x[kTake][C];
+    const auto load = [&](int s) {
+#pragma unroll
+        for (int k = 0; k < kTake; ++k)
+#pragma unroll
+            for (int c = 0; c < C; ++c) x[k][c] = s + k < a.parts ? sums[(s + k) * D + c] : 0.f;
+    };
+    load(wave * kTake);  // (on their way while the reference points are compared)
     float m = -__builtin_inff();
     for (int s = lane; s < a.parts; s += kWave) m = fmaxf(m, ml[2 * s]);
     m = wave_max(m);
@@ -375,11 +389,7 @@ __global__ __launch_bounds__(256) void int4_merge_kernel(Int4Attention a, int dt
             l = fmaf(w, ml[2 * (s0 + lane) + 1], l);
         }
         for (int k0 = wave * kTake; k0 < kWave && s0 + k0 < a.parts; k0 += waves * kTake) {
-            float x[kTake][C];
-#pragma unroll
-            for (int k = 0; k < kTake; ++k)
-#pragma unroll
-                for (int c = 0; c < C; ++c) x[k][c] = s0 + k0 + k < a.parts ? parts[(s0 + k0 + k) * D + c] : 0.f;
+            if (s0 > 0 || k0 > wave * kTake) load(s0 + k0);
 #pragma unroll
             for (int k = 0; k < kTake; ++k) {
                 const float wk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), k0 + k));

@@ -108,6 +108,12 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
     constexpr int LR = D / 8, RP = kWave / LR, Passes = kBlock / RP;  // lanes per row, rows per pass
     const int lane = threadIdx.x & (kWave - 1), w = lane % LR;
     uint32_t* words = reinterpret_cast<uint32_t*>(rec);
+    const int quad = lane >> 4, c0 = lane & 15;
+    u32x4* vw = reinterpret_cast<u32x4*>(rec + R::v) + lane;
+    u32x4 old[Whole ? 1 : D / 64];  // the Value words that a part of the record's tokens joins
+    if constexpr (!Whole)
+#pragma unroll
+        for (int u = 0; u < D / 64; ++u) old[u] = vw[u * kWave];
     const auto load = [&](int kv, int row) {
         return load8<Dt>(a.src[kv], b * a.sb[kv] + h * a.sh[kv] + 8 * w + (src0 + static_cast<int64_t>(row) - t0) * a.st[kv], a.vec);
     };
@@ -154,7 +160,6 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const int quad = lane >> 4, c0 = lane & 15;
     uint32_t fresh = 0;  // the nibbles this write replaces
     if constexpr (!Whole)
 #pragma unroll
@@ -162,7 +167,6 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
             const int tok = 4 * quad + (e & 3) + 16 * (e >> 2);
             if (tok >= t0 && tok < t1) fresh |= turn(15u << (4 * e), 29);
         }
-    u32x4* vw = reinterpret_cast<u32x4*>(rec + R::v) + lane;
 #pragma unroll
     for (int u = 0; u < D / 64; ++u) {
         uint32_t tok[8];
@@ -179,7 +183,7 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
         }
         const u32x4 word = value_words(tok);
         if constexpr (Whole) vw[u * kWave] = word;
-        else if (fresh) vw[u * kWave] = (vw[u * kWave] & ~fresh) | (word & fresh);
+        else if (fresh) vw[u * kWave] = (old[u] & ~fresh) | (word & fresh);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -318,12 +322,68 @@ struct ReadArgs {
     int32_t starts[kInlineSeqs];
 };
 
-// A wave per record: a Key word and row segment of eight channels per lane, then Values of four (two and two) channels
-// and eight tokens.
+// Rows from .. to - 1 of a record, zeros from row ``seen`` on: a Key word and row segment of eight channels per lane, and
+// Values of four (two and two) channels and eight tokens.
+template <int D, int GROUP, int Dt, bool Whole>
+__device__ __forceinline__ void read_record(const ReadArgs& a, const uint8_t* rec, int64_t dst, int from, int to, int seen, int lane) {
+    using R = Int4Rec<D, GROUP>;
+    constexpr int LR = D / 8, RP = kWave / LR, Passes = kBlock / RP, U = D / 64;
+    const int w = lane % LR, quad = lane >> 4, c0 = lane & 15;
+    uint32_t word[Passes], key[Passes];
+    u32x4 values[U], pairs[U][2][2];
+#pragma unroll
+    for (int p = 0; p < Passes; ++p) {
+        if (!Whole && (p * RP + RP <= from || p * RP >= to)) continue;
+        const int row = p * RP + lane / LR;
+        word[p] = reinterpret_cast<const uint32_t*>(rec)[row * LR + key_word(D, w)];
+        key[p] = reinterpret_cast<const uint32_t*>(rec + R::ksm)[w / (GROUP / 8) * kBlock + row];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        values[u] = reinterpret_cast<const u32x4*>(rec + R::v)[u * kWave + lane];
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)  // of the four channels, or of the lower and the upper two
+                pairs[u][v][k] = reinterpret_cast<const u32x4*>(rec + R::vsm)[(GROUP == 32 ? 2 * u + k : 64 * u / GROUP) * (kBlock / 4) + 4 * v + quad];
+    }
+    if (a.out[0])
+#pragma unroll
+        for (int p = 0; p < Passes; ++p) {
+            if (!Whole && (p * RP + RP <= from || p * RP >= to)) continue;
+            const int row = p * RP + lane / LR;
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = Whole || row < seen ? fmaf(static_cast<float>(code_at(word[p], e)), pair_scale(key[p]), pair_min(key[p])) : 0.f;
+            if (Whole || (row >= from && row < to)) store_row<Dt>(a.out[0], dst + row * D + 8 * w, x);
+        }
+    if (a.out[1])
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int row = 16 * (e >> 2) + 4 * quad + (e & 3);
+                if (!Whole && (row < from || row >= to)) continue;
+                float x[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    const uint32_t pair = pairs[u][e >> 2][t >> 1][e & 3];
+                    x[t] = Whole || row < seen ? fmaf(static_cast<float>(code_at(values[u][t], e)), pair_scale(pair), pair_min(pair)) : 0.f;
+                }
+                if constexpr (GROUP == 32) {
+                    const float a0[2] = {x[0], x[1]}, a1[2] = {x[2], x[3]};
+                    store_row<Dt>(a.out[1], dst + row * D + 64 * u + 2 * c0, a0);
+                    store_row<Dt>(a.out[1], dst + row * D + 64 * u + 32 + 2 * c0, a1);
+                } else {
+                    store_row<Dt>(a.out[1], dst + row * D + 64 * u + 4 * c0, x);
+                }
+            }
+}
+
+// A wave per record.
 template <int D, int GROUP, int Dt>
 __global__ __launch_bounds__(256) void int4_read_kernel(ReadArgs a) {
     using R = Int4Rec<D, GROUP>;
-    constexpr int LR = D / 8, RP = kWave / LR;
     const int b = a.b0 + blockIdx.z, h = blockIdx.y, lane = threadIdx.x % kWave;
     const int start = a.starts[blockIdx.z], len = int4_len(a.L, b);
     const int block = start / kBlock + static_cast<int>(blockIdx.x) * 4 + in_sgpr(static_cast<int>(threadIdx.x / kWave));
@@ -333,51 +393,11 @@ __global__ __launch_bounds__(256) void int4_read_kernel(ReadArgs a) {
     const uint8_t* rec = int4_block(a.L, b, h, there ? block : 0, R::bytes);
     // element 0 of the row of the record's token 0, which may lie in front of the first
     const int64_t dst = ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.tokens + (pos0 - start)) * D;
-    if (a.out[0]) {
-        const int w = lane % LR;
-#pragma unroll
-        for (int p = 0; p < kBlock / RP; ++p) {
-            const int row = p * RP + lane / LR;
-            const uint32_t word = reinterpret_cast<const uint32_t*>(rec)[row * LR + key_word(D, w)];
-            const uint32_t sm = reinterpret_cast<const uint32_t*>(rec + R::ksm)[w / (GROUP / 8) * kBlock + row];
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = pos0 + row < len ? fmaf(static_cast<float>(code_at(word, e)), pair_scale(sm), pair_min(sm)) : 0.f;
-            if (pos0 + row >= start && pos0 + row < end) store_row<Dt>(a.out[0], dst + row * D + 8 * w, x);
-        }
-    }
-    if (a.out[1]) {
-        const int quad = lane >> 4, c0 = lane & 15;
-#pragma unroll
-        for (int u = 0; u < D / 64; ++u) {
-            const u32x4 word = reinterpret_cast<const u32x4*>(rec + R::v)[u * kWave + lane];
-#pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                u32x4 sm[2];  // of the four channels, or of the lower and the upper two
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int g = GROUP == 32 ? 2 * u + k : 64 * u / GROUP;
-                    sm[k] = reinterpret_cast<const u32x4*>(rec + R::vsm)[g * (kBlock / 4) + 4 * v + quad];
-                }
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * v + 4 * quad + r;
-                    float x[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        x[t] = pos0 + row < len ? fmaf(static_cast<float>(code_at(word[t], r + 4 * v)), pair_scale(sm[t >> 1][r]), pair_min(sm[t >> 1][r])) : 0.f;
-                    if (pos0 + row < start || pos0 + row >= end) continue;
-                    if constexpr (GROUP == 32) {
-                        const float a0[2] = {x[0], x[1]}, a1[2] = {x[2], x[3]};
-                        store_row<Dt>(a.out[1], dst + row * D + 64 * u + 2 * c0, a0);
-                        store_row<Dt>(a.out[1], dst + row * D + 64 * u + 32 + 2 * c0, a1);
-                    } else {
-                        store_row<Dt>(a.out[1], dst + row * D + 64 * u + 4 * c0, x);
-                    }
-                }
-            }
-        }
-    }
+    const int from = static_cast<int>(max(start - pos0, static_cast<int64_t>(0))), to = static_cast<int>(min(end - pos0, static_cast<int64_t>(kBlock)));
+    const int seen = static_cast<int>(min(max(len - pos0, static_cast<int64_t>(0)), static_cast<int64_t>(kBlock)));
+    // (a whole record: all of its loads on their way before the first store)
+    if (from == 0 && to == kBlock && seen == kBlock) read_record<D, GROUP, Dt, true>(a, rec, dst, 0, kBlock, kBlock, lane);
+    else read_record<D, GROUP, Dt, false>(a, rec, dst, from, to, seen, lane);
 }
 
 template <int D, int GROUP, int Dt>
