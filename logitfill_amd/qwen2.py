@@ -14,11 +14,15 @@ past_key_values=None, **kwargs)``), with two differences: the packed output
 reference reshapes it directly, which is right only for ``q_len == 1``), and the model runs
 without a transformers cache -- the packed cache holds the history, so callers pass explicit
 ``position_ids`` (``PackedDecoder`` does).  ``detach_packed`` restores the original forwards.
+
+With an ``Int4KVManager`` the layers run ``int4_attention`` instead, which caches the new tokens
+before it reads (of a manager with ``top_pages``, over the pages it selects).
 """
 from __future__ import annotations
 
 import torch
 
+from logitfill_amd.packed.int4 import Int4KVManager, int4_attention
 from logitfill_amd.packed.reference import packed_attention
 
 
@@ -49,6 +53,8 @@ def _make_forward(attn, manager, attention_fn):
         if past == 0:
             out = _dense_attention(attn, query, key, value, attention_mask, kwargs)
             manager.commit(layer_idx, key, value)
+        elif getattr(manager, "commits_new_tokens", False):
+            out = attention_fn(manager, layer_idx, query, key, value, attn.scaling).transpose(1, 2)
         elif attention_fn is packed_attention:
             # attention then commit, the commit folded into the decode launch where it can be
             out = packed_attention(manager, layer_idx, query, key, value, attn.scaling, commit=True).transpose(1, 2)
@@ -66,7 +72,10 @@ def _make_forward(attn, manager, attention_fn):
 def attach_packed(model, manager, attention_fn=packed_attention) -> None:
     """Route every decoder layer's attention through ``manager`` (a ``PackedKVManager`` whose
     layers match the model's).  ``attention_fn`` is ``packed_attention`` (the HIP path) or
-    ``reference_attention`` (dense dequantise-then-attend), same signature."""
+    ``reference_attention`` (dense dequantise-then-attend), same signature.  An ``Int4KVManager``
+    takes ``int4_attention`` in place of the default."""
+    if isinstance(manager, Int4KVManager) and attention_fn is packed_attention:
+        attention_fn = int4_attention
     cfg = model.config
     n_kv = int(cfg.num_key_value_heads)
     layers = model.model.layers
