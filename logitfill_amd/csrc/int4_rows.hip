@@ -64,28 +64,55 @@ __device__ __forceinline__ void widen8(const Raw8<Dt>& r, float (&x)[8]) {
     }
 }
 
-// Codes of a lane's eight channels; scale and minimum of their group in every lane.  The quotient is formed from the
-// correctly rounded reciprocal of the scale, which the group's codes share, and one correction by the exact residual
-// (Markstein): the correctly rounded quotient, as the division gives it.  A range beyond float32's is cut to its
-// largest number, whose quotient clamps to 15 as the infinite one does.  Adding 2^23 rounds to an integer, half to even.
-template <int GROUP>
+// The smallest x of 4, 8 or 16 neighbouring lanes, in every one of them: exchanges within a row of 16 lanes that ride on
+// the comparison (lanes i and i ^ 1, i ^ 2, then 7 - i and 15 - i, whose fours and eights hold one value by then).
+template <int Ctrl>
+__device__ __forceinline__ float row_other(float x) {
+    const int i = __builtin_bit_cast(int, x);
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, Ctrl, 0xf, 0xf, true));
+}
+template <int N>
+__device__ __forceinline__ float lanes_min(float x) {
+    x = fminf(x, row_other<0xB1>(x));                       // quad_perm 1, 0, 3, 2
+    x = fminf(x, row_other<0x4E>(x));                       // quad_perm 2, 3, 0, 1
+    if constexpr (N > 4) x = fminf(x, row_other<0x141>(x)); // row_half_mirror
+    if constexpr (N > 8) x = fminf(x, row_other<0x140>(x)); // row_mirror
+    return x;
+}
+
+// a / b, rounded to nearest, from y = RN(1 / b) and one correction by the exact residual (Markstein): the correctly
+// rounded quotient, as the division gives it, where no step overflows.
+__device__ __forceinline__ float quotient(float a, float b, float y) {
+    const float q = a * y;
+    return fmaf(fmaf(-q, b, a), y, q);
+}
+
+// Codes of a lane's eight channels, each with kCodeCarry; scale and minimum of their group in every lane.  The codes of
+// a group share the reciprocal of the scale.  A range beyond float32's is cut to its largest number, whose quotient
+// clamps to 15 as the infinite one does.  Adding 2^23 rounds to an integer, half to even, in the lower bits.
+constexpr uint32_t kCodeCarry = 0x4B000000u;
+template <int GROUP, int Dt>
 __device__ __forceinline__ void quantise8(const float (&x)[8], uint32_t (&code)[8], float& s, float& lo) {
     lo = x[0];
     float hi = x[0];
 #pragma unroll
     for (int e = 1; e < 8; ++e) { lo = fminf(lo, x[e]); hi = fmaxf(hi, x[e]); }
-#pragma unroll
-    for (int m = 1; m < GROUP / 8; m <<= 1) {
-        lo = fminf(lo, __shfl_xor(lo, m, kWave));
-        hi = fmaxf(hi, __shfl_xor(hi, m, kWave));
-    }
-    s = fminf(fmaxf((hi - lo) / 15.f, 1e-5f), 1e5f);
+    lo = lanes_min<GROUP / 8>(lo);
+    hi = -lanes_min<GROUP / 8>(-hi);
+    constexpr float kMost = 3.40282347e38f;
+    s = __builtin_amdgcn_fmed3f(quotient(fminf(hi - lo, kMost), 15.f, 1.f / 15.f), 1e-5f, 1e5f);
     const float y = 1.f / s;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const float d = fminf(x[e] - lo, 3.40282347e38f), q0 = d * y, q = fmaf(fmaf(-q0, s, d), y, q0);
-        code[e] = __float_as_uint(__builtin_amdgcn_fmed3f(q, 0.f, 15.f) + 8388608.f) & 15u;
+        const float d = Dt == LF_FP16 ? x[e] - lo : fminf(x[e] - lo, kMost);
+        code[e] = __float_as_uint(__builtin_amdgcn_fmed3f(quotient(d, s, y), 0.f, 15.f) + 8388608.f);
     }
+}
+// The sum of kCodeCarry << (step e), e = 0 .. n - 1: what a word of n codes added up in their places carries too much.
+constexpr uint32_t carried(int n, int step) {
+    uint32_t c = 0;
+    for (int e = 0; e < n; ++e) c += kCodeCarry << (step * e);
+    return c;
 }
 
 // Four Value words from eight tokens' codes of four channels, a byte each: word c's nibble e is byte c of tok[e].
@@ -101,7 +128,8 @@ __device__ __forceinline__ u32x4 value_words(const uint32_t (&tok)[8]) {
 }
 
 // Tokens t0 .. t1 - 1 of a record, from source rows src0 .. of (b, h); one wave.  ``codes``: its 32 x D bytes of LDS.
-// Whole: all 32, every row's load on its way before the first is used.
+// Whole: all 32, of rows that start on 16 bytes, every row's load on its way before the first is used (a branch around
+// each load, for rows that do not, made each wait for the one before).
 template <int D, int GROUP, int Dt, bool Whole>
 __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int src0, int t0, int t1, uint8_t* codes) {
     using R = Int4Rec<D, GROUP>;
@@ -115,30 +143,40 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
 #pragma unroll
         for (int u = 0; u < D / 64; ++u) old[u] = vw[u * kWave];
     const auto load = [&](int kv, int row) {
-        return load8<Dt>(a.src[kv], b * a.sb[kv] + h * a.sh[kv] + 8 * w + (src0 + static_cast<int64_t>(row) - t0) * a.st[kv], a.vec);
+        return load8<Dt>(a.src[kv], b * a.sb[kv] + h * a.sh[kv] + 8 * w + (src0 + static_cast<int64_t>(row) - t0) * a.st[kv], Whole || a.vec);
     };
     const auto take = [&](int kv, int row, const Raw8<Dt>& raw, bool real) {
         float x[8], s, lo;
         widen8<Dt>(raw, x);
         uint32_t code[8];
-        quantise8<GROUP>(x, code, s, lo);
+        quantise8<GROUP, Dt>(x, code, s, lo);
         if (!real) return;
         uint32_t* sm = reinterpret_cast<uint32_t*>(rec + (kv ? R::vsm : R::ksm));
         if (w % (GROUP / 8) == 0)
             sm[w / (GROUP / 8) * kBlock + row] = f32_to_f16(s) | static_cast<uint32_t>(f32_to_f16(lo)) << 16;
         if (kv == 0) {
-            uint32_t word = 0;
+            uint32_t word = -carried(8, 4);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) word |= code[e] << (4 * e);
+            for (int e = 0; e < 8; ++e) word += code[e] << (4 * e);
             words[row * LR + key_word(D, w)] = turn(word, 29);
         } else {
-            u32x2 packed = {0, 0};
+            u32x2 packed = {-carried(4, 8), -carried(4, 8)};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) packed[e >> 2] |= code[e] << (8 * (e & 3));
+            for (int e = 0; e < 8; ++e) packed[e >> 2] += code[e] << (8 * (e & 3));
             *reinterpret_cast<u32x2*>(codes + row * D + 8 * w) = packed;
         }
     };
-    if constexpr (Whole) {
+    if constexpr (Whole && Dt != LF_FP32 && Passes <= 8) {
+        Raw8<Dt> raw[2][Passes];
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int p = 0; p < Passes; ++p) raw[kv][p] = load(kv, p * RP + lane / LR);
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int p = 0; p < Passes; ++p) take(kv, p * RP + lane / LR, raw[kv][p], true);
+    } else if constexpr (Whole) {
         constexpr int Ahead = Dt == LF_FP32 || Passes > 8 ? 4 : 8;  // rows on their way
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv)
@@ -267,7 +305,7 @@ __global__ __launch_bounds__(256) void int4_append_pages_kernel(RowsArgs a) {
         const int t0 = max(lo - k0, 0), t1 = min(hi - k0, kBlock);
         if (t0 >= t1) continue;
         uint8_t* rec = int4_block(a.L, b, h, k0 / kBlock, Int4Rec<D, GROUP>::bytes);
-        if (t1 - t0 == kBlock) write_block<D, GROUP, Dt, true>(a, rec, b, h, k0 - start, 0, kBlock, lds + wave * kBlock * D);
+        if (t1 - t0 == kBlock && a.vec) write_block<D, GROUP, Dt, true>(a, rec, b, h, k0 - start, 0, kBlock, lds + wave * kBlock * D);
         else write_block<D, GROUP, Dt, false>(a, rec, b, h, k0 + t0 - start, t0, t1, lds + wave * kBlock * D);
     }
     if (hi < p0 + P) return;
