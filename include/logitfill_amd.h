@@ -388,10 +388,12 @@ int32_t lf_unpack_ints(const int32_t* words, int64_t rows, int32_t n_words, int3
  *                                             64 s + 4 c + t, with groups of 32 64 s + 32 (t / 2) + 2 c + t % 2
  *     Key scale, min fp16 [head_dim / group][32][2]
  *     Value scale, min fp16 [head_dim / group][32][2]
- *   A code word's nibble e is in bits (4 e + 3) % 32 .. of the word: the word rotated left by 3.
+ *   A Key word's nibble e is in bits (4 e + 3) % 32 .. of the word, a Value word's in bits (4 e + 6) % 32 ..: the
+ *   words rotated left by 3 and by 6.
  * ``bounds``: bf16 [batch][n_kv][cap_tokens / page_size][2][head_dim], every full page's smallest and
  * largest Key per channel (of the values read back), rounded outward (infinities: bf16's largest number).  ``lens``: DEVICE int32 [batch],
- * the sequences' tokens; the write position never leaves the device.
+ * the sequences' tokens; the write position never leaves the device.  ``tops``: fp16 [batch][n_kv][cap_tokens / 32],
+ * every record's largest Value scale (or more: of rows that were taken back).
  *
  * head_dim 64, 128 or 256; group 32, 64 or 128, at most head_dim; page_size a multiple of 32 up to 1024;
  * cap_tokens a multiple of page_size; blocks and bounds 16-byte aligned (others: LF_E_UNSUPPORTED or
@@ -401,6 +403,7 @@ typedef struct lf_int4_layer {
     uint8_t* blocks;
     uint16_t* bounds;
     int32_t* lens;
+    uint16_t* tops;
     int32_t batch, n_kv, head_dim;
     int32_t cap_tokens, page_size, group;
 } lf_int4_layer;

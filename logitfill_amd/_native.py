@@ -99,7 +99,7 @@ class Int4Layer(ctypes.Structure):
     """``lf_int4_layer``."""
 
     _fields_ = [
-        ("blocks", c_void_p), ("bounds", c_void_p), ("lens", c_void_p),
+        ("blocks", c_void_p), ("bounds", c_void_p), ("lens", c_void_p), ("tops", c_void_p),
         ("batch", c_int32), ("n_kv", c_int32), ("head_dim", c_int32),
         ("cap_tokens", c_int32), ("page_size", c_int32), ("group", c_int32),
     ]

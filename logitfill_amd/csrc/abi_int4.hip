@@ -23,7 +23,7 @@ bool valid_dtype(int32_t d) { return d == LF_BF16 || d == LF_FP16 || d == LF_FP3
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 int32_t check_int4(const lf_int4_layer* L) {
-    if (!L || !L->blocks || !L->bounds || !L->lens) return LF_E_NULL;
+    if (!L || !L->blocks || !L->bounds || !L->lens || !L->tops) return LF_E_NULL;
     if (L->batch <= 0 || L->n_kv <= 0 || L->batch > kGrid || L->n_kv > kGrid) return LF_E_SHAPE;
     if (L->head_dim != 64 && L->head_dim != 128 && L->head_dim != 256) return LF_E_UNSUPPORTED;
     if ((L->group != 32 && L->group != 64 && L->group != 128) || L->group > L->head_dim) return LF_E_UNSUPPORTED;

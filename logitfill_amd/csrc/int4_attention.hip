@@ -7,11 +7,14 @@
 // A score's lane holds the tokens of exactly the P' operand its lane of the second product needs (Value words hold
 // eight tokens of a channel in that order), so nothing is exchanged between the two products.
 //
-// Codes enter as bf16 16 + code (one and-or per pair); the 16 is taken out of the scores by the accumulator's start
-// value, -16 sum(q_g), and out of the output by a product of P' with a constant.  Queries are split into bf16 parts
-// that add up to them exactly (bf16 one, fp16 two, fp32 three).  P' is rounded to as many parts as the output's
-// type asks for; the codes count from their middle, 7.5, there (sum p (min + 7.5 scale) is kept in fp32), so that a
-// rounding of P' weighs as the code's distance from it.
+// Codes enter as 16 + code, Keys' in bf16 and Values' in fp16 (one and-or per pair); the 16 is taken out of the scores
+// by the accumulator's start value, -16 sum(q_g), and out of the output by a product of P' with a constant.  Queries are
+// split into bf16 parts that add up to them exactly (bf16 one, fp16 two, fp32 three).  P' is rounded to fp16, in as many
+// parts as the output's type asks for (one, two, two); the codes count from their middle, 7.5, there (sum p (min +
+// 7.5 scale) is kept in fp32), so that a rounding of P' weighs as the code's distance from it.  In one part of bf16 the
+// roundings of P' were as large as the bf16 output's own (rel. error 2.4e-3 to 2.7e-3 against 1.7e-3); fp16's eight times
+// smaller ones need P' in its range: the reference point is moved by log2 of the largest Value scale of the wave's records
+// (tops), so that P' stays below 2^15.
 //
 // A workgroup's four waves take the records of its split in turn, each with its own running reference point and
 // sums, merged through LDS at the end; several splits of a sequence are merged by int4_merge_kernel.  The
@@ -58,6 +61,37 @@ __device__ __forceinline__ Parts<NT> split(const float (&a)[4], const float (&b)
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Element pairs (a[i], b[i]) in NP fp16 parts, each rounded to nearest.
+template <int NP>
+struct Weights {
+    f16x8 t[NP];
+};
+template <int NP>
+__device__ __forceinline__ Weights<NP> weights(const float (&a)[4], const float (&b)[4]) {
+    Weights<NP> r;
+    float x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { x[i] = a[i]; y[i] = b[i]; }
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = pack_f16(x[i], y[i]);
+            if (n + 1 < NP) {
+                const uint32_t pair = w[i];
+                x[i] -= pair_scale(pair);
+                y[i] -= pair_min(pair);  // (the pair's upper half)
+            }
+        }
+        r.t[n] = __builtin_bit_cast(f16x8, w);
+    }
+    return r;
+}
 
 // LDS reads stay behind this point: hoisted all to a record's start they take more registers than three waves a
 // SIMD leave.
@@ -95,7 +129,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     using R = Int4Rec<D, GROUP>;
     using S = Ring<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
-    constexpr int NT = Dt == LF_BF16 ? 1 : Dt == LF_FP16 ? 2 : 3;
+    constexpr int NT = Dt == LF_BF16 ? 1 : Dt == LF_FP16 ? 2 : 3, NP = Dt == LF_BF16 ? 1 : 2;  // parts of q and of P'
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float lds_ml[kWaves][kTile][2];
     int32_t* lds_pages = reinterpret_cast<int32_t*>(smem + S::lds);  // with pages only
@@ -180,6 +214,21 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         if (k < count) fill(k, k);
     if (ahead && count == 0) wait_ring<0>();
 
+    // The weights are 2^(score - ref) with ref = largest score + lift: P' <= 2^8 2^-lift scale < 2^15 for this wave's
+    // records, whose largest Value scales lie below 2^(lift + 7).
+    uint32_t most_scale = 0;
+    for (int k = lane; k < count; k += kWave) {
+        int block = first + wave + k * kWaves;
+        if (a.n_pages) {
+            const int e = block / per_page, page = lds_pages[e - first / per_page];
+            block = max(page, 0) * per_page + (block - e * per_page);
+        }
+        most_scale = max(most_scale, static_cast<uint32_t>(*int4_top(a.L, b, h, block)));
+    }
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) most_scale = max(most_scale, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most_scale), m, kWave)));
+    const float lift = static_cast<float>(static_cast<int>(__float_as_uint(f16_to_f32(static_cast<uint16_t>(most_scale))) >> 23) - 126 - 7);
+
     Parts<NT> q[CH];
     float qsum[G];
     const bool flip = a.qscale < 0.f;  // a negative scale goes into the queries: scores are then compared unscaled
@@ -200,9 +249,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
 #pragma unroll
     for (int g = 0; g < G; ++g) qsum[g] = rows_sum(qsum[g]);
 
-    const uint32_t code_base = in_vgpr(kCodeBase);
-    constexpr uint32_t kMiddle = 0xC1BCC1BCu;  // bf16 -23.5: the bias of the codes and their middle
-    const bf16x8 middle = __builtin_bit_cast(bf16x8, u32x4{kMiddle, kMiddle, kMiddle, kMiddle});
+    const uint32_t key_base = in_vgpr(kKeyBase), value_base = in_vgpr(kValueBase);
+    constexpr uint32_t kMiddle = 0xCDE0CDE0u;  // fp16 -23.5: the bias of the codes and their middle
+    const f16x8 middle = __builtin_bit_cast(f16x8, u32x4{kMiddle, kMiddle, kMiddle, kMiddle});
     f32x4 o[VT], fix[G];
     float pm[G], l = 0.f, ref = 0.f, limit = -__builtin_inff();
 #pragma unroll
@@ -230,7 +279,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
                 f32x4 acc = {start, start, start, start};
 #pragma unroll
                 for (int c = g * CG; c < (g + 1) * CG; ++c) {
-                    const bf16x8 codes = codes8(kw[c], code_base);
+                    const bf16x8 codes = __builtin_bit_cast(bf16x8, codes8<kKeyMask>(kw[c], key_base));
 #pragma unroll
                     for (int m = NT - 1; m >= 0; --m) acc = mfma(codes, q[c].t[m], acc);
                 }
@@ -252,8 +301,8 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         if (__any(most > limit)) {
             most = rows_max(most);
             const bool moves = most > limit;
-            const float scale = !moves ? 1.f : limit == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - most);
-            if (moves) { ref = most; limit = most + 8.f; }
+            const float scale = !moves ? 1.f : limit == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - most - lift);
+            if (moves) { ref = most + lift; limit = most + 8.f; }
             l *= scale;
 #pragma unroll
             for (int g = 0; g < G; ++g) { pm[g] *= scale; fix[g] *= scale; }
@@ -288,14 +337,14 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
                     pm[g] = fmaf(p[t][r], pair_min(pair[t][r]), pm[g]);
                     pm[g] = fmaf(7.5f, x[t][r], pm[g]);
                 }
-            const Parts<NT> w = split<NT>(x[0], x[1]);
+            const Weights<NP> w = weights<NP>(x[0], x[1]);
 #pragma unroll
-            for (int m = NT - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
+            for (int m = NP - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
 #pragma unroll
             for (int t = g * TG; t < (g + 1) * TG; ++t) {
-                const bf16x8 codes = codes8(vw[(t >> 2) * kWave][t & 3], code_base);
+                const f16x8 codes = __builtin_bit_cast(f16x8, codes8<kValueMask>(vw[(t >> 2) * kWave][t & 3], value_base));
 #pragma unroll
-                for (int m = NT - 1; m >= 0; --m) o[t] = mfma(codes, w.t[m], o[t]);
+                for (int m = NP - 1; m >= 0; --m) o[t] = mfma(codes, w.t[m], o[t]);
             }
             phase();
         }

@@ -8,6 +8,7 @@ namespace lf {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
@@ -25,11 +26,13 @@ struct Int4Rec {
     static_assert(bytes == LF_INT4_BLOCK_BYTES(D, GROUP), "record size");
 };
 
-// Nibble e of a code word is in bits 4 e + 3 .. 4 e + 6, the last one wrapping to bits 31, 0, 1, 2: with the
-// word turned by 4 e bits, nibbles e and e + 4 are the upper four mantissa bits of the bf16 halves
-// 0x4180 | code << 3 = 16 + code, without a shift of their own.
+// Nibble e of a Key word is in bits 4 e + 3 .. of it, of a Value word in bits 4 e + 6 .., the last one's upper bits
+// wrapping to the lowest: with the word turned by 4 e bits, nibbles e and e + 4 are the upper four mantissa bits of the
+// bf16 halves 0x4180 | code << 3 or the fp16 halves 0x4C00 | code << 6, 16 + code, without a shift of their own.
+constexpr int kKeyTurn = 3, kValueTurn = 6;
 __device__ __forceinline__ uint32_t turn(uint32_t w, int bits) { return __builtin_amdgcn_alignbit(w, w, bits); }
-__device__ __forceinline__ uint32_t code_at(uint32_t w, int e) { return turn(w, (4 * e + 3) & 31) & 15u; }
+template <int Turn>
+__device__ __forceinline__ uint32_t code_at(uint32_t w, int e) { return turn(w, (4 * e + Turn) & 31) & 15u; }
 
 // A constant in a vector register: the and-or of a code's pair takes one literal-free scalar and vector operands (with
 // both as literals it is an and, then an or).
@@ -38,14 +41,13 @@ __device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
     return x;
 }
 
-// A word's eight codes as bf16 16 + code; element 2 i is nibble i, element 2 i + 1 nibble i + 4.  ``base``: kCodeBase
-// in a vector register.
+// A Key word's eight codes as bf16, a Value word's as fp16 16 + code; element 2 i is nibble i, element 2 i + 1 nibble
+// i + 4.  ``base``: kKeyBase or kValueBase in a vector register.
 constexpr float kCodeBias = 16.f;
-constexpr uint32_t kCodeBase = 0x41804180u;
-__device__ __forceinline__ bf16x8 codes8(uint32_t w, uint32_t base) {
-    constexpr uint32_t mask = 0x00780078u;
-    return __builtin_bit_cast(bf16x8, u32x4{(w & mask) | base, (turn(w, 4) & mask) | base, (turn(w, 8) & mask) | base,
-                                            (turn(w, 12) & mask) | base});
+constexpr uint32_t kKeyBase = 0x41804180u, kValueBase = 0x4C004C00u, kKeyMask = 0x00780078u, kValueMask = 0x03C003C0u;
+template <uint32_t Mask>
+__device__ __forceinline__ u32x4 codes8(uint32_t w, uint32_t base) {
+    return u32x4{(w & Mask) | base, (turn(w, 4) & Mask) | base, (turn(w, 8) & Mask) | base, (turn(w, 12) & Mask) | base};
 }
 
 // Where a Key row's word w (channels 8 w .. 8 w + 7) stands in it.
@@ -67,7 +69,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    return f32_to_f16(a) | static_cast<uint32_t>(f32_to_f16(b)) << 16;
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
 }
 
 // N (2, 4 or 8) floats to consecutive elements, rounded to nearest.
@@ -92,6 +95,10 @@ __device__ __forceinline__ void store_row(void* p, int64_t at, const float (&x)[
 // Record ``block`` of (sequence b, kv head h).
 __device__ __forceinline__ uint8_t* int4_block(const lf_int4_layer& L, int b, int h, int block, int bytes) {
     return L.blocks + ((static_cast<int64_t>(b) * L.n_kv + h) * (L.cap_tokens / kBlock) + block) * bytes;
+}
+
+__device__ __forceinline__ uint16_t* int4_top(const lf_int4_layer& L, int b, int h, int block) {
+    return L.tops + (static_cast<int64_t>(b) * L.n_kv + h) * (L.cap_tokens / kBlock) + block;
 }
 
 __device__ __forceinline__ int int4_len(const lf_int4_layer& L, int b) {

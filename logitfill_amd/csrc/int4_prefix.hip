@@ -16,8 +16,6 @@
 namespace lf {
 namespace {
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr int kWaves = 4, kTile = 16, MT = kManyRows / (kWaves * kTile);  // row tiles of a wave
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
@@ -26,14 +24,18 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 __device__ __forceinline__ uint32_t lower_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t upper_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// A word's eight codes times s[i] plus m[i], element pairs (nibble i, nibble i + 4): the fp16 bits 0x5800 | code << 3
-// are 128 + code.
+// A word's eight codes times s[i] plus m[i], element pairs (nibble i, nibble i + 4).  The fp16 bits of a Key word's,
+// 0x5800 | code << 3, are 128 + code; of a Value word's, 0x4C00 | code << 6, 16 + code.
+constexpr uint32_t kWideBase = 0x58005800u;
+template <uint32_t Mask>
 __device__ __forceinline__ u32x4 dequant8(uint32_t w, const uint32_t (&s)[4], const uint32_t (&m)[4], uint32_t base) {
+    constexpr _Float16 bias = static_cast<_Float16>(Mask == kKeyMask ? 128 : 16);
+    const u32x4 bits = codes8<Mask>(w, base);
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = ((i ? turn(w, 4 * i) : w) & 0x00780078u) | base;
-        const f16x2 code = __builtin_bit_cast(f16x2, bits) - f16x2{static_cast<_Float16>(128), static_cast<_Float16>(128)};
+        const uint32_t pair = bits[i];
+        const f16x2 code = __builtin_bit_cast(f16x2, pair) - f16x2{bias, bias};
         r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, m[i])));
     }
     return r;
@@ -57,7 +59,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
     const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
     constexpr int VW = VT / 2;                          // a lane's Value words
     constexpr int VG = GROUP == 32 ? VW / 2 : 1;        // and the groups they lie in
-    const uint32_t code_base = in_vgpr(0x58005800u);
+    const uint32_t code_base = in_vgpr(wave < 2 ? kWideBase : kValueBase);  // (a wave stages Keys or Values)
     // Every wave loads the same pieces, whichever it stages: with a branch around the loads, what it joins waited for them.
     struct Raw {
         uint32_t w[4];
@@ -93,7 +95,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
             for (int c = 0; c < CH; ++c) {
                 const uint32_t pair = r.key[c / (CH / G)], s = lower_pair(pair, pair), m = upper_pair(pair, pair);
                 const uint32_t ss[4] = {s, s, s, s}, mm[4] = {m, m, m, m};
-                to[(half * CH + c) * kWave + lane] = dequant8(r.w[c], ss, mm, code_base);
+                to[(half * CH + c) * kWave + lane] = dequant8<kKeyMask>(r.w[c], ss, mm, code_base);
             }
         } else {
 #pragma unroll
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
                 }
 #pragma unroll
                 for (int c = k * (VW / VG); c < (k + 1) * (VW / VG); ++c)
-                    to[kK + (half * VW + c) * kWave + lane] = dequant8(r.w[c], s, m, code_base);
+                    to[kK + (half * VW + c) * kWave + lane] = dequant8<kValueMask>(r.w[c], s, m, code_base);
             }
         }
     };

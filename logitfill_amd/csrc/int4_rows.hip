@@ -124,14 +124,15 @@ __device__ __forceinline__ u32x4 value_words(const uint32_t (&tok)[8]) {
     const uint32_t c = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u), d = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
     const u32x4 w = {__builtin_amdgcn_perm(b, a, 0x05040100u), __builtin_amdgcn_perm(b, a, 0x07060302u),
                      __builtin_amdgcn_perm(d, c, 0x05040100u), __builtin_amdgcn_perm(d, c, 0x07060302u)};
-    return u32x4{turn(w[0], 29), turn(w[1], 29), turn(w[2], 29), turn(w[3], 29)};
+    constexpr int left = 32 - kValueTurn;
+    return u32x4{turn(w[0], left), turn(w[1], left), turn(w[2], left), turn(w[3], left)};
 }
 
-// Tokens t0 .. t1 - 1 of a record, from source rows src0 .. of (b, h); one wave.  ``codes``: its 32 x D bytes of LDS.
-// Whole: all 32, of rows that start on 16 bytes, every row's load on its way before the first is used (a branch around
+// Tokens t0 .. t1 - 1 of a record, from source rows src0 .. of (b, h); one wave.  ``codes``: its 32 x D bytes of LDS;
+// ``most``: the record's largest Value scale.  Whole: all 32, of rows that start on 16 bytes, every row's load on its way before the first is used (a branch around
 // each load, for rows that do not, made each wait for the one before).
 template <int D, int GROUP, int Dt, bool Whole>
-__device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int src0, int t0, int t1, uint8_t* codes) {
+__device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int b, int h, int src0, int t0, int t1, uint8_t* codes, uint16_t* most) {
     using R = Int4Rec<D, GROUP>;
     constexpr int LR = D / 8, RP = kWave / LR, Passes = kBlock / RP;  // lanes per row, rows per pass
     const int lane = threadIdx.x & (kWave - 1), w = lane % LR;
@@ -145,6 +146,7 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
     const auto load = [&](int kv, int row) {
         return load8<Dt>(a.src[kv], b * a.sb[kv] + h * a.sh[kv] + 8 * w + (src0 + static_cast<int64_t>(row) - t0) * a.st[kv], Whole || a.vec);
     };
+    uint32_t top = Whole || t0 == 0 ? 0 : *most;  // (fp16 numbers above zero are ordered as their bits)
     const auto take = [&](int kv, int row, const Raw8<Dt>& raw, bool real) {
         float x[8], s, lo;
         widen8<Dt>(raw, x);
@@ -154,11 +156,12 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
         uint32_t* sm = reinterpret_cast<uint32_t*>(rec + (kv ? R::vsm : R::ksm));
         if (w % (GROUP / 8) == 0)
             sm[w / (GROUP / 8) * kBlock + row] = f32_to_f16(s) | static_cast<uint32_t>(f32_to_f16(lo)) << 16;
+        if (kv) top = max(top, static_cast<uint32_t>(f32_to_f16(s)));
         if (kv == 0) {
             uint32_t word = -carried(8, 4);
 #pragma unroll
             for (int e = 0; e < 8; ++e) word += code[e] << (4 * e);
-            words[row * LR + key_word(D, w)] = turn(word, 29);
+            words[row * LR + key_word(D, w)] = turn(word, 32 - kKeyTurn);
         } else {
             u32x2 packed = {-carried(4, 8), -carried(4, 8)};
 #pragma unroll
@@ -198,12 +201,16 @@ __device__ __forceinline__ void write_block(const RowsArgs& a, uint8_t* rec, int
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+    top = min(top, 0x7bffu);  // (an infinite scale counts as the largest)
+#pragma unroll
+    for (int m = 1; m < kWave; m <<= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), m, kWave)));
+    if (lane == 0) *most = static_cast<uint16_t>(top);
     uint32_t fresh = 0;  // the nibbles this write replaces
     if constexpr (!Whole)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int tok = 4 * quad + (e & 3) + 16 * (e >> 2);
-            if (tok >= t0 && tok < t1) fresh |= turn(15u << (4 * e), 29);
+            if (tok >= t0 && tok < t1) fresh |= turn(15u << (4 * e), 32 - kValueTurn);
         }
 #pragma unroll
     for (int u = 0; u < D / 64; ++u) {
@@ -255,7 +262,7 @@ __device__ void page_bounds(const lf_int4_layer& L, int b, int h, int page, int 
         const float s = pair_scale(sm), m = pair_min(sm);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float x = fmaf(static_cast<float>(code_at(word, e)), s, m);
+            const float x = fmaf(static_cast<float>(code_at<kKeyTurn>(word, e)), s, m);
             lo[e] = fminf(lo[e], x);
             hi[e] = fmaxf(hi[e], x);
         }
@@ -305,13 +312,14 @@ __global__ __launch_bounds__(256) void int4_append_pages_kernel(RowsArgs a) {
         const int t0 = max(lo - k0, 0), t1 = min(hi - k0, kBlock);
         if (t0 >= t1) continue;
         uint8_t* rec = int4_block(a.L, b, h, k0 / kBlock, Int4Rec<D, GROUP>::bytes);
-        if (t1 - t0 == kBlock && a.vec) write_block<D, GROUP, Dt, true>(a, rec, b, h, k0 - start, 0, kBlock, lds + wave * kBlock * D);
-        else write_block<D, GROUP, Dt, false>(a, rec, b, h, k0 + t0 - start, t0, t1, lds + wave * kBlock * D);
+        if (t1 - t0 == kBlock && a.vec) write_block<D, GROUP, Dt, true>(a, rec, b, h, k0 - start, 0, kBlock, lds + wave * kBlock * D, int4_top(a.L, b, h, k0 / kBlock));
+        else write_block<D, GROUP, Dt, false>(a, rec, b, h, k0 + t0 - start, t0, t1, lds + wave * kBlock * D, int4_top(a.L, b, h, k0 / kBlock));
     }
-    if (hi < p0 + P) return;
-    __threadfence_block();
-    __syncthreads();
-    page_bounds<D, GROUP>(a.L, b, h, page, threadIdx.x, blockDim.x, reinterpret_cast<float*>(lds));
+    if (hi == p0 + P) {
+        __threadfence_block();
+        __syncthreads();
+        page_bounds<D, GROUP>(a.L, b, h, page, threadIdx.x, blockDim.x, reinterpret_cast<float*>(lds));
+    }
 }
 
 __global__ void int4_advance_kernel(RowsArgs a) {
@@ -331,7 +339,7 @@ __global__ __launch_bounds__(512) void int4_append_few_kernel(RowsArgs a) {
         for (int k = start / kBlock; k * kBlock < end; ++k) {
             const int t0 = max(start - k * kBlock, 0), t1 = min(end - k * kBlock, kBlock);
             write_block<D, GROUP, Dt, false>(a, int4_block(a.L, b, h, k, Int4Rec<D, GROUP>::bytes), b, h,
-                                             k * kBlock + t0 - start, t0, t1, lds + wave * kBlock * D);
+                                             k * kBlock + t0 - start, t0, t1, lds + wave * kBlock * D, int4_top(a.L, b, h, k));
         }
     __threadfence_block();
     __syncthreads();  // every wave has read the length, and its rows are there
@@ -392,7 +400,7 @@ __device__ __forceinline__ void read_record(const ReadArgs& a, const uint8_t* re
             const int row = p * RP + lane / LR;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = Whole || row < seen ? fmaf(static_cast<float>(code_at(word[p], e)), pair_scale(key[p]), pair_min(key[p])) : 0.f;
+            for (int e = 0; e < 8; ++e) x[e] = Whole || row < seen ? fmaf(static_cast<float>(code_at<kKeyTurn>(word[p], e)), pair_scale(key[p]), pair_min(key[p])) : 0.f;
             if (Whole || (row >= from && row < to)) store_row<Dt>(a.out[0], dst + row * D + 8 * w, x);
         }
     if (a.out[1])
@@ -406,7 +414,7 @@ __device__ __forceinline__ void read_record(const ReadArgs& a, const uint8_t* re
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     const uint32_t pair = pairs[u][e >> 2][t >> 1][e & 3];
-                    x[t] = Whole || row < seen ? fmaf(static_cast<float>(code_at(values[u][t], e)), pair_scale(pair), pair_min(pair)) : 0.f;
+                    x[t] = Whole || row < seen ? fmaf(static_cast<float>(code_at<kValueTurn>(values[u][t], e)), pair_scale(pair), pair_min(pair)) : 0.f;
                 }
                 if constexpr (GROUP == 32) {
                     const float a0[2] = {x[0], x[1]}, a1[2] = {x[2], x[3]};

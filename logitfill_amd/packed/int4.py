@@ -106,6 +106,7 @@ class _Int4Store:
         with torch.inference_mode(False):
             self._lens = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
         self._dirty = False  # the device's lengths are behind the host's
+        self._tops: Optional[torch.Tensor] = None
         if capacity_tokens:
             self.reserve(capacity_tokens)
 
@@ -139,10 +140,13 @@ class _Int4Store:
             blocks = torch.zeros(B, H, cap // BLOCK, _block_bytes(D, self.group_size), dtype=torch.uint8,
                                  device=self.device)
             bounds = torch.zeros(B, H, cap // P, 2, D, dtype=torch.bfloat16, device=self.device)
+            tops = torch.zeros(B, H, cap // BLOCK, dtype=torch.float16, device=self.device)
             if self._cap:
+                tops[:, :, : self._cap // BLOCK].copy_(self._tops)
                 blocks[:, :, : self._cap // BLOCK].copy_(self._blocks)
                 bounds[:, :, : self._cap // P].copy_(self._bounds)
-        self._blocks, self._bounds, self._cap, self._struct = blocks, bounds, cap, None
+        self._blocks, self._bounds, self._tops = blocks, bounds, tops
+        self._cap, self._struct = cap, None
 
     def layer_struct(self, lengths: bool = True) -> _native.Int4Layer:
         """The ``lf_int4_layer`` describing this store; ``lengths``: the device's up to date on the current stream."""
@@ -151,6 +155,7 @@ class _Int4Store:
         if self._struct is None:
             s = _native.Int4Layer()
             s.blocks, s.bounds, s.lens = self._blocks.data_ptr(), self._bounds.data_ptr(), self._lens.data_ptr()
+            s.tops = self._tops.data_ptr()
             s.batch, s.n_kv, s.head_dim = self.batch, self.n_kv, self.head_dim
             s.cap_tokens, s.page_size, s.group = self._cap, self.page_size, self.group_size
             self._struct = s

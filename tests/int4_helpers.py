@@ -9,8 +9,8 @@ from tests.helpers import f32
 
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 HALF_STEP = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -11, "fp32": 2.0 ** -24}
-# P' = p * scale is kept in one, two and three bf16 parts; all but the last are cut off (2^-7), that is rounded
-WEIGHT_STEP = {"bf16": 2.0 ** -8, "fp16": 2.0 ** -15, "fp32": 2.0 ** -22}
+# P' = p * scale is kept in one, two and two fp16 parts, each rounded
+WEIGHT_STEP = {"bf16": 2.0 ** -11, "fp16": 2.0 ** -22, "fp32": 2.0 ** -22}
 
 
 def rows(shape, dtype: str, seed: int):
@@ -45,11 +45,13 @@ def many_rows_bound(q, k, v, scaling):
     return (2 * d + 3 * 2.0 ** -11) * np.abs(v).max() + 2.0 ** -25
 
 
-def attention_bound(q, k_size, v_size, scaling, ref, dtype: str, smax: float):
+def attention_bound(q, k_size, v_size, scaling, ref, dtype: str, smax: float, top: float):
     """Largest admitted |out - ref| per element of ``ref [rows, D]``.
 
     * the output's rounding;
-    * a rounding of P' = p * scale moves the output by at most that step times scale * |code - 7.5|;
+    * a rounding of P' = p * scale moves the output by at most that step times scale * |code - 7.5|, and by
+      2^-25 times 7.5 over the sum of the weights where P' is subnormal: the weights' largest is at least
+      2^7 over the largest scale of a record, ``top`` where rows of it were taken back;
     * float32: a score's term passes 5 sums inside a product of 32, one per product and part, two per
       group, each off by 2^-24 of sum |q| (|k| + 32 scale); the exponential is off by 2^-20; a score off by
       d moves the weights by a factor e^d above and below the quotient; the Value sums pass T / 32
@@ -63,13 +65,13 @@ def attention_bound(q, k_size, v_size, scaling, ref, dtype: str, smax: float):
     size = (np.abs(q).astype(np.float64) @ k_size.T).max(-1, keepdims=True)
     d = abs(scaling) * steps * 2.0 ** -24 * size + 2.0 ** -20
     reach = v_size.max()
-    return (HALF_STEP[dtype] * np.abs(ref) + WEIGHT_STEP[dtype] * 7.5 * smax + 2 * d * reach
+    return (HALF_STEP[dtype] * np.abs(ref) + 7.5 * (WEIGHT_STEP[dtype] * smax + T * 2.0 ** -32 * top) + 2 * d * reach
             + (T / 32 + 40) * 2.0 ** -23 * reach)
 
 
-def expected(q, key, value, lengths, group: int, scaling: float, dtype: str, *, page=0, pages=None, q_lens=None):
+def expected(q, key, value, lengths, group: int, scaling: float, dtype: str, *, page=0, pages=None, q_lens=None, top=0.0):
     """Float64 output and its bound, ``[B, n_q, n, D]``: ``key/value [B, H, T, D]`` are the rows written, sequence b
-    holding the first ``lengths[b]``; with ``pages`` [B, H, n, K] the attended pages."""
+    holding the first ``lengths[b]`` (``top``: the largest Value scale of rows taken back); with ``pages`` [B, H, n, K] the attended pages."""
     qn, kn, vn = f32(q), f32(key), f32(value)
     B, n_q, n, D = qn.shape
     H = kn.shape[1]
@@ -96,7 +98,8 @@ def expected(q, key, value, lengths, group: int, scaling: float, dtype: str, *, 
                 head = slice(h * g, (h + 1) * g)
                 r = o4.attend(qn[b, head, j], k, v, scaling, np.broadcast_to(seen, (g, total)))
                 out[b, head, j] = r
-                tol[b, head, j] = attention_bound(qn[b, head, j], k_size[seen], v_size[seen], scaling, r, dtype, smax)
+                tol[b, head, j] = attention_bound(qn[b, head, j], k_size[seen], v_size[seen], scaling, r, dtype, smax,
+                                                   max(smax, top))
                 if pages is None and g * n >= 64 and k.shape[-1] <= 128 and dtype != "fp32":
                     tol[b, head, j] += many_rows_bound(qn[b, head, j], k[seen], v[seen], scaling)
     return out, tol

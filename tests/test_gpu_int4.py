@@ -272,6 +272,30 @@ def test_attention_sharp_and_flat(gpu, scaling):
     assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, scaling), ref, tol)
 
 
+@pytest.mark.parametrize("dtype,n", [("bf16", 1), ("fp16", 2), ("bf16", 40)])
+def test_values_of_any_size(gpu, dtype, n):
+    """Value rows of 2^-14 to 2^14, zeros among them, and rows as large that were taken back."""
+    D, group, T = 128, 64, 600
+    key, value = rows((1, 2, T, D), "fp32", 13)
+    size = torch.exp2(torch.randint(-14, 12, (T,), generator=torch.Generator().manual_seed(2)).float())
+    value = value * size[:, None]
+    value[:, :, ::7] = 0
+    key, value = key.to(TYPES[dtype]), value.to(TYPES[dtype])
+    q = query((1, 6, n, D), dtype, 13)
+    mgr = manager(gpu, D, group, 64, 6, 2)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    ref, tol = expected(q, key, value, [T], group, D ** -0.5, dtype)
+    assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol)
+    top = float(o4.quantise(f32(value), group)[1].max())
+    small = value * (2.0 ** -10 / size[:, None].clamp(min=2.0 ** -10)).to(value.dtype)
+    for keep, s_top in ((1, top), (0, 0.0)):  # a row is left, and none
+        mgr.truncate(keep)
+        mgr.commit(0, key[:, :, keep:].to(gpu), small[:, :, keep:].to(gpu))
+        v = torch.cat([value[:, :, :keep], small[:, :, keep:]], 2)
+        ref, tol = expected(q, key, v, [T], group, D ** -0.5, dtype, top=s_top)
+        assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol)
+
+
 def test_growing_scores_move_the_reference_point(gpu):
     """Every record's scores pass the last one's by more than the step that moves the reference point."""
     D, T = 64, 700

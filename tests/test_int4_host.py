@@ -37,7 +37,7 @@ def test_struct_layouts_match_c(tmp_path):
 
 def _layer(**kw):
     L = _native.Int4Layer()
-    L.blocks, L.bounds, L.lens = AT, AT, AT
+    L.blocks, L.bounds, L.lens, L.tops = AT, AT, AT, AT
     L.batch, L.n_kv, L.head_dim, L.cap_tokens, L.page_size, L.group = 2, 4, 128, 1024, 128, 64
     for k, v in kw.items():
         setattr(L, k, v)
@@ -57,7 +57,7 @@ def _args(**kw):
 NULL, SHAPE, UNSUPPORTED, WORKSPACE, DTYPE = (_native.LF_E_NULL, _native.LF_E_SHAPE, _native.LF_E_UNSUPPORTED,
                                               _native.LF_E_WORKSPACE, _native.LF_E_DTYPE)
 BAD_LAYERS = [
-    ({"blocks": 0}, NULL), ({"bounds": 0}, NULL), ({"lens": 0}, NULL), ({"batch": 0}, SHAPE), ({"n_kv": 0}, SHAPE),
+    ({"blocks": 0}, NULL), ({"bounds": 0}, NULL), ({"lens": 0}, NULL), ({"tops": 0}, NULL), ({"batch": 0}, SHAPE), ({"n_kv": 0}, SHAPE),
     ({"batch": 65536}, SHAPE), ({"head_dim": 96}, UNSUPPORTED), ({"head_dim": 512}, UNSUPPORTED),
     ({"group": 16}, UNSUPPORTED), ({"group": 128, "head_dim": 64}, UNSUPPORTED), ({"page_size": 48}, SHAPE),
     ({"page_size": 2048, "cap_tokens": 4096}, SHAPE), ({"page_size": 0}, SHAPE), ({"cap_tokens": 1000}, SHAPE),
