@@ -9,18 +9,24 @@
 //
 // Codes enter as 16 + code, Keys' in bf16 and Values' in fp16 (one and-or per pair); the 16 is taken out of the scores
 // by the accumulator's start value, -16 sum(q_g), and out of the output by a product of P' with a constant.  Queries are
-// split into bf16 parts that add up to them exactly (bf16 one, fp16 two, fp32 three).  P' is rounded to fp16, in as many
+// split into bf16 parts that add up to them exactly (bf16 one, fp16 two).  P' is rounded to fp16, in as many
 // parts as the output's type asks for (one, two, two); the codes count from their middle, 7.5, there (sum p (min +
 // 7.5 scale) is kept in fp32), so that a rounding of P' weighs as the code's distance from it.  In one part of bf16 the
 // roundings of P' were as large as the bf16 output's own (rel. error 2.4e-3 to 2.7e-3 against 1.7e-3); fp16's eight times
 // smaller ones need P' in its range: the reference point is moved by log2 of the largest Value scale of the wave's records
 // (tops), so that P' stays below 2^15.
 //
+// float32 rows keep more: there both products take code - 7.5 in fp16 (one packed sum per pair), for the 16 and the middle
+// are three times what the codes themselves reach and leave their roundings in the scores (rel. error 1.7e-6 to 2.7e-6
+// with them, 2e-7 to 4e-7 without), and the queries, times the power of two that fits them into fp16, enter in three fp16 parts.
+//
 // A workgroup's four waves take the records of its split in turn, each with its own running reference point and
 // sums, merged through LDS at the end; several splits of a sequence are merged by int4_merge_kernel.  The
 // reference point of a row moves only when a score passes it by 2^8: p stays below 2^8 and the sums are rescaled
 // rarely.
 #include "int4_common.hpp"
+
+#include <type_traits>
 
 namespace lf {
 int launch_int4_prefix(const Int4Attention& a, int dtype, hipStream_t stream);
@@ -67,12 +73,12 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
 
 // Element pairs (a[i], b[i]) in NP fp16 parts, each rounded to nearest.
 template <int NP>
-struct Weights {
+struct HalfParts {
     f16x8 t[NP];
 };
 template <int NP>
-__device__ __forceinline__ Weights<NP> weights(const float (&a)[4], const float (&b)[4]) {
-    Weights<NP> r;
+__device__ __forceinline__ HalfParts<NP> half_parts(const float (&a)[4], const float (&b)[4]) {
+    HalfParts<NP> r;
     float x[4], y[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { x[i] = a[i]; y[i] = b[i]; }
@@ -130,6 +136,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     using S = Ring<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
     constexpr int NT = Dt == LF_BF16 ? 1 : Dt == LF_FP16 ? 2 : 3, NP = Dt == LF_BF16 ? 1 : 2;  // parts of q and of P'
+    constexpr bool kCentred = Dt == LF_FP32;
+    using Codes = std::conditional_t<kCentred, f16x8, bf16x8>;
+    using QueryParts = std::conditional_t<kCentred, HalfParts<NT>, Parts<NT>>;
     extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
     __shared__ float lds_ml[kWaves][kTile][2];
     int32_t* lds_pages = reinterpret_cast<int32_t*>(smem + S::lds);  // with pages only
@@ -229,29 +238,50 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     for (int m = 1; m < kWave; m <<= 1) most_scale = max(most_scale, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most_scale), m, kWave)));
     const float lift = static_cast<float>(static_cast<int>(__float_as_uint(f16_to_f32(static_cast<uint16_t>(most_scale))) >> 23) - 126 - 7);
 
-    Parts<NT> q[CH];
+    QueryParts q[CH];
     float qsum[G];
     const bool flip = a.qscale < 0.f;  // a negative scale goes into the queries: scores are then compared unscaled
-    const float qscale = fmaxf(fabsf(a.qscale), 1e-37f);
+    const int64_t at_q = b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 8 * quad;
+    float qscale = fabsf(a.qscale), fit = 1.f;  // ``fit``: the power of two that takes the row's largest to 2^13 .. 2^14
+    if constexpr (kCentred) {
+        float most = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            float x[8] = {};
+            if (real) query8<Dt>(a, at_q + 32 * c, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[e]));
+        }
+        const uint32_t e = min(max(__float_as_uint(rows_max(most)) >> 23, 27u), 254u);
+        fit = __uint_as_float((267u - e) << 23);
+        qscale *= __uint_as_float((e - 13u) << 23);
+    }
+    qscale = fmaxf(qscale, 1e-37f);
 #pragma unroll
     for (int g = 0; g < G; ++g) qsum[g] = 0.f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         float x[8] = {};
-        if (real) query8<Dt>(a, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 32 * c + 8 * quad, x);
+        if (real) query8<Dt>(a, at_q + 32 * c, x);
+        if constexpr (kCentred)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] *= fit;
         if (flip)
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = -x[e];
         const float lo[4] = {x[0], x[1], x[2], x[3]}, hi[4] = {x[4], x[5], x[6], x[7]};
-        q[c] = split<NT>(lo, hi);
+        if constexpr (kCentred) q[c] = half_parts<NT>(lo, hi);
+        else q[c] = split<NT>(lo, hi);
         qsum[c / CG] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) qsum[g] = rows_sum(qsum[g]);
 
-    const uint32_t key_base = in_vgpr(kKeyBase), value_base = in_vgpr(kValueBase);
-    constexpr uint32_t kMiddle = 0xCDE0CDE0u;  // fp16 -23.5: the bias of the codes and their middle
+    const uint32_t key_base = in_vgpr(kCentred ? kKeyBaseHalf : kKeyBase), value_base = in_vgpr(kValueBase);
+    // the bias of the codes and their middle: fp16 -23.5 (Values), and -135.5 (Keys that are read as fp16)
+    constexpr uint32_t kMiddle = 0xCDE0CDE0u, kKeyMiddle = 0xD83CD83Cu;
     const f16x8 middle = __builtin_bit_cast(f16x8, u32x4{kMiddle, kMiddle, kMiddle, kMiddle});
+    const f16x8 key_middle = __builtin_bit_cast(f16x8, u32x4{kKeyMiddle, kKeyMiddle, kKeyMiddle, kKeyMiddle});
     f32x4 o[VT], fix[G];
     float pm[G], l = 0.f, ref = 0.f, limit = -__builtin_inff();
 #pragma unroll
@@ -273,20 +303,22 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 const u32x4 pair = sm[8 * g];
-                float start = -kCodeBias * qsum[g];
+                float start = kCentred ? 0.f : -kCodeBias * qsum[g];
                 // (formed anew per record: kept, the G accumulator starts take the registers of a third wave)
                 if constexpr (G > 2) asm volatile("" : "+v"(start));
                 f32x4 acc = {start, start, start, start};
 #pragma unroll
                 for (int c = g * CG; c < (g + 1) * CG; ++c) {
-                    const bf16x8 codes = __builtin_bit_cast(bf16x8, codes8<kKeyMask>(kw[c], key_base));
+                    Codes codes = __builtin_bit_cast(Codes, codes8<kKeyMask>(kw[c], key_base));
+                    if constexpr (kCentred) codes += key_middle;
 #pragma unroll
                     for (int m = NT - 1; m >= 0; --m) acc = mfma(codes, q[c].t[m], acc);
                 }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     // (a sum with zero where it is a product: it takes the fp16 factor as it is)
-                    const float m = fmaf(pair_min(pair[r]), qsum[g], g == 0 ? 0.f : y[t][r]);
+                    const float low = kCentred ? fmaf(7.5f, pair_scale(pair[r]), pair_min(pair[r])) : pair_min(pair[r]);
+                    const float m = fmaf(low, qsum[g], g == 0 ? 0.f : y[t][r]);
                     y[t][r] = fmaf(pair_scale(pair[r]), acc[r], m);
                 }
             }
@@ -337,12 +369,14 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
                     pm[g] = fmaf(p[t][r], pair_min(pair[t][r]), pm[g]);
                     pm[g] = fmaf(7.5f, x[t][r], pm[g]);
                 }
-            const Weights<NP> w = weights<NP>(x[0], x[1]);
+            const HalfParts<NP> w = half_parts<NP>(x[0], x[1]);
+            if constexpr (!kCentred)
 #pragma unroll
-            for (int m = NP - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
+                for (int m = NP - 1; m >= 0; --m) fix[g] = mfma(middle, w.t[m], fix[g]);
 #pragma unroll
             for (int t = g * TG; t < (g + 1) * TG; ++t) {
-                const f16x8 codes = __builtin_bit_cast(f16x8, codes8<kValueMask>(vw[(t >> 2) * kWave][t & 3], value_base));
+                f16x8 codes = __builtin_bit_cast(f16x8, codes8<kValueMask>(vw[(t >> 2) * kWave][t & 3], value_base));
+                if constexpr (kCentred) codes += middle;
 #pragma unroll
                 for (int m = NP - 1; m >= 0; --m) o[t] = mfma(codes, w.t[m], o[t]);
             }

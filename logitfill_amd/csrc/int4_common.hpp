@@ -44,7 +44,7 @@ __device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
 // A Key word's eight codes as bf16, a Value word's as fp16 16 + code; element 2 i is nibble i, element 2 i + 1 nibble
 // i + 4.  ``base``: kKeyBase or kValueBase in a vector register.
 constexpr float kCodeBias = 16.f;
-constexpr uint32_t kKeyBase = 0x41804180u, kValueBase = 0x4C004C00u, kKeyMask = 0x00780078u, kValueMask = 0x03C003C0u;
+constexpr uint32_t kKeyBase = 0x41804180u, kValueBase = 0x4C004C00u, kKeyBaseHalf = 0x58005800u, kKeyMask = 0x00780078u, kValueMask = 0x03C003C0u;
 template <uint32_t Mask>
 __device__ __forceinline__ u32x4 codes8(uint32_t w, uint32_t base) {
     return u32x4{(w & Mask) | base, (turn(w, 4) & Mask) | base, (turn(w, 8) & Mask) | base, (turn(w, 12) & Mask) | base};

@@ -26,7 +26,6 @@ __device__ __forceinline__ uint32_t upper_pair(uint32_t a, uint32_t b) { return 
 
 // A word's eight codes times s[i] plus m[i], element pairs (nibble i, nibble i + 4).  The fp16 bits of a Key word's,
 // 0x5800 | code << 3, are 128 + code; of a Value word's, 0x4C00 | code << 6, 16 + code.
-constexpr uint32_t kWideBase = 0x58005800u;
 template <uint32_t Mask>
 __device__ __forceinline__ u32x4 dequant8(uint32_t w, const uint32_t (&s)[4], const uint32_t (&m)[4], uint32_t base) {
     constexpr _Float16 bias = static_cast<_Float16>(Mask == kKeyMask ? 128 : 16);
@@ -59,7 +58,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
     const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
     constexpr int VW = VT / 2;                          // a lane's Value words
     constexpr int VG = GROUP == 32 ? VW / 2 : 1;        // and the groups they lie in
-    const uint32_t code_base = in_vgpr(wave < 2 ? kWideBase : kValueBase);  // (a wave stages Keys or Values)
+    const uint32_t code_base = in_vgpr(wave < 2 ? kKeyBaseHalf : kValueBase);  // (a wave stages Keys or Values)
     // Every wave loads the same pieces, whichever it stages: with a branch around the loads, what it joins waited for them.
     struct Raw {
         uint32_t w[4];
