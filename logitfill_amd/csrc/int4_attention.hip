@@ -24,6 +24,9 @@
 // sums, merged through LDS at the end; several splits of a sequence are merged by int4_merge_kernel.  The
 // reference point of a row moves only when a score passes it by 2^8: p stays below 2^8 and the sums are rescaled
 // rarely.
+// A layer of 16 sequences of 32K tokens (28 / 4 heads of 128, groups of 64, one query each): 55 us for 304 MB, 5.5 TB/s,
+// VALU 61 % and matrix cores 14 % busy.  32 ragged ones of 4K to 64K (40 / 8 heads, groups of 32): 290 us, 1.36 GB, 4.7 TB/s,
+// VALU 65 %: the memory first, then the unpacking (four masks and shifts a word) and the factors of 32 channels each.
 #include "int4_common.hpp"
 
 #include <type_traits>

@@ -435,10 +435,24 @@ def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3, overhead: float = 
     return -(-max(max(tokens), 1) // size), size
 
 
-# From this many query rows per kv head up, and this many tokens in front of the queries, the many-row kernel takes
-# what every query sees.
+# From this many query rows per kv head up, this many tokens in front of the queries, and this many products of a
+# row's channel and a token's in front of them, the many-row kernel takes what every query sees.  It unpacks a record once
+# for 128 rows and costs two launches and 128-row partial sums: bf16, 28 / 4 heads of 128, groups of 128 over 16K tokens,
+# general against many-row, us: 32 queries (1.9e9 products) 31 / 45, 64 49 / 59, 128 (7.5e9) 80 / 74, 512
+# (3e10) 235 / 179; four sequences of 4K, 128 queries 73 / 77.  Groups of 32 cost the general kernel twice the products'
+# instructions (64 queries 68 / 61, 512 369 / 215), and so do queries of two parts (fp16; 32 queries, groups of 32 56 / 47).
 MANY_ROWS = 64
 MANY_ROWS_HISTORY = 256
+MANY_ROWS_WORK = 6e9
+
+
+def _many_rows(group: int, q_len: int, n_kv: int, head_dim: int, group_size: int, dtype, tokens) -> bool:
+    """Whether the many-row kernel takes part in the attention of sequences of ``tokens``."""
+    rows = group * q_len
+    if rows < MANY_ROWS or head_dim > 128 or dtype == torch.float32 or max(tokens) < q_len + MANY_ROWS_HISTORY:
+        return False
+    work = sum(n - q_len for n in tokens if n > q_len) * rows * n_kv * head_dim
+    return work >= MANY_ROWS_WORK * (0.5 if dtype == torch.float16 else 1.0) * (0.5 if group_size == 32 else 1.0)
 
 
 def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, key_new: Optional[torch.Tensor],
@@ -499,8 +513,7 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
         a.pages, a.n_pages = pages.data_ptr(), pages.shape[3]
         # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
         tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
-    if pages is None and group * q_len >= MANY_ROWS and D <= 128 and query.dtype != torch.float32 \
-            and max(tokens) >= q_len + MANY_ROWS_HISTORY:
+    if pages is None and _many_rows(group, q_len, manager.n_kv, D, manager.group_size, query.dtype, tokens):
         a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
                                          overhead=MANY_ROWS_OVERHEAD)
         a.splits = 1

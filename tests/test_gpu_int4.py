@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from logitfill_amd import _native
-from logitfill_amd.packed import Int4KVManager, int4_attention, layout, select_pages
+from logitfill_amd.packed import Int4KVManager, int4, int4_attention, layout, select_pages
 from oracle import int4 as o4
 from tests.helpers import f32
 from tests.int4_helpers import TYPES, assert_within, expected, query, rows
@@ -207,9 +207,10 @@ MANY = [
 
 
 @pytest.mark.parametrize("D,group,page,n_q,n_kv,lengths,q_len,dtype", MANY)
-def test_many_query_rows(gpu, D, group, page, n_q, n_kv, lengths, q_len, dtype):
+def test_many_query_rows(gpu, monkeypatch, D, group, page, n_q, n_kv, lengths, q_len, dtype):
     """The many-row kernel in front of the general one; the whole output close in the mean, too: independent roundings
     of weights, Keys and Values (fp16) and of the output."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)  # (the rule wants longer calls)
     B = len(lengths)
     key, value = rows((B, n_kv, max(lengths), D), dtype, sum(lengths) + 1)
     q = query((B, n_q, q_len, D), dtype, D + q_len)
@@ -228,8 +229,9 @@ def test_many_query_rows(gpu, D, group, page, n_q, n_kv, lengths, q_len, dtype):
     assert_within(out, ref, tol)
 
 
-def test_many_query_rows_of_any_size(gpu):
+def test_many_query_rows_of_any_size(gpu, monkeypatch):
     """Rows of 2^-60 to 2^60 (float16's range is passed through the rows' factor), of zeros, and one of NaN."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)
     D, T, n = 128, 700, 70
     key, value = rows((1, 1, T, D), "bf16", 8)
     q = query((1, 1, n, D), "bf16", 8).float()
@@ -249,8 +251,9 @@ def test_many_query_rows_of_any_size(gpu):
 
 
 @pytest.mark.parametrize("n", [1, 64])
-def test_a_nan_key_reaches_every_query_that_sees_it(gpu, n):
+def test_a_nan_key_reaches_every_query_that_sees_it(gpu, monkeypatch, n):
     """In a split of its own, too, far below the others' scores."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)
     D, T = 64, 5000
     key, value = rows((1, 1, T, D), "bf16", 9)
     key[0, 0, 3] = float("nan")
@@ -273,8 +276,9 @@ def test_attention_sharp_and_flat(gpu, scaling):
 
 
 @pytest.mark.parametrize("dtype,n", [("bf16", 1), ("fp16", 2), ("bf16", 40)])
-def test_values_of_any_size(gpu, dtype, n):
+def test_values_of_any_size(gpu, monkeypatch, dtype, n):
     """Value rows of 2^-14 to 2^14, zeros among them, and rows as large that were taken back."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)
     D, group, T = 128, 64, 600
     key, value = rows((1, 2, T, D), "fp32", 13)
     size = torch.exp2(torch.randint(-14, 12, (T,), generator=torch.Generator().manual_seed(2)).float())
@@ -294,6 +298,57 @@ def test_values_of_any_size(gpu, dtype, n):
         v = torch.cat([value[:, :, :keep], small[:, :, keep:]], 2)
         ref, tol = expected(q, key, v, [T], group, D ** -0.5, dtype, top=s_top)
         assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol)
+
+
+def test_float32_queries_of_any_size(gpu):
+    """Rows of 2^-90 to 2^90, of zeros, and one of NaN: the factor that fits a row into float16 parts is its own."""
+    D, T, n = 128, 700, 40
+    key, value = rows((1, 1, T, D), "fp32", 31)
+    size = torch.exp2(torch.linspace(-90, 0, n))[:, None]
+    q = query((1, 1, n, D), "fp32", 31) * size
+    q[0, 0, 11] = 0
+    mgr = manager(gpu, D, 64, 64, 1, 1)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    ref, tol = expected(q, key, value, [T], 64, D ** -0.5, "fp32")
+    assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol)
+    big = q * 2.0 ** 90
+    ref, tol = expected(big, key, value, [T], 64, 2.0 ** -91, "fp32")
+    assert_within(int4_attention(mgr, 0, big.to(gpu), None, None, 2.0 ** -91), ref, tol)
+    q[0, 0, 30] = float("nan")
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5)[0, 0]
+    assert out[30].isnan().all() and torch.isfinite(out[:30]).all() and torch.isfinite(out[31:]).all()
+
+
+def test_more_sequences_than_a_launch_takes(gpu):
+    """70 ragged sequences: written by pages, then a few tokens each, read from starts of their own, attended."""
+    B, H, D, group, page = 70, 2, 64, 32, 32
+    g = torch.Generator().manual_seed(6)
+    first = torch.randint(0, 80, (B,), generator=g).tolist()
+    more = torch.randint(0, 4, (B,), generator=g).tolist()
+    lengths = [a + c for a, c in zip(first, more)]
+    key, value = rows((B, H, max(lengths), D), "bf16", 33)
+    mgr = manager(gpu, D, group, page, 4, H, B)
+    mgr.commit(0, key[:, :, :max(first)].to(gpu), value[:, :, :max(first)].to(gpu), first)
+    new = [torch.stack([torch.nn.functional.pad(x[b], (0, 0, 0, 3))[:, first[b]:first[b] + 3] for b in range(B)]) for x in (key, value)]
+    mgr.commit(0, new[0].to(gpu), new[1].to(gpu), more)
+    check_rows(mgr, key, value, lengths, group, page)
+    q = query((B, 4, 1, D), "bf16", 33)
+    ref, tol = expected(q, key, value, lengths, group, D ** -0.5, "bf16")
+    assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol)
+
+
+def test_broadcast_rows_and_queries(gpu):
+    """Inputs whose batch, heads or tokens stand on one another (strides of zero)."""
+    B, H, T, D, group, page = 2, 2, 70, 128, 64, 64
+    key, value = rows((1, 1, T, D), "bf16", 34)
+    q = query((1, 1, 1, D), "bf16", 34)
+    mgr = manager(gpu, D, group, page, 4, H, B)
+    mgr.commit(0, key.to(gpu).expand(B, H, T, D), value.to(gpu)[:, :, :1].expand(B, H, T, D))
+    k, v = key.expand(B, H, T, D), value[:, :, :1].expand(B, H, T, D)
+    check_rows(mgr, k, v, [T] * B, group, page)
+    out = int4_attention(mgr, 0, q.to(gpu).expand(B, 4, 3, D), None, None, D ** -0.5)
+    ref, tol = expected(q.expand(B, 4, 3, D), k, v, [T] * B, group, D ** -0.5, "bf16")
+    assert_within(out, ref, tol)
 
 
 def test_growing_scores_move_the_reference_point(gpu):
@@ -407,6 +462,19 @@ def test_selected_pages(gpu, D, group, page, n_q, n_kv, lengths, q_len, top, dty
     out = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5, pages=pages)
     ref, tol = expected(q, key, value, lengths, group, D ** -0.5, dtype, page=page, pages=want)
     assert_within(out, ref, tol)
+
+
+def test_more_pages_than_registers_hold(gpu):
+    """17 000 pages: the choice reads its scores from memory."""
+    D, group, page, T, top = 64, 64, 32, 17000 * 32 + 5, 300
+    g = torch.Generator().manual_seed(35)
+    key = torch.randn(1, 1, T, D, generator=g).to(torch.bfloat16)
+    q = query((1, 2, 1, D), "bf16", 35)
+    mgr = manager(gpu, D, group, page, 2, 1)
+    mgr.commit(0, key.to(gpu), key.to(gpu))
+    bnd = f32(mgr.layers[0].page_bounds())[0, 0]
+    want = o4.select(f32(q)[0, :, 0], bnd, T // page, top)
+    assert np.array_equal(select_pages(mgr, 0, q.to(gpu), top)[0, 0, 0].cpu().numpy(), want)
 
 
 def test_equal_scores_take_the_lower_pages(gpu):

@@ -175,3 +175,14 @@ def test_oracle_known_answers():
     v = np.eye(3)
     out = o4.attend(np.zeros((2, 3)), v, v, 1.0, np.array([[True, True, False], [False] * 3]))
     assert np.allclose(out, [[0.5, 0.5, 0], [0, 0, 0]])
+
+
+def test_many_row_rule():
+    """Long calls of many rows, twice as soon in fp16 and with groups of 32; never in float32 or at head_dim 256."""
+    bf16, fp16 = torch.bfloat16, torch.float16
+    for args, want in (((7, 512, 4, 128, 128, bf16, [16896]), True), ((7, 32, 4, 128, 128, bf16, [16384]), False),
+                       ((7, 64, 4, 128, 32, bf16, [16384]), True), ((7, 64, 4, 128, 64, bf16, [16384]), False),
+                       ((7, 32, 4, 128, 32, fp16, [16384]), True), ((7, 512, 4, 128, 32, torch.float32, [16896]), False),
+                       ((7, 512, 4, 256, 64, bf16, [16896]), False), ((7, 512, 4, 128, 128, bf16, [700]), False),
+                       ((1, 63, 4, 128, 32, bf16, [1 << 24]), False), ((7, 512, 4, 128, 32, bf16, [0, 3]), False)):
+        assert int4._many_rows(*args) is want, args
