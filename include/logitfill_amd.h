@@ -450,7 +450,7 @@ typedef struct lf_int4_args {
                                                  what is behind them too; with pages: unused  */
     int32_t prefix_splits;                    /* > 0: the rows that every query of a 128-row tile sees go to the
                                                  many-row kernel, in that many workgroups per tile (1 .. 1024, of
-                                                 2-byte queries, head_dim 64 or 128, no pages; else
+                                                 bf16 queries, head_dim 64 or 128, no pages; else
                                                  LF_E_UNSUPPORTED), and splits is 1 for what is behind them  */
     void* workspace; int64_t workspace_bytes; /* 16-byte aligned, no initialisation           */
 } lf_int4_args;

@@ -109,7 +109,7 @@ int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, 
     if (A.prefix_splits < 0 || A.prefix_splits > kMaxSplits) return LF_E_SHAPE;
     if (A.prefix_splits > 0) {
         if (A.splits != 1) return LF_E_SHAPE;
-        if (A.n_pages > 0 || A.dtype == LF_FP32 || layer->head_dim > 128) return LF_E_UNSUPPORTED;
+        if (A.n_pages > 0 || A.dtype != LF_BF16 || layer->head_dim > 128) return LF_E_UNSUPPORTED;
     }
     const int parts = A.splits + A.prefix_splits;
     if (parts > 1) {

@@ -32,7 +32,7 @@
 #include <type_traits>
 
 namespace lf {
-int launch_int4_prefix(const Int4Attention& a, int dtype, hipStream_t stream);
+int launch_int4_prefix(const Int4Attention& a, hipStream_t stream);
 
 namespace {
 
@@ -504,7 +504,7 @@ int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
     int lds = Ring<D, GROUP>::lds;
     if (a.n_pages) lds += 4 * (a.split_tokens / (a.L.page_size / kBlock) + 2);  // the split's entries of the page list
     int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
-    if (st == LF_OK && a.prefix) st = launch_int4_prefix(a, Dt, stream);
+    if (st == LF_OK && a.prefix) st = launch_int4_prefix(a, stream);
     if (st != LF_OK) return st;
     hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, a);
     if (a.parts > 1) {

@@ -107,6 +107,8 @@ class _Int4Store:
             self._lens = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
         self._dirty = False  # the device's lengths are behind the host's
         self._tops: Optional[torch.Tensor] = None
+        self._captured = False  # a graph names the arrays, and its replays move the device's lengths
+        self._kept: list = []   # arrays that a captured graph may still name
         if capacity_tokens:
             self.reserve(capacity_tokens)
 
@@ -122,7 +124,8 @@ class _Int4Store:
     # ---- storage -------------------------------------------------------------
     def reserve(self, tokens: int) -> None:
         """Grow the capacity to at least ``tokens`` per sequence (doubling, page aligned).  The new arrays have
-        other addresses: a captured graph keeps the old ones, so reserve before the capture."""
+        other addresses: a captured graph keeps the old ones (which live as long as the cache), so reserve before the
+        capture."""
         P = self.page_size
         need = -(-int(tokens) // P) * P
         if need <= self._cap:
@@ -145,6 +148,12 @@ class _Int4Store:
                 tops[:, :, : self._cap // BLOCK].copy_(self._tops)
                 blocks[:, :, : self._cap // BLOCK].copy_(self._blocks)
                 bounds[:, :, : self._cap // P].copy_(self._bounds)
+            # the copies run on this stream, which need not be the arrays' own; a captured graph may still name them
+            old = (self._blocks, self._bounds, self._tops)
+            for t in old if self._cap else ():
+                t.record_stream(torch.cuda.current_stream(self.device))
+            if self._captured:
+                self._kept.append(old)
         self._blocks, self._bounds, self._tops = blocks, bounds, tops
         self._cap, self._struct = cap, None
 
@@ -159,10 +168,12 @@ class _Int4Store:
             s.batch, s.n_kv, s.head_dim = self.batch, self.n_kv, self.head_dim
             s.cap_tokens, s.page_size, s.group = self._cap, self.page_size, self.group_size
             self._struct = s
-        if lengths and self._dirty:
-            if torch.cuda.is_current_stream_capturing():
+        if torch.cuda.is_current_stream_capturing():
+            self._captured = True
+            if lengths and self._dirty:
                 raise RuntimeError("the cache was truncated or reset since its last launch: "
                                    "call manager.sync_lengths() before the capture")
+        elif lengths and self._dirty:
             _native.check(_native.load().lf_int4_set_lens(self._struct, _ints(self.lengths),
                                                           _native.current_stream_ptr(self.device)), "lf_int4_set_lens")
             self._dirty = False
@@ -171,7 +182,7 @@ class _Int4Store:
     def set_lengths(self, lengths) -> None:
         """Host lengths; the device's follow before the next launch."""
         lengths = [int(n) for n in lengths]
-        if lengths != self.lengths:
+        if lengths != self.lengths or self._captured:
             self.lengths = lengths
             self._dirty = True
 
@@ -216,16 +227,16 @@ class _Int4Store:
         new = [n + T for n in old] if lengths is None else [n + t for n, t in zip(old, lengths)]
         if max(new) > self._cap:
             self.reserve(max(new))
-        # the rows go where the host's lengths end and the device's follow; a captured commit moves the device's own
+        # the rows go where the host's lengths end and the device's follow; a captured commit moves the device's own, when
+        # it is replayed, and advance() the host's
         captured = torch.cuda.is_current_stream_capturing()
         st = _native.load().lf_int4_append(
             self.layer_struct(captured), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
             _strides(value), None if captured else _ints(old), None if lengths is None else _ints(lengths), T,
             _native.current_stream_ptr(self.device))
         _native.check(st, "lf_int4_append")
-        self.lengths = new
         if not captured:
-            self._dirty = False
+            self.lengths, self._dirty = new, False
 
     @_here
     def read(self, starts, tokens: int, dtype=torch.float32):
@@ -436,11 +447,11 @@ def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3, overhead: float = 
 
 
 # From this many query rows per kv head up, this many tokens in front of the queries, and this many products of a
-# row's channel and a token's in front of them, the many-row kernel takes what every query sees.  It unpacks a record once
-# for 128 rows and costs two launches and 128-row partial sums: bf16, 28 / 4 heads of 128, groups of 128 over 16K tokens,
-# general against many-row, us: 32 queries (1.9e9 products) 31 / 45, 64 49 / 59, 128 (7.5e9) 80 / 74, 512
-# (3e10) 235 / 179; four sequences of 4K, 128 queries 73 / 77.  Groups of 32 cost the general kernel twice the products'
-# instructions (64 queries 68 / 61, 512 369 / 215), and so do queries of two parts (fp16; 32 queries, groups of 32 56 / 47).
+# row's channel and a token's in front of them, the many-row kernel takes what every query sees (bf16: it holds Keys and
+# weights in fp16).  It unpacks a record once for 128 rows and costs two launches and 128-row partial sums: 28 / 4 heads of
+# 128, groups of 128 over 16K tokens, general against many-row, us: 32 queries (1.9e9 products) 31 / 45, 64 49 / 59, 128
+# (7.5e9) 80 / 74, 512 (3e10) 235 / 179; four sequences of 4K, 128 queries 73 / 77.  Groups of 32 cost the general kernel
+# more (64 queries 68 / 61, 512 369 / 215).
 MANY_ROWS = 64
 MANY_ROWS_HISTORY = 256
 MANY_ROWS_WORK = 6e9
@@ -449,10 +460,10 @@ MANY_ROWS_WORK = 6e9
 def _many_rows(group: int, q_len: int, n_kv: int, head_dim: int, group_size: int, dtype, tokens) -> bool:
     """Whether the many-row kernel takes part in the attention of sequences of ``tokens``."""
     rows = group * q_len
-    if rows < MANY_ROWS or head_dim > 128 or dtype == torch.float32 or max(tokens) < q_len + MANY_ROWS_HISTORY:
+    if rows < MANY_ROWS or head_dim > 128 or dtype != torch.bfloat16 or max(tokens) < q_len + MANY_ROWS_HISTORY:
         return False
     work = sum(n - q_len for n in tokens if n > q_len) * rows * n_kv * head_dim
-    return work >= MANY_ROWS_WORK * (0.5 if dtype == torch.float16 else 1.0) * (0.5 if group_size == 32 else 1.0)
+    return work >= MANY_ROWS_WORK * (0.5 if group_size == 32 else 1.0)
 
 
 def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, key_new: Optional[torch.Tensor],

@@ -198,11 +198,12 @@ def test_attention(gpu, D, group, page, n_q, n_kv, lengths, q_len, dtype):
 MANY = [
     # rows of several 128-row tiles, tiles of one head and of several, ragged histories, a history of whole records
     (128, 128, 128, 28, 4, [1500], 61, "bf16"),
-    (128, 64, 64, 8, 2, [900, 400, 290], 40, "fp16"),
+    (128, 64, 64, 8, 2, [900, 400, 290], 40, "bf16"),
     (128, 32, 32, 12, 2, [1024, 77], 130, "bf16"),
     (64, 64, 64, 4, 2, [2000], 300, "bf16"),
-    (64, 32, 32, 16, 1, [640, 0, 5], 9, "fp16"),
+    (64, 32, 32, 16, 1, [640, 0, 5], 9, "bf16"),
     (128, 64, 128, 64, 1, [1333], 1, "bf16"),
+    (64, 32, 32, 16, 1, [640], 90, "fp16"),  # (the general kernel)
 ]
 
 
@@ -558,9 +559,7 @@ def test_a_captured_step_replays_as_the_cache_grows(gpu, top):
         with torch.cuda.graph(graph):
             outs = step(graphed)
         graphs.append((graph, outs))
-    # the captures moved the host's lengths, not the device's
-    for layer in graphed.layers:
-        layer.lengths = [T, 29]
+    assert [layer.lengths for layer in graphed.layers] == [[T, 29]] * 2  # a capture commits nothing
     for t in range(T, T + 50):
         load(t)
         want = step(eager)
@@ -593,10 +592,47 @@ def test_replays_past_the_capacity_write_nothing(gpu):
         graph.replay()
         torch.cuda.synchronize()
     assert mgr.layers[0]._lens.tolist() == [32]
-    mgr.layers[0].lengths = [32]
+    mgr.advance(2)
     assert not torch.equal(mgr.layers[0]._blocks, before)
     got = mgr.layers[0].read(0, 32)[0]
     assert torch.equal(got[:, :, 30], got[:, :, 31])
+
+
+def test_commits_around_a_capture(gpu):
+    """A capture commits nothing; replays are told of with advance() or taken back with truncate(), to the host's own
+    lengths too, and eager commits go behind what is left."""
+    D, page, T = 64, 32, 90
+    key, value = rows((1, 2, T, D), "bf16", 92)
+    k, v = key.to(gpu), value.to(gpu)
+    mgr = manager(gpu, D, 32, page, 2, 2, capacity_tokens=128)
+    mgr.commit(0, k[:, :, :30], v[:, :, :30])
+    step_k, step_v = k[:, :, 30:31].clone(), v[:, :, 30:31].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mgr.commit(0, step_k, step_v)
+    assert mgr.seq_len == 30
+    mgr.commit(0, k[:, :, 30:33], v[:, :, 30:33])
+    check_rows(mgr, key, value, [33], 32, page)
+    step_k.copy_(k[:, :, 33:34])
+    step_v.copy_(v[:, :, 33:34])
+    graph.replay()
+    mgr.advance(1)
+    mgr.commit(0, k[:, :, 34:60], v[:, :, 34:60])
+    check_rows(mgr, key, value, [60], 32, page)
+    for _ in range(3):
+        graph.replay()
+    mgr.truncate(60)
+    check_rows(mgr, key, value, [60], 32, page)
+    mgr.commit(0, k[:, :, 60:], v[:, :, 60:])
+    check_rows(mgr, key, value, [T], 32, page)
+    # the cache grows away from the graph, whose replays reach arrays that are still theirs
+    mgr.layers[0].reserve(1000)
+    others = [torch.zeros(1 << 16, dtype=torch.uint8, device=gpu) for _ in range(8)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not any(bool(t.any()) for t in others)
+    mgr.truncate(T)
+    check_rows(mgr, key, value, [T], 32, page)
 
 
 def test_on_another_stream(gpu):

@@ -108,7 +108,7 @@ def test_append_and_read_refusals():
     ({"n_pages": 1025, "pages": AT}, SHAPE), ({"n_pages": -1}, SHAPE),
     ({"n_pages": 4, "pages": AT, "q_len": 20000}, SHAPE),
     ({"prefix_splits": -1}, SHAPE), ({"prefix_splits": 1025}, SHAPE), ({"prefix_splits": 4}, SHAPE),
-    ({"prefix_splits": 4, "splits": 1, "dtype": 2}, UNSUPPORTED),
+    ({"prefix_splits": 4, "splits": 1, "dtype": 1}, UNSUPPORTED), ({"prefix_splits": 4, "splits": 1, "dtype": 2}, UNSUPPORTED),
     ({"prefix_splits": 4, "splits": 1, "n_pages": 2, "pages": AT}, UNSUPPORTED),
     ({"prefix_splits": 4, "splits": 1, "workspace_bytes": 5 * 2 * 28 * 130 * 4 - 1}, WORKSPACE),
 ])
@@ -178,11 +178,11 @@ def test_oracle_known_answers():
 
 
 def test_many_row_rule():
-    """Long calls of many rows, twice as soon in fp16 and with groups of 32; never in float32 or at head_dim 256."""
+    """Long calls of many rows in bf16, twice as soon with groups of 32; never at head_dim 256."""
     bf16, fp16 = torch.bfloat16, torch.float16
     for args, want in (((7, 512, 4, 128, 128, bf16, [16896]), True), ((7, 32, 4, 128, 128, bf16, [16384]), False),
                        ((7, 64, 4, 128, 32, bf16, [16384]), True), ((7, 64, 4, 128, 64, bf16, [16384]), False),
-                       ((7, 32, 4, 128, 32, fp16, [16384]), True), ((7, 512, 4, 128, 32, torch.float32, [16896]), False),
+                       ((7, 512, 4, 128, 32, fp16, [16896]), False), ((7, 512, 4, 128, 32, torch.float32, [16896]), False),
                        ((7, 512, 4, 256, 64, bf16, [16896]), False), ((7, 512, 4, 128, 128, bf16, [700]), False),
                        ((1, 63, 4, 128, 32, bf16, [1 << 24]), False), ((7, 512, 4, 128, 32, bf16, [0, 3]), False)):
         assert int4._many_rows(*args) is want, args
