@@ -437,11 +437,12 @@ int32_t lf_int4_read(const lf_int4_layer* layer, const int32_t* starts, int32_t 
 /* Arguments of lf_int4_attention and lf_int4_select. */
 typedef struct lf_int4_args {
     const void* query; int32_t dtype;         /* [batch][n_q][q_len][head_dim] by strides   */
-    int32_t n_q, q_len;
+    int32_t n_q, q_len;                       /* n_q * q_len at most 2^20, times batch below 2^24 */
     int64_t q_strides[3];                     /* elements per sequence, head and token; unit channel stride */
     const int32_t* q_lens;                    /* DEVICE int32 [batch] of 0 .. q_len: query tokens of every
                                                  sequence (NULL: q_len); out rows behind them are zeros */
-    void* out;                                /* [batch][n_q][q_len][head_dim] contiguous, of ``dtype`` */
+    void* out;                                /* [batch][n_q][q_len][head_dim] contiguous, of ``dtype``,
+                                                 16-byte aligned                              */
     float scaling;
     int32_t n_pages;                          /* pages per query token (select; attention: 0 = all) */
     int32_t* pages;                           /* DEVICE int32 [batch][n_kv][q_len][n_pages]   */

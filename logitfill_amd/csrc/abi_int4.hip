@@ -41,6 +41,7 @@ int32_t check_query(const lf_int4_layer* L, const lf_int4_args* A) {
     if (!valid_dtype(A->dtype)) return LF_E_DTYPE;
     if (A->n_q <= 0 || A->n_q % L->n_kv != 0 || A->q_len <= 0) return LF_E_SHAPE;
     if (static_cast<int64_t>(A->n_q) * A->q_len > (1 << 20)) return LF_E_SHAPE;
+    if (static_cast<int64_t>(A->n_q) * A->q_len * L->batch >= 1 << 24) return LF_E_SHAPE;  // (256 threads a row, 2^32 in a grid)
     // a workgroup row per (kv head, query token) or (kv head, 16 rows), whichever are more
     const int64_t g = A->n_q / L->n_kv, rows = A->n_pages > 0 ? (g + 15) / 16 * A->q_len : (g * A->q_len + 15) / 16;
     if (rows * L->n_kv > kGrid) return LF_E_SHAPE;
@@ -104,6 +105,7 @@ int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, 
     if (st != LF_OK) return st;
     const lf_int4_args& A = *args;
     if (!A.out) return LF_E_NULL;
+    if (!aligned16(A.out)) return LF_E_SHAPE;
     if (A.splits <= 0 || A.splits > kMaxSplits) return LF_E_SHAPE;
     if (A.n_pages == 0 && A.splits > 1 && (A.split_tokens <= 0 || A.split_tokens % 32 != 0)) return LF_E_SHAPE;
     if (A.prefix_splits < 0 || A.prefix_splits > kMaxSplits) return LF_E_SHAPE;

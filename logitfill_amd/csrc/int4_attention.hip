@@ -187,8 +187,10 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     const int own = top > 0 ? (top - 1) / a.L.page_size : 0;
     int first, last;
     if (a.n_pages) {
-        first = part * a.split_tokens;
-        last = min(first + a.split_tokens, per_page * (a.n_pages + 1));
+        // (rounded up, splits can pass the list's end: those take nothing and read none of it)
+        const int records = per_page * (a.n_pages + 1);
+        first = min(part * a.split_tokens, records);
+        last = min(first + a.split_tokens, records);
         if (top == 0) last = first;
         // the pages of the list that the split takes, -1 for an entry that is none in front of the own page
         const int32_t* list = a.pages + ((static_cast<int64_t>(b) * a.L.n_kv + h) * a.q_len + j) * a.n_pages;

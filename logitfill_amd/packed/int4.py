@@ -344,13 +344,18 @@ class Int4KVManager:
         self.seq_len = 0
 
 
-def _check_query(manager, query: torch.Tensor) -> torch.Tensor:
+def _check_query(manager, query: torch.Tensor, paged: bool) -> torch.Tensor:
     shape = query.shape
     if len(shape) != 4 or shape[0] != manager.batch_size or shape[1] != manager.n_q or shape[3] != manager.head_dim:
         raise ValueError(f"query must be [{manager.batch_size}, {manager.n_q}, q_len, {manager.head_dim}], "
                          f"got {tuple(shape)}")
-    if shape[2] < 1:
+    n, group = shape[2], manager.n_q // manager.n_kv
+    if n < 1:
         raise ValueError("query holds no token")
+    # (the kernels' grids)
+    tiles = -(-group // 16) * n if paged else -(-group * n // 16)
+    if n * manager.n_q > 1 << 20 or shape[0] * n * manager.n_q >= 1 << 24 or manager.n_kv * tiles > 65535:
+        raise ValueError(f"{n} query tokens are too many for one call: feed them in chunks")
     return _check_rows(query, manager.device, "query")
 
 
@@ -484,7 +489,7 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     Everything is enqueued on the current stream.
     """
     layer = manager.layers[layer_idx]
-    query = _check_query(manager, query)
+    query = _check_query(manager, query, pages is not None or manager.top_pages > 0)
     q_len = query.shape[2]
     B = manager.batch_size
     new = None
@@ -567,7 +572,7 @@ def select_pages(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, to
     score is the largest, over the kv head's query heads, of ``sum_c max(q_c lo_c, q_c hi_c)`` with the
     page's ``page_bounds``, formed in float64.  Equal scores: the lower page first.
     """
-    query = _check_query(manager, query)
+    query = _check_query(manager, query, True)
     top_pages = int(top_pages)
     if not 1 <= top_pages <= MAX_PAGES:
         raise ValueError(f"top_pages must lie in 1 .. {MAX_PAGES}, got {top_pages}")

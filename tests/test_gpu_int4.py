@@ -465,6 +465,22 @@ def test_selected_pages(gpu, D, group, page, n_q, n_kv, lengths, q_len, top, dty
     assert_within(out, ref, tol)
 
 
+@pytest.mark.parametrize("splits", [2, 5, 50, 64])
+def test_pages_in_any_number_of_splits(gpu, monkeypatch, splits):
+    """Splits that end inside a page, pass the list's end, and belong to a sequence without a token."""
+    D, group, page, n = 64, 32, 256, 5
+    lengths = [3000, 0, 700, 1]
+    key, value = rows((4, 2, 3000, D), "bf16", 36)
+    q = query((4, 4, 1, D), "bf16", 36)
+    mgr = manager(gpu, D, group, page, 4, 2, 4)
+    mgr.commit(0, key.to(gpu), value.to(gpu), lengths)
+    pages = select_pages(mgr, 0, q.to(gpu), n)
+    monkeypatch.setattr(int4, "plan_splits", lambda *a, **k: (splits, 128))
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5, pages=pages)
+    ref, tol = expected(q, key, value, lengths, group, D ** -0.5, "bf16", page=page, pages=pages.cpu().numpy())
+    assert_within(out, ref, tol)
+
+
 def test_more_pages_than_registers_hold(gpu):
     """17 000 pages: the choice reads its scores from memory."""
     D, group, page, T, top = 64, 64, 32, 17000 * 32 + 5, 300

@@ -101,7 +101,7 @@ def test_append_and_read_refusals():
 
 
 @pytest.mark.parametrize("change,want", [
-    ({"query": 0}, NULL), ({"out": 0}, NULL), ({"dtype": 7}, DTYPE), ({"n_q": 27}, SHAPE), ({"n_q": 0}, SHAPE),
+    ({"query": 0}, NULL), ({"out": 0}, NULL), ({"out": AT + 8}, SHAPE), ({"dtype": 7}, DTYPE), ({"n_q": 27}, SHAPE), ({"n_q": 0}, SHAPE),
     ({"q_len": 0}, SHAPE), ({"q_len": 1 << 20}, SHAPE), ({"splits": 0}, SHAPE), ({"splits": 1025}, SHAPE),
     ({"split_tokens": 100}, SHAPE), ({"split_tokens": 0}, SHAPE), ({"workspace": 0}, NULL),
     ({"workspace": AT + 4}, SHAPE), ({"workspace_bytes": 100}, WORKSPACE), ({"n_pages": 4}, NULL),
@@ -114,6 +114,21 @@ def test_append_and_read_refusals():
 ])
 def test_attention_refusals(change, want):
     assert _native.load().lf_int4_attention(_layer(), _args(**change), None) == want
+
+
+def test_more_rows_than_a_grid_holds():
+    layer, args = _layer(batch=1 << 13), _args(q_len=64, splits=1)
+    layer.n_kv, args.n_q = 32, 32
+    assert _native.load().lf_int4_attention(layer, args, None) == SHAPE
+
+    class Manager:
+        batch_size, n_q, n_kv, head_dim, device = 2, 28, 4, 128, torch.device("cpu")
+    for n, paged in ((40000, False), (16384, True), (0, False)):
+        with pytest.raises(ValueError):
+            int4._check_query(Manager, torch.empty(2, 28, n, 1, dtype=torch.bfloat16).expand(2, 28, n, 128), paged)
+    Manager.batch_size = 9000
+    with pytest.raises(ValueError, match="too many"):
+        int4._check_query(Manager, torch.empty(1, 28, 70, 1, dtype=torch.bfloat16).expand(9000, 28, 70, 128), False)
 
 
 @pytest.mark.parametrize("change,want", [
