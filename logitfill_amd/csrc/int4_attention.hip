@@ -311,14 +311,17 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
                 float start = kCentred ? 0.f : -kCodeBias * qsum[g];
                 // (formed anew per record: kept, the G accumulator starts take the registers of a third wave)
                 if constexpr (G > 2) asm volatile("" : "+v"(start));
-                f32x4 acc = {start, start, start, start};
+                f32x4 rest = {start, start, start, start}, acc = {0.f, 0.f, 0.f, 0.f};  // (float32: the lower parts by themselves)
 #pragma unroll
                 for (int c = g * CG; c < (g + 1) * CG; ++c) {
                     Codes codes = __builtin_bit_cast(Codes, codes8<kKeyMask>(kw[c], key_base));
                     if constexpr (kCentred) codes += key_middle;
 #pragma unroll
-                    for (int m = NT - 1; m >= 0; --m) acc = mfma(codes, q[c].t[m], acc);
+                    for (int m = NT - 1; m >= (kCentred ? 1 : 0); --m) rest = mfma(codes, q[c].t[m], rest);
+                    if constexpr (kCentred) acc = mfma(codes, q[c].t[0], acc);
                 }
+                if constexpr (kCentred) acc += rest;
+                else acc = rest;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     // (a sum with zero where it is a product: it takes the fp16 factor as it is)
