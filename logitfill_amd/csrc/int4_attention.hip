@@ -451,7 +451,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
 }
 
 // The splits' sums at their largest reference point: a workgroup per output row, whose waves take the splits in
-// turn (sixteen of every 64, all loads on their way at once) and add up through LDS.
+// turn (sixteen of every 64, all loads on their way at once) and add up through LDS.  3 to 5 us, a launch and two dependent
+// loads; of 512 queries (14 336 rows, 51 MB of sums) 12.  One wave up to 16 splits, four from there on: attention and
+// merge of one sequence of 2K tokens, 16 splits 9.1 us with one and 9.3 with four, 64 splits 11.5 and 9.5.
 template <int D>
 __global__ __launch_bounds__(256) void int4_merge_kernel(Int4Attention a, int dtype) {
     constexpr int C = D / kWave, kTake = 16;

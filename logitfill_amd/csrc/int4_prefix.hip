@@ -11,7 +11,7 @@
 // output that is little (rel. error 1.7e-3 to 1.8e-3, at head_dim 64 2.2e-3, its own 1.65e-3); against fp16's it is not
 // (4e-4 to 1.5e-3 against 2.1e-4), so bf16 rows alone come here.
 //
-// 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128: 155 to 167 us, 0.73 PFLOP/s; matrix cores 34 %, VALU
+// 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128: 150 us of the call's 175, 0.8 PFLOP/s; matrix cores 34 %, VALU
 // 47 % and LDS 41 % busy: the operands' LDS reads and the softmax beside the products, two workgroups a CU.
 //
 // Double-buffered: a record's codes are loaded into registers two records ahead (a lane's sixteen bytes are exactly

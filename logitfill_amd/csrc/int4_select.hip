@@ -112,7 +112,8 @@ __global__ __launch_bounds__(256) void int4_score_kernel(SelectArgs a) {
 
 // A workgroup per (query token, kv head): the n_pages-th largest key, eight bits at a time (as far as the pages at
 // the prefix are more than are needed), then the pages above it and the first of those at it, in order.  Thread t
-// holds keys t, t + T, .. in registers (``Hold`` of them, 0: any number, read anew).
+// holds keys t, t + T, .. in registers (``Hold`` of them, 0: any number, read anew).  4.5 us for 128 pages, 11.5 for 4 096:
+// bound by the rounds' barriers, some five of eight bits each, not by the keys.
 template <int T, int Hold>
 __global__ __launch_bounds__(T) void int4_top_kernel(SelectArgs a) {
     constexpr int W = T / kWave;
@@ -243,8 +244,10 @@ int launch_int4_select(const lf_int4_layer& L, const lf_int4_args& A, hipStream_
         return LF_OK;
     });
     if (st != LF_OK) return st;
-    if (pages <= 256) launch_top<256, 1>(a, stream);
-    else if (pages <= 1024) launch_top<256, 4>(a, stream);
+    // By the capacity: the device alone knows the lengths.  Scores and choice of 8 (sequence, kv head)s, us: 1 000 pages
+    // 12.2 with four waves, 16.2 with sixteen; 4 000 pages from sixteen waves' registers 25.0, from memory 29.5, 16 000 61.5
+    // and 79.6.
+    if (pages <= 1024) launch_top<256, 4>(a, stream);
     else if (pages <= 16384) launch_top<1024, 16>(a, stream);
     else launch_top<1024, 0>(a, stream);
     const hipError_t err = hipGetLastError();
