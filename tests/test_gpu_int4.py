@@ -1,6 +1,8 @@
 """The 4-bit row cache on the device against its float64 oracle: rows written and read back bit for bit,
 attention within the rounding's bounds, page selection equal, for lengths, layouts, strides and masks where
 each can go wrong."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -685,6 +687,37 @@ def test_two_streams_attend_one_cache_at_once(gpu):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_two_threads_attend_one_cache_at_once(gpu):
+    """Each on a stream of its own, with queries of unlike forms."""
+    D, T = 128, 2000
+    key, value = (t.to(gpu) for t in rows((2, 2, T, D), "bf16", 97))
+    mgr = manager(gpu, D, 64, 64, 8, 2, 2)
+    mgr.commit(0, key, value)
+    qs = [query((2, 8, n, D), "bf16", 97 + n).to(gpu) for n in (1, 3)]
+
+    def call(q):
+        return int4_attention(mgr, 0, q, None, None, D ** -0.5, pages=select_pages(mgr, 0, q, 5))
+
+    want = [call(q) for q in qs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i].append(call(qs[i]))
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    for i in range(2):
+        assert len(got[i]) == 20 and all(torch.equal(x, want[i]) for x in got[i])
 
 
 def test_refusals(gpu):
