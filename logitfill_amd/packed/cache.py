@@ -694,15 +694,16 @@ class LogitFillCache(_HFCache):
         self.manager.reset()
 
     def crop(self, tokens_to_remove: int) -> None:
-        """transformers' ``crop``: keep that many tokens, or, negative, all but that many (a 4-bit row cache;
-        packed pages cannot be cropped)."""
+        """transformers' ``crop``, of every sequence by itself: keep that many of its tokens, or, negative, all but
+        that many of its last (a 4-bit row cache; packed pages cannot be cropped)."""
         truncate = getattr(self.manager, "truncate", None)
         if truncate is None:
             raise NotImplementedError("packed pages cannot be cropped")
         keep = int(tokens_to_remove)
-        keep = max(keep + int(self.manager.seq_len), 0) if keep < 0 else keep
-        if keep < int(self.manager.seq_len):
-            truncate([min(keep, n) for n in self.manager.layers[-1].lengths])
+        have = self.manager.layers[-1].lengths
+        left = [min(keep, n) if keep >= 0 else max(n + keep, 0) for n in have]
+        if left != have:
+            truncate(left)
 
     def reorder_cache(self, beam_idx) -> None:
         raise NotImplementedError("beam search is not supported by the packed cache")
