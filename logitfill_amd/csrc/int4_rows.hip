@@ -356,10 +356,11 @@ __global__ __launch_bounds__(512) void int4_append_few_kernel(RowsArgs a) {
         }
 }
 
+constexpr int kInlineLens = 512;  // 2 of a launch's 4 KB of arguments
 struct LensArgs {
     int32_t* lens;
     int b0, n;
-    int32_t value[kInlineSeqs];
+    int32_t value[kInlineLens];
 };
 __global__ void int4_set_lens_kernel(LensArgs a) {
     if (static_cast<int>(threadIdx.x) < a.n) a.lens[a.b0 + threadIdx.x] = a.value[threadIdx.x];
@@ -474,10 +475,10 @@ int last_error() {
 }  // namespace
 
 int launch_int4_set_lens(const lf_int4_layer& L, const int32_t* lens, hipStream_t stream) {
-    for (int b0 = 0; b0 < L.batch; b0 += kInlineSeqs) {
-        LensArgs a{L.lens, b0, min(kInlineSeqs, L.batch - b0), {}};
+    for (int b0 = 0; b0 < L.batch; b0 += kInlineLens) {
+        LensArgs a{L.lens, b0, min(kInlineLens, L.batch - b0), {}};
         for (int i = 0; i < a.n; ++i) a.value[i] = lens[b0 + i];
-        hipLaunchKernelGGL(int4_set_lens_kernel, dim3(1), dim3(kInlineSeqs), 0, stream, a);
+        hipLaunchKernelGGL(int4_set_lens_kernel, dim3(1), dim3(kInlineLens), 0, stream, a);
     }
     return last_error();
 }

@@ -86,11 +86,44 @@ def _ints(values):
     return (ctypes.c_int32 * len(values))(*values)
 
 
-class _Int4Store:
-    """One layer's 4-bit rows for ``batch`` sequences."""
+class _Lengths:
+    """The device's lengths of a cache's layers, int32 ``[layers, batch]``.  Appends move them on the stream of their call;
+    what the host sets is a launch of its own, which calls on other streams wait for."""
 
-    def __init__(self, n_kv: int, head_dim: int, page_size: int, group_size: int, *, device="cuda", batch: int = 1,
-                 capacity_tokens: int = 0):
+    def __init__(self, layers: int, batch: int, device: torch.device):
+        self.device = device
+        with torch.inference_mode(False):
+            self.rows = torch.zeros(layers, batch, dtype=torch.int32, device=device)
+        self._last = None  # (event, stream) of what the host set last
+
+    def set(self, layer: _native.Int4Layer, lengths) -> None:
+        """``lengths`` (per layer, per sequence) on the current stream; ``layer``: a struct whose capacity holds them."""
+        stream = torch.cuda.current_stream(self.device)
+        batch = self.rows.shape[1]
+        some = max(1, 65535 // batch)  # layers in one call: to it they are more sequences
+        for i in range(0, len(lengths), some):
+            part = [n for row in lengths[i : i + some] for n in row]
+            s = _native.Int4Layer.from_buffer_copy(layer)
+            s.lens, s.batch = self.rows[i].data_ptr(), len(part)
+            _native.check(_native.load().lf_int4_set_lens(s, _ints(part), stream.cuda_stream), "lf_int4_set_lens")
+        event = torch.cuda.Event()
+        event.record(stream)
+        self._last = (event, stream.cuda_stream)
+
+    def wait(self) -> None:
+        """The current stream behind what the host set last."""
+        if self._last is not None:
+            event, at = self._last
+            stream = torch.cuda.current_stream(self.device)
+            if stream.cuda_stream != at:
+                stream.wait_event(event)
+
+
+class _Int4Store:
+    """One layer's 4-bit rows for ``batch`` sequences; ``lens``: its row of ``order``."""
+
+    def __init__(self, n_kv: int, head_dim: int, page_size: int, group_size: int, order: _Lengths, lens: torch.Tensor, *,
+                 device="cuda", batch: int = 1, capacity_tokens: int = 0):
         self.device = _check_device(device)
         self.n_kv, self.head_dim = int(n_kv), int(head_dim)
         self.page_size, self.group_size = int(page_size), int(group_size)
@@ -103,9 +136,7 @@ class _Int4Store:
         self._blocks: Optional[torch.Tensor] = None
         self._bounds: Optional[torch.Tensor] = None
         self._struct: Optional[_native.Int4Layer] = None
-        with torch.inference_mode(False):
-            self._lens = torch.zeros(self.batch, dtype=torch.int32, device=self.device)
-        self._dirty = False  # the device's lengths are behind the host's
+        self._order, self._lens = order, lens
         self._tops: Optional[torch.Tensor] = None
         self._captured = False  # a graph names the arrays, and its replays move the device's lengths
         self._kept: list = []   # arrays that a captured graph may still name
@@ -157,8 +188,8 @@ class _Int4Store:
         self._blocks, self._bounds, self._tops = blocks, bounds, tops
         self._cap, self._struct = cap, None
 
-    def layer_struct(self, lengths: bool = True) -> _native.Int4Layer:
-        """The ``lf_int4_layer`` describing this store; ``lengths``: the device's up to date on the current stream."""
+    def layer_struct(self) -> _native.Int4Layer:
+        """The ``lf_int4_layer`` describing this store; the current stream is behind the lengths that the host set."""
         if self._cap == 0:
             self.reserve(self.page_size)
         if self._struct is None:
@@ -170,21 +201,9 @@ class _Int4Store:
             self._struct = s
         if torch.cuda.is_current_stream_capturing():
             self._captured = True
-            if lengths and self._dirty:
-                raise RuntimeError("the cache was truncated or reset since its last launch: "
-                                   "call manager.sync_lengths() before the capture")
-        elif lengths and self._dirty:
-            _native.check(_native.load().lf_int4_set_lens(self._struct, _ints(self.lengths),
-                                                          _native.current_stream_ptr(self.device)), "lf_int4_set_lens")
-            self._dirty = False
+        else:
+            self._order.wait()
         return self._struct
-
-    def set_lengths(self, lengths) -> None:
-        """Host lengths; the device's follow before the next launch."""
-        lengths = [int(n) for n in lengths]
-        if lengths != self.lengths or self._captured:
-            self.lengths = lengths
-            self._dirty = True
 
     def page_bounds(self) -> torch.Tensor:
         """bf16 ``[batch, n_kv, capacity / page_size, 2, head_dim]``: every full page's smallest and largest Key per
@@ -231,12 +250,12 @@ class _Int4Store:
         # it is replayed, and advance() the host's
         captured = torch.cuda.is_current_stream_capturing()
         st = _native.load().lf_int4_append(
-            self.layer_struct(captured), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
+            self.layer_struct(), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
             _strides(value), None if captured else _ints(old), None if lengths is None else _ints(lengths), T,
             _native.current_stream_ptr(self.device))
         _native.check(st, "lf_int4_append")
         if not captured:
-            self.lengths, self._dirty = new, False
+            self.lengths = new
 
     @_here
     def read(self, starts, tokens: int, dtype=torch.float32):
@@ -280,13 +299,17 @@ class Int4KVManager:
         self.batch_size, self.top_pages = int(batch_size), int(top_pages)
         if self.n_kv <= 0 or self.n_q <= 0 or self.n_q % self.n_kv:
             raise ValueError("query heads must divide into KV heads")
+        if self.batch_size <= 0 or int(n_layers) < 0:
+            raise ValueError("batch_size must be positive and n_layers not negative")
         if not 0 <= self.top_pages <= MAX_PAGES:
             raise ValueError(f"top_pages must lie in 0 .. {MAX_PAGES}, got {top_pages}")
         check_layout(self.head_dim, self.page_size, self.group_size)
         self.device = _check_device(device)
         self.seq_len = 0
-        self.layers = [_Int4Store(self.n_kv, self.head_dim, self.page_size, self.group_size, device=self.device,
-                                  batch=self.batch_size, capacity_tokens=capacity_tokens) for _ in range(int(n_layers))]
+        self._lens = _Lengths(int(n_layers), self.batch_size, self.device)
+        self.layers = [_Int4Store(self.n_kv, self.head_dim, self.page_size, self.group_size, self._lens, row,
+                                  device=self.device, batch=self.batch_size, capacity_tokens=capacity_tokens)
+                       for row in self._lens.rows]
         self._args: dict = {}
 
     def commit(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor, lengths=None) -> None:
@@ -307,16 +330,32 @@ class Int4KVManager:
 
     def truncate(self, lengths) -> None:
         """Forget every layer's tokens past ``lengths[b]`` (an int for all; rejected draft tokens, a prompt's common
-        start).  The device's lengths follow with the next call; before a capture, call ``sync_lengths``."""
+        start).  A write on the current stream: it follows the calls and replays that stand on it, and later calls on
+        other streams wait for it (a replay there does not by itself)."""
         lengths = [int(lengths)] * self.batch_size if isinstance(lengths, int) else [int(n) for n in lengths]
         if len(lengths) != self.batch_size:
             raise ValueError("truncate takes one length per sequence")
         for layer in self.layers:
             if any(n < 0 or n > have for n, have in zip(lengths, layer.lengths)):
                 raise ValueError(f"truncate to {lengths}: the cache holds {layer.lengths}")
-        for layer in self.layers:
-            layer.set_lengths(lengths)
+        self._set_lengths(lengths)
+
+    @_here
+    def _set_lengths(self, lengths: list) -> None:
+        """Every layer's lengths, the device's at once."""
+        if any(layer.lengths != lengths or layer._captured for layer in self.layers):
+            self._send_lengths([lengths] * len(self.layers))
+            for layer in self.layers:
+                layer.lengths = list(lengths)
         self.seq_len = self.layers[-1].length if self.layers else 0
+
+    def _send_lengths(self, lengths: list) -> None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("lengths that the host sets are its own step: set them before the capture")
+        widest = max(self.layers, key=lambda layer: layer.capacity)
+        if widest.capacity:  # (else no layer holds a token)
+            self._lens.wait()
+            self._lens.set(widest.layer_struct(), lengths)
 
     def advance(self, tokens) -> None:
         """Tell the host of tokens that replays of a captured step committed on the device (per sequence, or an int for
@@ -333,15 +372,15 @@ class Int4KVManager:
 
     @_here
     def sync_lengths(self) -> None:
-        """Bring the device's lengths up to the host's on the current stream (before a capture)."""
-        for layer in self.layers:
-            layer.layer_struct()
+        """Set the device's lengths to the host's on the current stream (after replays that ``advance`` is not told of)."""
+        if self.layers:
+            for layer in self.layers:
+                layer.layer_struct()
+            self._send_lengths([layer.lengths for layer in self.layers])
 
     def reset(self) -> None:
-        """Forget every token (storage is kept for reuse)."""
-        for layer in self.layers:
-            layer.set_lengths([0] * self.batch_size)
-        self.seq_len = 0
+        """Forget every token (storage is kept for reuse); a write on the current stream, as ``truncate``."""
+        self._set_lengths([0] * self.batch_size)
 
 
 def _check_query(manager, query: torch.Tensor, paged: bool) -> torch.Tensor:
