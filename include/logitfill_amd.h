@@ -443,7 +443,7 @@ typedef struct lf_int4_args {
                                                  sequence (NULL: q_len); out rows behind them are zeros */
     void* out;                                /* [batch][n_q][q_len][head_dim] contiguous, of ``dtype``,
                                                  16-byte aligned                              */
-    float scaling;
+    float scaling;                            /* finite (else LF_E_SHAPE)                    */
     int32_t n_pages;                          /* pages per query token (select; attention: 0 = all) */
     int32_t* pages;                           /* DEVICE int32 [batch][n_kv][q_len][n_pages]   */
     int32_t splits;                           /* workgroups that share a sequence's tokens, 1 .. 1024 */

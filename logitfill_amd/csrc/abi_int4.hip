@@ -1,6 +1,8 @@
 // extern "C" entry points of the 4-bit row cache: arguments are checked here, before anything is enqueued.
 #include "int4_common.hpp"
 
+#include <cmath>
+
 namespace lf {
 int launch_int4_set_lens(const lf_int4_layer& L, const int32_t* lens, hipStream_t stream);
 int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_src, int dtype, const int64_t* k_strides,
@@ -106,6 +108,7 @@ int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, 
     const lf_int4_args& A = *args;
     if (!A.out) return LF_E_NULL;
     if (!aligned16(A.out)) return LF_E_SHAPE;
+    if (!std::isfinite(A.scaling)) return LF_E_SHAPE;  // (the kernels take the larger of it and 1e-37)
     if (A.splits <= 0 || A.splits > kMaxSplits) return LF_E_SHAPE;
     if (A.n_pages == 0 && A.splits > 1 && (A.split_tokens <= 0 || A.split_tokens % 32 != 0)) return LF_E_SHAPE;
     if (A.prefix_splits < 0 || A.prefix_splits > kMaxSplits) return LF_E_SHAPE;

@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 from typing import Optional
 
 import torch
@@ -527,6 +528,9 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
 
     Everything is enqueued on the current stream.
     """
+    scaling = float(scaling)
+    if not math.isfinite(scaling):
+        raise ValueError(f"scaling must be finite, got {scaling}")
     layer = manager.layers[layer_idx]
     query = _check_query(manager, query, pages is not None or manager.top_pages > 0)
     q_len = query.shape[2]

@@ -1,0 +1,20 @@
+"""Calls of the 4-bit row cache that are refused before anything runs (no GPU)."""
+import pytest
+import torch
+
+from logitfill_amd import _native
+from logitfill_amd.packed import int4
+from tests.test_int4_host import _args, _layer
+
+
+@pytest.mark.parametrize("scaling", [float("nan"), float("inf"), -float("inf")])
+def test_a_scaling_that_is_not_finite(scaling):
+    """NaN became the smallest factor: finite outputs, every row's weight equal."""
+    assert _native.load().lf_int4_attention(_layer(), _args(scaling=scaling), None) == _native.LF_E_SHAPE
+
+    class Manager:
+        batch_size, n_q, n_kv, head_dim, device, top_pages = 1, 2, 1, 64, torch.device("cpu"), 0
+        layers = [None]
+    for s in (scaling, torch.tensor(scaling)):
+        with pytest.raises(ValueError, match="finite"):
+            int4.int4_attention(Manager, 0, torch.empty(1, 2, 1, 64), None, None, s)
