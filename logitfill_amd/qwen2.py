@@ -23,7 +23,7 @@ from __future__ import annotations
 import torch
 
 from logitfill_amd.packed.int4 import Int4KVManager, int4_attention
-from logitfill_amd.packed.reference import packed_attention
+from logitfill_amd.packed.reference import packed_attention, reference_attention
 
 
 def _dense_attention(attn, query, key, value, attention_mask, kwargs):
@@ -73,9 +73,13 @@ def attach_packed(model, manager, attention_fn=packed_attention) -> None:
     """Route every decoder layer's attention through ``manager`` (a ``PackedKVManager`` whose
     layers match the model's).  ``attention_fn`` is ``packed_attention`` (the HIP path) or
     ``reference_attention`` (dense dequantise-then-attend), same signature.  An ``Int4KVManager``
-    takes ``int4_attention`` in place of the default."""
-    if isinstance(manager, Int4KVManager) and attention_fn is packed_attention:
-        attention_fn = int4_attention
+    takes ``int4_attention`` in place of the default; any other function given for it commits the new
+    tokens itself (``reference_attention``, which reads packed pages, does not: ``ValueError``)."""
+    if isinstance(manager, Int4KVManager):
+        if attention_fn is reference_attention:
+            raise ValueError("reference_attention reads packed pages; an Int4KVManager takes int4_attention")
+        if attention_fn is packed_attention:
+            attention_fn = int4_attention
     cfg = model.config
     n_kv = int(cfg.num_key_value_heads)
     layers = model.model.layers

@@ -4,6 +4,8 @@ import torch
 
 from logitfill_amd import _native
 from logitfill_amd.packed import int4
+from logitfill_amd.packed.reference import reference_attention
+from logitfill_amd.qwen2 import attach_packed
 from tests.test_int4_host import _args, _layer
 
 
@@ -18,3 +20,10 @@ def test_a_scaling_that_is_not_finite(scaling):
     for s in (scaling, torch.tensor(scaling)):
         with pytest.raises(ValueError, match="finite"):
             int4.int4_attention(Manager, 0, torch.empty(1, 2, 1, 64), None, None, s)
+
+
+def test_the_dense_path_of_packed_pages():
+    """It failed at the first decode step, the prompt committed."""
+    manager = int4.Int4KVManager.__new__(int4.Int4KVManager)
+    with pytest.raises(ValueError, match="int4_attention"):
+        attach_packed(None, manager, reference_attention)
