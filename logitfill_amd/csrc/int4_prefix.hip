@@ -2,17 +2,22 @@
 // prompt's chunk over what is in front of it).
 //
 // Per record the general kernel's waves unpack the codes and form scale and minimum terms for 16 rows each.  Here the
-// workgroup dequantises a record once -- Keys and Values as fp16 s * code + m, by packed fp16 arithmetic -- into LDS,
-// in the order in which the products' lanes read it, and its four waves take it for 32 rows each:
-//     S^T = K . Q^T,  p = 2^(S c - ref),  O^T = V^T . P^T,  l = 1 . P^T   on v_mfma_f32_16x16x32_f16.
-// A query row is scaled by a power of two so that its largest element lies in [1, 2); the factor goes into c.  The
-// fp16 steps: a Key and a Value element are off by 2^-12 of their size (a Key's error in a score is that of a sum of
-// head_dim independent ones), a weight p by 2^-12; l is the sum of the rounded weights.  Against bf16's rounding of the
-// output that is little (rel. error 1.7e-3 to 1.8e-3, at head_dim 64 2.2e-3, its own 1.65e-3); against fp16's it is not
-// (4e-4 to 1.5e-3 against 2.1e-4), so bf16 rows alone come here.
+// workgroup unpacks a record once, by packed fp16 arithmetic, into LDS, in the order in which the products' lanes read it, and
+// its four waves take it for 32 rows each, on v_mfma_f32_16x16x32_f16:
+//     S_t = sum_g scale_t,g (code_t,g . q_g) + min_t,g sum(q_g),  p = 2^(S c - ref),  O^T = V^T . P^T,  l = sum p.
+// Keys enter as their codes, which fp16 holds, and scale and minimum in fp32 as in the general kernel: as fp16 s * code + m a
+// Key was off by 2^-12 of itself, which beside a channel that is large in every token (a bias of 400) moved weights by a
+// hundredth and more.  (In two exact fp16 parts, scale * code, Keys take twice the LDS reads and products: 263 us against 223
+// below.)  With several groups, the minima's terms are a product of their own, sixteen deep, of the fp16 factors as
+// they stand and the queries' sums in two fp16 parts (2^-22 of them); with one group of 128 they are a sum per score, for
+// the product's registers spill (223 us against 238).
+// A query row is scaled by a power of two so that its largest element lies in [1, 2); the factor goes into c.  Values enter as
+// fp16 s * code + m, off by 2^-12 of their size, and so does a weight p; against bf16's rounding of the output that
+// is little (rel. error 1.66e-3 to 1.69e-3, its own 1.64e-3 to 1.66e-3), against fp16's it is not, so bf16 rows
+// alone come here.
 //
-// 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128: 150 us of the call's 175, 0.8 PFLOP/s; matrix cores 34 %, VALU
-// 47 % and LDS 41 % busy: the operands' LDS reads and the softmax beside the products, two workgroups a CU.
+// 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128 / 64 / 32: calls of 223 / 250 / 278 us where the general
+// kernel alone takes 273 / 324 / 417; 14 / 2 heads of 64, groups of 64 / 32: 85 / 91 and 105 / 136.
 //
 // Double-buffered: a record's codes are loaded into registers two records ahead (a lane's sixteen bytes are exactly
 // what it turns into operands), dequantised one ahead, one barrier per record.
@@ -26,49 +31,64 @@ constexpr int kWaves = 4, kTile = 16, MT = kManyRows / (kWaves * kTile);  // row
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ uint32_t lower_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ uint32_t upper_pair(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// A word's eight codes times s[i] plus m[i], element pairs (nibble i, nibble i + 4).  The fp16 bits of a Key word's,
-// 0x5800 | code << 3, are 128 + code; of a Value word's, 0x4C00 | code << 6, 16 + code.
+// A word's eight codes in fp16, element pairs (nibble i, nibble i + 4).  The fp16 bits of a Key word's, 0x5800 | code << 3,
+// are 128 + code; of a Value word's, 0x4C00 | code << 6, 16 + code.
 template <uint32_t Mask>
-__device__ __forceinline__ u32x4 dequant8(uint32_t w, const uint32_t (&s)[4], const uint32_t (&m)[4], uint32_t base) {
+__device__ __forceinline__ f16x2 code_pair(const u32x4& bits, int i) {
     constexpr _Float16 bias = static_cast<_Float16>(Mask == kKeyMask ? 128 : 16);
-    const u32x4 bits = codes8<Mask>(w, base);
+    const uint32_t pair = bits[i];
+    return __builtin_bit_cast(f16x2, pair) - f16x2{bias, bias};
+}
+// A Key word's codes.
+__device__ __forceinline__ u32x4 keys8(uint32_t w, uint32_t base) {
+    const u32x4 bits = codes8<kKeyMask>(w, base);
     u32x4 r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t pair = bits[i];
-        const f16x2 code = __builtin_bit_cast(f16x2, pair) - f16x2{bias, bias};
-        r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, m[i])));
-    }
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, code_pair<kKeyMask>(bits, i));
     return r;
 }
+// A Value word's codes times s[i] plus m[i].
+__device__ __forceinline__ u32x4 values8(uint32_t w, const f16x2 (&s)[4], const f16x2 (&m)[4], uint32_t base) {
+    const u32x4 bits = codes8<kValueMask>(w, base);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code_pair<kValueMask>(bits, i), s[i], m[i]));
+    return r;
+}
+// LDS reads stay behind this point: hoisted to a record's start they take more registers than three waves a SIMD leave.
+__device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
+__device__ __forceinline__ f16x2 halves(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
 
 template <int D, int GROUP>
-__global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Attention a) {
+__global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) void int4_prefix_kernel(Int4Attention a) {
     using R = Int4Rec<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, VT = D / 16;
+    constexpr bool kOne = D == 128 && G == 1;  // the minima's terms by sums
     constexpr int kK = 2 * CH * kWave, kV = VT * kWave;  // 16-byte pieces of a record's Keys and Values
     __shared__ u32x4 lds[2][kK + kV];
+    __shared__ __attribute__((aligned(16))) uint32_t key_pairs[2][G * kBlock];  // Keys' scales and minima
     const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
+    const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
     const int len = int4_len(a.L, b);
     const int n = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
     const int records = prefix_records(a, len, n, tile);
     const int per = (records + a.prefix - 1) / a.prefix, first = min(part * per, records), last = min(first + per, records);
 
     // This wave's share of a record: 0, 1: sixteen Key rows; 2, 3: half of a lane's Value words.
-    const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
     constexpr int VW = VT / 2;                          // a lane's Value words
     constexpr int VG = GROUP == 32 ? VW / 2 : 1;        // and the groups they lie in
     const uint32_t code_base = in_vgpr(wave < 2 ? kKeyBaseHalf : kValueBase);  // (a wave stages Keys or Values)
+    constexpr int NP = 2 * VG > G ? 2 * VG : G;
     // Every wave loads the same pieces, whichever it stages: with a branch around the loads, what it joins waited for them.
     struct Raw {
         uint32_t w[4];
-        uint32_t key[G];        // scale and minimum of a Key row's groups
-        u32x4 value[2 * VG];    // of tokens 4 quad .. and 16 + 4 quad .. of a Value word's groups
+        u32x4 pair[NP];  // scale and minimum: [g][0] a Key row's, or a Value word's of tokens 4 quad .. and 16 + 4 quad ..
     };
     const int half = wave & 1;
     const uint32_t word_at = wave < 2 ? (16 * half + col) * (D / 2) + CH * 4 * quad
@@ -88,48 +108,47 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
             r.w[1] = x[1];
         }
 #pragma unroll
-        for (int g = 0; g < G; ++g) r.key[g] = *reinterpret_cast<const uint32_t*>(rec + key_at + 4 * kBlock * g);
-#pragma unroll
-        for (int k = 0; k < 2 * VG; ++k)
-            r.value[k] = *reinterpret_cast<const u32x4*>(rec + value_at + 4 * kBlock * (k >> 1) + 64 * (k & 1));
+        for (int k = 0; k < NP; ++k) {
+            const uint32_t at = wave < 2 ? key_at + 4 * kBlock * min(k, G - 1) : value_at + 4 * kBlock * (k >> 1) + 64 * (k & 1);
+            __builtin_memcpy(&r.pair[k], __builtin_assume_aligned(rec + at, 4), 16);
+        }
     };
-    const auto stage = [&](const Raw& r, u32x4* to) {
+    const auto stage = [&](const Raw& r, u32x4* to, uint32_t* pairs) {
         if (wave < 2) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const uint32_t pair = r.key[c / (CH / G)], s = lower_pair(pair, pair), m = upper_pair(pair, pair);
-                const uint32_t ss[4] = {s, s, s, s}, mm[4] = {m, m, m, m};
-                to[(half * CH + c) * kWave + lane] = dequant8<kKeyMask>(r.w[c], ss, mm, code_base);
-            }
+            for (int c = 0; c < CH; ++c) to[(half * CH + c) * kWave + lane] = keys8(r.w[c], code_base);
+            if (quad == 0)
+#pragma unroll
+                for (int g = 0; g < G; ++g) pairs[g * kBlock + 16 * half + col] = r.pair[g][0];
         } else {
 #pragma unroll
             for (int k = 0; k < VG; ++k) {
-                uint32_t s[4], m[4];
+                f16x2 s[4], m[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[i] = lower_pair(r.value[2 * k][i], r.value[2 * k + 1][i]);
-                    m[i] = upper_pair(r.value[2 * k][i], r.value[2 * k + 1][i]);
+                    s[i] = halves(lower_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i]));
+                    m[i] = halves(upper_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i]));
                 }
 #pragma unroll
                 for (int c = k * (VW / VG); c < (k + 1) * (VW / VG); ++c)
-                    to[kK + (half * VW + c) * kWave + lane] = dequant8<kValueMask>(r.w[c], s, m, code_base);
+                    to[kK + (half * VW + c) * kWave + lane] = values8(r.w[c], s, m, code_base);
             }
         }
     };
 
     // rows (head of the group, token), tokens fastest: this lane's, one of each row tile
     f16x8 q[MT][CH];
+    f16x4 qsum[MT];  // the query's sum over lane quad's group: 0 (for the scale), upper part, 0, lower part
+    float qall[MT];  // or over the one group
     float scale[MT], ref[MT], limit[MT];  // limit: how far a score may pass ref; -inf until one is seen
-    int row[MT];  // head of the group * q_len + token, or -1
     const bool flip = a.qscale < 0.f;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
         const int r = tile * kManyRows + (wave * MT + t) * kTile + col, i = r / a.q_len, j = r % a.q_len;
-        row[t] = i < a.g ? r : -1;
         float x[CH][8] = {}, most = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (row[t] >= 0) query8<LF_BF16>(a, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 32 * c + 8 * quad, x[c]);
+            if (i < a.g) query8<LF_BF16>(a, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 32 * c + 8 * quad, x[c]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[c][e]));
         }
@@ -138,6 +157,7 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
         const int exponent = static_cast<int>(__float_as_uint(most) >> 23);
         const float down = __uint_as_float(static_cast<uint32_t>(min(max(254 - exponent, 1), 253)) << 23);
         scale[t] = fmaxf(fabsf(a.qscale) / down, 1e-37f);
+        float sums[G] = {}, mine = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -145,43 +165,74 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
                 // operand element 2 i is channel i of the word, element 2 i + 1 channel 4 + i
                 const float v = x[c][(e >> 1) + 4 * (e & 1)] * down;
                 q[t][c][e] = static_cast<_Float16>(flip ? -v : v);
+                sums[c / (CH / G)] += flip ? -v : v;
             }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const float sum = rows_sum(sums[g]);  // (in every quad)
+            mine = kOne || quad == g ? sum : mine;
+        }
+        qall[t] = mine;
+        const _Float16 upper = static_cast<_Float16>(mine);
+        qsum[t] = f16x4{0, upper, 0, static_cast<_Float16>(mine - static_cast<float>(upper))};
         ref[t] = 0.f;
         limit[t] = -__builtin_inff();
     }
-    f32x4 o[MT][VT], l[MT];
+    f32x4 o[MT][VT];
+    float l[MT];
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        l[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        l[t] = 0.f;
 #pragma unroll
         for (int v = 0; v < VT; ++v) o[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    const f16x8 ones = {1, 1, 1, 1, 1, 1, 1, 1};
 
     Raw raw;
     if (first < last) {
         load(first, raw);
-        stage(raw, lds[0]);
+        stage(raw, lds[0], key_pairs[0]);
         load(min(first + 1, last - 1), raw);
     }
     __syncthreads();
     for (int k = first; k < last; ++k) {
         const u32x4* rec = lds[(k - first) & 1];
+        const uint32_t* pairs = key_pairs[(k - first) & 1];
         if (k + 1 < last) {
-            stage(raw, lds[(k + 1 - first) & 1]);
+            stage(raw, lds[(k + 1 - first) & 1], key_pairs[(k + 1 - first) & 1]);
             load(min(k + 2, last - 1), raw);
         }
         f32x4 y[MT][2];
 #pragma unroll
-        for (int t = 0; t < MT; ++t) y[t][0] = y[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int u = 0; u < 2; ++u) {
+            if constexpr (!kOne) {
+                const uint32_t pair = pairs[min(quad, G - 1) * kBlock + 16 * u + col];  // (a quad past the groups: times zero)
+                const f16x4 factors = __builtin_bit_cast(f16x4, u32x2{pair, pair});
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const f16x8 key = __builtin_bit_cast(f16x8, rec[(u * CH + c) * kWave + lane]);
-#pragma unroll
-                for (int t = 0; t < MT; ++t) y[t][u] = mfma(key, q[t][c], y[t][u]);
+                for (int t = 0; t < MT; ++t) y[t][u] = __builtin_amdgcn_mfma_f32_16x16x16f16(factors, qsum[t], f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
             }
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                f32x4 acc[MT];
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = g * (CH / G); c < (g + 1) * (CH / G); ++c) {
+                    const f16x8 key = __builtin_bit_cast(f16x8, rec[(u * CH + c) * kWave + lane]);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) acc[t] = mfma(key, q[t][c], acc[t]);
+                }
+                const u32x4 pair = *reinterpret_cast<const u32x4*>(pairs + g * kBlock + 16 * u + 4 * quad);
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // (a sum with zero where it is a product: it takes the fp16 factor as it is)
+                        const float low = kOne ? fmaf(pair_min(pair[i]), qall[t], 0.f) : y[t][u][i];
+                        y[t][u][i] = fmaf(pair_scale(pair[i]), acc[t][i], low);
+                    }
+                phase();
+            }
+        }
         f16x8 p[MT];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -212,8 +263,11 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) p[t][2 * i + u] = static_cast<_Float16>(__builtin_amdgcn_exp2f(z[u][i]));
-            l[t] = mfma(ones, p[t], l[t]);
+                for (int u = 0; u < 2; ++u) {
+                    const float e = __builtin_amdgcn_exp2f(z[u][i]);
+                    l[t] += e;
+                    p[t][2 * i + u] = static_cast<_Float16>(e);
+                }
         }
 #pragma unroll
         for (int v = 0; v < VT; ++v) {
@@ -225,13 +279,15 @@ __global__ __launch_bounds__(kWaves * kWave, 3) void int4_prefix_kernel(Int4Atte
     }
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        if (row[t] < 0) continue;
-        const int64_t at = ((static_cast<int64_t>(b) * a.n_q + h * a.g) * a.q_len + row[t]) * a.parts + part;
+        l[t] = rows_sum(l[t]);
+        const int r = tile * kManyRows + (wave * MT + t) * kTile + col;  // head of the group * q_len + token
+        if (r >= a.g * a.q_len) continue;
+        const int64_t at = ((static_cast<int64_t>(b) * a.n_q + h * a.g) * a.q_len + r) * a.parts + part;
         // (a sum of NaN counts as seen; rows behind the sequence's last token are zeros whatever they saw)
-        const bool token = row[t] % a.q_len < n;
+        const bool token = r % a.q_len < n;
         if (quad == 0) {
-            a.part_ml[2 * at] = token && l[t][0] != 0.f ? ref[t] : -__builtin_inff();
-            a.part_ml[2 * at + 1] = token ? l[t][0] : 0.f;
+            a.part_ml[2 * at] = token && l[t] != 0.f ? ref[t] : -__builtin_inff();
+            a.part_ml[2 * at + 1] = token ? l[t] : 0.f;
         }
         if (!token)
 #pragma unroll

@@ -453,6 +453,11 @@ def workgroups_per_cu(head_dim: int, group: int) -> int:
     return {64: 4, 128: 3, 256: 2 if group > 32 else 1}[head_dim]
 
 
+def many_rows_per_cu(head_dim: int, group: int) -> int:
+    """Many-row workgroups that a CU holds, by registers."""
+    return 2 if head_dim == 128 and group < 128 else 3
+
+
 @functools.lru_cache(maxsize=512)
 def _plan(units: tuple, rows: int, slots: int, overhead: float) -> int:
     """Units a split takes, of sequences of ``units`` (their work, ``rows`` workgroups a split): the size of least
@@ -574,7 +579,7 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
         tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
     if pages is None and _many_rows(group, q_len, manager.n_kv, D, manager.group_size, query.dtype, tokens):
         a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
-                                         overhead=MANY_ROWS_OVERHEAD)
+                                         many_rows_per_cu(D, manager.group_size), MANY_ROWS_OVERHEAD)
         a.splits = 1
     else:
         a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,

@@ -1,0 +1,31 @@
+"""The many-row kernel where float16 does not hold what it is given."""
+import pytest
+import torch
+
+from logitfill_amd.packed import Int4KVManager, int4, int4_attention
+from tests.int4_exact import exact, prefixes  # noqa: F401  (a fixture)
+from tests.int4_helpers import assert_within
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 64), (128, 32), (64, 64), (64, 32)])
+def test_keys_beside_a_constant(gpu, monkeypatch, prefixes, D, group):  # noqa: F811
+    """Channels that are large in every token (Keys with a bias): scores within float32's error, and no step in the results
+    where the rule passes from one kernel to the other."""
+    T, n, n_q, H = 1500, 61, 8, 2
+    g = torch.Generator().manual_seed(D + group)
+    key = torch.randn(1, H, T, D, generator=g) * 3
+    key[..., 5] += 400
+    key[..., D // 2 + 3] -= 300
+    key, value = key.bfloat16(), torch.randn(1, H, T, D, generator=g).bfloat16()
+    q = torch.randn(1, n_q, n, D, generator=g) * 12 / D ** 0.5
+    q[..., [5, D // 2 + 3]] = 12
+    q = q.bfloat16()
+    mgr = Int4KVManager(1, n_q, H, D, 64, group, gpu)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    ref, tol = exact(q, key, value, [T], group, D ** -0.5, "bf16", many=True)
+    for work in (0, 1e30):
+        monkeypatch.setattr(int4, "MANY_ROWS_WORK", work)
+        assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol, f"work {work}")
+    assert [p > 0 for p in prefixes()] == [True, False]
