@@ -26,6 +26,11 @@
 namespace lf {
 namespace {
 
+// A weight is formed as up to 2^15: 2^7 where the reference point is, 2^8 before that moves.  fp16 keeps it down to 2^-24,
+// 2^-31 of a row's largest, and it takes 2^22 smaller ones to show in bf16.  (With 1 where the reference point is, 131 071
+// tokens of 2^-26 each, 2^-9 of their row, were lost.)
+constexpr float kHeadroom = 7.f;
+
 constexpr int kWaves = 4, kTile = 16, MT = kManyRows / (kWaves * kTile);  // row tiles of a wave
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
@@ -247,10 +252,10 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
             if (__any(most > limit[t])) {
                 most = rows_max(most);
                 const bool moves = most > limit[t];
-                const float by = moves ? most : 0.f;
+                const float by = moves ? most - kHeadroom : 0.f;
                 const float down = limit[t] < 0.f && moves ? 0.f : __builtin_amdgcn_exp2f(-by);
                 ref[t] += by;
-                limit[t] = moves ? 8.f : limit[t];
+                limit[t] = moves ? kHeadroom + 8.f : limit[t];
                 l[t] *= down;
 #pragma unroll
                 for (int v = 0; v < VT; ++v) o[t][v] *= down;

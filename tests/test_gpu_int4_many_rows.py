@@ -29,3 +29,23 @@ def test_keys_beside_a_constant(gpu, monkeypatch, prefixes, D, group):  # noqa: 
         monkeypatch.setattr(int4, "MANY_ROWS_WORK", work)
         assert_within(int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5), ref, tol, f"work {work}")
     assert [p > 0 for p in prefixes()] == [True, False]
+    assert [p > 0 for p in prefixes()] == [True, False]
+
+
+def test_very_many_tokens_of_small_weight(gpu, monkeypatch, prefixes):  # noqa: F811
+    """131 071 tokens of 2^-26 of the first one's weight each, in one split: 2^-9 of the whole together."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)
+    monkeypatch.setattr(int4, "plan_splits", lambda *a, **k: (1, 128))
+    D, T, n = 64, 1 << 17, 64
+    key = torch.zeros(1, 1, T, D, dtype=torch.bfloat16)
+    key[:, :, 0] = 18  # (rows of one number are kept as they are)
+    value = torch.full((1, 1, T, D), 512.0, dtype=torch.bfloat16)
+    value[:, :, 0] = 0
+    q = torch.zeros(1, 1, n, D, dtype=torch.bfloat16)
+    q[..., 7] = 1
+    mgr = Int4KVManager(1, 1, 1, D, 32, 64, gpu, capacity_tokens=T)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    ref, tol = exact(q[:, :, -1:], key, value, [T], 64, 1.0, "bf16", many=True)
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, 1.0)
+    assert_within(out[:, :, -1:], ref, tol)
+    assert prefixes() == [1] and 0.9 < float(ref.min()) < 1.1
