@@ -7,16 +7,16 @@
 //     S_t = sum_g scale_t,g (code_t,g . q_g) + min_t,g sum(q_g),  p = 2^(S c - ref),  O^T = V^T . P^T,  l = sum p.
 // Keys enter as their codes, which fp16 holds, and scale and minimum in fp32 as in the general kernel: as fp16 s * code + m a
 // Key was off by 2^-12 of itself, which beside a channel that is large in every token (a bias of 400) moved weights by a
-// hundredth and more.  (In two exact fp16 parts, scale * code, Keys take twice the LDS reads and products: 263 us against 223
-// below.)  With several groups, the minima's terms are a product of their own, sixteen deep, of the fp16 factors as
+// hundredth and more.  (In two exact fp16 parts, scale * code, Keys take twice the LDS reads and products: 263 us in
+// place of 222 below.)  With several groups, the minima's terms are a product of their own, sixteen deep, of the fp16 factors as
 // they stand and the queries' sums in two fp16 parts (2^-22 of them); with one group of 128 they are a sum per score, for
 // the product's registers spill (223 us against 238).
 // A query row is scaled by a power of two so that its largest element lies in [1, 2); the factor goes into c.  Values enter as
-// fp16 s * code + m, off by 2^-12 of their size, and so does a weight p; against bf16's rounding of the output that
+// fp16 s * code + m, times a power of two of the split's, off by 2^-12 of their size, and so does a weight p; against bf16's rounding of the output that
 // is little (rel. error 1.66e-3 to 1.69e-3, its own 1.64e-3 to 1.66e-3), against fp16's it is not, so bf16 rows
 // alone come here.
 //
-// 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128 / 64 / 32: calls of 223 / 250 / 278 us where the general
+// 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128 / 64 / 32: calls of 222 / 237 / 266 us where the general
 // kernel alone takes 273 / 324 / 417; 14 / 2 heads of 64, groups of 64 / 32: 85 / 91 and 105 / 136.
 //
 // Double-buffered: a record's codes are loaded into registers two records ahead (a lane's sixteen bytes are exactly
@@ -76,6 +76,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     constexpr int kK = 2 * CH * kWave, kV = VT * kWave;  // 16-byte pieces of a record's Keys and Values
     __shared__ u32x4 lds[2][kK + kV];
     __shared__ __attribute__((aligned(16))) uint32_t key_pairs[2][G * kBlock];  // Keys' scales and minima
+    __shared__ float widest[kWaves];
     const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
@@ -84,6 +85,26 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     const int n = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
     const int records = prefix_records(a, len, n, tile);
     const int per = (records + a.prefix - 1) / a.prefix, first = min(part * per, records), last = min(first + per, records);
+
+    // 2^up takes the split's largest Value to 2^14 .. 2^15: read back a Value reaches 16 * 65 504, fp16's infinity, and 2^-14 is
+    // where fp16 begins to lose bits.  (One that is not finite takes no part.)  The scales and minima are read twice for it: 3, 5
+    // and 9 us of the calls above with groups of 128, 64 and 32.
+    float most_value = 0.f;
+    for (int k = threadIdx.x; k < (last - first) * 8 * G; k += kWaves * kWave) {
+        const u32x4 pair = reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(first + k / (8 * G)) * R::bytes + R::vsm)[k % (8 * G)];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float m = pair_min(pair[i]), v = fmaxf(fabsf(m), fabsf(fmaf(15.f, pair_scale(pair[i]), m)));
+            most_value = fmaxf(most_value, v < 4e6f ? v : 0.f);
+        }
+    }
+    most_value = wave_max(most_value);
+    if (lane == 0) widest[wave] = most_value;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) most_value = fmaxf(most_value, widest[w]);
+    const int up = in_sgpr(min(max(141 - static_cast<int>(__float_as_uint(most_value) >> 23), -14), 15));
+    const f16x2 raise = halves(static_cast<uint32_t>(15 + up) * 0x04000400u);
 
     // This wave's share of a record: 0, 1: sixteen Key rows; 2, 3: half of a lane's Value words.
     constexpr int VW = VT / 2;                          // a lane's Value words
@@ -131,8 +152,8 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
                 f16x2 s[4], m[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[i] = halves(lower_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i]));
-                    m[i] = halves(upper_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i]));
+                    s[i] = halves(lower_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i])) * raise;
+                    m[i] = halves(upper_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i])) * raise;
                 }
 #pragma unroll
                 for (int c = k * (VW / VG); c < (k + 1) * (VW / VG); ++c)
@@ -297,6 +318,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
         if (!token)
 #pragma unroll
             for (int v = 0; v < VT; ++v) o[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+#pragma unroll
+        for (int v = 0; v < VT; ++v) o[t][v] *= down;
         each_run<D, GROUP>(o[t], quad, [&](int c, const float (&x)[4]) { store_row<LF_FP32>(a.part_o, at * D + c, x); });
     }
 }

@@ -4,7 +4,7 @@ import torch
 
 from logitfill_amd.packed import Int4KVManager, int4, int4_attention
 from tests.int4_exact import exact, prefixes  # noqa: F401  (a fixture)
-from tests.int4_helpers import assert_within
+from tests.int4_helpers import assert_within, query, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,27 @@ def test_very_many_tokens_of_small_weight(gpu, monkeypatch, prefixes):  # noqa: 
     out = int4_attention(mgr, 0, q.to(gpu), None, None, 1.0)
     assert_within(out[:, :, -1:], ref, tol)
     assert prefixes() == [1] and 0.9 < float(ref.min()) < 1.1
+
+
+@pytest.mark.parametrize("D,group", [(128, 128), (128, 64), (128, 32), (64, 64), (64, 32)])
+def test_rows_past_fp16(gpu, monkeypatch, prefixes, D, group):  # noqa: F811
+    """Values read back of up to 9e5 in one group, of 1e-4 in the next sequence, and Keys as large beside small queries; in
+    rows of float32, for minima and scales are float16."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)
+    T, n, n_q, H = 900, 40, 8, 2
+    key, value = rows((3, H, T, D), "fp32", D + group)
+    key[0, :, :, :group] = key[0, :, :, :group] / key[0, :, :, :group].abs().amax() * 4e5 + 3.4e5
+    value[0, :, ::3, :group] = value[0, :, ::3, :group] / value[0, :, :, :group].abs().amax() * 4.5e5 + 4.2e5
+    key[0, :, :, 0] = -6e4  # (every row's minimum within fp16)
+    value[0, :, ::3, 0] = -3e4
+    value[1] *= 1e-4
+    value[2, :, ::50] *= 2.0 ** 12
+    q = query((3, n_q, n, D), "bf16", D)
+    q[0, :, :, :group] *= 2.0 ** -16
+    mgr = Int4KVManager(1, n_q, H, D, 32, group, gpu, batch_size=3)
+    mgr.commit(0, key.to(gpu), value.to(gpu))
+    assert float(mgr.layers[0].read(0, T)[1][0].max()) > 7e5
+    out = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5)
+    ref, tol = exact(q, key, value, [T] * 3, group, D ** -0.5, "bf16", many=True)
+    assert_within(out, ref, tol)
+    assert all(p > 0 for p in prefixes())
