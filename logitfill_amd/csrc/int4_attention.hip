@@ -14,7 +14,9 @@
 // 7.5 scale) is kept in fp32), so that a rounding of P' weighs as the code's distance from it.  In one part of bf16 the
 // roundings of P' were as large as the bf16 output's own (rel. error 2.4e-3 to 2.7e-3 against 1.7e-3); fp16's eight times
 // smaller ones need P' in its range: the reference point is moved by log2 of the largest Value scale of the wave's records
-// (tops), so that P' stays below 2^15.
+// (tops), so that P' stays below 2^15; in two parts, where a group's scales are 2^r below that, its P' is raised by 2^r (a group
+// whose Values are 2^10 smaller had a rel. error of 9e-6 in float32, 2^14 smaller 2e-4, against 4e-8 alone).  One part
+// loses a weight 2^-31 2^r of its row's largest.
 //
 // float32 rows keep more: there both products take code - 7.5 in fp16 (one packed sum per pair), for the 16 and the middle
 // are three times what the codes themselves reach and leave their roundings in the scores (rel. error 1.7e-6 to 2.7e-6
@@ -229,19 +231,43 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     if (ahead && count == 0) wait_ring<0>();
 
     // The weights are 2^(score - ref) with ref = largest score + lift: P' <= 2^8 2^-lift scale < 2^15 for this wave's
-    // records, whose largest Value scales lie below 2^(lift + 7).
+    // records, whose largest Value scales lie below 2^(lift + 7).  In two parts P' is multiplied by ``raise``, too, up to that bound of
+    // its own group's scales: its second part would be lost where they are much smaller.  The scales are read twice for it
+    // (16 sequences of 32K tokens, 28 / 4 heads of 128, groups of 64: fp16 73 -> 77 us, float32 85 -> 87).
+    const auto block_at = [&](int k) {  // (of an entry that is not attended, the first page's)
+        const int at = first + wave + k * kWaves;
+        if (!a.n_pages) return at;
+        const int e = at / per_page, page = lds_pages[e - first / per_page];
+        return max(page, 0) * per_page + (at - e * per_page);
+    };
+    const auto exponent = [](uint32_t scale) { return static_cast<int>(__float_as_uint(f16_to_f32(static_cast<uint16_t>(scale))) >> 23); };
     uint32_t most_scale = 0;
-    for (int k = lane; k < count; k += kWave) {
-        int block = first + wave + k * kWaves;
-        if (a.n_pages) {
-            const int e = block / per_page, page = lds_pages[e - first / per_page];
-            block = max(page, 0) * per_page + (block - e * per_page);
-        }
-        most_scale = max(most_scale, static_cast<uint32_t>(*int4_top(a.L, b, h, block)));
-    }
+    float raise[G];
+    if constexpr (NP == 1) {
+        for (int k = lane; k < count; k += kWave) most_scale = max(most_scale, static_cast<uint32_t>(*int4_top(a.L, b, h, block_at(k))));
 #pragma unroll
-    for (int m = 1; m < kWave; m <<= 1) most_scale = max(most_scale, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most_scale), m, kWave)));
-    const float lift = static_cast<float>(static_cast<int>(__float_as_uint(f16_to_f32(static_cast<uint16_t>(most_scale))) >> 23) - 126 - 7);
+        for (int m = 1; m < kWave; m <<= 1) most_scale = max(most_scale, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most_scale), m, kWave)));
+    } else {
+        constexpr int Piece = 8 * G, Take = kWave / Piece;  // 16-byte pieces of a record's pairs, and records a load takes
+        uint32_t mine = 0;
+        for (int k = lane / Piece; k < count; k += Take) {
+            const u32x4 pair = reinterpret_cast<const u32x4*>(base + static_cast<int64_t>(block_at(k)) * R::bytes + R::vsm)[lane % Piece];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mine = max(mine, pair[r] & 0xffffu);  // (fp16 numbers above zero are ordered as their bits)
+        }
+        mine = min(mine, 0x7bffu);
+#pragma unroll
+        for (int m = 1; m < kWave; m <<= 1)
+            if (m < 8 || m >= Piece) mine = max(mine, static_cast<uint32_t>(__shfl_xor(static_cast<int>(mine), m, kWave)));
+#pragma unroll
+        for (int g = 0; g < G; ++g) most_scale = max(most_scale, static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), 8 * g)));
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const uint32_t of = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), 8 * g));
+            raise[g] = __uint_as_float(static_cast<uint32_t>(127 + (of ? exponent(most_scale) - exponent(of) : 0)) << 23);
+        }
+    }
+    const float lift = static_cast<float>(exponent(most_scale) - 126 - 7);
 
     QueryParts q[CH];
     float qsum[G];
@@ -377,6 +403,11 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
                     pm[g] = fmaf(p[t][r], pair_min(pair[t][r]), pm[g]);
                     pm[g] = fmaf(7.5f, x[t][r], pm[g]);
                 }
+            if constexpr (NP > 1)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[t][r] *= raise[g];
             const HalfParts<NP> w = half_parts<NP>(x[0], x[1]);
             if constexpr (!kCentred)
 #pragma unroll
@@ -419,7 +450,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     const float mine = m_wave == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m_wave - m_all);
 #pragma unroll
     for (int t = 0; t < VT; ++t) {
-        o[t] = (o[t] + fix[t / TG] + pm[t / TG]) * mine;
+        o[t] += fix[t / TG];
+        if constexpr (NP > 1) o[t] *= __uint_as_float((254u << 23) - __float_as_uint(raise[t / TG]));  // (its reciprocal)
+        o[t] = (o[t] + pm[t / TG]) * mine;
         if (wave > 0) *reinterpret_cast<f32x4*>(lds_o + ((wave - 1) * kTile + col) * S::pad + 16 * t + 4 * quad) = o[t];
     }
     __syncthreads();

@@ -11,7 +11,8 @@ Per element, with w the weights, e a weight's relative error and o the output:
 * many-row kernel: a weight and a Value in fp16 (half a step 2^-11), a weight below 2^-14 off by 2^-25 where the largest
   is at least 2^7, a Value by 2^-25 where the split's largest is at least 2^14 (or all times 2^15), a query off by
   2^-25 of its row's largest element; its sum over a group in two fp16 parts (2^-22);
-* sums over the records and merges: 2^-23 per record of sum w (|v| + 32 scale);
+* sums: 5 steps inside a product of 32, one per record and the merges', 2^-23 each of sum w (|v| + 32 scale), in float32,
+  whose codes count from their middle, of sum w (|v| + 8 scale);
 * the output's own rounding, half a step."""
 from __future__ import annotations
 
@@ -69,7 +70,7 @@ def row_bound(q, k: Rows, v: Rows, scaling, w, peak, out, dtype: str, many: bool
         small = T * 2.0 ** -32 * peak
         floor = 2.0 ** -25 * max(av.max() * 2.0 ** -13, 2.0 ** -15)
         bound += 2.0 ** -11 * (w @ av) + small * (av.max(0) + np.abs(out)) + 16 * floor
-    bound += (T / 32 + 40) * 2.0 ** -23 * (w @ v.size + np.abs(out))
+    bound += (T / 32 + 20) * 2.0 ** -23 * (w @ (av + (8 if dtype == "fp32" else 32) * v.scale) + np.abs(out))
     return bound + HALF_STEP[dtype] * (np.abs(out) + bound) + 1e-37
 
 
