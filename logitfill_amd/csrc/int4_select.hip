@@ -1,8 +1,10 @@
 // Page selection of the 4-bit row cache: a score per page from its Keys' bounds, and the pages of highest score.
 //
 // score(page) = max over the kv head's query heads of sum_c max(q_c lo_c, q_c hi_c): no Key of the page has a larger
-// q . k.  Products of a bf16 bound and a query element are exact in float64 and so, but for queries whose elements
-// span more than 2^20, are their sums: the choice does not hang on the order in which they are formed.
+// q . k.  Products of a bf16 bound and a query element are exact in float64: 16 bits of a bf16 query's, 19 of fp16's, 32
+// of float32's.  So is their sum, and the choice then does not hang on its order, where the product's bits, the spans of the
+// query's elements and of the page's bounds and log2(head_dim) come to 53 together: at head_dim 128 spans of 2^30, 2^27 and 2^14
+// in all.  Beyond that a sum is off by 2^-53 of sum |q bound| a step, and of pages closer than that any may be chosen.
 #include "int4_common.hpp"
 
 namespace lf {
@@ -38,8 +40,9 @@ __device__ __forceinline__ uint64_t score_key(double x) {
 
 // D / 8 lanes take a page, eight channels each, and eight heads at a time: the heads' elements stay in registers, the
 // bounds are widened once for all heads, and the heads' sums are exchanged so that each step of the butterfly halves the
-// heads a lane still adds up.  Bound by the float64 arithmetic (a sum and its select per head, channel and page: 11 us for
-// 16 384 pages of 128 channels and 7 heads, 8.4 MB).  Measured beside it: four pages a lane with the queries kept in
+// heads a lane still adds up.  11 us for 16 384 pages of 128 channels and 7 heads, 8.4 MB, and neither of them bounds it: a
+// wave issues some 970 vector instructions around 64 float64 sums a lane (both operands widened, a select per product, the
+// exchanges of doubles), one after the other's result, the VALU 32 % busy.  Measured beside it: four pages a lane with the queries kept in
 // float64, 21 us (256 registers, one wave a SIMD); products of float64 matrix instructions, max(q, 0) hi + min(q, 0) lo
 // over tiles of sixteen heads, 9 us, and 22 in one launch with the choice below (they do four times the products).
 constexpr int kHeads = 8;

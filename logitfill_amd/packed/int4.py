@@ -618,7 +618,8 @@ def select_pages(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, to
     ``query [B, n_q, q_len, D]``: the sequence's last ``q_len`` tokens, already committed.  Candidates
     are the pages before the query's own one (which ``int4_attention`` attends by itself); a page's
     score is the largest, over the kv head's query heads, of ``sum_c max(q_c lo_c, q_c hi_c)`` with the
-    page's ``page_bounds``, formed in float64.  Equal scores: the lower page first.
+    page's ``page_bounds``, formed in float64 (exact but for elements that span very much: ``lf_int4_select``).  Equal
+    scores: the lower page first, NaN ones last.
     """
     query = _check_query(manager, query, True)
     top_pages = int(top_pages)
