@@ -497,14 +497,18 @@ def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3, overhead: float = 
 
 
 # From this many query rows per kv head up, this many tokens in front of the queries, and this many products of a
-# row's channel and a token's in front of them, the many-row kernel takes what every query sees (bf16: it holds Keys and
-# weights in fp16).  It unpacks a record once for 128 rows and costs two launches and 128-row partial sums: 28 / 4 heads of
-# 128, groups of 128 over 16K tokens, general against many-row, us: 32 queries (1.9e9 products) 31 / 45, 64 49 / 59, 128
-# (7.5e9) 80 / 74, 512 (3e10) 235 / 179; four sequences of 4K, 128 queries 73 / 77.  Groups of 32 cost the general kernel
-# more (64 queries 68 / 61, 512 369 / 215).
+# row's channel and a token's in front of them (per 32 channels of a group: the general kernel takes a term per group), the
+# many-row kernel takes what every query sees (bf16: it holds weights and Values in fp16).  It unpacks a record once for 128
+# rows, and costs two launches, 128-row partial sums and their merge, which is work per row: past MANY_ROWS_FULL rows in all
+# the products have to grow with them.  28 / 4 heads of 128, general against many-row, us, groups of 128, 64 and 32 (32 / 8
+# heads): one sequence of 16K tokens, 64 queries 45 / 58, 51 / 53, 67 / 54 (28 / 4), 128 73 / 74, 86 / 75, 118 / 81, 512 225 /
+# 192, 266 / 203, 359 / 241; four of 4K, 512 queries 210 / 236, 254 / 237, 390 / 284; of 2K 108 / 154, 131 / 153, 201 / 181;
+# of 16K 827 / 624, 993 / 741, 1 556 / 896.  14 / 2 heads of 64, one sequence of 16K, 512 queries, groups of 64 and 32: 95 / 76
+# and 119 / 79; four of 2K 42 / 63 and 53 / 65.
 MANY_ROWS = 64
 MANY_ROWS_HISTORY = 256
-MANY_ROWS_WORK = 6e9
+MANY_ROWS_WORK = 3e9
+MANY_ROWS_FULL = 12000
 
 
 def _many_rows(group: int, q_len: int, n_kv: int, head_dim: int, group_size: int, dtype, tokens) -> bool:
@@ -513,7 +517,7 @@ def _many_rows(group: int, q_len: int, n_kv: int, head_dim: int, group_size: int
     if rows < MANY_ROWS or head_dim > 128 or dtype != torch.bfloat16 or max(tokens) < q_len + MANY_ROWS_HISTORY:
         return False
     work = sum(n - q_len for n in tokens if n > q_len) * rows * n_kv * head_dim
-    return work >= MANY_ROWS_WORK * (0.5 if group_size == 32 else 1.0)
+    return work >= MANY_ROWS_WORK * {32: 1, 64: 2, 128: 3}[group_size] * max(1.0, rows * n_kv * len(tokens) / MANY_ROWS_FULL)
 
 
 def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, key_new: Optional[torch.Tensor],

@@ -27,3 +27,12 @@ def test_the_dense_path_of_packed_pages():
     manager = int4.Int4KVManager.__new__(int4.Int4KVManager)
     with pytest.raises(ValueError, match="int4_attention"):
         attach_packed(None, manager, reference_attention)
+
+
+def test_many_row_rule_by_the_work_in_front_of_every_row():
+    """Rows add partial sums and their merge: short histories stay with the general kernel, however many rows there are (four
+    sequences of 2K tokens, 1 024 queries, groups of 128: 277 us by the many-row kernel, 186 without)."""
+    for args, want in (((7, 1024, 4, 128, 128, torch.bfloat16, [2048] * 4), False), ((7, 512, 4, 128, 128, torch.bfloat16, [4096] * 4), False),
+                       ((7, 512, 4, 128, 128, torch.bfloat16, [16384] * 4), True), ((4, 512, 8, 128, 32, torch.bfloat16, [4096] * 4), True),
+                       ((7, 256, 2, 64, 64, torch.bfloat16, [32768]), True), ((7, 1024, 2, 64, 64, torch.bfloat16, [2048] * 4), False)):
+        assert int4._many_rows(*args) is want, args
