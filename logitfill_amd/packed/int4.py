@@ -88,36 +88,63 @@ def _ints(values):
 
 
 class _Lengths:
-    """The device's lengths of a cache's layers, int32 ``[layers, batch]``.  Appends move them on the stream of their call;
-    what the host sets is a launch of its own, which calls on other streams wait for."""
+    """The device's lengths of a cache's layers, int32 ``[layers, batch]``, and their order among streams.
+
+    Appends move them on the stream of their call.  What the host sets (``truncate``, ``reset``) belongs to the stream that
+    was current there: the next call on it brings a layer's lengths along (an append in its arguments, any other
+    call by a launch), and the first call on any other stream sets there what is still to be set and waits for that
+    stream.  Where graphs name the arrays, whose replays ask nobody, the lengths are set at once."""
 
     def __init__(self, layers: int, batch: int, device: torch.device):
         self.device = device
         with torch.inference_mode(False):
             self.rows = torch.zeros(layers, batch, dtype=torch.int32, device=device)
-        self._last = None  # (event, stream) of what the host set last
+        self.layers: list = []
+        self._at = None     # the handle of the stream of the host's last change
+        self._event = None  # there, once another stream has asked
 
-    def set(self, layer: _native.Int4Layer, lengths) -> None:
-        """``lengths`` (per layer, per sequence) on the current stream; ``layer``: a struct whose capacity holds them."""
-        stream = torch.cuda.current_stream(self.device)
+    def changed(self) -> None:
+        """The host has changed lengths (of layers now ``_dirty``) at this place of the current stream."""
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("lengths that the host sets are a step of their own: set them before the capture")
+        self._at, self._event = _native.current_stream_ptr(self.device), None
+
+    def order(self, at: int) -> None:
+        """The current stream, ``at``, behind the host's last change."""
+        if self._at is None or at == self._at:
+            return
+        event = self._event
+        if event is None:
+            there = torch.cuda.ExternalStream(self._at, self.device) if self._at else torch.cuda.default_stream(self.device)
+            with torch.cuda.stream(there):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("the stream on which the cache was truncated is being captured: "
+                                       "call manager.sync_lengths() before the capture")
+                self.send()
+                event = torch.cuda.Event()
+                event.record()
+            self._event = event
+        torch.cuda.current_stream(self.device).wait_event(event)
+
+    def send(self, every: bool = False) -> None:
+        """The host's lengths to the device, of the layers that wait for it (or all), on the current stream."""
+        todo = [layer for layer in self.layers if (layer._dirty or every) and layer.capacity]
+        if not todo:
+            return
+        if len(todo) < len(self.layers):
+            for layer in todo:
+                layer.send_lengths()
+            return
+        s = _native.Int4Layer.from_buffer_copy(max(todo, key=lambda layer: layer.capacity).describe())
         batch = self.rows.shape[1]
         some = max(1, 65535 // batch)  # layers in one call: to it they are more sequences
-        for i in range(0, len(lengths), some):
-            part = [n for row in lengths[i : i + some] for n in row]
-            s = _native.Int4Layer.from_buffer_copy(layer)
+        for i in range(0, len(todo), some):
+            part = [n for layer in todo[i : i + some] for n in layer.lengths]
             s.lens, s.batch = self.rows[i].data_ptr(), len(part)
-            _native.check(_native.load().lf_int4_set_lens(s, _ints(part), stream.cuda_stream), "lf_int4_set_lens")
-        event = torch.cuda.Event()
-        event.record(stream)
-        self._last = (event, stream.cuda_stream)
-
-    def wait(self) -> None:
-        """The current stream behind what the host set last."""
-        if self._last is not None:
-            event, at = self._last
-            stream = torch.cuda.current_stream(self.device)
-            if stream.cuda_stream != at:
-                stream.wait_event(event)
+            _native.check(_native.load().lf_int4_set_lens(s, _ints(part), _native.current_stream_ptr(self.device)),
+                          "lf_int4_set_lens")
+        for layer in todo:
+            layer._dirty = False
 
 
 class _Int4Store:
@@ -138,6 +165,7 @@ class _Int4Store:
         self._bounds: Optional[torch.Tensor] = None
         self._struct: Optional[_native.Int4Layer] = None
         self._order, self._lens = order, lens
+        self._dirty = False  # the device's lengths are behind the host's
         self._tops: Optional[torch.Tensor] = None
         self._captured = False  # a graph names the arrays, and its replays move the device's lengths
         self._kept: list = []   # arrays that a captured graph may still name
@@ -189,8 +217,8 @@ class _Int4Store:
         self._blocks, self._bounds, self._tops = blocks, bounds, tops
         self._cap, self._struct = cap, None
 
-    def layer_struct(self) -> _native.Int4Layer:
-        """The ``lf_int4_layer`` describing this store; the current stream is behind the lengths that the host set."""
+    def describe(self) -> _native.Int4Layer:
+        """The ``lf_int4_layer`` describing this store."""
         if self._cap == 0:
             self.reserve(self.page_size)
         if self._struct is None:
@@ -200,11 +228,28 @@ class _Int4Store:
             s.batch, s.n_kv, s.head_dim = self.batch, self.n_kv, self.head_dim
             s.cap_tokens, s.page_size, s.group = self._cap, self.page_size, self.group_size
             self._struct = s
-        if torch.cuda.is_current_stream_capturing():
-            self._captured = True
-        else:
-            self._order.wait()
         return self._struct
+
+    def send_lengths(self) -> None:
+        """The host's lengths to the device, on the current stream."""
+        _native.check(_native.load().lf_int4_set_lens(self.describe(), _ints(self.lengths),
+                                                      _native.current_stream_ptr(self.device)), "lf_int4_set_lens")
+        self._dirty = False
+
+    def layer_struct(self, lengths: bool = True) -> _native.Int4Layer:
+        """``describe()`` for a call on the current stream, in its place behind what the host set; ``lengths``: the device's
+        up to date there."""
+        s = self.describe()
+        if torch.cuda.is_current_stream_capturing():
+            if lengths and self._dirty:
+                raise RuntimeError("the cache was truncated or reset since its last launch: "
+                                   "call manager.sync_lengths() before the capture")
+            self._captured = True
+            return s
+        self._order.order(_native.current_stream_ptr(self.device))
+        if lengths and self._dirty:
+            self.send_lengths()
+        return s
 
     def page_bounds(self) -> torch.Tensor:
         """bf16 ``[batch, n_kv, capacity / page_size, 2, head_dim]``: every full page's smallest and largest Key per
@@ -251,12 +296,12 @@ class _Int4Store:
         # it is replayed, and advance() the host's
         captured = torch.cuda.is_current_stream_capturing()
         st = _native.load().lf_int4_append(
-            self.layer_struct(), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
+            self.layer_struct(captured), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
             _strides(value), None if captured else _ints(old), None if lengths is None else _ints(lengths), T,
             _native.current_stream_ptr(self.device))
         _native.check(st, "lf_int4_append")
         if not captured:
-            self.lengths = new
+            self.lengths, self._dirty = new, False
 
     @_here
     def read(self, starts, tokens: int, dtype=torch.float32):
@@ -311,6 +356,7 @@ class Int4KVManager:
         self.layers = [_Int4Store(self.n_kv, self.head_dim, self.page_size, self.group_size, self._lens, row,
                                   device=self.device, batch=self.batch_size, capacity_tokens=capacity_tokens)
                        for row in self._lens.rows]
+        self._lens.layers = self.layers
         self._args: dict = {}
 
     def commit(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor, lengths=None) -> None:
@@ -331,8 +377,8 @@ class Int4KVManager:
 
     def truncate(self, lengths) -> None:
         """Forget every layer's tokens past ``lengths[b]`` (an int for all; rejected draft tokens, a prompt's common
-        start).  A write on the current stream: it follows the calls and replays that stand on it, and later calls on
-        other streams wait for it (a replay there does not by itself)."""
+        start).  A write on the current stream: it follows the calls and replays that stand there, and later calls on
+        other streams wait for that stream (a replay does not by itself).  Before a capture, call ``sync_lengths``."""
         lengths = [int(lengths)] * self.batch_size if isinstance(lengths, int) else [int(n) for n in lengths]
         if len(lengths) != self.batch_size:
             raise ValueError("truncate takes one length per sequence")
@@ -343,20 +389,14 @@ class Int4KVManager:
 
     @_here
     def _set_lengths(self, lengths: list) -> None:
-        """Every layer's lengths, the device's at once."""
-        if any(layer.lengths != lengths or layer._captured for layer in self.layers):
-            self._send_lengths([lengths] * len(self.layers))
+        captured = any(layer._captured for layer in self.layers)
+        if captured or any(layer.lengths != lengths for layer in self.layers):
+            self._lens.changed()
             for layer in self.layers:
-                layer.lengths = list(lengths)
+                layer.lengths, layer._dirty = list(lengths), True
+            if captured:
+                self._lens.send()
         self.seq_len = self.layers[-1].length if self.layers else 0
-
-    def _send_lengths(self, lengths: list) -> None:
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("lengths that the host sets are its own step: set them before the capture")
-        widest = max(self.layers, key=lambda layer: layer.capacity)
-        if widest.capacity:  # (else no layer holds a token)
-            self._lens.wait()
-            self._lens.set(widest.layer_struct(), lengths)
 
     def advance(self, tokens) -> None:
         """Tell the host of tokens that replays of a captured step committed on the device (per sequence, or an int for
@@ -373,11 +413,13 @@ class Int4KVManager:
 
     @_here
     def sync_lengths(self) -> None:
-        """Set the device's lengths to the host's on the current stream (after replays that ``advance`` is not told of)."""
-        if self.layers:
-            for layer in self.layers:
-                layer.layer_struct()
-            self._send_lengths([layer.lengths for layer in self.layers])
+        """Set the device's lengths to the host's on the current stream (before a capture; after replays that ``advance`` is
+        not told of)."""
+        for layer in self.layers:
+            layer.describe()
+        self._lens.order(_native.current_stream_ptr(self.device))
+        self._lens.changed()
+        self._lens.send(every=True)
 
     def reset(self) -> None:
         """Forget every token (storage is kept for reuse); a write on the current stream, as ``truncate``."""

@@ -44,6 +44,38 @@ def test_the_second_stream_after_a_truncation(gpu, how):
     assert mgr.layers[0]._lens.tolist() == mgr.layers[1]._lens.tolist() == left
 
 
+def test_streams_that_take_turns(gpu):
+    """Truncations on one busy stream and calls on another, append and attention, a layer each, again and again."""
+    T = 300
+    key, value = rows((1, H, 400, D), "bf16", 24)
+    k, v = key.to(gpu), value.to(gpu)
+    q = query((1, N_Q, 1, D), "bf16", 24)
+    dq = q.to(gpu)
+    mgr = Int4KVManager(3, N_Q, H, D, PAGE, GROUP, gpu, capacity_tokens=512)
+    for layer in range(3):
+        mgr.commit(layer, k[:, :, :T], v[:, :, :T])
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for left in (200, 100, 37):
+        with torch.cuda.stream(first):
+            first.wait_stream(second)
+            _busy(gpu)
+            mgr.truncate(left)
+            mgr.commit(0, k[:, :, 350:352], v[:, :, 350:352])
+        with torch.cuda.stream(second):
+            outs = [int4_attention(mgr, layer, dq, None, None, D ** -0.5) for layer in (1, 0)]
+            mgr.commit(2, k[:, :, 360:361], v[:, :, 360:361])
+            outs.append(int4_attention(mgr, 2, dq, None, None, D ** -0.5))
+        torch.cuda.synchronize()
+        assert [layer.lengths for layer in mgr.layers] == [[left + 2], [left], [left + 1]]
+        assert mgr._lens.rows.tolist() == [[left + 2], [left], [left + 1]]
+        for out, more in zip(outs, ([], [350, 351], [360])):
+            at = list(range(left)) + more
+            ref, tol = expected(q, key[:, :, at], value[:, :, at], [len(at)], GROUP, D ** -0.5, "bf16")
+            assert_within(out, ref, tol)
+        mgr.truncate(left)
+
+
 def test_a_replay_after_a_truncation(gpu):
     """Rejected tokens are taken back between replays of one captured step, with no other call."""
     T = 60
@@ -55,6 +87,12 @@ def test_a_replay_after_a_truncation(gpu):
     for layer in range(2):
         mgr.commit(layer, k[:, :, :T], v[:, :, :T])
     graph = torch.cuda.CUDAGraph()
+    mgr.truncate(T - 1)
+    with pytest.raises(RuntimeError, match="sync_lengths"), torch.cuda.graph(torch.cuda.CUDAGraph()):
+        int4_attention(mgr, 0, dq, None, None, D ** -0.5)
+    mgr.sync_lengths()
+    for layer in range(2):
+        mgr.commit(layer, k[:, :, T - 1:T], v[:, :, T - 1:T])
     with torch.cuda.graph(graph):
         outs = [int4_attention(mgr, layer, dq, step_k, step_v, D ** -0.5) for layer in range(2)]
         with pytest.raises(RuntimeError):
@@ -93,8 +131,10 @@ def test_more_lengths_than_a_launch_takes(gpu):
     mgr.commit(0, key, value)
     mgr.commit(1, key, value)
     mgr.truncate(counts)
+    mgr.sync_lengths()
     assert [layer._lens.tolist() for layer in mgr.layers] == [counts] * 2
     mgr.reset()
+    mgr.sync_lengths()
     assert not mgr._lens.rows.any()
 
 
