@@ -4,7 +4,8 @@ import pytest
 import torch
 
 from logitfill_amd.packed import Int4KVManager, int4_attention
-from tests.int4_helpers import assert_within, expected, query, rows
+from tests.int4_exact import exact
+from tests.int4_helpers import assert_within, query, rows
 
 pytestmark = pytest.mark.gpu
 D, GROUP, PAGE, N_Q, H = 128, 64, 32, 4, 2
@@ -37,7 +38,7 @@ def test_the_second_stream_after_a_truncation(gpu, how):
         outs += [int4_attention(mgr, layer, dq, None, None, D ** -0.5) for layer in range(2)]
         k, v = mgr.layers[1].read(0, 500)
     torch.cuda.synchronize()
-    ref, tol = expected(q, key, value, left, GROUP, D ** -0.5, "bf16")
+    ref, tol = exact(q, key, value, left, GROUP, D ** -0.5, "bf16")
     for out in outs:
         assert_within(out, ref, tol)
     assert not k[0, :, left[0]:].any() and not v[1, :, left[1]:].any()
@@ -71,7 +72,7 @@ def test_streams_that_take_turns(gpu):
         assert mgr._lens.rows.tolist() == [[left + 2], [left], [left + 1]]
         for out, more in zip(outs, ([], [350, 351], [360])):
             at = list(range(left)) + more
-            ref, tol = expected(q, key[:, :, at], value[:, :, at], [len(at)], GROUP, D ** -0.5, "bf16")
+            ref, tol = exact(q, key[:, :, at], value[:, :, at], [len(at)], GROUP, D ** -0.5, "bf16")
             assert_within(out, ref, tol)
         mgr.truncate(left)
 
@@ -110,7 +111,7 @@ def test_a_replay_after_a_truncation(gpu):
         torch.cuda.synchronize()
         assert torch.isfinite(noise) and mgr.layers[1]._lens.tolist() == [n + 1]
         kk, vv = (torch.cat([t[:, :, :n], t[:, :, 70:71]], 2) for t in (key, value))
-        ref, tol = expected(q, kk, vv, [n + 1], GROUP, D ** -0.5, "bf16")
+        ref, tol = exact(q, kk, vv, [n + 1], GROUP, D ** -0.5, "bf16")
         for out in outs:
             assert_within(out, ref, tol)
         mgr.truncate(n)

@@ -73,3 +73,51 @@ def test_rows_past_fp16(gpu, monkeypatch, prefixes, D, group):  # noqa: F811
     ref, tol = exact(q, key, value, [T] * 3, group, D ** -0.5, "bf16", many=True)
     assert_within(out, ref, tol)
     assert all(p > 0 for p in prefixes())
+
+
+def test_chunks_of_a_prompt_are_committed_and_attended(gpu, monkeypatch, prefixes):  # noqa: F811
+    """Ragged chunks through the call the model makes, then a captured one replayed over page ends: both kernels over the
+    device's lengths, the plan the capture's."""
+    monkeypatch.setattr(int4, "MANY_ROWS_WORK", 0)
+    D, group, page, n_q, H, n = 128, 64, 64, 8, 2, 45
+    key, value = rows((2, H, 900, D), "bf16", 41)
+    q = query((2, n_q, 900, D), "bf16", 41)
+    k, v, dq = key.to(gpu), value.to(gpu), q.to(gpu)
+    mgr = Int4KVManager(1, n_q, H, D, page, group, gpu, batch_size=2, capacity_tokens=960)
+    starts = [400, 333]
+    mgr.commit(0, k[:, :, :400], v[:, :, :400], starts)
+
+    def chunk(x, counts):
+        out = torch.zeros(2, x.shape[1], n, D, dtype=x.dtype, device=x.device)
+        for b, (t, c) in enumerate(zip(starts, counts)):
+            out[b, :, :c] = x[b, :, t:t + c]
+        return out
+
+    def check(out, at, counts):
+        ends = [t + c for t, c in zip(starts, counts)]
+        ref, tol = exact(at, key, value, ends, group, D ** -0.5, "bf16", q_lens=counts, many=True)
+        assert_within(out, ref, tol)
+        starts[:] = ends
+
+    for counts in ([n, n], [n, 20], [7, n], [n, 0]):
+        out = int4_attention(mgr, 0, chunk(dq, counts), chunk(k, counts), chunk(v, counts), D ** -0.5, lengths=counts)
+        check(out, chunk(q, counts), counts)
+    assert mgr.layers[0].lengths == starts and prefixes()[0] > 0
+    step = [chunk(x, [n, n]) for x in (dq, k, v)]
+    int4_attention(mgr, 0, *step, D ** -0.5)
+    mgr.truncate(starts)
+    mgr.sync_lengths()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = int4_attention(mgr, 0, *step, D ** -0.5)
+    assert prefixes()[-1] > 0
+    for _ in range(5):
+        for held, x in zip(step, (dq, k, v)):
+            held.copy_(chunk(x, [n, n]))
+        graph.replay()
+        noise = torch.randn(1 << 16, device=gpu).sum()
+        torch.cuda.synchronize()
+        assert torch.isfinite(noise)
+        mgr.advance(n)
+        check(out, chunk(q, [n, n]), [n, n])
+    assert mgr.layers[0].lengths == starts
