@@ -378,7 +378,8 @@ int32_t lf_unpack_ints(const int32_t* words, int64_t rows, int32_t n_words, int3
  * Value of one kv head -- is kept per group of ``group`` channels as 4-bit codes, an fp16 scale and an
  * fp16 minimum, by the rule of lf_asymmetric_codes at 4 bits: lo = min, s = clamp((max - lo) / 15, 1e-5,
  * 1e5), code = clamp(rint((x - lo) / s), 0, 15) in IEEE float32; the value read back is the float32
- * code * fp16(s) + fp16(lo).
+ * code * fp16(s) + fp16(lo).  A group that spans more than 15 * 65 504 or whose minimum lies beyond +-65 504 is not
+ * finite when it is read back (fp16 scales and minima).
  *
  * Storage: ``blocks``, one record per 32 tokens of a (sequence, kv head):
  *   [batch][n_kv][cap_tokens / 32][LF_INT4_BLOCK_BYTES(head_dim, group)], each record

@@ -331,7 +331,8 @@ __global__ void int4_advance_kernel(RowsArgs a) {
 
 // A few tokens behind lengths that only the device knows: a workgroup per sequence, a wave per kv head; the workgroup
 // advances the length, which with a workgroup per page and head takes a launch of its own.  Captured appends of 1, 4 and
-// 8 tokens, 16 sequences of 4 heads of 128: 4.2, 4.5 and 5.5 us; 9 tokens, by pages, 6.6.  With the lengths in the
+// 8 tokens, 16 sequences of 4 heads of 128: 4.2, 4.5 and 5.5 us; 9 tokens, by pages, 6.6.  (A page that is completed gets
+// its bounds head after head: not measured with more than 4.)  With the lengths in the
 // arguments pages are the faster way for any count (one token to 8 sequences that fill a page 6.4 us against 8.1).
 constexpr int kFewTokens = 8;
 template <int D, int GROUP, int Dt>

@@ -490,8 +490,9 @@ MANY_ROWS_OVERHEAD = 4.0
 
 
 def workgroups_per_cu(head_dim: int, group: int) -> int:
-    """Attention workgroups that a CU holds: by registers 4, 3 and 2 at head_dim 64, 128 and 256, and by the record
-    rings' LDS 1 at head_dim 256 with groups of 32."""
+    """Attention workgroups that a plan counts per CU: the 4, 3 and 2 of the kernels' launch bounds at head_dim 64, 128
+    and 256 (the registers of bf16 groups of 128 at head_dim 128, 123, admit 4, those of groups of 64 at head_dim 64,
+    78, admit 6), and by the record rings' LDS 1 at head_dim 256 with groups of 32."""
     return {64: 4, 128: 3, 256: 2 if group > 32 else 1}[head_dim]
 
 

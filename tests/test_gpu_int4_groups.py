@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("D,group", [(64, 32), (128, 32), (128, 64), (256, 32), (256, 128)])
-@pytest.mark.parametrize("dtype", ["fp32", "fp16"])
+@pytest.mark.parametrize("dtype", ["fp32", "fp16", "bf16"])
 @pytest.mark.parametrize("ratio", [10, 20])
 def test_groups_of_unlike_size(gpu, D, group, dtype, ratio):
     T, n, n_q, H, page = 500, 2, 4, 2, 32
