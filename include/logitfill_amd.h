@@ -479,7 +479,8 @@ int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t
  * sum_c max(q_c lo_c, q_c hi_c) with the page's bounds, an upper bound of the page's q . k, summed in
  * float64: exactly, so that the choice does not depend on the order of the sum, where the query's elements and
  * the bounds together span no more than 2^(53 - log2(head_dim) - b), b = 16, 19 and 32 for bf16, fp16 and fp32
- * queries; beyond that to 2^-53 of sum |q bound| a step.  Equal scores: the lower page first; NaN scores come last.  Writes ``pages`` in ascending order, -1 behind the last one.  n_pages <= 1024.
+ * queries; beyond that to 2^-53 of sum |q bound| a step.  Equal scores: the lower page first; NaN scores come
+ * last.  Writes ``pages`` in ascending order, -1 behind the last one.  n_pages <= 1024.
  * Workspace: lf_int4_select_workspace_bytes().
  */
 int32_t lf_int4_select(const lf_int4_layer* layer, const lf_int4_args* args, void* stream);

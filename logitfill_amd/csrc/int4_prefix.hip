@@ -12,9 +12,9 @@
 // they stand and the queries' sums in two fp16 parts (2^-22 of them); with one group of 128 they are a sum per score, for
 // the product's registers spill (223 us against 238).
 // A query row is scaled by a power of two so that its largest element lies in [1, 2); the factor goes into c.  Values enter as
-// fp16 s * code + m, times a power of two of the split's, off by 2^-12 of their size, and so does a weight p; against bf16's rounding of the output that
-// is little (rel. error 1.66e-3 to 1.69e-3, its own 1.64e-3 to 1.66e-3), against fp16's it is not, so bf16 rows
-// alone come here.
+// fp16 s * code + m, times a power of two of the split's, off by 2^-12 of their size, and so does a weight p; against bf16's
+// rounding of the output that is little (rel. error 1.66e-3 to 1.69e-3, its own 1.64e-3 to 1.66e-3), against fp16's it is not,
+// so bf16 rows alone come here.
 //
 // 512 queries of 28 / 4 heads of 128 over 16 384 tokens, groups of 128 / 64 / 32: calls of 222 / 237 / 266 us where the general
 // kernel alone takes 273 / 324 / 417; 14 / 2 heads of 64, groups of 64 / 32: 85 / 91 and 105 / 136.

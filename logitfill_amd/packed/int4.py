@@ -23,6 +23,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import threading
 from typing import Optional
 
 import torch
@@ -100,6 +101,7 @@ class _Lengths:
         with torch.inference_mode(False):
             self.rows = torch.zeros(layers, batch, dtype=torch.int32, device=device)
         self.layers: list = []
+        self.lock = threading.RLock()  # over a layer's host lengths and the launch that takes them to the device
         self._at = None     # the handle of the stream of the host's last change
         self._event = None  # there, once another stream has asked
 
@@ -113,21 +115,22 @@ class _Lengths:
         """The current stream, ``at``, behind the host's last change."""
         if self._at is None or at == self._at:
             return
-        event = self._event
-        if event is None:
-            there = torch.cuda.ExternalStream(self._at, self.device) if self._at else torch.cuda.default_stream(self.device)
-            with torch.cuda.stream(there):
-                if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("the stream on which the cache was truncated is being captured: "
-                                       "call manager.sync_lengths() before the capture")
-                self.send()
-                event = torch.cuda.Event()
-                event.record()
-            self._event = event
+        with self.lock:
+            if self._event is None:
+                there = torch.cuda.ExternalStream(self._at, self.device) if self._at else torch.cuda.default_stream(self.device)
+                with torch.cuda.stream(there):
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("the stream on which the cache was truncated is being captured: "
+                                           "call manager.sync_lengths() before the capture")
+                    self.send()
+                    event = torch.cuda.Event()
+                    event.record()
+                self._event = event
+            event = self._event
         torch.cuda.current_stream(self.device).wait_event(event)
 
     def send(self, every: bool = False) -> None:
-        """The host's lengths to the device, of the layers that wait for it (or all), on the current stream."""
+        """The host's lengths to the device, of the layers that wait for it (or all), on the current stream; under the lock."""
         todo = [layer for layer in self.layers if (layer._dirty or every) and layer.capacity]
         if not todo:
             return
@@ -248,7 +251,8 @@ class _Int4Store:
             return s
         self._order.order(_native.current_stream_ptr(self.device))
         if lengths and self._dirty:
-            self.send_lengths()
+            with self._order.lock:
+                self.send_lengths()
         return s
 
     def page_bounds(self) -> torch.Tensor:
@@ -295,13 +299,15 @@ class _Int4Store:
         # the rows go where the host's lengths end and the device's follow; a captured commit moves the device's own, when
         # it is replayed, and advance() the host's
         captured = torch.cuda.is_current_stream_capturing()
-        st = _native.load().lf_int4_append(
-            self.layer_struct(captured), key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key),
-            _strides(value), None if captured else _ints(old), None if lengths is None else _ints(lengths), T,
-            _native.current_stream_ptr(self.device))
-        _native.check(st, "lf_int4_append")
-        if not captured:
-            self.lengths, self._dirty = new, False
+        s = self.layer_struct(captured)
+        with self._order.lock:
+            st = _native.load().lf_int4_append(
+                s, key.data_ptr(), value.data_ptr(), _native.dtype_code(key.dtype), _strides(key), _strides(value),
+                None if captured else _ints(old), None if lengths is None else _ints(lengths), T,
+                _native.current_stream_ptr(self.device))
+            _native.check(st, "lf_int4_append")
+            if not captured:
+                self.lengths, self._dirty = new, False
 
     @_here
     def read(self, starts, tokens: int, dtype=torch.float32):
@@ -391,11 +397,12 @@ class Int4KVManager:
     def _set_lengths(self, lengths: list) -> None:
         captured = any(layer._captured for layer in self.layers)
         if captured or any(layer.lengths != lengths for layer in self.layers):
-            self._lens.changed()
-            for layer in self.layers:
-                layer.lengths, layer._dirty = list(lengths), True
-            if captured:
-                self._lens.send()
+            with self._lens.lock:
+                self._lens.changed()
+                for layer in self.layers:
+                    layer.lengths, layer._dirty = list(lengths), True
+                if captured:
+                    self._lens.send()
         self.seq_len = self.layers[-1].length if self.layers else 0
 
     def advance(self, tokens) -> None:
@@ -418,8 +425,9 @@ class Int4KVManager:
         for layer in self.layers:
             layer.describe()
         self._lens.order(_native.current_stream_ptr(self.device))
-        self._lens.changed()
-        self._lens.send(every=True)
+        with self._lens.lock:
+            self._lens.changed()
+            self._lens.send(every=True)
 
     def reset(self) -> None:
         """Forget every token (storage is kept for reuse); a write on the current stream, as ``truncate``."""

@@ -1,5 +1,7 @@
 """Lengths that the host sets (truncate, reset) reach the device in their place: before replays on the same stream, and
 before calls on any other."""
+import threading
+
 import pytest
 import torch
 
@@ -75,6 +77,50 @@ def test_streams_that_take_turns(gpu):
             ref, tol = exact(q, key[:, :, at], value[:, :, at], [len(at)], GROUP, D ** -0.5, "bf16")
             assert_within(out, ref, tol)
         mgr.truncate(left)
+
+
+def test_threads_with_a_layer_and_a_stream_each(gpu):
+    """After a truncation one thread appends to its layer while others read theirs; the streams have waited for it."""
+    T, L = 120, 4
+    key, value = rows((1, H, 200, D), "bf16", 25)
+    k, v = key.to(gpu), value.to(gpu)
+    q = query((1, N_Q, 1, D), "bf16", 25)
+    dq = q.to(gpu)
+    mgr = Int4KVManager(L, N_Q, H, D, PAGE, GROUP, gpu, capacity_tokens=256)
+    for layer in range(L):
+        mgr.commit(layer, k[:, :, :T], v[:, :, :T])
+    streams = [torch.cuda.Stream() for _ in range(L)]
+    torch.cuda.synchronize()
+    for left in range(100, 60, -2):
+        with torch.cuda.stream(streams[0]):
+            mgr.truncate(left)
+        outs, failed = [None] * L, []
+        start = threading.Barrier(L)
+
+        def work(i):
+            try:
+                with torch.cuda.stream(streams[i]):
+                    start.wait(30)
+                    if i % 2 == 0:
+                        mgr.commit(i, k[:, :, 150:153], v[:, :, 150:153])
+                    outs[i] = int4_attention(mgr, i, dq, None, None, D ** -0.5)
+                streams[i].synchronize()
+            except Exception as e:  # (a thread's error is not the test's by itself)
+                failed.append(e)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(L)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(60)
+        assert not failed, failed
+        torch.cuda.synchronize()
+        want = [[left + 3 if i % 2 == 0 else left] for i in range(L)]
+        assert [layer.lengths for layer in mgr.layers] == want and mgr._lens.rows.tolist() == want
+        for i in range(L):
+            at = list(range(left)) + ([150, 151, 152] if i % 2 == 0 else [])
+            ref, tol = exact(q, key[:, :, at], value[:, :, at], [len(at)], GROUP, D ** -0.5, "bf16")
+            assert_within(outs[i], ref, tol)
 
 
 def test_a_replay_after_a_truncation(gpu):
