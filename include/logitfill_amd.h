@@ -486,6 +486,33 @@ int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t
 int32_t lf_int4_select(const lf_int4_layer* layer, const lf_int4_args* args, void* stream);
 int64_t lf_int4_select_workspace_bytes(const lf_int4_layer* layer, int32_t q_len);
 
+/*
+ * Rotary positions: rows of ``query`` and ``key`` turned by their tokens' positions.  Pair j of a row's first
+ * ``rotary_dim`` channels -- (j, rotary_dim / 2 + j), or (2 j, 2 j + 1) where ``interleaved`` -- becomes
+ * (x cos t - y sin t, y cos t + x sin t) times ``factor``, t = 2 pi * position * turns[j]; the other channels
+ * pass through.  Angles are formed in float64, rows rotated in float32 and rounded once.  Outputs do not overlap inputs.
+ * head_dim even, 2 .. 512; rotary_dim even, 2 .. head_dim; batch * tokens below 2^31; n_q + n_kv at most 4096 (either
+ * may be 0, its pointers then NULL).
+ */
+typedef struct lf_rotary_args {
+    const void *query, *key;                  /* [batch][heads][tokens][head_dim] by strides  */
+    void *query_out, *key_out;
+    int32_t dtype;                            /* of all four                                  */
+    int32_t batch, tokens, n_q, n_kv, head_dim, rotary_dim;
+    int32_t interleaved;
+    int64_t q_strides[3], k_strides[3];       /* elements per sequence, head and token; unit channel stride */
+    int64_t qo_strides[3], ko_strides[3];
+    const void* positions;                    /* DEVICE, by strides per sequence and token (0: the same for
+                                                 all); NULL: token s is at position start + s */
+    int64_t position_strides[2];
+    int32_t wide;                             /* positions are int64, else int32              */
+    int64_t start;
+    const double* turns;                      /* DEVICE [rotary_dim / 2]: frequency / 2 pi    */
+    double factor;
+} lf_rotary_args;
+
+int32_t lf_rotary(const lf_rotary_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

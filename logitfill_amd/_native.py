@@ -8,7 +8,7 @@ The library is loaded lazily and only after ``torch`` is imported, so that its
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().with_name("liblogitfill_amd.so")
@@ -122,6 +122,23 @@ class Int4Args(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    """``lf_rotary_args``."""
+
+    _fields_ = [
+        ("query", c_void_p), ("key", c_void_p), ("query_out", c_void_p), ("key_out", c_void_p),
+        ("dtype", c_int32),
+        ("batch", c_int32), ("tokens", c_int32), ("n_q", c_int32), ("n_kv", c_int32),
+        ("head_dim", c_int32), ("rotary_dim", c_int32),
+        ("interleaved", c_int32),
+        ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3),
+        ("qo_strides", c_int64 * 3), ("ko_strides", c_int64 * 3),
+        ("positions", c_void_p), ("position_strides", c_int64 * 2), ("wide", c_int32),
+        ("start", c_int64),
+        ("turns", c_void_p), ("factor", c_double),
+    ]
+
+
 _SIGNATURES = {
     "lf_abi_version": (c_int32, []),
     "lf_build_info": (c_char_p, []),
@@ -158,6 +175,7 @@ _SIGNATURES = {
     "lf_int4_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32, c_int32, c_int32]),
     "lf_int4_select": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
     "lf_int4_select_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32]),
+    "lf_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
 }
 
 ABI_VERSION = 8
