@@ -513,6 +513,46 @@ typedef struct lf_rotary_args {
 
 int32_t lf_rotary(const lf_rotary_args* args, void* stream);
 
+/*
+ * Causal attention of whole prompts: query token j of a sequence, one of its n_q last, sees Keys 0 .. n_k - n_q + j of
+ * the sequence's n_k: out = softmax(scaling q . K^T) V; a token that sees no Key gives zeros.  Query head i reads kv head
+ * i / (n_q / n_kv).  Sequences lie in rows of a batch, padded or one behind another, as the work items say; rows
+ * that no item names are neither read nor written.
+ *
+ * A work item is a tile of tile_rows query rows of a sequence (row r: token r / g, head r % g of the group) and a
+ * range of its Keys in tiles of LF_PROMPT_KEYS(head_dim, dtype); every (item, kv head) is a workgroup, in this order.  A
+ * row tile has one item of slot -1, whose rows go to ``out``, or several that divide its Keys, of consecutive slots
+ * 0 .. n_slots - 1 of the workspace, and an entry of ``merges`` with the first one's slot and their number (parts).
+ */
+typedef struct lf_prompt_item {
+    int32_t q_row, q_start, n_q;              /* the sequence's queries: row of the batch, first token, tokens */
+    int32_t k_row, k_start, n_k;              /* its Keys and Values                          */
+    int32_t tile;                             /* rows tile * tile_rows ..                     */
+    int32_t begin, end;                       /* Key tiles (those behind the last one seen are left out) */
+    int32_t slot, parts;
+    int32_t unused;
+} lf_prompt_item;
+
+#define LF_PROMPT_KEYS(head_dim, dtype) ((head_dim) == 256 || (dtype) == LF_FP32 ? 32 : 64)
+
+typedef struct lf_prompt_args {
+    const void *query, *key, *value;          /* [row][heads][token][head_dim] by strides, 16-byte aligned rows */
+    void* out;
+    int32_t dtype;                            /* of all four                                  */
+    int32_t n_q, n_kv, head_dim;              /* heads; head_dim 64, 128 or 256               */
+    int64_t q_strides[3], k_strides[3];       /* elements per row of the batch, head and token; unit channel stride */
+    int64_t v_strides[3], out_strides[3];
+    float scaling;                            /* finite                                       */
+    int32_t tile_rows;                        /* 32 or 128                                    */
+    const lf_prompt_item* items;              /* DEVICE                                       */
+    const lf_prompt_item* merges;             /* DEVICE (NULL: no row tile is divided)        */
+    int32_t n_items, n_merges, n_slots;
+    void* workspace; int64_t workspace_bytes; /* lf_prompt_workspace_bytes, 16-byte aligned, no initialisation */
+} lf_prompt_args;
+
+int32_t lf_prompt_attention(const lf_prompt_args* args, void* stream);
+int64_t lf_prompt_workspace_bytes(int32_t n_kv, int32_t head_dim, int32_t tile_rows, int32_t n_slots);
+
 #ifdef __cplusplus
 }
 #endif

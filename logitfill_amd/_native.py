@@ -139,6 +139,22 @@ class RotaryArgs(ctypes.Structure):
     ]
 
 
+class PromptArgs(ctypes.Structure):
+    """``lf_prompt_args``."""
+
+    _fields_ = [
+        ("query", c_void_p), ("key", c_void_p), ("value", c_void_p), ("out", c_void_p),
+        ("dtype", c_int32), ("n_q", c_int32), ("n_kv", c_int32), ("head_dim", c_int32),
+        ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3),
+        ("v_strides", c_int64 * 3), ("out_strides", c_int64 * 3),
+        ("scaling", c_float),
+        ("tile_rows", c_int32),
+        ("items", c_void_p), ("merges", c_void_p),
+        ("n_items", c_int32), ("n_merges", c_int32), ("n_slots", c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 _SIGNATURES = {
     "lf_abi_version": (c_int32, []),
     "lf_build_info": (c_char_p, []),
@@ -176,6 +192,8 @@ _SIGNATURES = {
     "lf_int4_select": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
     "lf_int4_select_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32]),
     "lf_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
+    "lf_prompt_attention": (c_int32, [POINTER(PromptArgs), c_void_p]),
+    "lf_prompt_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
 }
 
 ABI_VERSION = 8

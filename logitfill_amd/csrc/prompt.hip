@@ -1,0 +1,415 @@
+// Causal attention of whole prompts on the matrix cores: sequences of any lengths, grouped heads, queries that are the last of
+// their sequence's Keys.
+//
+// A workgroup takes a tile of query rows of one kv head -- row r is token r / g of the sequence and head r % g of the group, so
+// that a tile's rows see nearly the same Keys -- and walks the Keys in tiles that reach LDS by DMA, one ahead.  Per
+// tile and wave, for 32 rows, on v_mfma_f32_32x32x16:
+//     S^T = K . Q^T,   p = 2^(c S - ref),   O^T += V^T . P^T,   l += sum p.
+// A score's lane holds eight of the sixteen Keys that its lane of the second product takes, so P goes from one to the other
+// in registers; the Value operand is read with its Keys in that order by LDS transpose reads.  The reference point of a row
+// moves only when a score passes it by 2^8.
+//
+// Scores and sums are fp32; P is rounded to the rows' type (bf16: 2^-9 of a weight at most, averaged over the Keys, beside the
+// output's own 2^-9; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).
+#include "lf_common.hpp"
+#include "decode_common.hpp"
+
+#include <type_traits>
+
+namespace lf {
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct Prompt {
+    const void *q, *k, *v;
+    void* out;
+    int64_t qs[3], ks[3], vs[3], os[3];  // elements per batch row, head and token
+    const lf_prompt_item* items;
+    int n_q, n_kv, g;
+    float qscale;   // scaling * log2(e)
+    float* part_o;  // [slots][n_kv][rows of a tile][D]
+    float* part_ml; // [slots][n_kv][rows of a tile][2]
+};
+
+template <int Dt> struct Element;
+template <> struct Element<LF_BF16> {
+    using x8 = bf16x8;
+    static constexpr float headroom = 0.f;
+    static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+    }
+};
+template <> struct Element<LF_FP16> {
+    using x8 = f16x8;
+    static constexpr float headroom = 7.f;
+    static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+    }
+};
+
+template <> struct Element<LF_FP32> {
+    using x8 = f32x4;  // (four channels or one Key a product: v_mfma_f32_32x32x2)
+    static constexpr float headroom = 0.f;
+};
+
+// A tile of Keys or Values in LDS: rows in 16-byte pieces, whose places are exchanged by row so that the products'
+// operand reads take all banks.
+template <int D, int Dt>
+struct Tile {
+    static constexpr int esize = Dt == LF_FP32 ? 4 : 2;
+    static constexpr int keys = D == 256 || Dt == LF_FP32 ? 32 : 64;
+    static constexpr int row = esize * D, bytes = keys * row, pieces = row / 16;
+    static constexpr int rows_per_load = 1024 / row, loads = bytes / 1024;
+    static constexpr int lds = 4 * bytes;  // Keys and Values, two tiles
+    static __device__ __forceinline__ int key_swap(int r) { return r & (pieces < 16 ? pieces - 1 : 15); }
+    static __device__ __forceinline__ int value_swap(int r) { return Dt == LF_FP32 ? (r & 4) << 1 : D == 64 ? (r & 2) << 1 : (r & 3) << 2; }
+};
+
+// Max and sum over the two lanes of a query.
+__device__ __forceinline__ float halves_max(float x) {
+    float a, b;
+    swap_rows<true>(x, a, b);
+    return fmaxf(a, b);
+}
+
+__device__ __forceinline__ u32x2 read_tr(uint32_t at) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(static_cast<uintptr_t>(at))));
+}
+__device__ __forceinline__ uint32_t read4(uint32_t at) {
+    typedef __attribute__((address_space(3))) const uint32_t lds_u32;
+    return *reinterpret_cast<lds_u32*>(static_cast<uintptr_t>(at));
+}
+__device__ __forceinline__ u32x4 read16(uint32_t at) {
+    typedef __attribute__((address_space(3))) const u32x4 lds_u32x4;
+    return *reinterpret_cast<lds_u32x4*>(static_cast<uintptr_t>(at));
+}
+
+// NW waves of 32 rows each.
+template <int D, int Dt, int NW>
+__global__ __launch_bounds__(NW * kWave, D == 256 && Dt == LF_FP32 ? 1 : 2) void prompt_kernel(Prompt a) {
+    using T = Tile<D, Dt>;
+    using E = Element<Dt>;
+    using x8 = typename E::x8;
+    constexpr bool kWide = Dt == LF_FP32;
+    constexpr int ES = T::esize, KT = T::keys, KB = KT / 32, SQ = D * ES / 32, CB = D / 32, KK = kWide ? KT / 8 : KT / 16;
+    constexpr int kRows = 32 * NW;
+    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    const int h = blockIdx.x % a.n_kv;
+    const lf_prompt_item item = a.items[blockIdx.x / a.n_kv];
+    const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    const int col = lane & 31, hi = lane >> 5;
+    const uint32_t lds = lds_addr(smem);
+
+    const int row = item.tile * kRows + wave * 32 + col;
+    const int j = row / a.g, i = row - j * a.g;
+    const bool real = j < item.n_q;
+    const int lim = real ? max(item.n_k - item.n_q + j + 1, 0) : 0;  // Keys this row sees
+    int all = real ? lim : 0x7fffffff, top = lim;                    // that every row of the wave sees, and any
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        all = min(all, __shfl_xor(all, m, kWave));
+        top = max(top, __shfl_xor(top, m, kWave));
+    }
+    all = in_sgpr(all);
+    top = in_sgpr(top);
+    // the workgroup's last row that is real sees the most
+    const int last_token = min((item.tile * kRows + kRows - 1) / a.g, item.n_q - 1);
+    const int reach = max(item.n_k - item.n_q + last_token + 1, 0);
+    const int first = item.begin, last = min(item.end, (reach + KT - 1) / KT);
+
+    const unsigned char* kbase = static_cast<const unsigned char*>(a.k) + ES * (item.k_row * a.ks[0] + h * a.ks[1] + static_cast<int64_t>(item.k_start) * a.ks[2]);
+    const unsigned char* vbase = static_cast<const unsigned char*>(a.v) + ES * (item.k_row * a.vs[0] + h * a.vs[1] + static_cast<int64_t>(item.k_start) * a.vs[2]);
+    // Tile t to buffer b: a load instruction takes rows_per_load rows (of Keys past the last one that is seen, that one).
+    const auto fill = [&](int t, int b) {
+#pragma unroll
+        for (int n = 0; n < T::loads / NW; ++n) {
+            const int r = (wave + n * NW) * T::rows_per_load + lane / T::pieces, piece = lane % T::pieces;
+            const int64_t at = min(t * KT + r, reach - 1);
+            const uint32_t to = lds + b * 2 * T::bytes + (wave + n * NW) * 1024;
+            dma16(kbase + ES * at * a.ks[2] + 16 * (piece ^ T::key_swap(r)), to);
+            dma16(vbase + ES * at * a.vs[2] + 16 * (piece ^ T::value_swap(r)), to + T::bytes);
+        }
+    };
+    if (first < last) fill(first, 0);
+
+    x8 q[SQ];
+    {
+        // a lane's channels: of every 16 (float32: 8), the half hi
+        const unsigned char* src = static_cast<const unsigned char*>(a.q) + 16 * hi +
+            ES * (item.q_row * a.qs[0] + static_cast<int64_t>(h * a.g + i) * a.qs[1] + static_cast<int64_t>(item.q_start + j) * a.qs[2]);
+#pragma unroll
+        for (int s = 0; s < SQ; ++s) {
+            u32x4 w = {0, 0, 0, 0};
+            if (real) w = *reinterpret_cast<const u32x4*>(src + 32 * s);
+            q[s] = __builtin_bit_cast(x8, w);
+        }
+    }
+    // A negative scale would make the largest score the smallest: it goes into the queries' signs.
+    if (a.qscale < 0.f)
+#pragma unroll
+        for (int s = 0; s < SQ; ++s) q[s] = -q[s];
+    const float scale = fmaxf(fabsf(a.qscale), 1e-37f);  // (above zero: -inf stays -inf)
+
+    f32x16 o[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) o[c] = f32x16{};
+    float l = 0.f, ref = 0.f, limit = -__builtin_inff();
+
+    // operand addresses inside a tile
+    const uint32_t key_at = col * T::row;
+    const int group = lane >> 4, in16 = lane & 15;  // 16 lanes transpose four rows of sixteen channels
+    const int vrow = 4 * (group >> 1) + (in16 >> 2), vcol = 16 * (group & 1) + 4 * (in16 & 3);
+
+    for (int t = first; t < last; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // tile t is there, and nobody reads the other buffer any more
+        const uint32_t buf = lds + ((t - first) & 1) * 2 * T::bytes;
+        if (t + 1 < last) fill(t + 1, (t + 1 - first) & 1);
+        const int k0 = t * KT;
+        if (k0 >= top) continue;
+        f32x16 s[KB];
+#pragma unroll
+        for (int b = 0; b < KB; ++b) s[b] = f32x16{};
+#pragma unroll
+        for (int n = 0; n < SQ; ++n)
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const int r = 32 * b + col;
+                const u32x4 w = read16(buf + 32 * b * T::row + key_at + 16 * ((2 * n + hi) ^ T::key_swap(r)));
+                if constexpr (kWide) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), q[n][e], s[b], 0, 0, 0);
+                } else {
+                    s[b] = E::mfma(__builtin_bit_cast(x8, w), q[n], s[b]);
+                }
+            }
+        const bool masked = k0 + KT > all;
+        if (masked)
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = k0 + 32 * b + 8 * (r / 4) + 4 * hi + r % 4 < lim ? s[b][r] : -__builtin_inff();
+        float most = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, s[b][r]);
+        most *= scale;
+        if (__any(most > limit)) {
+            most = halves_max(most);
+            const bool moves = most > limit;
+            const float down = !moves ? 1.f : limit == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - most + E::headroom);
+            if (moves) { ref = most - E::headroom; limit = most + 8.f; }
+            l *= down;
+#pragma unroll
+            for (int c = 0; c < CB; ++c) o[c] *= down;
+        }
+        // P as the second product's operands: eight Keys each, 16 kk + 4 hi .. + 3 and 16 kk + 8 + 4 hi .. + 3 (float32: four in
+        // turn, one a product)
+        x8 p[KK];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            if constexpr (kWide) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[kk][e] = __builtin_amdgcn_exp2f(fmaf(s[0][4 * kk + e], scale, -ref));
+                    l += p[kk][e];
+                }
+            } else {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(s[kk / 2][8 * (kk & 1) + 2 * e], scale, -ref));
+                    const float y = __builtin_amdgcn_exp2f(fmaf(s[kk / 2][8 * (kk & 1) + 2 * e + 1], scale, -ref));
+                    l += x + y;
+                    w[e] = E::pack(x, y);
+                }
+                p[kk] = __builtin_bit_cast(x8, w);
+            }
+        }
+        // The same Keys' Values in channels 32 c + col.
+        const auto value = [&](int kk, int c) {
+            if constexpr (kWide) {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int r = 8 * kk + 4 * hi + e;
+                    w[e] = read4(buf + T::bytes + r * T::row + 16 * ((8 * c + col / 4) ^ T::value_swap(r)) + 4 * (col & 3));
+                }
+                return w;
+            } else {
+                const int r = 16 * kk + vrow;  // (8 rows further on, the pieces' exchange is the same)
+                const int piece = (32 * c + vcol) / 8;
+                const uint32_t at = buf + T::bytes + r * T::row + 16 * (piece ^ T::value_swap(vrow)) + 2 * (vcol & 7);
+                const u32x2 x = read_tr(at), y = read_tr(at + 8 * T::row);
+                return u32x4{x[0], x[1], y[0], y[1]};
+            }
+        };
+        const auto multiply = [](u32x4 w, x8 weights, f32x16 sum) {
+            if constexpr (kWide) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), weights[e], sum, 0, 0, 0);
+                return sum;
+            } else {
+                return E::mfma(__builtin_bit_cast(x8, w), weights, sum);
+            }
+        };
+        if (!masked) {
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int c = 0; c < CB; ++c) o[c] = multiply(value(kk, c), p[kk], o[c]);
+        } else {
+            // What stands where a row does not see need not be finite, and 0 * NaN is NaN: where a sum is not finite, one Key
+            // at a time is added to the rows that see it.
+#pragma unroll
+            for (int c = 0; c < CB; ++c) {
+                f32x16 sum = f32x16{};
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) sum = multiply(value(kk, c), p[kk], sum);
+                float test = 0.f;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) test = fmaf(sum[r], 0.f, test);
+                if (__any(test != 0.f)) {
+                    sum = f32x16{};
+#pragma unroll 1
+                    for (int key = 0; key < KT; ++key) {
+                        const int kk = kWide ? key >> 3 : key >> 4, half = (key >> 2) & 1;
+                        const int word = kWide ? key & 3 : ((key & 3) + 4 * ((key >> 3) & 1)) >> 1;
+                        const uint32_t keep = kWide ? 0xffffffffu : 0xffffu << (16 * (key & 1));
+                        u32x4 w = value(kk, c), pk = __builtin_bit_cast(u32x4, p[0]);
+#pragma unroll
+                        for (int n = 1; n < KK; ++n)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) pk[x] = kk == n ? __builtin_bit_cast(u32x4, p[n])[x] : pk[x];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) w[x] &= hi == half && word == x ? keep : 0u;
+                        const f32x16 one = multiply(w, __builtin_bit_cast(x8, pk), f32x16{});
+                        const bool seen = k0 + key < lim;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) sum[r] += seen ? one[r] : 0.f;
+                    }
+                }
+                o[c] += sum;
+            }
+        }
+    }
+
+    l = halves_sum(l);
+    if (!real) return;
+    // channels 32 c + 8 n + 4 hi .. + 3
+    if (item.slot < 0) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // (no Key seen: zeros)
+        const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2] + 4 * hi;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const f32x4 x = {o[c][4 * n] * inv, o[c][4 * n + 1] * inv, o[c][4 * n + 2] * inv, o[c][4 * n + 3] * inv};
+                if constexpr (kWide) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to + 32 * c + 8 * n) = x;
+                else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to + 32 * c + 8 * n) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+            }
+        return;
+    }
+    const int64_t at = (static_cast<int64_t>(item.slot) * a.n_kv + h) * kRows + wave * 32 + col;
+    float* dst = a.part_o + at * D + 4 * hi;
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            *reinterpret_cast<f32x4*>(dst + 32 * c + 8 * n) = f32x4{o[c][4 * n], o[c][4 * n + 1], o[c][4 * n + 2], o[c][4 * n + 3]};
+    if (hi == 0) {
+        a.part_ml[2 * at] = l == 0.f ? -__builtin_inff() : ref;
+        a.part_ml[2 * at + 1] = l;
+    }
+}
+
+// The splits' sums of a tile's rows at their largest reference point: D / 4 lanes a row, a split after the other.
+template <int D, int Dt>
+__global__ __launch_bounds__(256) void prompt_merge_kernel(Prompt a, const lf_prompt_item* items, int tile_rows) {
+    constexpr int L = D / 4;
+    const int h = blockIdx.x % a.n_kv;
+    const lf_prompt_item item = items[blockIdx.x / a.n_kv];
+    const int r = blockIdx.y * (256 / L) + threadIdx.x / L, c = threadIdx.x % L * 4;
+    const int row = item.tile * tile_rows + r, j = row / a.g, i = row - j * a.g;
+    if (r >= tile_rows || j >= item.n_q) return;
+    const int64_t step = static_cast<int64_t>(a.n_kv) * tile_rows, at = item.slot * step + static_cast<int64_t>(h) * tile_rows + r;
+    float m = -__builtin_inff();
+    for (int s = 0; s < item.parts; ++s) m = fmaxf(m, a.part_ml[2 * (at + s * step)]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int s = 0; s < item.parts; ++s) {
+        const float ms = a.part_ml[2 * (at + s * step)], w = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - m);
+        l = fmaf(w, a.part_ml[2 * (at + s * step) + 1], l);
+        o += w * *reinterpret_cast<const f32x4*>(a.part_o + (at + s * step) * D + c);
+    }
+    o *= l == 0.f ? 0.f : 1.f / l;
+    const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2] + c;
+    if constexpr (Dt == LF_FP32) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to) = o;
+    else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to) = u32x2{Element<Dt>::pack(o[0], o[1]), Element<Dt>::pack(o[2], o[3])};
+}
+
+template <int D, int Dt, int NW>
+int launch_rows(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
+    const auto fn = prompt_kernel<D, Dt, NW>;
+    const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), Tile<D, Dt>::lds);
+    if (st != LF_OK) return st;
+    hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(A.n_items) * A.n_kv), dim3(NW * kWave), (Tile<D, Dt>::lds), stream, a);
+    if (A.n_merges) {
+        const int rows = 32 * NW, per = 256 / (D / 4);
+        hipLaunchKernelGGL((prompt_merge_kernel<D, Dt>), dim3(static_cast<uint32_t>(A.n_merges) * A.n_kv, (rows + per - 1) / per), dim3(256), 0,
+                           stream, a, A.merges, rows);
+    }
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? LF_OK : static_cast<int>(err);
+}
+
+template <int D, int Dt>
+int launch_typed(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
+    return A.tile_rows == 32 ? launch_rows<D, Dt, 1>(a, A, stream) : launch_rows<D, Dt, 4>(a, A, stream);
+}
+
+template <int D>
+int launch_dim(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
+    return A.dtype == LF_BF16 ? launch_typed<D, LF_BF16>(a, A, stream)
+           : A.dtype == LF_FP16 ? launch_typed<D, LF_FP16>(a, A, stream)
+                                : launch_typed<D, LF_FP32>(a, A, stream);
+}
+
+}  // namespace
+
+int64_t prompt_part_bytes(int n_kv, int head_dim, int tile_rows, int slots) {
+    return static_cast<int64_t>(slots) * n_kv * tile_rows * (head_dim + 2) * 4;
+}
+
+int launch_prompt(const lf_prompt_args& A, hipStream_t stream) {
+    Prompt a{};
+    a.q = A.query; a.k = A.key; a.v = A.value; a.out = A.out;
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = A.q_strides[i]; a.ks[i] = A.k_strides[i];
+        a.vs[i] = A.v_strides[i]; a.os[i] = A.out_strides[i];
+    }
+    a.items = A.items;
+    a.n_q = A.n_q; a.n_kv = A.n_kv; a.g = A.n_q / A.n_kv;
+    a.qscale = A.scaling * kLog2e;
+    a.part_o = static_cast<float*>(A.workspace);
+    a.part_ml = a.part_o + static_cast<int64_t>(A.n_slots) * A.n_kv * A.tile_rows * A.head_dim;
+    return A.head_dim == 64 ? launch_dim<64>(a, A, stream) : A.head_dim == 128 ? launch_dim<128>(a, A, stream) : launch_dim<256>(a, A, stream);
+}
+
+}  // namespace lf

@@ -1,0 +1,244 @@
+"""Causal attention of whole prompts: sequences of unlike lengths, packed one behind another or padded to a batch.
+
+* ``PromptPlan``       -- the lengths of a batch of prompts and the work they make; kept for all layers.
+* ``prompt_attention`` -- attention of every sequence's tokens to its Keys up to their own.
+
+It is a prompt's first pass, whose rows are not in a cache yet (the caches' own attention serves what follows);
+with more Keys than queries the queries are the last tokens: a prompt fed in pieces, single tokens.  No reference
+counterpart (its prefill runs the model's dense attention, ``src/logitfill/models/qwen2_attention.py:76-146``).
+Nothing here runs on the CPU.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from typing import NamedTuple, Optional
+
+import numpy as np
+import torch
+
+from logitfill_amd import _native
+from logitfill_amd.packed.cache import _check_device
+from logitfill_amd.packed.reference import _cu_count
+
+MAX_TOKENS = 1 << 24  # of a sequence
+# A workgroup's fixed cost, and what a row tile's division into several adds to each (its partial sums written and
+# merged), in Key tiles.
+ITEM_COST, PART_COST = 2.0, 2.0
+
+
+def key_tile(head_dim: int, dtype) -> int:
+    """``LF_PROMPT_KEYS``."""
+    return 32 if head_dim == 256 or dtype == torch.float32 else 64
+
+
+def tile_rows(lengths, group: int) -> int:
+    """Query rows of a workgroup: one wave's 32 where no sequence has more, else four waves' 128."""
+    return 32 if max(lengths) * group <= 32 else 128
+
+
+def split_size(tiles: np.ndarray, n_kv: int, slots: int) -> int:
+    """Key tiles that a workgroup takes at most, of row tiles that see ``tiles`` each: the size of least estimated
+    time over ``slots`` workgroups at once."""
+    longest = int(tiles.max(initial=1))
+    best, size = None, longest
+    for parts in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128):
+        s = max(1, -(-longest // parts))
+        n = -(-np.maximum(tiles, 1) // s)
+        total = float((tiles + n * (ITEM_COST + np.where(n > 1, PART_COST, 0.0))).sum()) * n_kv
+        one = s + ITEM_COST + (PART_COST if parts > 1 else 0.0)
+        cost = max(total / slots + 0.5 * one, one)
+        if best is None or cost < 0.97 * best:
+            best, size = cost, s
+    return size
+
+
+class _Form(NamedTuple):
+    """A plan's work for one form of call, on the device."""
+
+    items: torch.Tensor
+    n_items: int
+    n_merges: int
+    n_slots: int
+    rows: int
+    stream: int
+    event: torch.cuda.Event
+
+
+def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int, rows: int, keys: int, n_kv: int, slots: int):
+    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``), the merges' and the number of partial sums."""
+    n, m = np.asarray(lengths, dtype=np.int64), np.asarray(key_lengths, dtype=np.int64)
+    per = -(-n * group // rows)  # row tiles of every sequence
+    seq = np.repeat(np.arange(len(n)), per)
+    tile = np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)
+    last_token = np.minimum((tile * rows + rows - 1) // group, n[seq] - 1)
+    reach = np.maximum(m[seq] - n[seq] + last_token + 1, 0)
+    tiles = -(-reach // keys)
+    size = split_size(tiles, n_kv, slots)
+    parts = np.maximum(-(-tiles // size), 1)
+    each = -(-tiles // parts)
+    parts = np.maximum(-(-tiles // np.maximum(each, 1)), 1)  # (no part is empty)
+    slot = np.where(parts > 1, np.cumsum(np.where(parts > 1, parts, 0)) - parts, -1)
+    base = np.zeros((len(seq), 12), dtype=np.int64)
+    q_start, k_start = np.cumsum(n) - n, np.cumsum(m) - m
+    base[:, 0], base[:, 1] = (0, q_start[seq]) if packed_q else (seq, 0)
+    base[:, 3], base[:, 4] = (0, k_start[seq]) if packed_k else (seq, 0)
+    base[:, 2], base[:, 5], base[:, 6] = n[seq], m[seq], tile
+    base[:, 9], base[:, 10] = slot, parts
+    merges = base[parts > 1]
+    at = np.repeat(np.arange(len(seq)), parts)
+    part = np.arange(len(at)) - np.repeat(np.cumsum(parts) - parts, parts)
+    items = base[at]
+    items[:, 7] = part * each[at]
+    items[:, 8] = np.minimum(items[:, 7] + each[at], tiles[at])
+    items[:, 9] = np.where(items[:, 9] < 0, -1, items[:, 9] + part)
+    # the longest first: the short ones fill what is left
+    items = items[np.argsort(items[:, 7] - items[:, 8], kind="stable")]
+    return items.astype(np.int32), merges.astype(np.int32), int(np.where(parts > 1, parts, 0).sum())
+
+
+class PromptPlan:
+    """The sequences of a batch of prompts: ``lengths[b]`` query tokens, the last of ``key_lengths[b]`` (default: as many)
+    Keys.  Holds the work of every form of call made with it (head counts, types), on the device: keep it for a
+    model's layers, and as long as a captured graph that used it."""
+
+    def __init__(self, lengths, key_lengths=None, *, device="cuda"):
+        self.lengths = [int(n) for n in lengths]
+        self.key_lengths = list(self.lengths) if key_lengths is None else [int(n) for n in key_lengths]
+        if not self.lengths or len(self.key_lengths) != len(self.lengths):
+            raise ValueError("a plan takes the lengths of at least one sequence, and as many key_lengths")
+        if min(self.lengths + self.key_lengths) < 0 or max(self.lengths + self.key_lengths) > MAX_TOKENS:
+            raise ValueError(f"lengths must lie in 0 .. {MAX_TOKENS}")
+        self.device = _check_device(device)
+        self._forms: dict = {}
+
+    @property
+    def batch(self) -> int:
+        return len(self.lengths)
+
+    def _rows(self, shape, lengths, name: str) -> bool:
+        """Whether sequences of ``lengths`` lie packed in ``[B, heads, T, D]``; ``ValueError`` where they do not fit."""
+        B, T = shape[0], shape[2]
+        if B == self.batch and max(lengths) <= T:
+            return False  # (one sequence: both forms are the same)
+        if B == 1 and self.batch > 1 and sum(lengths) <= T:
+            return True
+        raise ValueError(f"{name} {tuple(shape)} does not hold sequences of {lengths[:8]}{'...' if self.batch > 8 else ''} tokens")
+
+    def _form(self, packed_q: bool, packed_k: bool, group: int, n_kv: int, head_dim: int, dtype) -> _Form:
+        key = (packed_q, packed_k, group, n_kv, head_dim, dtype)
+        form = self._forms.get(key)
+        stream = _native.current_stream_ptr(self.device)
+        if form is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a plan's first call uploads its work: run the step once before the capture")
+            rows, keys = tile_rows(self.lengths, group), key_tile(head_dim, dtype)
+            per_cu = 8 if rows == 32 else 2
+            if dtype == torch.float32 and head_dim == 256:
+                per_cu = 1
+            items, merges, slots = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, keys, n_kv,
+                                              per_cu * _cu_count(self.device))
+            with torch.inference_mode(False):
+                device = _native.upload(np.concatenate([items, merges]).reshape(-1), torch.int32, self.device)
+            event = torch.cuda.Event()
+            event.record(torch.cuda.current_stream(self.device))
+            form = self._forms[key] = _Form(device, len(items), len(merges), slots, rows, stream, event)
+        elif stream != form.stream and not torch.cuda.is_current_stream_capturing():
+            here = torch.cuda.current_stream(self.device)
+            here.wait_event(form.event)
+            form.items.record_stream(here)
+        return form
+
+
+def _check_rows(t: torch.Tensor, name: str, query: torch.Tensor) -> torch.Tensor:
+    """``t`` as the kernel reads it: unit channel stride, rows on 16 bytes."""
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} is on {t.device}; logitfill_amd runs on ROCm devices only")
+    if t.device != query.device:
+        raise ValueError(f"{name} is on {t.device}, the query on {query.device}")
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be [batch, heads, tokens, head_dim], got {tuple(t.shape)}")
+    if t.dtype != query.dtype:
+        raise TypeError("query, key and value must share a dtype")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, which prompt_attention does not give: call it under torch.no_grad()")
+    size = t.element_size()
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:3]):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling: float,
+                     plan: Optional[PromptPlan] = None) -> torch.Tensor:
+    """Causal attention: ``query [B, n_q, T, D]``, ``key / value [B, n_kv, S, D]`` -> ``[B, n_q, T, D]`` (tokens
+    outermost in memory, as an output projection takes it); bf16, fp16 or fp32, any strides, head_dim 64, 128 or 256.
+
+    ``plan``: the sequences.  B of them, each from the start of its own row (padded), or, in a batch of one row, all
+    behind one another (packed); queries and Keys each in one of the two ways.  None: every row is a sequence of
+    all its tokens.  A sequence's queries are the last of its Keys, and each sees the Keys up to its own.  Rows of
+    the output behind a sequence's last token, and rows of queries that see no Key, are zeros.
+
+    Everything is enqueued on the current stream."""
+    scaling = float(scaling)
+    if not math.isfinite(scaling):
+        raise ValueError(f"scaling must be finite, got {scaling}")
+    query, key, value = (_check_rows(t, name, query) for t, name in ((query, "query"), (key, "key"), (value, "value")))
+    B, n_q, T, D = query.shape
+    n_kv = key.shape[1]
+    if key.shape != value.shape or key.shape[3] != D:
+        raise ValueError(f"key and value must be of one shape [B, n_kv, S, {D}], got {tuple(key.shape)} and {tuple(value.shape)}")
+    if n_kv <= 0 or n_q <= 0 or n_q % n_kv:
+        raise ValueError("query heads must divide into KV heads")
+    if D not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256, got {D}")
+    code = _native.dtype_code(query.dtype)
+    if plan is None:
+        if key.shape[0] != B:
+            raise ValueError(f"query has {B} rows, key {key.shape[0]}")
+        if B == 0:
+            return torch.empty(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
+        plan = _whole(B, T, key.shape[2], query.device)
+    elif plan.device != query.device:
+        raise ValueError(f"query is on {query.device}, the plan on {plan.device}")
+    packed_q, packed_k = plan._rows(query.shape, plan.lengths, "query"), plan._rows(key.shape, plan.key_lengths, "key")
+    if max(plan.lengths) * (n_q // n_kv) > 1 << 30:
+        raise ValueError("too many query tokens for one call: feed them in chunks")
+    if torch.cuda.current_device() == query.device.index:
+        return _attend(query, key, value, scaling, plan, packed_q, packed_k, code)
+    with torch.cuda.device(query.device):
+        return _attend(query, key, value, scaling, plan, packed_q, packed_k, code)
+
+
+@functools.lru_cache(maxsize=64)
+def _whole(B: int, T: int, S: int, device) -> PromptPlan:
+    return PromptPlan([T] * B, [S] * B, device=device)
+
+
+def _attend(query, key, value, scaling: float, plan: PromptPlan, packed_q: bool, packed_k: bool, code: int) -> torch.Tensor:
+    """``prompt_attention`` of checked arguments."""
+    B, n_q, T, D = query.shape
+    n_kv = key.shape[1]
+    # (rows that no sequence has are not written by the kernel)
+    make = torch.empty if sum(plan.lengths) == B * T else torch.zeros
+    out = make(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
+    if max(plan.lengths) == 0 or max(plan.key_lengths) == 0:
+        return out.zero_()
+    form = plan._form(packed_q, packed_k, n_q // n_kv, n_kv, D, query.dtype)
+    a = _native.PromptArgs()
+    a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
+    a.dtype, a.n_q, a.n_kv, a.head_dim = code, n_q, n_kv, D
+    a.q_strides[:], a.k_strides[:] = query.stride()[:3], key.stride()[:3]
+    a.v_strides[:], a.out_strides[:] = value.stride()[:3], out.stride()[:3]
+    a.scaling, a.tile_rows = scaling, form.rows
+    a.items, a.n_items = form.items.data_ptr(), form.n_items
+    if form.n_merges:
+        a.merges, a.n_merges, a.n_slots = a.items + 48 * form.n_items, form.n_merges, form.n_slots
+        nbytes = 4 * form.n_slots * n_kv * form.rows * (D + 2)  # lf_prompt_workspace_bytes
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _native.check(_native.load().lf_prompt_attention(ctypes.byref(a), _native.current_stream_ptr(query.device)),
+                  "lf_prompt_attention")
+    return out

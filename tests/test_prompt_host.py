@@ -1,0 +1,100 @@
+"""The prompt attention's work list and its refusals on the host (no GPU)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from logitfill_amd import _native
+from logitfill_amd.packed import PromptPlan, prompt_attention
+from logitfill_amd.packed.prompt import split_size, tile_rows, work_items
+
+
+@pytest.mark.parametrize("seed", range(12))
+@pytest.mark.parametrize("rows,keys", [(32, 64), (128, 64), (128, 32)])
+def test_every_row_tile_s_keys_are_covered_once(seed, rows, keys):
+    rng = np.random.default_rng(seed)
+    B, g, n_kv = int(rng.integers(1, 7)), int(rng.integers(1, 9)), int(rng.integers(1, 9))
+    n = rng.integers(0, 700, B)
+    m = np.maximum(0, n + rng.integers(-20, 4000, B))
+    packed = bool(seed % 2)
+    items, merges, slots = work_items(n, m, packed, not packed, g, rows, keys, n_kv, 512)
+    assert (np.diff(items[:, 8] - items[:, 7]) <= 0).all()  # the longest first
+    assert sorted(items[items[:, 9] >= 0, 9]) == list(range(slots))
+    by_tile = {}
+    for x in items:
+        b = int(x[3])  # (packed queries: Keys are padded, and the other way about)
+        if not packed:
+            b = int(x[0])
+        assert (x[2], x[5]) == (n[b], m[b])
+        assert (x[0], x[1]) == ((0, n[:b].sum()) if packed else (b, 0))
+        assert (x[3], x[4]) == ((b, 0) if packed else (0, m[:b].sum()))
+        by_tile.setdefault((b, int(x[6])), []).append(x)
+    assert len(by_tile) == sum(-(-int(k) * g // rows) for k in n)
+    divided = {(int(x[0] if not packed else x[3]), int(x[6])): x for x in merges}
+    for (b, t), parts in by_tile.items():
+        parts.sort(key=lambda x: x[7])
+        seen = max(0, m[b] - n[b] + min((t * rows + rows - 1) // g, n[b] - 1) + 1)
+        assert parts[0][7] == 0 and parts[-1][8] == -(-seen // keys)
+        assert all(x[8] == y[7] for x, y in zip(parts, parts[1:]))
+        if len(parts) == 1:
+            assert parts[0][9] == -1 and (b, t) not in divided
+        else:
+            assert [x[9] for x in parts] == list(range(parts[0][9], parts[0][9] + len(parts)))
+            assert all(x[8] > x[7] for x in parts)
+            assert (divided[b, t][9], divided[b, t][10]) == (parts[0][9], len(parts))
+
+
+def test_long_keys_of_few_rows_are_divided():
+    assert split_size(np.array([512]), 4, 2048) < 32
+    assert split_size(np.full(4096, 256), 8, 512) == 256  # enough row tiles
+    assert tile_rows([1, 4], 8) == 32 and tile_rows([5], 8) == 128
+
+
+@pytest.mark.parametrize("lengths,keys", [([], None), ([3, -1], None), ([3], [3, 4]), ([1 << 25], None), ([1], [1 << 25])])
+def test_refused_plans(lengths, keys):
+    with pytest.raises(ValueError):
+        PromptPlan(lengths, keys)
+
+
+def test_the_cpu():
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        PromptPlan([3], device="cpu")
+    t = torch.zeros(1, 2, 3, 64)
+    with pytest.raises(RuntimeError, match="ROCm devices only"):
+        prompt_attention(t, t, t, 0.1)
+    with pytest.raises(ValueError, match="finite"):
+        prompt_attention(t, t, t, float("nan"))
+
+
+def _args(**changes):
+    a = _native.PromptArgs()
+    a.dtype, a.n_q, a.n_kv, a.head_dim, a.scaling, a.tile_rows, a.n_items = 0, 4, 2, 64, 0.1, 128, 1
+    for name in ("query", "key", "value", "out", "items"):
+        setattr(a, name, 4096)
+    for name, value in changes.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("changes,status", [
+    ({"dtype": 3}, _native.LF_E_DTYPE), ({"head_dim": 96}, _native.LF_E_UNSUPPORTED), ({"n_q": 3}, _native.LF_E_SHAPE),
+    ({"n_kv": 0}, _native.LF_E_SHAPE), ({"n_items": -1}, _native.LF_E_SHAPE), ({"tile_rows": 64}, _native.LF_E_SHAPE),
+    ({"n_items": 1 << 30, "n_kv": 2}, _native.LF_E_SHAPE), ({"scaling": float("nan")}, _native.LF_E_SHAPE),
+    ({"scaling": float("inf")}, _native.LF_E_SHAPE), ({"n_items": 0}, _native.LF_OK), ({"query": None}, _native.LF_E_NULL),
+    ({"out": None}, _native.LF_E_NULL), ({"items": None}, _native.LF_E_NULL), ({"n_merges": 1}, _native.LF_E_NULL),
+    ({"key": 4098}, _native.LF_E_SHAPE), ({"n_slots": 2}, _native.LF_E_NULL),
+    ({"n_slots": 2, "workspace": 4100}, _native.LF_E_SHAPE), ({"n_slots": 2, "workspace": 4096, "workspace_bytes": 2 * 2 * 128 * 66 * 4 - 1}, _native.LF_E_WORKSPACE),
+])
+def test_the_c_entry_refuses(changes, status):
+    assert _native.load().lf_prompt_attention(ctypes.byref(_args(**changes)), None) == status
+
+
+def test_strides_off_16_bytes_and_null_arguments():
+    lib = _native.load()
+    a = _args()
+    a.v_strides[2] = 68
+    assert lib.lf_prompt_attention(ctypes.byref(a), None) == _native.LF_E_SHAPE
+    assert lib.lf_prompt_attention(None, None) == _native.LF_E_NULL
+    assert lib.lf_prompt_workspace_bytes(2, 64, 128, 2) == 2 * 2 * 128 * 66 * 4
+    assert lib.lf_prompt_workspace_bytes(0, 64, 128, 2) == _native.LF_E_SHAPE
