@@ -474,6 +474,19 @@ int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, 
 int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t q_len, int32_t splits);
 
 /*
+ * The same for sequences that share prefixes: the rows of ``prefix``'s sequence b / (batch / prefix->batch) stand in front of
+ * sequence b's own (batch a multiple of prefix->batch; n_kv, head_dim and group alike), and every prefix is read once for the
+ * queries of all its sequences.  Query token j of a sequence sees rows 0 .. p + lens[b] - n + j of the p + lens[b] rows.  No
+ * pages.  ``shared_splits`` workgroups (1 .. 1024, with splits and prefix_splits at most 1025) share a prefix's tokens,
+ * ``shared_split_tokens`` (a multiple of 32) each, the last one also what is behind them; with ``many_rows`` (bf16, head_dim
+ * 64 or 128) 128 query rows at a time by the many-row kernel, in even shares; there every row that is not finite counts for
+ * queries that stand in front of it, too (of a sequence shorter than its queries).
+ * Workspace: lf_int4_workspace_bytes() of all three.
+ */
+int32_t lf_int4_shared_attention(const lf_int4_layer* layer, const lf_int4_layer* prefix, const lf_int4_args* args,
+                                 int32_t shared_splits, int32_t shared_split_tokens, int32_t many_rows, void* stream);
+
+/*
  * Page selection: for every query token j (at position lens[b] - n + j) and kv head, the n_pages pages of
  * highest score among those before its own page: score = max over the kv head's query heads of
  * sum_c max(q_c lo_c, q_c hi_c) with the page's bounds, an upper bound of the page's q . k, summed in

@@ -188,6 +188,8 @@ _SIGNATURES = {
                                  c_void_p, c_int32, c_void_p]),
     "lf_int4_read": (c_int32, [POINTER(Int4Layer), c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p]),
     "lf_int4_attention": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
+    "lf_int4_shared_attention": (c_int32, [POINTER(Int4Layer), POINTER(Int4Layer), POINTER(Int4Args), c_int32, c_int32, c_int32,
+                                           c_void_p]),
     "lf_int4_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32, c_int32, c_int32]),
     "lf_int4_select": (c_int32, [POINTER(Int4Layer), POINTER(Int4Args), c_void_p]),
     "lf_int4_select_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32]),

@@ -11,6 +11,8 @@ int launch_int4_append(const lf_int4_layer& L, const void* k_src, const void* v_
 int launch_int4_read(const lf_int4_layer& L, const int32_t* starts, int tokens, void* k_out, void* v_out, int dtype,
                      hipStream_t stream);
 int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream);
+int launch_int4_shared(const lf_int4_layer& L, const lf_int4_layer& P, const lf_int4_args& A, int splits, int split_tokens, bool many_rows,
+                       hipStream_t stream);
 int launch_int4_select(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream);
 int64_t int4_part_bytes(const lf_int4_layer& L, int n_q, int q_len, int splits);
 int64_t int4_keys_bytes(const lf_int4_layer& L, int q_len);
@@ -49,6 +51,30 @@ int32_t check_query(const lf_int4_layer* L, const lf_int4_args* A) {
     if (rows * L->n_kv > kGrid) return LF_E_SHAPE;
     if (A->n_pages < 0 || A->n_pages > kMaxPages) return LF_E_SHAPE;
     if (A->n_pages > 0 && !A->pages) return LF_E_NULL;
+    return LF_OK;
+}
+
+// An attention call's arguments, with ``shared`` parts in front of its own.
+int32_t check_attention(const lf_int4_layer* layer, const lf_int4_args* args, int shared) {
+    const int32_t st = check_query(layer, args);
+    if (st != LF_OK) return st;
+    const lf_int4_args& A = *args;
+    if (!A.out) return LF_E_NULL;
+    if (!aligned16(A.out)) return LF_E_SHAPE;
+    if (!std::isfinite(A.scaling)) return LF_E_SHAPE;  // (the kernels take the larger of it and 1e-37)
+    if (A.splits <= 0 || A.splits > kMaxSplits) return LF_E_SHAPE;
+    if (A.n_pages == 0 && A.splits > 1 && (A.split_tokens <= 0 || A.split_tokens % 32 != 0)) return LF_E_SHAPE;
+    if (A.prefix_splits < 0 || A.prefix_splits > kMaxSplits) return LF_E_SHAPE;
+    if (A.prefix_splits > 0) {
+        if (A.splits != 1) return LF_E_SHAPE;
+        if (A.n_pages > 0 || A.dtype != LF_BF16 || layer->head_dim > 128) return LF_E_UNSUPPORTED;
+    }
+    const int parts = A.splits + A.prefix_splits + shared;
+    if (parts > 1) {
+        if (!A.workspace) return LF_E_NULL;
+        if (!aligned16(A.workspace)) return LF_E_SHAPE;
+        if (A.workspace_bytes < lf::int4_part_bytes(*layer, A.n_q, A.q_len, parts)) return LF_E_WORKSPACE;
+    }
     return LF_OK;
 }
 
@@ -103,26 +129,25 @@ int64_t lf_int4_workspace_bytes(const lf_int4_layer* layer, int32_t n_q, int32_t
 }
 
 int32_t lf_int4_attention(const lf_int4_layer* layer, const lf_int4_args* args, void* stream) {
-    const int32_t st = check_query(layer, args);
+    const int32_t st = check_attention(layer, args, 0);
+    return st != LF_OK ? st : lf::launch_int4_attention(*layer, *args, static_cast<hipStream_t>(stream));
+}
+
+int32_t lf_int4_shared_attention(const lf_int4_layer* layer, const lf_int4_layer* prefix, const lf_int4_args* args,
+                                 int32_t shared_splits, int32_t shared_split_tokens, int32_t many_rows, void* stream) {
+    int32_t st = check_int4(prefix);
+    if (st != LF_OK) return st;
+    if (shared_splits <= 0 || shared_splits > kMaxSplits) return LF_E_SHAPE;
+    st = check_attention(layer, args, shared_splits);
     if (st != LF_OK) return st;
     const lf_int4_args& A = *args;
-    if (!A.out) return LF_E_NULL;
-    if (!aligned16(A.out)) return LF_E_SHAPE;
-    if (!std::isfinite(A.scaling)) return LF_E_SHAPE;  // (the kernels take the larger of it and 1e-37)
-    if (A.splits <= 0 || A.splits > kMaxSplits) return LF_E_SHAPE;
-    if (A.n_pages == 0 && A.splits > 1 && (A.split_tokens <= 0 || A.split_tokens % 32 != 0)) return LF_E_SHAPE;
-    if (A.prefix_splits < 0 || A.prefix_splits > kMaxSplits) return LF_E_SHAPE;
-    if (A.prefix_splits > 0) {
-        if (A.splits != 1) return LF_E_SHAPE;
-        if (A.n_pages > 0 || A.dtype != LF_BF16 || layer->head_dim > 128) return LF_E_UNSUPPORTED;
-    }
-    const int parts = A.splits + A.prefix_splits;
-    if (parts > 1) {
-        if (!A.workspace) return LF_E_NULL;
-        if (!aligned16(A.workspace)) return LF_E_SHAPE;
-        if (A.workspace_bytes < lf::int4_part_bytes(*layer, A.n_q, A.q_len, parts)) return LF_E_WORKSPACE;
-    }
-    return lf::launch_int4_attention(*layer, A, static_cast<hipStream_t>(stream));
+    if (A.splits + A.prefix_splits + shared_splits > kMaxSplits + 1) return LF_E_SHAPE;
+    if (prefix->n_kv != layer->n_kv || prefix->head_dim != layer->head_dim || prefix->group != layer->group) return LF_E_SHAPE;
+    if (layer->batch % prefix->batch != 0) return LF_E_SHAPE;
+    if (A.n_pages > 0) return LF_E_UNSUPPORTED;
+    if (many_rows ? A.dtype != LF_BF16 || layer->head_dim > 128 : shared_split_tokens <= 0 || shared_split_tokens % 32 != 0)
+        return many_rows ? LF_E_UNSUPPORTED : LF_E_SHAPE;
+    return lf::launch_int4_shared(*layer, *prefix, A, shared_splits, shared_split_tokens, many_rows != 0, static_cast<hipStream_t>(stream));
 }
 
 int64_t lf_int4_select_workspace_bytes(const lf_int4_layer* layer, int32_t q_len) {

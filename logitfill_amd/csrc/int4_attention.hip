@@ -40,6 +40,7 @@
 
 namespace lf {
 int launch_int4_prefix(const Int4Attention& a, hipStream_t stream);
+int launch_int4_shared_rows(const Int4Attention& a, hipStream_t stream);
 
 namespace {
 
@@ -140,7 +141,8 @@ __device__ __forceinline__ void wait_ring() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-template <int D, int GROUP, int Dt>
+// Shared: of a prefix that ``each`` sequences share; the rows are all their queries, and the sums always partial ones.
+template <int D, int GROUP, int Dt, bool Shared>
 __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(Int4Attention a) {
     using R = Int4Rec<D, GROUP>;
     using S = Ring<D, GROUP>;
@@ -156,12 +158,17 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     // of sequences of unlike lengths (splits first: 32 ragged contexts of 4K-64K tokens in 4 splits 545 us, against 429: 2 of 8 XCDs
     // had the last, mostly empty split) and the row tiles of a head, which read the same records, few of them; the
     // splits last, so that a long sequence's later ones follow everyone's first.
-    const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = a.prefix + blockIdx.z;
+    const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
     // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
     int i, j;
-    if (a.n_pages) {
+    SharedRow row_at;
+    if constexpr (Shared) {
+        row_at = shared_row(a, b, tile * kTile + col);
+        i = row_at.i;
+        j = row_at.j;
+    } else if (a.n_pages) {
         j = tile % a.q_len;
         i = tile / a.q_len * kTile + col;
     } else {
@@ -169,17 +176,18 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         i = r / a.q_len;
         j = r % a.q_len;
     }
-    const bool real = i < a.g;
+    const bool real = Shared ? row_at.real : i < a.g;
+    const int seq = Shared ? row_at.b : b;
     // The first record is on its way before the sequence's length is: where it lies hangs on neither (with pages or
     // behind a many-row prefix it does).  A wave that finds it has none waits for the load all the same.
     const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
     const uint32_t ring = lds_addr(smem) + wave * kRing * R::bytes;
     const int64_t early = static_cast<int64_t>(part) * (a.split_tokens / kBlock) + wave;
-    const bool ahead = !a.n_pages && !a.prefix && early < a.L.cap_tokens / kBlock;
+    const bool ahead = (Shared || (!a.n_pages && !a.prefix)) && early < a.L.cap_tokens / kBlock;
     if (ahead) S::load(base + early * R::bytes, ring, lane);
     const int len = int4_len(a.L, b);
-    const int n = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-    const int lim = real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
+    const int n = Shared ? 0 : a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+    const int lim = Shared ? shared_limit(a, row_at, len) : real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
     int all = real ? lim : 0x7fffffff, top = lim;                 // rows every query of the tile sees, and any
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {
@@ -193,7 +201,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     const int per_page = a.L.page_size / kBlock;
     const int own = top > 0 ? (top - 1) / a.L.page_size : 0;
     int first, last;
-    if (a.n_pages) {
+    if (!Shared && a.n_pages) {
         // (rounded up, splits can pass the list's end: those take nothing and read none of it)
         const int records = per_page * (a.n_pages + 1);
         first = min(part * a.split_tokens, records);
@@ -213,15 +221,15 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         __syncthreads();
     } else {
         const int blocks = (top + kBlock - 1) / kBlock, per = a.split_tokens / kBlock;
-        first = a.prefix ? min(prefix_records(a, len, n, tile / (kManyRows / kTile)), blocks)
-                         : static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
-        last = part + 1 == a.parts ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
+        first = !Shared && a.prefix ? min(prefix_records(a, len, n, tile / (kManyRows / kTile)), blocks)
+                                    : static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
+        last = part + 1 == a.splits ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
     }
     const int count = last > first + wave ? (last - first - wave + kWaves - 1) / kWaves : 0;  // this wave's records
     // The k-th of them, or -1 for one that is not attended (its place in the ring is filled with another).
     const auto block_of = [&](int k) {
         const int at = first + wave + k * kWaves;
-        if (!a.n_pages) return at;
+        if (Shared || !a.n_pages) return at;
         const int e = at / per_page, page = in_sgpr(lds_pages[e - first / per_page]);
         const int block = page * per_page + (at - e * per_page);
         return page < 0 || block * kBlock >= top ? -1 : block;
@@ -241,7 +249,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     // (16 sequences of 32K tokens, 28 / 4 heads of 128, groups of 64: fp16 73 -> 77 us, float32 85 -> 87).
     const auto block_at = [&](int k) {  // (of an entry that is not attended, the first page's)
         const int at = first + wave + k * kWaves;
-        if (!a.n_pages) return at;
+        if (Shared || !a.n_pages) return at;
         const int e = at / per_page, page = lds_pages[e - first / per_page];
         return max(page, 0) * per_page + (at - e * per_page);
     };
@@ -277,7 +285,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     QueryParts q[CH];
     float qsum[G];
     const bool flip = a.qscale < 0.f;  // a negative scale goes into the queries: scores are then compared unscaled
-    const int64_t at_q = b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 8 * quad;
+    const int64_t at_q = seq * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 8 * quad;
     float qscale = fabsf(a.qscale), fit = 1.f;  // ``fit``: the power of two that takes the row's largest to 2^13 .. 2^14
     if constexpr (kCentred) {
         float most = 0.f;
@@ -471,18 +479,18 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         for (int t = 0; t < VT; ++t) o[t] += *reinterpret_cast<const f32x4*>(lds_o + ((w - 1) * kTile + col) * S::pad + 16 * t + 4 * quad);
     }
     if (!real) return;
-    const int64_t row = (static_cast<int64_t>(b) * a.n_q + h * a.g + i) * a.q_len + j;
-    if (a.parts == 1) {
+    const int64_t row = (static_cast<int64_t>(seq) * a.n_q + h * a.g + i) * a.q_len + j;
+    if (!Shared && a.parts == 1) {
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;  // (no row seen: zeros)
 #pragma unroll
         for (int t = 0; t < VT; ++t) o[t] *= inv;
         each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<Dt>(a.out, row * D + c, x); });
         return;
     }
-    float* dst = a.part_o + (row * a.parts + part) * D;
+    float* dst = a.part_o + (row * a.parts + a.part0 + part) * D;
     each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<LF_FP32>(dst, c, x); });
     if (quad == 0) {
-        float* ml = a.part_ml + (row * a.parts + part) * 2;
+        float* ml = a.part_ml + (row * a.parts + a.part0 + part) * 2;
         ml[0] = m_all;
         ml[1] = l_all;
     }
@@ -545,13 +553,15 @@ __global__ __launch_bounds__(256) void int4_merge_kernel(Int4Attention a, int dt
 
 template <int D, int GROUP, int Dt>
 int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
-    const auto fn = int4_attention_kernel<D, GROUP, Dt>;
+    const auto fn = int4_attention_kernel<D, GROUP, Dt, false>;
     int lds = Ring<D, GROUP>::lds;
     if (a.n_pages) lds += 4 * (a.split_tokens / (a.L.page_size / kBlock) + 2);  // the split's entries of the page list
     int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
     if (st == LF_OK && a.prefix) st = launch_int4_prefix(a, stream);
     if (st != LF_OK) return st;
-    hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, a);
+    Int4Attention rest = a;  // what a many-row launch leaves
+    rest.part0 += a.prefix;
+    hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, rest);
     if (a.parts > 1) {
         const uint32_t rows = static_cast<uint32_t>(a.L.batch) * a.n_q * a.q_len;
         hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.parts > 16 ? 256 : 64), 0, stream, a, Dt);
@@ -560,13 +570,19 @@ int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
     return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }
 
-}  // namespace
-
-int64_t int4_part_bytes(const lf_int4_layer& L, int n_q, int q_len, int splits) {
-    return splits <= 1 ? 0 : static_cast<int64_t>(L.batch) * n_q * q_len * splits * (L.head_dim + 2) * 4;
+// The rows of a shared prefix, 16 at a time.
+template <int D, int GROUP, int Dt>
+int launch_shared_typed(const Int4Attention& a, hipStream_t stream) {
+    const auto fn = int4_attention_kernel<D, GROUP, Dt, true>;
+    const int lds = Ring<D, GROUP>::lds, tiles = (a.g * a.q_len * a.each + kTile - 1) / kTile;
+    const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
+    if (st != LF_OK) return st;
+    hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, a);
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }
 
-int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream) {
+Int4Attention attention_of(const lf_int4_layer& L, const lf_int4_args& A, int more_parts) {
     Int4Attention a{};
     a.L = L;
     a.q = A.query;
@@ -581,11 +597,18 @@ int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStre
     a.pages = A.pages; a.n_pages = A.n_pages;
     a.splits = A.splits;
     a.prefix = A.prefix_splits;
-    a.parts = a.splits + a.prefix;
+    a.parts = a.splits + a.prefix + more_parts;
+    a.part0 = more_parts;
     a.split_tokens = A.split_tokens;
     const int64_t rows = static_cast<int64_t>(L.batch) * A.n_q * A.q_len;
     a.part_o = static_cast<float*>(A.workspace);
     a.part_ml = a.part_o + rows * a.parts * L.head_dim;
+    return a;
+}
+
+// The attention of ``a``'s rows over their own cache, and the merge of all parts.
+int launch_own(Int4Attention a, const lf_int4_args& A, hipStream_t stream) {
+    const lf_int4_layer& L = a.L;
     int tiles = (a.g * A.q_len + kTile - 1) / kTile;
     if (A.n_pages) {
         tiles = (a.g + kTile - 1) / kTile * A.q_len;
@@ -598,6 +621,37 @@ int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStre
                : A.dtype == LF_FP16 ? launch_typed<D, GROUP, LF_FP16>(a, tiles, stream)
                                     : launch_typed<D, GROUP, LF_FP32>(a, tiles, stream);
     });
+}
+
+}  // namespace
+
+int64_t int4_part_bytes(const lf_int4_layer& L, int n_q, int q_len, int splits) {
+    return splits <= 1 ? 0 : static_cast<int64_t>(L.batch) * n_q * q_len * splits * (L.head_dim + 2) * 4;
+}
+
+int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStream_t stream) {
+    return launch_own(attention_of(L, A, 0), A, stream);
+}
+
+// The prefix's parts come first, then the sequences' own.
+int launch_int4_shared(const lf_int4_layer& L, const lf_int4_layer& P, const lf_int4_args& A, int splits, int split_tokens, bool many_rows,
+                       hipStream_t stream) {
+    const Int4Attention own = attention_of(L, A, splits);
+    Int4Attention a = own;
+    a.L = P;
+    a.part0 = a.prefix = 0;
+    a.splits = splits;
+    a.split_tokens = split_tokens;
+    a.each = L.batch / P.batch;
+    a.own_lens = L.lens;
+    a.own_cap = L.cap_tokens;
+    const int st = many_rows ? launch_int4_shared_rows(a, stream) : int4_dispatch(P, [&](auto shape) {
+        constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
+        return A.dtype == LF_BF16 ? launch_shared_typed<D, GROUP, LF_BF16>(a, stream)
+               : A.dtype == LF_FP16 ? launch_shared_typed<D, GROUP, LF_FP16>(a, stream)
+                                    : launch_shared_typed<D, GROUP, LF_FP32>(a, stream);
+    });
+    return st == LF_OK ? launch_own(own, A, stream) : st;
 }
 
 }  // namespace lf

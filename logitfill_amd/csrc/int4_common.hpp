@@ -122,10 +122,32 @@ struct Int4Attention {
     int n_pages;
     int splits, split_tokens;  // with pages: split_tokens is in records of the page list
     int prefix;                // splits of the many-row kernel in front of them
-    int parts;                 // prefix + splits
+    int parts;                 // of every output row
+    int part0;                 // the first one of this launch
+    // A shared prefix (the kernels' Shared forms): L holds the prefixes, one for ``each`` sequences in turn.
+    int each;
+    const int32_t* own_lens;   // [batch] of the sequences behind them
+    int own_cap;
     float* part_o;             // [batch * n_q * q_len][parts][D]
     float* part_ml;            // [batch * n_q * q_len][parts][2]
 };
+
+// Query row ``r`` of a prefix's (sequence, head of the group, token), tokens fastest.
+struct SharedRow {
+    int b, i, j;   // sequence of the whole batch
+    bool real;
+};
+__device__ __forceinline__ SharedRow shared_row(const Int4Attention& a, int prefix, int r) {
+    const int per = a.g * a.q_len, s = r / per, rest = r - s * per, i = rest / a.q_len;
+    return {prefix * a.each + s, i, rest - i * a.q_len, s < a.each};
+}
+// Rows of a prefix of ``len`` that the row's query sees: all of them, unless its sequence is shorter than its queries.
+__device__ __forceinline__ int shared_limit(const Int4Attention& a, const SharedRow& row, int len) {
+    if (!row.real) return 0;
+    const int n = a.q_lens ? min(max(a.q_lens[row.b], 0), a.q_len) : a.q_len;
+    const int own = min(max(a.own_lens[row.b], 0), a.own_cap);
+    return row.j < n ? min(max(len + own - n + row.j + 1, 0), len) : 0;
+}
 
 constexpr int kManyRows = 128;  // query rows of a many-row workgroup
 

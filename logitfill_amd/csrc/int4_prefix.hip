@@ -68,7 +68,8 @@ __device__ __forceinline__ u32x4 values8(uint32_t w, const f16x2 (&s)[4], const 
 __device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ f16x2 halves(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
 
-template <int D, int GROUP>
+// Shared: of a prefix that ``each`` sequences share; the rows are all their queries, and its last record may be a part of one.
+template <int D, int GROUP, bool Shared>
 __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) void int4_prefix_kernel(Int4Attention a) {
     using R = Int4Rec<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, VT = D / 16;
@@ -82,9 +83,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     const int col = lane & 15, quad = lane >> 4;
     const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
     const int len = int4_len(a.L, b);
-    const int n = a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-    const int records = prefix_records(a, len, n, tile);
-    const int per = (records + a.prefix - 1) / a.prefix, first = min(part * per, records), last = min(first + per, records);
+    const int n = Shared ? 0 : a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+    const int records = Shared ? (len + kBlock - 1) / kBlock : prefix_records(a, len, n, tile), splits = Shared ? a.splits : a.prefix;
+    const int per = (records + splits - 1) / splits, first = min(part * per, records), last = min(first + per, records);
 
     // 2^up takes the split's largest Value to 2^14 .. 2^15: read back a Value reaches 16 * 65 504, fp16's infinity, and 2^-14 is
     // where fp16 begins to lose bits.  (One that is not finite takes no part.)  The scales and minima are read twice for it: 3, 5
@@ -95,7 +96,8 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float m = pair_min(pair[i]), v = fmaxf(fabsf(m), fabsf(fmaf(15.f, pair_scale(pair[i]), m)));
-            most_value = fmaxf(most_value, v < 4e6f ? v : 0.f);
+            const bool row = !Shared || (first + k / (8 * G)) * kBlock + 4 * (k % 8) + i < len;
+            most_value = fmaxf(most_value, row && v < 4e6f ? v : 0.f);
         }
     }
     most_value = wave_max(most_value);
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
             __builtin_memcpy(&r.pair[k], __builtin_assume_aligned(rec + at, 4), 16);
         }
     };
-    const auto stage = [&](const Raw& r, u32x4* to, uint32_t* pairs) {
+    const auto stage = [&](const Raw& r, u32x4* to, uint32_t* pairs, int left) {  // left: the record's tokens
         if (wave < 2) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) to[(half * CH + c) * kWave + lane] = keys8(r.w[c], code_base);
@@ -152,8 +154,13 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
                 f16x2 s[4], m[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    s[i] = halves(lower_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i])) * raise;
-                    m[i] = halves(upper_pair(r.pair[2 * k][i], r.pair[2 * k + 1][i])) * raise;
+                    uint32_t lower = r.pair[2 * k][i], upper = r.pair[2 * k + 1][i];
+                    if (Shared && left < kBlock) {  // (what stands behind the last token need not be finite)
+                        lower = 4 * quad + i < left ? lower : 0u;
+                        upper = 16 + 4 * quad + i < left ? upper : 0u;
+                    }
+                    s[i] = halves(lower_pair(lower, upper)) * raise;
+                    m[i] = halves(upper_pair(lower, upper)) * raise;
                 }
 #pragma unroll
                 for (int c = k * (VW / VG); c < (k + 1) * (VW / VG); ++c)
@@ -166,15 +173,19 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     f16x8 q[MT][CH];
     f16x4 qsum[MT];  // the query's sum over lane quad's group: 0 (for the scale), upper part, 0, lower part
     float qall[MT];  // or over the one group
+    int lim[MT];     // Shared: the prefix's rows that it sees
     float scale[MT], ref[MT], limit[MT];  // limit: how far a score may pass ref; -inf until one is seen
     const bool flip = a.qscale < 0.f;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        const int r = tile * kManyRows + (wave * MT + t) * kTile + col, i = r / a.q_len, j = r % a.q_len;
+        const int r = tile * kManyRows + (wave * MT + t) * kTile + col;
+        SharedRow at = {b, r / a.q_len, r % a.q_len, r / a.q_len < a.g};
+        if constexpr (Shared) at = shared_row(a, b, r);
+        lim[t] = Shared ? shared_limit(a, at, len) : 0;
         float x[CH][8] = {}, most = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-            if (i < a.g) query8<LF_BF16>(a, b * a.qb + static_cast<int64_t>(h * a.g + i) * a.qh + j * a.qt + 32 * c + 8 * quad, x[c]);
+            if (at.real) query8<LF_BF16>(a, at.b * a.qb + static_cast<int64_t>(h * a.g + at.i) * a.qh + at.j * a.qt + 32 * c + 8 * quad, x[c]);
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[c][e]));
         }
@@ -216,7 +227,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     Raw raw;
     if (first < last) {
         load(first, raw);
-        stage(raw, lds[0], key_pairs[0]);
+        stage(raw, lds[0], key_pairs[0], len - first * kBlock);
         load(min(first + 1, last - 1), raw);
     }
     __syncthreads();
@@ -224,7 +235,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
         const u32x4* rec = lds[(k - first) & 1];
         const uint32_t* pairs = key_pairs[(k - first) & 1];
         if (k + 1 < last) {
-            stage(raw, lds[(k + 1 - first) & 1], key_pairs[(k + 1 - first) & 1]);
+            stage(raw, lds[(k + 1 - first) & 1], key_pairs[(k + 1 - first) & 1], len - (k + 1) * kBlock);
             load(min(k + 2, last - 1), raw);
         }
         f32x4 y[MT][2];
@@ -258,6 +269,16 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
                     }
                 phase();
             }
+        }
+        if constexpr (Shared) {
+            // (rows that are no queries see nothing)
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+                if (__any(k * kBlock + kBlock > lim[t]))
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) y[t][u][i] = k * kBlock + 16 * u + 4 * quad + i < lim[t] ? y[t][u][i] : -__builtin_inff();
         }
         f16x8 p[MT];
 #pragma unroll
@@ -307,10 +328,12 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     for (int t = 0; t < MT; ++t) {
         l[t] = rows_sum(l[t]);
         const int r = tile * kManyRows + (wave * MT + t) * kTile + col;  // head of the group * q_len + token
-        if (r >= a.g * a.q_len) continue;
-        const int64_t at = ((static_cast<int64_t>(b) * a.n_q + h * a.g) * a.q_len + r) * a.parts + part;
+        SharedRow of = {b, r / a.q_len, r % a.q_len, r < a.g * a.q_len};
+        if constexpr (Shared) of = shared_row(a, b, r);
+        if (!of.real) continue;
+        const int64_t at = ((static_cast<int64_t>(of.b) * a.n_q + h * a.g + of.i) * a.q_len + of.j) * a.parts + a.part0 + part;
         // (a sum of NaN counts as seen; rows behind the sequence's last token are zeros whatever they saw)
-        const bool token = r % a.q_len < n;
+        const bool token = Shared || of.j < n;
         if (quad == 0) {
             a.part_ml[2 * at] = token && l[t] != 0.f ? ref[t] : -__builtin_inff();
             a.part_ml[2 * at + 1] = token ? l[t] : 0.f;
@@ -325,25 +348,28 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
     }
 }
 
-}  // namespace
-
-int launch_int4_prefix(const Int4Attention& a, hipStream_t stream) {
-    const int tiles = (a.g * a.q_len + kManyRows - 1) / kManyRows;
-    const dim3 grid(a.L.n_kv * tiles, a.L.batch, a.prefix);
-    const auto launch = [&](auto shape) {
+template <bool Shared>
+int launch(const Int4Attention& a, int rows, int splits, hipStream_t stream) {
+    const dim3 grid(a.L.n_kv * ((rows + kManyRows - 1) / kManyRows), a.L.batch, splits);
+    const auto of = [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
-        hipLaunchKernelGGL((int4_prefix_kernel<D, GROUP>), grid, dim3(kWaves * kWave), 0, stream, a);
+        hipLaunchKernelGGL((int4_prefix_kernel<D, GROUP, Shared>), grid, dim3(kWaves * kWave), 0, stream, a);
         const hipError_t err = hipGetLastError();
         return err == hipSuccess ? LF_OK : static_cast<int>(err);
     };
     switch (a.L.head_dim * 1000 + a.L.group) {
-        case 64032: return launch(Int4Shape<64, 32>());
-        case 64064: return launch(Int4Shape<64, 64>());
-        case 128032: return launch(Int4Shape<128, 32>());
-        case 128064: return launch(Int4Shape<128, 64>());
-        case 128128: return launch(Int4Shape<128, 128>());
+        case 64032: return of(Int4Shape<64, 32>());
+        case 64064: return of(Int4Shape<64, 64>());
+        case 128032: return of(Int4Shape<128, 32>());
+        case 128064: return of(Int4Shape<128, 64>());
+        case 128128: return of(Int4Shape<128, 128>());
         default: return LF_E_UNSUPPORTED;
     }
 }
+
+}  // namespace
+
+int launch_int4_prefix(const Int4Attention& a, hipStream_t stream) { return launch<false>(a, a.g * a.q_len, a.prefix, stream); }
+int launch_int4_shared_rows(const Int4Attention& a, hipStream_t stream) { return launch<true>(a, a.g * a.q_len * a.each, a.splits, stream); }
 
 }  // namespace lf

@@ -659,17 +659,22 @@ class LogitFillCache(_HFCache):
         self.manager = manager
 
     # -- lengths ------------------------------------------------------------------------------
+    def _prefix(self) -> int:
+        """Tokens of a prefix that the manager's sequences share (sequence 0's, as ``seq_len``)."""
+        prefix = getattr(self.manager, "prefix", None)
+        return 0 if prefix is None else prefix.seq_len
+
     def get_seq_length(self, layer_idx: int = 0) -> int:
-        return int(self.manager.seq_len)
+        return int(self.manager.seq_len) + self._prefix()
 
     def get_query_offset(self, layer_idx: int = 0) -> int:
-        return int(self.manager.seq_len)
+        return self.get_seq_length()
 
     def get_mask_sizes(self, query, layer_idx: int = 0):
         """``(kv_length, kv_offset)``: the packed tokens plus the ``query`` tokens (an int, or
         the tensor of cache positions older transformers pass), offset 0."""
         q_len = int(query) if isinstance(query, int) else int(query.shape[0])
-        return int(self.manager.seq_len) + q_len, 0
+        return self.get_seq_length() + q_len, 0
 
     def get_max_length(self, layer_idx: int | None = None) -> int:
         return -1  # grows without a bound
@@ -695,13 +700,17 @@ class LogitFillCache(_HFCache):
 
     def crop(self, tokens_to_remove: int) -> None:
         """transformers' ``crop``, of every sequence by itself: keep that many of its tokens, or, negative, all but
-        that many of its last (a 4-bit row cache; packed pages cannot be cropped)."""
+        that many of its last (a 4-bit row cache; packed pages cannot be cropped).  A shared prefix's tokens are among them,
+        and stay: a crop into it is a ``ValueError``."""
         truncate = getattr(self.manager, "truncate", None)
         if truncate is None:
             raise NotImplementedError("packed pages cannot be cropped")
         keep = int(tokens_to_remove)
         have = self.manager.layers[-1].lengths
-        left = [min(keep, n) if keep >= 0 else max(n + keep, 0) for n in have]
+        before = [0] * len(have) if self._prefix() == 0 else self.manager.prefix_lengths(-1)
+        left = [min(keep, p + n) - p if keep >= 0 else max(p + n + keep, 0) - p for n, p in zip(have, before)]
+        if min(left) < 0:
+            raise ValueError(f"a crop to {keep} would cut the shared prefix of {max(before)} tokens")
         if left != have:
             truncate(left)
 

@@ -340,12 +340,14 @@ class Int4KVManager:
     ``head_dim`` 64, 128 or 256; ``group_size`` 32, 64 or 128 channels per scale and minimum;
     ``page_size`` (a multiple of 32 up to 1024) is the unit of ``select_pages``.  ``top_pages``: the
     model integration attends that many selected pages per query and kv head (0: every row).
+    ``prefix``: another manager whose sequences stand in front of this one's (the attribute, too).
     """
 
     commits_new_tokens = True  # the attention writes the new tokens before it reads
 
     def __init__(self, n_layers: int, n_q: int, n_kv: int, head_dim: int, page_size: int = 128, group_size: int = 64,
-                 device="cuda", *, batch_size: int = 1, capacity_tokens: int = 0, top_pages: int = 0):
+                 device="cuda", *, batch_size: int = 1, capacity_tokens: int = 0, top_pages: int = 0,
+                 prefix: Optional["Int4KVManager"] = None):
         self.n_q, self.n_kv, self.head_dim = int(n_q), int(n_kv), int(head_dim)
         self.page_size, self.group_size = int(page_size), int(group_size)
         self.batch_size, self.top_pages = int(batch_size), int(top_pages)
@@ -364,6 +366,41 @@ class Int4KVManager:
                        for row in self._lens.rows]
         self._lens.layers = self.layers
         self._args: dict = {}
+        self._prefix: Optional[Int4KVManager] = None
+        self.prefix = prefix
+
+    @property
+    def prefix(self) -> Optional["Int4KVManager"]:
+        """The manager of a prefix that this one's sequences share, or None: of ``prefix.batch_size`` prefixes, each in
+        front of ``batch_size / prefix.batch_size`` sequences in turn (all the samples of a prompt, the chats behind a system
+        prompt).  ``int4_attention`` then attends a prefix's rows, read once for all its sequences, and the sequence's own
+        behind them; commits, ``truncate`` and ``reset`` are of the own rows, and the prefix may be written between calls
+        as any cache.  A captured call holds the prefix's split plan too."""
+        return self._prefix
+
+    @prefix.setter
+    def prefix(self, prefix: Optional["Int4KVManager"]) -> None:
+        if prefix is not None:
+            if not isinstance(prefix, Int4KVManager):
+                raise TypeError(f"prefix must be an Int4KVManager, got {type(prefix).__name__}")
+            mine = (self.n_q, self.n_kv, self.head_dim, self.group_size, len(self.layers), self.device)
+            its = (prefix.n_q, prefix.n_kv, prefix.head_dim, prefix.group_size, len(prefix.layers), prefix.device)
+            if mine != its:
+                raise ValueError(f"the prefix has (n_q, n_kv, head_dim, group_size, layers, device) {its}, the manager {mine}")
+            if self.batch_size % prefix.batch_size:
+                raise ValueError(f"{prefix.batch_size} prefixes do not divide {self.batch_size} sequences")
+            if prefix is self or prefix.prefix is not None:
+                raise ValueError("a prefix stands in front of every row: it has no prefix of its own")
+            if self.top_pages:
+                raise ValueError("a manager of top_pages takes no prefix: pages are selected among its own rows")
+        self._prefix = prefix
+
+    def prefix_lengths(self, layer_idx: int) -> list:
+        """Tokens in front of every sequence's own (zeros without a prefix)."""
+        if self._prefix is None:
+            return [0] * self.batch_size
+        lengths = self._prefix.layers[layer_idx].lengths
+        return [n for n in lengths for _ in range(self.batch_size // len(lengths))]
 
     def commit(self, layer_idx: int, key: torch.Tensor, value: torch.Tensor, lengths=None) -> None:
         """Append ``key/value [batch, n_kv, T, head_dim]`` to layer ``layer_idx``, quantised as they are written.
@@ -586,6 +623,9 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     not before the own page or not above its predecessor is not attended.  Without it a manager of
     ``top_pages`` selects that many itself.
 
+    Of a manager with a ``prefix``, whose rows stand in front of the sequences' own, each prefix is read once for all
+    its sequences (no ``pages``).
+
     Everything is enqueued on the current stream.
     """
     scaling = float(scaling)
@@ -595,6 +635,11 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     query = _check_query(manager, query, pages is not None or manager.top_pages > 0)
     q_len = query.shape[2]
     B = manager.batch_size
+    if manager.prefix is not None:
+        if pages is not None:
+            raise ValueError("pages are of a sequence's own rows: a manager with a prefix attends them all")
+        if manager.prefix.prefix is not None:
+            raise ValueError("the manager's prefix has a prefix of its own")
     new = None
     if (key_new is None) != (value_new is None):
         raise ValueError("key_new and value_new come together")
@@ -639,14 +684,44 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
     else:
         a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,
                                                workgroups_per_cu(D, manager.group_size))
-    parts = a.splits + a.prefix_splits
+    shared = _shared_plan(manager, layer_idx, q_len, query.dtype, lengths, cus)
+    parts = a.splits + a.prefix_splits + (shared[0] if shared else 0)
     if parts > 1:
         nbytes = 4 * B * n_q * q_len * parts * (D + 2)  # lf_int4_workspace_bytes
         ws = _workspace(manager, nbytes)
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    st = _native.load().lf_int4_attention(layer.layer_struct(), a, _native.current_stream_ptr(manager.device))
+    stream = _native.current_stream_ptr(manager.device)
+    if shared:
+        prefix = manager.prefix.layers[layer_idx].layer_struct()
+        st = _native.load().lf_int4_shared_attention(layer.layer_struct(), prefix, a, *shared, stream)
+        _native.check(st, "lf_int4_shared_attention")
+        return out
+    st = _native.load().lf_int4_attention(layer.layer_struct(), a, stream)
     _native.check(st, "lf_int4_attention")
     return out
+
+
+# Query rows per kv head, of all the sequences of a prefix, from which on the many-row kernel takes it.
+SHARED_ROWS = 33
+
+
+def _shared_plan(manager, layer_idx: int, q_len: int, dtype, lengths, cus: int):
+    """``(splits, split_tokens, many_rows)`` of the manager's prefix, or None where there is none."""
+    prefix = manager.prefix
+    if prefix is None:
+        return None
+    tokens = prefix.layers[layer_idx].lengths
+    if not max(tokens):
+        return None
+    D, group = manager.head_dim, manager.group_size
+    rows = manager.n_q // manager.n_kv * q_len * (manager.batch_size // prefix.batch_size)
+    own = manager.layers[layer_idx].lengths
+    behind = all(n >= (q_len if lengths is None else lengths[b]) for b, n in enumerate(own))  # every query sees all of it
+    if rows >= SHARED_ROWS and dtype == torch.bfloat16 and D <= 128 and behind:
+        splits, size = plan_splits(tokens, manager.n_kv * -(-rows // 128), cus, many_rows_per_cu(D, group), MANY_ROWS_OVERHEAD)
+        return min(splits, MAX_SPLITS // 2), size, 1
+    splits, size = plan_splits(tokens, manager.n_kv * -(-rows // 16), cus, workgroups_per_cu(D, group))
+    return splits, size, 0
 
 
 @_here
