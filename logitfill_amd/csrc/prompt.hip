@@ -34,6 +34,7 @@ struct Prompt {
     const lf_prompt_item* items;
     int n_q, n_kv, g;
     float qscale;   // scaling * log2(e)
+    int far;        // a tile's rows span more than 32-bit offsets reach
     float* part_o;  // [slots][n_kv][rows of a tile][D]
     float* part_ml; // [slots][n_kv][rows of a tile][2]
 };
@@ -41,6 +42,7 @@ struct Prompt {
 template <int Dt> struct Element;
 template <> struct Element<LF_BF16> {
     using x8 = bf16x8;
+    static constexpr uint32_t bits = 0x7fff7fffu, least = 0x00800080u;  // all but the signs; infinity's distance from the next sign
     static constexpr float headroom = 0.f;
     static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -51,6 +53,7 @@ template <> struct Element<LF_BF16> {
 };
 template <> struct Element<LF_FP16> {
     using x8 = f16x8;
+    static constexpr uint32_t bits = 0x7fff7fffu, least = 0x04000400u;
     static constexpr float headroom = 7.f;
     static __device__ __forceinline__ f32x16 mfma(x8 a, x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -61,7 +64,8 @@ template <> struct Element<LF_FP16> {
 };
 
 template <> struct Element<LF_FP32> {
-    using x8 = f32x4;  // (four channels or one Key a product: v_mfma_f32_32x32x2)
+    using x8 = f32x4;  // (four channels or Keys, one a product: v_mfma_f32_32x32x2)
+    static constexpr uint32_t bits = 0x7fffffffu, least = 0x00800000u;
     static constexpr float headroom = 0.f;
 };
 
@@ -89,6 +93,16 @@ __device__ __forceinline__ u32x2 read_tr(uint32_t at) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s16x4*>(static_cast<uintptr_t>(at))));
 }
+// LDS-DMA (dma16 without its streaming hint: other workgroups read the same Keys): each lane's 16 bytes, at an offset from a
+// uniform base or at an address of its own, land at lds + 16 * lane.  (A base that a vector instruction wrote, as a
+// readfirstlane, is read five wait states later at the earliest, and M0 one after its write.)
+__device__ __forceinline__ void dma16_at(const unsigned char* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(in_sgpr(base)), "{m0}"(lds) : "memory");
+}
+__device__ __forceinline__ void dma16_far(const unsigned char* g, uint32_t lds) {
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(lds) : "memory");
+}
+
 __device__ __forceinline__ uint32_t read4(uint32_t at) {
     typedef __attribute__((address_space(3))) const uint32_t lds_u32;
     return *reinterpret_cast<lds_u32*>(static_cast<uintptr_t>(at));
@@ -98,18 +112,25 @@ __device__ __forceinline__ u32x4 read16(uint32_t at) {
     return *reinterpret_cast<lds_u32x4*>(static_cast<uintptr_t>(at));
 }
 
+// LDS reads stay behind this point: all hoisted to a tile's start they take more registers than there are.
+__device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
+
 // NW waves of 32 rows each.
 template <int D, int Dt, int NW>
-__global__ __launch_bounds__(NW * kWave, D == 256 && Dt == LF_FP32 ? 1 : 2) void prompt_kernel(Prompt a) {
+__global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Prompt a) {
     using T = Tile<D, Dt>;
     using E = Element<Dt>;
     using x8 = typename E::x8;
     constexpr bool kWide = Dt == LF_FP32;
     constexpr int ES = T::esize, KT = T::keys, KB = KT / 32, SQ = D * ES / 32, CB = D / 32, KK = kWide ? KT / 8 : KT / 16;
     constexpr int kRows = 32 * NW;
-    extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const int h = blockIdx.x % a.n_kv;
-    const lf_prompt_item item = a.items[blockIdx.x / a.n_kv];
+    lf_prompt_item item = a.items[blockIdx.x / a.n_kv];
+    item.q_row = in_sgpr(item.q_row); item.q_start = in_sgpr(item.q_start); item.n_q = in_sgpr(item.n_q);
+    item.k_row = in_sgpr(item.k_row); item.k_start = in_sgpr(item.k_start); item.n_k = in_sgpr(item.n_k);
+    item.tile = in_sgpr(item.tile); item.slot = in_sgpr(item.slot);
+    item.begin = in_sgpr(item.begin); item.end = in_sgpr(item.end);
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 31, hi = lane >> 5;
     const uint32_t lds = lds_addr(smem);
@@ -131,17 +152,33 @@ __global__ __launch_bounds__(NW * kWave, D == 256 && Dt == LF_FP32 ? 1 : 2) void
     const int reach = max(item.n_k - item.n_q + last_token + 1, 0);
     const int first = item.begin, last = min(item.end, (reach + KT - 1) / KT);
 
-    const unsigned char* kbase = static_cast<const unsigned char*>(a.k) + ES * (item.k_row * a.ks[0] + h * a.ks[1] + static_cast<int64_t>(item.k_start) * a.ks[2]);
-    const unsigned char* vbase = static_cast<const unsigned char*>(a.v) + ES * (item.k_row * a.vs[0] + h * a.vs[1] + static_cast<int64_t>(item.k_start) * a.vs[2]);
-    // Tile t to buffer b: a load instruction takes rows_per_load rows (of Keys past the last one that is seen, that one).
-    const auto fill = [&](int t, int b) {
+    const unsigned char* kbase = in_sgpr(static_cast<const unsigned char*>(a.k) + ES * (item.k_row * a.ks[0] + h * a.ks[1] + static_cast<int64_t>(item.k_start) * a.ks[2]));
+    const unsigned char* vbase = in_sgpr(static_cast<const unsigned char*>(a.v) + ES * (item.k_row * a.vs[0] + h * a.vs[1] + static_cast<int64_t>(item.k_start) * a.vs[2]));
+    // The next tile to buffer b: a load instruction takes rows_per_load rows.  Of a whole tile a lane's offset from the tile's
+    // start is the same in every tile, but for the pieces' exchange, which is linear in the row's bits.
+    constexpr int kStep = NW * T::rows_per_load;
+    const int row0 = wave * T::rows_per_load + lane / T::pieces, piece0 = lane % T::pieces;
+    const uint32_t krow = static_cast<uint32_t>(row0 * a.ks[2] * ES), vrow0 = static_cast<uint32_t>(row0 * a.vs[2] * ES);
+    const uint32_t kpiece = 16 * (piece0 ^ T::key_swap(row0)), vpiece = 16 * (piece0 ^ T::value_swap(row0));
+    const auto fill = [&](int t, int b) __attribute__((always_inline)) {
+        const uint32_t to = lds + b * 2 * T::bytes + wave * 1024;
+        if (!a.far && t * KT + KT <= reach) {
+            const unsigned char *kt = kbase + static_cast<int64_t>(t) * KT * ES * a.ks[2], *vt = vbase + static_cast<int64_t>(t) * KT * ES * a.vs[2];
+#pragma unroll
+            for (int n = 0; n < T::loads / NW; ++n)
+                dma16_at(kt + static_cast<int64_t>(n * kStep) * ES * a.ks[2], krow + (kpiece ^ (16 * T::key_swap(n * kStep))), to + n * NW * 1024);
+#pragma unroll
+            for (int n = 0; n < T::loads / NW; ++n)
+                dma16_at(vt + static_cast<int64_t>(n * kStep) * ES * a.vs[2], vrow0 + (vpiece ^ (16 * T::value_swap(n * kStep))), to + T::bytes + n * NW * 1024);
+            return;
+        }
+        // (in place of Keys past the last one that is seen, that one)
 #pragma unroll
         for (int n = 0; n < T::loads / NW; ++n) {
-            const int r = (wave + n * NW) * T::rows_per_load + lane / T::pieces, piece = lane % T::pieces;
+            const int r = row0 + n * kStep;
             const int64_t at = min(t * KT + r, reach - 1);
-            const uint32_t to = lds + b * 2 * T::bytes + (wave + n * NW) * 1024;
-            dma16(kbase + ES * at * a.ks[2] + 16 * (piece ^ T::key_swap(r)), to);
-            dma16(vbase + ES * at * a.vs[2] + 16 * (piece ^ T::value_swap(r)), to + T::bytes);
+            dma16_far(kbase + ES * at * a.ks[2] + 16 * (piece0 ^ T::key_swap(r)), to + n * NW * 1024);
+            dma16_far(vbase + ES * at * a.vs[2] + 16 * (piece0 ^ T::value_swap(r)), to + T::bytes + n * NW * 1024);
         }
     };
     if (first < last) fill(first, 0);
@@ -170,36 +207,53 @@ __global__ __launch_bounds__(NW * kWave, D == 256 && Dt == LF_FP32 ? 1 : 2) void
     float l = 0.f, ref = 0.f, limit = -__builtin_inff();
 
     // operand addresses inside a tile
-    const uint32_t key_at = col * T::row;
+    // (the rows are whole multiples of what is exchanged: further pieces are an exclusive or away, further rows a constant)
+    const uint32_t key_at = col * T::row + 16 * (hi ^ T::key_swap(col));
     const int group = lane >> 4, in16 = lane & 15;  // 16 lanes transpose four rows of sixteen channels
     const int vrow = 4 * (group >> 1) + (in16 >> 2), vcol = 16 * (group & 1) + 4 * (in16 & 3);
+    const uint32_t value_at = T::bytes + (kWide ? 4 * hi * T::row + 16 * ((col / 4) ^ T::value_swap(4 * hi)) + 4 * (col & 3)
+                                                : vrow * T::row + 16 * ((vcol / 8) ^ T::value_swap(vrow)) + 2 * (vcol & 7));
 
-    for (int t = first; t < last; ++t) {
+    // Tiles that every row of the wave sees whole come first (a branch in one body became selects in every tile).
+    const auto tile = [&](auto masked_tile, int t) __attribute__((always_inline)) {
+        constexpr bool masked = decltype(masked_tile)::value;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // tile t is there, and nobody reads the other buffer any more
         const uint32_t buf = lds + ((t - first) & 1) * 2 * T::bytes;
         if (t + 1 < last) fill(t + 1, (t + 1 - first) & 1);
         const int k0 = t * KT;
-        if (k0 >= top) continue;
+        if (masked && k0 >= top) return;
+        // What stands where a row does not see need not be finite, and 0 * NaN is NaN: of a tile that holds such Values, one Key at
+        // a time is added to the rows that see it.
+        bool odd = false;
+        if constexpr (masked) {
+            uint32_t found = 0;
+#pragma unroll 4
+            for (int n = 0; n < T::loads; ++n) {
+                const u32x4 w = read16(buf + T::bytes + 1024 * n + 16 * lane);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) found |= (w[x] & E::bits) + E::least;
+            }
+            odd = __any((found & ~E::bits) != 0);
+        }
+        const uint32_t keys = buf + key_at, values = buf + value_at;
         f32x16 s[KB];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) s[b] = f32x16{};
-#pragma unroll
-        for (int n = 0; n < SQ; ++n)
+        for (int n = 0; n < SQ; ++n) {
+            if (n % 4 == 0) phase();
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
-                const int r = 32 * b + col;
-                const u32x4 w = read16(buf + 32 * b * T::row + key_at + 16 * ((2 * n + hi) ^ T::key_swap(r)));
+                const u32x4 w = read16((keys ^ (32 * n)) + 32 * b * T::row);
                 if constexpr (kWide) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), q[n][e], s[b], 0, 0, 0);
+                        s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), q[n][e], n + e == 0 ? f32x16{} : s[b], 0, 0, 0);
                 } else {
-                    s[b] = E::mfma(__builtin_bit_cast(x8, w), q[n], s[b]);
+                    s[b] = E::mfma(__builtin_bit_cast(x8, w), q[n], n == 0 ? f32x16{} : s[b]);
                 }
             }
-        const bool masked = k0 + KT > all;
-        if (masked)
+        }
+        if constexpr (masked)
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -243,24 +297,19 @@ __global__ __launch_bounds__(NW * kWave, D == 256 && Dt == LF_FP32 ? 1 : 2) void
             }
         }
         // The same Keys' Values in channels 32 c + col.
-        const auto value = [&](int kk, int c) {
+        const auto value = [&](int kk, int c) __attribute__((always_inline)) {
             if constexpr (kWide) {
                 u32x4 w;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = 8 * kk + 4 * hi + e;
-                    w[e] = read4(buf + T::bytes + r * T::row + 16 * ((8 * c + col / 4) ^ T::value_swap(r)) + 4 * (col & 3));
-                }
+                for (int e = 0; e < 4; ++e) w[e] = read4((values ^ (128 * c)) + (8 * kk + e) * T::row);
                 return w;
             } else {
-                const int r = 16 * kk + vrow;  // (8 rows further on, the pieces' exchange is the same)
-                const int piece = (32 * c + vcol) / 8;
-                const uint32_t at = buf + T::bytes + r * T::row + 16 * (piece ^ T::value_swap(vrow)) + 2 * (vcol & 7);
+                const uint32_t at = (values ^ (64 * c)) + 16 * kk * T::row;
                 const u32x2 x = read_tr(at), y = read_tr(at + 8 * T::row);
                 return u32x4{x[0], x[1], y[0], y[1]};
             }
         };
-        const auto multiply = [](u32x4 w, x8 weights, f32x16 sum) {
+        const auto multiply = [](u32x4 w, x8 weights, f32x16 sum) __attribute__((always_inline)) {
             if constexpr (kWide) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[e]), weights[e], sum, 0, 0, 0);
@@ -269,46 +318,41 @@ __global__ __launch_bounds__(NW * kWave, D == 256 && Dt == LF_FP32 ? 1 : 2) void
                 return E::mfma(__builtin_bit_cast(x8, w), weights, sum);
             }
         };
-        if (!masked) {
+        if (!odd) {
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk)
+            for (int kk = 0; kk < KK; ++kk) {
+                phase();
 #pragma unroll
                 for (int c = 0; c < CB; ++c) o[c] = multiply(value(kk, c), p[kk], o[c]);
+            }
         } else {
-            // What stands where a row does not see need not be finite, and 0 * NaN is NaN: where a sum is not finite, one Key
-            // at a time is added to the rows that see it.
-#pragma unroll
-            for (int c = 0; c < CB; ++c) {
-                f32x16 sum = f32x16{};
-#pragma unroll
-                for (int kk = 0; kk < KK; ++kk) sum = multiply(value(kk, c), p[kk], sum);
-                float test = 0.f;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) test = fmaf(sum[r], 0.f, test);
-                if (__any(test != 0.f)) {
-                    sum = f32x16{};
 #pragma unroll 1
-                    for (int key = 0; key < KT; ++key) {
-                        const int kk = kWide ? key >> 3 : key >> 4, half = (key >> 2) & 1;
-                        const int word = kWide ? key & 3 : ((key & 3) + 4 * ((key >> 3) & 1)) >> 1;
-                        const uint32_t keep = kWide ? 0xffffffffu : 0xffffu << (16 * (key & 1));
-                        u32x4 w = value(kk, c), pk = __builtin_bit_cast(u32x4, p[0]);
+            for (int key = 0; key < KT; ++key) {
+                const int kk = kWide ? key >> 3 : key >> 4, half = (key >> 2) & 1;
+                const int word = kWide ? key & 3 : ((key & 3) + 4 * ((key >> 3) & 1)) >> 1;
+                const uint32_t keep = kWide ? 0xffffffffu : 0xffffu << (16 * (key & 1));
+                u32x4 pk = __builtin_bit_cast(u32x4, p[0]);
 #pragma unroll
-                        for (int n = 1; n < KK; ++n)
+                for (int n = 1; n < KK; ++n)
 #pragma unroll
-                            for (int x = 0; x < 4; ++x) pk[x] = kk == n ? __builtin_bit_cast(u32x4, p[n])[x] : pk[x];
+                    for (int x = 0; x < 4; ++x) pk[x] = kk == n ? __builtin_bit_cast(u32x4, p[n])[x] : pk[x];
+                const bool seen = k0 + key < lim;
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) w[x] &= hi == half && word == x ? keep : 0u;
-                        const f32x16 one = multiply(w, __builtin_bit_cast(x8, pk), f32x16{});
-                        const bool seen = k0 + key < lim;
+                for (int c = 0; c < CB; ++c) {
+                    u32x4 w = value(kk, c);
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) sum[r] += seen ? one[r] : 0.f;
-                    }
+                    for (int x = 0; x < 4; ++x) w[x] &= hi == half && word == x ? keep : 0u;
+                    const f32x16 one = multiply(w, __builtin_bit_cast(x8, pk), f32x16{});
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[c][r] += seen ? one[r] : 0.f;
                 }
-                o[c] += sum;
             }
         }
-    }
+    };
+    const int whole = min(all / KT, last);
+    int t = first;
+    for (; t < whole; ++t) tile(std::false_type(), t);
+    for (; t < last; ++t) tile(std::true_type(), t);
 
     l = halves_sum(l);
     if (!real) return;
@@ -407,6 +451,8 @@ int launch_prompt(const lf_prompt_args& A, hipStream_t stream) {
     a.items = A.items;
     a.n_q = A.n_q; a.n_kv = A.n_kv; a.g = A.n_q / A.n_kv;
     a.qscale = A.scaling * kLog2e;
+    const int64_t near = (1ll << 31) / (64 * 4);
+    a.far = A.k_strides[2] < 0 || A.v_strides[2] < 0 || A.k_strides[2] >= near || A.v_strides[2] >= near;
     a.part_o = static_cast<float*>(A.workspace);
     a.part_ml = a.part_o + static_cast<int64_t>(A.n_slots) * A.n_kv * A.tile_rows * A.head_dim;
     return A.head_dim == 64 ? launch_dim<64>(a, A, stream) : A.head_dim == 128 ? launch_dim<128>(a, A, stream) : launch_dim<256>(a, A, stream);
