@@ -77,7 +77,7 @@ struct Tile {
     static constexpr int keys = D == 256 || Dt == LF_FP32 ? 32 : 64;
     static constexpr int row = esize * D, bytes = keys * row, pieces = row / 16;
     static constexpr int rows_per_load = 1024 / row, loads = bytes / 1024;
-    static constexpr int lds = 4 * bytes;  // Keys and Values, two tiles
+    static constexpr int lds = 2 * bytes;  // Keys, then Values
     static __device__ __forceinline__ int key_swap(int r) { return r & (pieces < 16 ? pieces - 1 : 15); }
     static __device__ __forceinline__ int value_swap(int r) { return Dt == LF_FP32 ? (r & 4) << 1 : D == 64 ? (r & 2) << 1 : (r & 3) << 2; }
 };
@@ -112,12 +112,132 @@ __device__ __forceinline__ u32x4 read16(uint32_t at) {
     return *reinterpret_cast<lds_u32x4*>(static_cast<uintptr_t>(at));
 }
 
+__device__ __forceinline__ lf_prompt_item load_item(const Prompt& a) {
+    lf_prompt_item item = a.items[blockIdx.x / a.n_kv];
+    item.q_row = in_sgpr(item.q_row); item.q_start = in_sgpr(item.q_start); item.n_q = in_sgpr(item.n_q);
+    item.k_row = in_sgpr(item.k_row); item.k_start = in_sgpr(item.k_start); item.n_k = in_sgpr(item.n_k);
+    item.tile = in_sgpr(item.tile); item.slot = in_sgpr(item.slot);
+    item.begin = in_sgpr(item.begin); item.end = in_sgpr(item.end);
+    return item;
+}
+
+// How a workgroup's NW waves bring tiles of an item's Keys and Values into LDS: a load instruction takes rows_per_load rows.
+// Of a whole tile a lane's offset from the tile's start is the same in every tile, but for the pieces' exchange, which is
+// linear in the row's bits.
+template <int D, int Dt, int NW>
+struct Loader {
+    using T = Tile<D, Dt>;
+    static constexpr int kStep = NW * T::rows_per_load;
+    struct Side {
+        const unsigned char* base;
+        int64_t stride;        // bytes from row to row
+        uint32_t row, piece;   // this lane's offsets
+        int swapped[2];        // (row0, its piece) for rows of their own
+        bool value;
+    };
+    Side keys, values;
+    int reach, wave;
+    bool far;
+
+    __device__ __forceinline__ Loader(const Prompt& a, const lf_prompt_item& item, int h, int wave_, int lane, int reach_) {
+        reach = reach_;
+        wave = wave_;
+        far = a.far;
+        const int row0 = wave * T::rows_per_load + lane / T::pieces, piece0 = lane % T::pieces;
+        keys = side(a.k, a.ks, item, h, row0, piece0, false);
+        values = side(a.v, a.vs, item, h, row0, piece0, true);
+    }
+    static __device__ __forceinline__ Side side(const void* p, const int64_t (&s)[3], const lf_prompt_item& item, int h, int row0, int piece0, bool value) {
+        const int64_t at = item.k_row * s[0] + h * s[1] + static_cast<int64_t>(item.k_start) * s[2];
+        const int64_t stride = s[2] * T::esize;
+        return {in_sgpr(static_cast<const unsigned char*>(p) + at * T::esize), stride, static_cast<uint32_t>(row0 * stride),
+                static_cast<uint32_t>(16 * (piece0 ^ (value ? T::value_swap(row0) : T::key_swap(row0)))), {row0, piece0}, value};
+    }
+    static __device__ __forceinline__ int swap(bool value, int r) { return value ? T::value_swap(r) : T::key_swap(r); }
+    // Tile t to LDS address ``at``.
+    __device__ __forceinline__ void fill(const Side& s, int t, uint32_t at) const {
+        const uint32_t to = at + wave * 1024;
+        if (!far && t * T::keys + T::keys <= reach) {
+            const unsigned char* from = s.base + static_cast<int64_t>(t) * T::keys * s.stride;
+#pragma unroll
+            for (int n = 0; n < T::loads / NW; ++n)
+                dma16_at(from + static_cast<int64_t>(n * kStep) * s.stride, s.row + (s.piece ^ (16 * swap(s.value, n * kStep))), to + n * NW * 1024);
+            return;
+        }
+        // (in place of Keys past the last one that is seen, that one; the empty statement keeps what this rare way needs out of the
+        // registers of the others)
+        int row0 = s.swapped[0], piece0 = s.swapped[1];
+        asm volatile("" : "+v"(row0), "+v"(piece0));
+#pragma unroll
+        for (int n = 0; n < T::loads / NW; ++n) {
+            const int r = row0 + n * kStep;
+            const int64_t row = min(t * T::keys + r, reach - 1);
+            dma16_far(s.base + row * s.stride + 16 * (piece0 ^ swap(s.value, r)), to + n * NW * 1024);
+        }
+    }
+};
+
 // LDS reads stay behind this point: all hoisted to a tile's start they take more registers than there are.
 __device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
 
+// A row's attention to Keys first .. end - 1 by itself, in the pair of lanes that holds it (half ``hi`` of its channels each): to
+// ``out``, or as a split's sums where that is null.
+template <int D, int Dt>
+__device__ __attribute__((noinline)) void one_row(const unsigned char* q, const unsigned char* k, const unsigned char* v, int64_t kstride,
+                                                  int64_t vstride, int first, int end, int hi, float qscale, unsigned char* out, float* part_o,
+                                                  float* part_ml) {
+    constexpr int H = D / 2;
+    float o[H], m = -__builtin_inff(), l = 0.f;
+#pragma unroll
+    for (int c = 0; c < H; ++c) o[c] = 0.f;
+#pragma unroll 1
+    for (int key = first; key < end; ++key) {
+        float s = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 8) {
+            float x[8], y[8];
+            load8_as_f32(q, c, Dt, x);
+            load8_as_f32(k + key * kstride, c, Dt, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+        }
+        s *= qscale;
+        if (s > m) {
+            const float down = __builtin_amdgcn_exp2f(m - s);
+            m = s;
+            l *= down;
+#pragma unroll
+            for (int c = 0; c < H; ++c) o[c] *= down;
+        }
+        const float w = s == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s - (m == -__builtin_inff() ? 0.f : m));
+        if (w == 0.f) continue;  // (as a masked one)
+        l += w;
+#pragma unroll
+        for (int c = 0; c < H; c += 8) {
+            float y[8];
+            load8_as_f32(v + key * vstride, hi * H + c, Dt, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[c + e] = fmaf(w, y[e], o[c + e]);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < H; ++c) {
+        if (out) store_from_f32(out, hi * H + c, Dt, o[c] * inv);
+        else part_o[hi * H + c] = o[c];
+    }
+    if (!out && hi == 0) {
+        part_ml[0] = l == 0.f ? -__builtin_inff() : m;
+        part_ml[1] = l;
+    }
+}
+
 // NW waves of 32 rows each.
+template <int D, int Dt>
+constexpr int kPerSimd = Dt == LF_FP32 ? (D == 64 ? 3 : D == 128 ? 2 : 1) : (D == 64 ? 4 : D == 128 ? 3 : 2);  // waves, by their registers
+
 template <int D, int Dt, int NW>
-__global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Prompt a) {
+__global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(Prompt a) {
     using T = Tile<D, Dt>;
     using E = Element<Dt>;
     using x8 = typename E::x8;
@@ -126,11 +246,7 @@ __global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Pr
     constexpr int kRows = 32 * NW;
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const int h = blockIdx.x % a.n_kv;
-    lf_prompt_item item = a.items[blockIdx.x / a.n_kv];
-    item.q_row = in_sgpr(item.q_row); item.q_start = in_sgpr(item.q_start); item.n_q = in_sgpr(item.n_q);
-    item.k_row = in_sgpr(item.k_row); item.k_start = in_sgpr(item.k_start); item.n_k = in_sgpr(item.n_k);
-    item.tile = in_sgpr(item.tile); item.slot = in_sgpr(item.slot);
-    item.begin = in_sgpr(item.begin); item.end = in_sgpr(item.end);
+    const lf_prompt_item item = load_item(a);
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 31, hi = lane >> 5;
     const uint32_t lds = lds_addr(smem);
@@ -152,36 +268,9 @@ __global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Pr
     const int reach = max(item.n_k - item.n_q + last_token + 1, 0);
     const int first = item.begin, last = min(item.end, (reach + KT - 1) / KT);
 
-    const unsigned char* kbase = in_sgpr(static_cast<const unsigned char*>(a.k) + ES * (item.k_row * a.ks[0] + h * a.ks[1] + static_cast<int64_t>(item.k_start) * a.ks[2]));
-    const unsigned char* vbase = in_sgpr(static_cast<const unsigned char*>(a.v) + ES * (item.k_row * a.vs[0] + h * a.vs[1] + static_cast<int64_t>(item.k_start) * a.vs[2]));
-    // The next tile to buffer b: a load instruction takes rows_per_load rows.  Of a whole tile a lane's offset from the tile's
-    // start is the same in every tile, but for the pieces' exchange, which is linear in the row's bits.
-    constexpr int kStep = NW * T::rows_per_load;
-    const int row0 = wave * T::rows_per_load + lane / T::pieces, piece0 = lane % T::pieces;
-    const uint32_t krow = static_cast<uint32_t>(row0 * a.ks[2] * ES), vrow0 = static_cast<uint32_t>(row0 * a.vs[2] * ES);
-    const uint32_t kpiece = 16 * (piece0 ^ T::key_swap(row0)), vpiece = 16 * (piece0 ^ T::value_swap(row0));
-    const auto fill = [&](int t, int b) __attribute__((always_inline)) {
-        const uint32_t to = lds + b * 2 * T::bytes + wave * 1024;
-        if (!a.far && t * KT + KT <= reach) {
-            const unsigned char *kt = kbase + static_cast<int64_t>(t) * KT * ES * a.ks[2], *vt = vbase + static_cast<int64_t>(t) * KT * ES * a.vs[2];
-#pragma unroll
-            for (int n = 0; n < T::loads / NW; ++n)
-                dma16_at(kt + static_cast<int64_t>(n * kStep) * ES * a.ks[2], krow + (kpiece ^ (16 * T::key_swap(n * kStep))), to + n * NW * 1024);
-#pragma unroll
-            for (int n = 0; n < T::loads / NW; ++n)
-                dma16_at(vt + static_cast<int64_t>(n * kStep) * ES * a.vs[2], vrow0 + (vpiece ^ (16 * T::value_swap(n * kStep))), to + T::bytes + n * NW * 1024);
-            return;
-        }
-        // (in place of Keys past the last one that is seen, that one)
-#pragma unroll
-        for (int n = 0; n < T::loads / NW; ++n) {
-            const int r = row0 + n * kStep;
-            const int64_t at = min(t * KT + r, reach - 1);
-            dma16_far(kbase + ES * at * a.ks[2] + 16 * (piece0 ^ T::key_swap(r)), to + n * NW * 1024);
-            dma16_far(vbase + ES * at * a.vs[2] + 16 * (piece0 ^ T::value_swap(r)), to + T::bytes + n * NW * 1024);
-        }
-    };
-    if (first < last) fill(first, 0);
+    const Loader<D, Dt, NW> loader(a, item, h, wave, lane, reach);
+    const unsigned char *kbase = loader.keys.base, *vbase = loader.values.base;
+    if (first < last) loader.fill(loader.keys, first, lds);
 
     x8 q[SQ];
     {
@@ -205,6 +294,7 @@ __global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Pr
 #pragma unroll
     for (int c = 0; c < CB; ++c) o[c] = f32x16{};
     float l = 0.f, ref = 0.f, limit = -__builtin_inff();
+    bool odd = false;
 
     // operand addresses inside a tile
     // (the rows are whole multiples of what is exchanged: further pieces are an exclusive or away, further rows a constant)
@@ -217,26 +307,12 @@ __global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Pr
     // Tiles that every row of the wave sees whole come first (a branch in one body became selects in every tile).
     const auto tile = [&](auto masked_tile, int t) __attribute__((always_inline)) {
         constexpr bool masked = decltype(masked_tile)::value;
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // tile t is there, and nobody reads the other buffer any more
-        const uint32_t buf = lds + ((t - first) & 1) * 2 * T::bytes;
-        if (t + 1 < last) fill(t + 1, (t + 1 - first) & 1);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();  // the tile's Keys are there, and nobody reads the last one's Values any more
+        loader.fill(loader.values, t, lds + T::bytes);
+        phase();
         const int k0 = t * KT;
-        if (masked && k0 >= top) return;
-        // What stands where a row does not see need not be finite, and 0 * NaN is NaN: of a tile that holds such Values, one Key at
-        // a time is added to the rows that see it.
-        bool odd = false;
-        if constexpr (masked) {
-            uint32_t found = 0;
-#pragma unroll 4
-            for (int n = 0; n < T::loads; ++n) {
-                const u32x4 w = read16(buf + T::bytes + 1024 * n + 16 * lane);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) found |= (w[x] & E::bits) + E::least;
-            }
-            odd = __any((found & ~E::bits) != 0);
-        }
-        const uint32_t keys = buf + key_at, values = buf + value_at;
+        const uint32_t keys = lds + key_at, values = lds + value_at;
         f32x16 s[KB];
 #pragma unroll
         for (int n = 0; n < SQ; ++n) {
@@ -318,35 +394,27 @@ __global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Pr
                 return E::mfma(__builtin_bit_cast(x8, w), weights, sum);
             }
         };
-        if (!odd) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();  // the tile's Values are there, and nobody reads its Keys any more
+        if (t + 1 < last) loader.fill(loader.keys, t + 1, lds);
+        phase();
+        // What stands where a row does not see need not be finite, and 0 * NaN is NaN: rows of a tile that holds such Values are
+        // formed anew.
+        if constexpr (masked) {
+            uint32_t found = 0;
+#pragma unroll 4
+            for (int n = 0; n < T::loads; ++n) {
+                const u32x4 w = read16(lds + T::bytes + 1024 * n + 16 * lane);
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                phase();
-#pragma unroll
-                for (int c = 0; c < CB; ++c) o[c] = multiply(value(kk, c), p[kk], o[c]);
+                for (int x = 0; x < 4; ++x) found |= (w[x] & E::bits) + E::least;
             }
-        } else {
-#pragma unroll 1
-            for (int key = 0; key < KT; ++key) {
-                const int kk = kWide ? key >> 3 : key >> 4, half = (key >> 2) & 1;
-                const int word = kWide ? key & 3 : ((key & 3) + 4 * ((key >> 3) & 1)) >> 1;
-                const uint32_t keep = kWide ? 0xffffffffu : 0xffffu << (16 * (key & 1));
-                u32x4 pk = __builtin_bit_cast(u32x4, p[0]);
+            odd = odd || __any((found & ~E::bits) != 0);
+        }
 #pragma unroll
-                for (int n = 1; n < KK; ++n)
+        for (int kk = 0; kk < KK; ++kk) {
+            phase();
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) pk[x] = kk == n ? __builtin_bit_cast(u32x4, p[n])[x] : pk[x];
-                const bool seen = k0 + key < lim;
-#pragma unroll
-                for (int c = 0; c < CB; ++c) {
-                    u32x4 w = value(kk, c);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) w[x] &= hi == half && word == x ? keep : 0u;
-                    const f32x16 one = multiply(w, __builtin_bit_cast(x8, pk), f32x16{});
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[c][r] += seen ? one[r] : 0.f;
-                }
-            }
+            for (int c = 0; c < CB; ++c) o[c] = multiply(value(kk, c), p[kk], o[c]);
         }
     };
     const int whole = min(all / KT, last);
@@ -354,6 +422,16 @@ __global__ __launch_bounds__(NW * kWave, D == 256 ? 1 : 2) void prompt_kernel(Pr
     for (; t < whole; ++t) tile(std::false_type(), t);
     for (; t < last; ++t) tile(std::true_type(), t);
 
+    if (odd) {
+        if (!real) return;
+        const unsigned char* src = static_cast<const unsigned char*>(a.q) +
+            ES * (item.q_row * a.qs[0] + static_cast<int64_t>(h * a.g + i) * a.qs[1] + static_cast<int64_t>(item.q_start + j) * a.qs[2]);
+        const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2];
+        const int64_t at = (static_cast<int64_t>(item.slot) * a.n_kv + h) * kRows + wave * 32 + col;
+        one_row<D, Dt>(src, kbase, vbase, ES * a.ks[2], ES * a.vs[2], first * KT, min(last * KT, lim), hi, a.qscale,
+                       item.slot < 0 ? static_cast<unsigned char*>(a.out) + ES * to : nullptr, a.part_o + at * D, a.part_ml + 2 * at);
+        return;
+    }
     l = halves_sum(l);
     if (!real) return;
     // channels 32 c + 8 n + 4 hi .. + 3

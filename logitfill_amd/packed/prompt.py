@@ -38,6 +38,14 @@ def tile_rows(lengths, group: int) -> int:
     return 32 if max(lengths) * group <= 32 else 128
 
 
+def workgroups_per_cu(rows: int, head_dim: int, dtype) -> int:
+    """Workgroups that a CU holds: of four waves by their registers, of one by the LDS of its tiles."""
+    wide = dtype == torch.float32
+    if rows == 32:
+        return (163840 // 2) // (key_tile(head_dim, dtype) * head_dim * (4 if wide else 2))
+    return {64: 3 if wide else 4, 128: 2 if wide else 3, 256: 1 if wide else 2}[head_dim]
+
+
 def split_size(tiles: np.ndarray, n_kv: int, slots: int) -> int:
     """Key tiles that a workgroup takes at most, of row tiles that see ``tiles`` each: the size of least estimated
     time over ``slots`` workgroups at once."""
@@ -134,11 +142,8 @@ class PromptPlan:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a plan's first call uploads its work: run the step once before the capture")
             rows, keys = tile_rows(self.lengths, group), key_tile(head_dim, dtype)
-            per_cu = 8 if rows == 32 else 2
-            if dtype == torch.float32 and head_dim == 256:
-                per_cu = 1
             items, merges, slots = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, keys, n_kv,
-                                              per_cu * _cu_count(self.device))
+                                              workgroups_per_cu(rows, head_dim, dtype) * _cu_count(self.device))
             with torch.inference_mode(False):
                 device = _native.upload(np.concatenate([items, merges]).reshape(-1), torch.int32, self.device)
             event = torch.cuda.Event()
