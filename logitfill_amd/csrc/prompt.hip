@@ -471,14 +471,32 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(Prompt a, const lf_pr
     const int row = item.tile * tile_rows + r, j = row / a.g, i = row - j * a.g;
     if (r >= tile_rows || j >= item.n_q) return;
     const int64_t step = static_cast<int64_t>(a.n_kv) * tile_rows, at = item.slot * step + static_cast<int64_t>(h) * tile_rows + r;
-    float m = -__builtin_inff();
-    for (int s = 0; s < item.parts; ++s) m = fmaxf(m, a.part_ml[2 * (at + s * step)]);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int s = 0; s < item.parts; ++s) {
-        const float ms = a.part_ml[2 * (at + s * step)], w = ms == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms - m);
-        l = fmaf(w, a.part_ml[2 * (at + s * step) + 1], l);
-        o += w * *reinterpret_cast<const f32x4*>(a.part_o + (at + s * step) * D + c);
+    float m = -__builtin_inff(), l = 0.f;
+    constexpr int kTake = 8;  // splits whose loads are on their way at once
+    for (int s0 = 0; s0 < item.parts; s0 += kTake) {
+        f32x4 x[kTake];
+        float ms[kTake], ls[kTake], top = m;
+#pragma unroll
+        for (int k = 0; k < kTake; ++k) {
+            const int64_t of = at + min(s0 + k, item.parts - 1) * step;
+            ms[k] = a.part_ml[2 * of];
+            ls[k] = a.part_ml[2 * of + 1];
+            x[k] = *reinterpret_cast<const f32x4*>(a.part_o + of * D + c);
+        }
+#pragma unroll
+        for (int k = 0; k < kTake; ++k) top = fmaxf(top, ms[k]);
+        const float down = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
+        m = top;
+        l *= down;
+        o *= down;
+#pragma unroll
+        for (int k = 0; k < kTake; ++k) {
+            if (s0 + k >= item.parts || ms[k] == -__builtin_inff()) continue;
+            const float w = __builtin_amdgcn_exp2f(ms[k] - m);
+            l = fmaf(w, ls[k], l);
+            o += w * x[k];
+        }
     }
     o *= l == 0.f ? 0.f : 1.f / l;
     const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2] + c;
