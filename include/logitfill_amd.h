@@ -557,6 +557,8 @@ typedef struct lf_prompt_args {
     int64_t v_strides[3], out_strides[3];
     float scaling;                            /* finite                                       */
     int32_t tile_rows;                        /* 32 or 128                                    */
+    int32_t groups;                           /* workgroups' halves that take Key tiles in turn: 1, or 2 with
+                                                 tile_rows 128, head_dim 64 or 128, bf16 or fp16 (else LF_E_SHAPE) */
     const lf_prompt_item* items;              /* DEVICE                                       */
     const lf_prompt_item* merges;             /* DEVICE (NULL: no row tile is divided)        */
     int32_t n_items, n_merges, n_slots;

@@ -148,7 +148,7 @@ class PromptArgs(ctypes.Structure):
         ("q_strides", c_int64 * 3), ("k_strides", c_int64 * 3),
         ("v_strides", c_int64 * 3), ("out_strides", c_int64 * 3),
         ("scaling", c_float),
-        ("tile_rows", c_int32),
+        ("tile_rows", c_int32), ("groups", c_int32),
         ("items", c_void_p), ("merges", c_void_p),
         ("n_items", c_int32), ("n_merges", c_int32), ("n_slots", c_int32),
         ("workspace", c_void_p), ("workspace_bytes", c_int64),

@@ -47,7 +47,8 @@ int32_t lf_prompt_attention(const lf_prompt_args* args, void* stream) {
     if (!valid_dtype(A.dtype)) return LF_E_DTYPE;
     if (A.head_dim != 64 && A.head_dim != 128 && A.head_dim != 256) return LF_E_UNSUPPORTED;
     if (A.n_kv <= 0 || A.n_q <= 0 || A.n_q % A.n_kv != 0 || A.n_items < 0 || A.n_merges < 0 || A.n_slots < 0) return LF_E_SHAPE;
-    if (A.tile_rows != 32 && A.tile_rows != 128 && (A.tile_rows != 256 || A.head_dim > 128 || A.dtype == LF_FP32)) return LF_E_SHAPE;
+    if (A.tile_rows != 32 && A.tile_rows != 128) return LF_E_SHAPE;
+    if (A.groups != 1 && (A.groups != 2 || A.tile_rows != 128 || A.head_dim > 128 || A.dtype == LF_FP32)) return LF_E_SHAPE;
     if (static_cast<int64_t>(A.n_items) * A.n_kv >= 1ll << 31 || static_cast<int64_t>(A.n_merges) * A.n_kv >= 1ll << 31) return LF_E_SHAPE;
     if (!std::isfinite(A.scaling)) return LF_E_SHAPE;
     if (A.n_items == 0) return LF_OK;

@@ -232,12 +232,18 @@ __device__ __attribute__((noinline)) void one_row(const unsigned char* q, const 
     }
 }
 
-// NW waves of 32 rows each.
+// Groups of NW waves of 32 rows each, that take an item's Key tiles in turn and are joined through LDS at its end.
 template <int D, int Dt>
 constexpr int kPerSimd = Dt == LF_FP32 ? (D == 64 ? 3 : D == 128 ? 2 : 1) : (D == 64 ? 4 : D == 128 ? 3 : 2);  // waves, by their registers
 
-template <int D, int Dt, int NW>
-__global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(Prompt a) {
+template <int D, int Dt, int NW, int Groups>
+struct Shape {
+    static constexpr int sums = NW * kWave * D * 2;  // bytes of a group's sums: D / 2 floats a lane
+    static constexpr int lds = Groups == 1 ? Tile<D, Dt>::lds : (2 * Tile<D, Dt>::lds > sums ? 2 * Tile<D, Dt>::lds : sums) + NW * kWave * 16;
+};
+
+template <int D, int Dt, int NW, int Groups>
+__global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, Dt>)) void prompt_kernel(Prompt a) {
     using T = Tile<D, Dt>;
     using E = Element<Dt>;
     using x8 = typename E::x8;
@@ -247,9 +253,10 @@ __global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(P
     extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];
     const int h = blockIdx.x % a.n_kv;
     const lf_prompt_item item = load_item(a);
-    const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    const int lane = threadIdx.x % kWave, turn = Groups == 1 ? 0 : in_sgpr(static_cast<int>(threadIdx.x / (NW * kWave)));
+    const int wave = in_sgpr(static_cast<int>(threadIdx.x / kWave)) - turn * NW;
     const int col = lane & 31, hi = lane >> 5;
-    const uint32_t lds = lds_addr(smem);
+    const uint32_t lds = lds_addr(smem) + turn * T::lds;
 
     const int row = item.tile * kRows + wave * 32 + col;
     const int j = row / a.g, i = row - j * a.g;
@@ -270,7 +277,7 @@ __global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(P
 
     const Loader<D, Dt, NW> loader(a, item, h, wave, lane, reach);
     const unsigned char *kbase = loader.keys.base, *vbase = loader.values.base;
-    if (first < last) loader.fill(loader.keys, first, lds);
+    if (first + turn < last) loader.fill(loader.keys, first + turn, lds);
 
     x8 q[SQ];
     {
@@ -396,7 +403,7 @@ __global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(P
         };
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __syncthreads();  // the tile's Values are there, and nobody reads its Keys any more
-        if (t + 1 < last) loader.fill(loader.keys, t + 1, lds);
+        if (t + Groups < last) loader.fill(loader.keys, t + Groups, lds);
         phase();
         // What stands where a row does not see need not be finite, and 0 * NaN is NaN: rows of a tile that holds such Values are
         // formed anew.
@@ -418,9 +425,42 @@ __global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(P
         }
     };
     const int whole = min(all / KT, last);
-    int t = first;
-    for (; t < whole; ++t) tile(std::false_type(), t);
-    for (; t < last; ++t) tile(std::true_type(), t);
+    int t = first + turn;
+    for (; t < whole; t += Groups) tile(std::false_type(), t);
+    for (; t < last; t += Groups) tile(std::true_type(), t);
+    l = halves_sum(l);
+    if constexpr (Groups == 2) {
+        if (turn == 1 && first < last && (last - first) % 2 != 0) {  // (a tile fewer: its two barriers)
+            __syncthreads();
+            __syncthreads();
+        }
+        __syncthreads();
+        f32x4* sums = reinterpret_cast<f32x4*>(smem) + wave * kWave + lane;
+        f32x4* stats = reinterpret_cast<f32x4*>(smem + Shape<D, Dt, NW, Groups>::lds - NW * kWave * 16) + wave * kWave + lane;
+        if (turn == 1) {
+#pragma unroll
+            for (int n = 0; n < 4 * CB; ++n) {
+                const f32x16& x = o[n / 4];
+                sums[n * NW * kWave] = f32x4{x[4 * (n % 4)], x[4 * (n % 4) + 1], x[4 * (n % 4) + 2], x[4 * (n % 4) + 3]};
+            }
+            *stats = f32x4{ref, l, odd ? 1.f : 0.f, 0.f};
+        }
+        __syncthreads();
+        if (turn == 1) return;
+        const f32x4 other = *stats;
+        const float mine = l == 0.f ? -__builtin_inff() : ref, its = other[1] == 0.f ? -__builtin_inff() : other[0];
+        const float top = fmaxf(mine, its);
+        const float w0 = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(mine - top), w1 = other[1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(its - top);
+        odd = odd || __any(other[2] != 0.f);
+        ref = top;
+        l = l * w0 + other[1] * w1;
+#pragma unroll
+        for (int n = 0; n < 4 * CB; ++n) {
+            const f32x4 x = sums[n * NW * kWave];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n / 4][4 * (n % 4) + e] = o[n / 4][4 * (n % 4) + e] * w0 + x[e] * w1;
+        }
+    }
 
     if (odd) {
         if (!real) return;
@@ -432,7 +472,6 @@ __global__ __launch_bounds__(NW * kWave, (kPerSimd<D, Dt>)) void prompt_kernel(P
                        item.slot < 0 ? static_cast<unsigned char*>(a.out) + ES * to : nullptr, a.part_o + at * D, a.part_ml + 2 * at);
         return;
     }
-    l = halves_sum(l);
     if (!real) return;
     // channels 32 c + 8 n + 4 hi .. + 3
     if (item.slot < 0) {
@@ -504,12 +543,13 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(Prompt a, const lf_pr
     else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to) = u32x2{Element<Dt>::pack(o[0], o[1]), Element<Dt>::pack(o[2], o[3])};
 }
 
-template <int D, int Dt, int NW>
+template <int D, int Dt, int NW, int Groups>
 int launch_rows(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
-    const auto fn = prompt_kernel<D, Dt, NW>;
-    const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), Tile<D, Dt>::lds);
+    const auto fn = prompt_kernel<D, Dt, NW, Groups>;
+    constexpr int lds = Shape<D, Dt, NW, Groups>::lds;
+    const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
     if (st != LF_OK) return st;
-    hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(A.n_items) * A.n_kv), dim3(NW * kWave), (Tile<D, Dt>::lds), stream, a);
+    hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(A.n_items) * A.n_kv), dim3(Groups * NW * kWave), lds, stream, a);
     if (A.n_merges) {
         const int rows = 32 * NW, per = 256 / (D / 4);
         hipLaunchKernelGGL((prompt_merge_kernel<D, Dt>), dim3(static_cast<uint32_t>(A.n_merges) * A.n_kv, (rows + per - 1) / per), dim3(256), 0,
@@ -521,7 +561,9 @@ int launch_rows(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
 
 template <int D, int Dt>
 int launch_typed(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
-    return A.tile_rows == 32 ? launch_rows<D, Dt, 1>(a, A, stream) : launch_rows<D, Dt, 4>(a, A, stream);
+    if constexpr (D <= 128 && Dt != LF_FP32)
+        if (A.groups == 2) return launch_rows<D, Dt, 4, 2>(a, A, stream);
+    return A.tile_rows == 32 ? launch_rows<D, Dt, 1, 1>(a, A, stream) : launch_rows<D, Dt, 4, 1>(a, A, stream);
 }
 
 template <int D>

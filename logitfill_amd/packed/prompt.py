@@ -23,9 +23,12 @@ from logitfill_amd.packed.cache import _check_device
 from logitfill_amd.packed.reference import _cu_count
 
 MAX_TOKENS = 1 << 24  # of a sequence
-# A workgroup's fixed cost, and what a row tile's division into several adds to each (its partial sums written and
-# merged), in Key tiles.
-ITEM_COST, PART_COST = 2.0, 2.0
+# Microseconds of a Key tile for a workgroup that has its compute unit to itself, and a compute unit's share of one where it
+# holds as many as it can (four waves; of the model's head_dim, float32 or not); of a workgroup's start and end; of the
+# launch that merges divided row tiles; of joining a workgroup's two groups.
+TILE_US = {(64, False): (0.9, 0.69), (128, False): (1.5, 0.95), (256, False): (1.5, 1.25),
+           (64, True): (2.2, 2.0), (128, True): (4.1, 3.9), (256, True): (8.4, 8.4)}
+ITEM_US, MERGE_US, PAIR_US = 3.0, 5.0, 1.5
 
 
 def key_tile(head_dim: int, dtype) -> int:
@@ -46,20 +49,38 @@ def workgroups_per_cu(rows: int, head_dim: int, dtype) -> int:
     return {64: 3 if wide else 4, 128: 2 if wide else 3, 256: 1 if wide else 2}[head_dim]
 
 
-def split_size(tiles: np.ndarray, n_kv: int, slots: int) -> int:
-    """Key tiles that a workgroup takes at most, of row tiles that see ``tiles`` each: the size of least estimated
-    time over ``slots`` workgroups at once."""
+def split_size(tiles: np.ndarray, n_kv: int, cus: int, per_cu: int, head_dim: int, dtype, rows: int = 128) -> tuple[int, int]:
+    """``(Key tiles that a workgroup takes at most, its groups)`` of row tiles that see ``tiles`` each: of least estimated time
+    on ``cus`` compute units of ``per_cu`` workgroups.  A division's gain is the compute units that it sets to work, its price
+    the partial sums, written and read once, and the launch that merges them.  Two groups share a workgroup's tiles
+    without either, where a compute unit has one workgroup at most."""
     longest = int(tiles.max(initial=1))
-    best, size = None, longest
-    for parts in (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128):
-        s = max(1, -(-longest // parts))
-        n = -(-np.maximum(tiles, 1) // s)
-        total = float((tiles + n * (ITEM_COST + np.where(n > 1, PART_COST, 0.0))).sum()) * n_kv
-        one = s + ITEM_COST + (PART_COST if parts > 1 else 0.0)
-        cost = max(total / slots + 0.5 * one, one)
-        if best is None or cost < 0.97 * best:
-            best, size = cost, s
-    return size
+    alone, shared = TILE_US[head_dim, dtype == torch.float32]
+    best, choice = None, (longest, 1)
+    pairs = rows == 128 and head_dim <= 128 and dtype != torch.float32
+    for parts in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256):
+        if parts > longest:
+            break
+        s = -(-longest // parts)
+        n = np.maximum(-(-tiles // s), 1)
+        sizes = np.sort(np.repeat(-(-tiles // n), n * n_kv))[::-1]
+        # the workgroups of a compute unit's first round, the longest of each rank
+        first = float(sizes[: cus * per_cu : cus].sum()) * shared + ITEM_US
+        even = (float(sizes.sum()) * shared + len(sizes) * 0.25 * ITEM_US) / cus
+        if len(sizes) > cus * per_cu:
+            even += 0.3 * float(sizes[cus * per_cu :].mean()) * shared
+        costs = [max(first, even, s * alone + ITEM_US)]
+        if pairs and len(sizes) <= cus and s > 1:
+            costs.append(-(-s // 2) * max(1.2 * alone, 2.2 * shared) + ITEM_US + PAIR_US)
+        more = MERGE_US + 8e-6 * float(n[n > 1].sum()) * n_kv * rows * (head_dim + 2) / 4 if parts > 1 else 0.0
+        for groups, cost in enumerate(costs, 1):
+            if best is None or cost + more < 0.97 * best:
+                best, choice = cost + more, (s, groups)
+        if parts == 1 and len(sizes) >= 4 * cus * per_cu:
+            break  # (as many row tiles keep every compute unit at work)
+        if min(costs) + more > 1.5 * best:
+            break
+    return choice
 
 
 class _Form(NamedTuple):
@@ -70,20 +91,21 @@ class _Form(NamedTuple):
     n_merges: int
     n_slots: int
     rows: int
+    groups: int
     stream: int
     event: torch.cuda.Event
 
 
-def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int, rows: int, keys: int, n_kv: int, slots: int):
-    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``), the merges' and the number of partial sums."""
+def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int, rows: int, head_dim: int, dtype, n_kv: int, cus: int):
+    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``), the merges', the number of partial sums and the groups of a workgroup."""
     n, m = np.asarray(lengths, dtype=np.int64), np.asarray(key_lengths, dtype=np.int64)
     per = -(-n * group // rows)  # row tiles of every sequence
     seq = np.repeat(np.arange(len(n)), per)
     tile = np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)
     last_token = np.minimum((tile * rows + rows - 1) // group, n[seq] - 1)
     reach = np.maximum(m[seq] - n[seq] + last_token + 1, 0)
-    tiles = -(-reach // keys)
-    size = split_size(tiles, n_kv, slots)
+    tiles = -(-reach // key_tile(head_dim, dtype))
+    size, groups = split_size(tiles, n_kv, cus, workgroups_per_cu(rows, head_dim, dtype), head_dim, dtype, rows)
     parts = np.maximum(-(-tiles // size), 1)
     each = -(-tiles // parts)
     parts = np.maximum(-(-tiles // np.maximum(each, 1)), 1)  # (no part is empty)
@@ -103,7 +125,7 @@ def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int,
     items[:, 9] = np.where(items[:, 9] < 0, -1, items[:, 9] + part)
     # the longest first: the short ones fill what is left
     items = items[np.argsort(items[:, 7] - items[:, 8], kind="stable")]
-    return items.astype(np.int32), merges.astype(np.int32), int(np.where(parts > 1, parts, 0).sum())
+    return items.astype(np.int32), merges.astype(np.int32), int(np.where(parts > 1, parts, 0).sum()), groups
 
 
 class PromptPlan:
@@ -141,14 +163,14 @@ class PromptPlan:
         if form is None:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a plan's first call uploads its work: run the step once before the capture")
-            rows, keys = tile_rows(self.lengths, group), key_tile(head_dim, dtype)
-            items, merges, slots = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, keys, n_kv,
-                                              workgroups_per_cu(rows, head_dim, dtype) * _cu_count(self.device))
+            rows = tile_rows(self.lengths, group)
+            items, merges, slots, groups = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, head_dim, dtype, n_kv,
+                                              _cu_count(self.device))
             with torch.inference_mode(False):
                 device = _native.upload(np.concatenate([items, merges]).reshape(-1), torch.int32, self.device)
             event = torch.cuda.Event()
             event.record(torch.cuda.current_stream(self.device))
-            form = self._forms[key] = _Form(device, len(items), len(merges), slots, rows, stream, event)
+            form = self._forms[key] = _Form(device, len(items), len(merges), slots, rows, groups, stream, event)
         elif stream != form.stream and not torch.cuda.is_current_stream_capturing():
             here = torch.cuda.current_stream(self.device)
             here.wait_event(form.event)
@@ -237,7 +259,7 @@ def _attend(query, key, value, scaling: float, plan: PromptPlan, packed_q: bool,
     a.dtype, a.n_q, a.n_kv, a.head_dim = code, n_q, n_kv, D
     a.q_strides[:], a.k_strides[:] = query.stride()[:3], key.stride()[:3]
     a.v_strides[:], a.out_strides[:] = value.stride()[:3], out.stride()[:3]
-    a.scaling, a.tile_rows = scaling, form.rows
+    a.scaling, a.tile_rows, a.groups = scaling, form.rows, form.groups
     a.items, a.n_items = form.items.data_ptr(), form.n_items
     if form.n_merges:
         a.merges, a.n_merges, a.n_slots = a.items + 48 * form.n_items, form.n_merges, form.n_slots

@@ -69,13 +69,13 @@ def test_divided_row_tiles_agree_with_whole_ones(gpu, monkeypatch):
     from logitfill_amd.packed import prompt
 
     q, k, v, _, out = run(gpu, [150, 40], [1500, 700], (4, 2), 128, "bf16", seed=2)
-    for size in (1, 2, 5, 1000):
-        monkeypatch.setattr(prompt, "split_size", lambda tiles, n_kv, slots: size)
+    for size, groups in ((1, 1), (2, 1), (5, 1), (1000, 1), (1, 2), (2, 2), (7, 2), (1000, 2)):
+        monkeypatch.setattr(prompt, "split_size", lambda *args: (size, groups))
         plan = PromptPlan([150, 40], [1500, 700], device=gpu)
         again = prompt_attention(q.to(gpu), k.to(gpu), v.to(gpu), 128 ** -0.5, plan)
         assert_within(again, *expected(q, k, v, [150, 40], [1500, 700], 128 ** -0.5, "bf16", True, True), f"split {size}")
         form, = plan._forms.values()
-        assert (form.n_merges > 0) == (size < 24)
+        assert (form.n_merges > 0) == (size < 24) and form.groups == groups
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
@@ -83,6 +83,17 @@ def test_divided_row_tiles_agree_with_whole_ones(gpu, monkeypatch):
 def test_scalings(gpu, scaling, dtype):
     """Zero weighs every Key alike, a negative one turns the order; sharp weights move the reference point often."""
     run(gpu, [140, 50], None, (4, 2), 64, dtype, seed=4, scaling=scaling)
+
+
+@pytest.mark.parametrize("dtype,D", [("bf16", 64), ("fp16", 128)])
+def test_two_groups_of_a_workgroup(gpu, monkeypatch, dtype, D):
+    """One, an even and an odd number of Key tiles; rows that see nothing; what is masked need not be finite."""
+    from logitfill_amd.packed import prompt
+
+    monkeypatch.setattr(prompt, "split_size", lambda *args: (1000, 2))
+    run(gpu, [1, 0, 37, 130, 300, 65, 64], None, (7, 1), D, dtype, seed=D)
+    run(gpu, [50, 130, 5], [700, 128, 3], (4, 2), D, dtype, packed_q=False, packed_k=False, seed=D + 1, spare=2)
+    test_what_is_masked_need_not_be_finite(gpu, D, dtype)
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])

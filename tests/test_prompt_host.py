@@ -7,18 +7,19 @@ import torch
 
 from logitfill_amd import _native
 from logitfill_amd.packed import PromptPlan, prompt_attention
-from logitfill_amd.packed.prompt import split_size, tile_rows, work_items
+from logitfill_amd.packed.prompt import key_tile, split_size, tile_rows, work_items
 
 
 @pytest.mark.parametrize("seed", range(12))
-@pytest.mark.parametrize("rows,keys", [(32, 64), (128, 64), (128, 32)])
-def test_every_row_tile_s_keys_are_covered_once(seed, rows, keys):
+@pytest.mark.parametrize("rows,D,dtype", [(32, 64, torch.bfloat16), (128, 128, torch.float16), (128, 64, torch.float32)])
+def test_every_row_tile_s_keys_are_covered_once(seed, rows, D, dtype):
+    keys = key_tile(D, dtype)
     rng = np.random.default_rng(seed)
     B, g, n_kv = int(rng.integers(1, 7)), int(rng.integers(1, 9)), int(rng.integers(1, 9))
     n = rng.integers(0, 700, B)
     m = np.maximum(0, n + rng.integers(-20, 4000, B))
     packed = bool(seed % 2)
-    items, merges, slots = work_items(n, m, packed, not packed, g, rows, keys, n_kv, 512)
+    items, merges, slots, groups = work_items(n, m, packed, not packed, g, rows, D, dtype, n_kv, 256)
     assert (np.diff(items[:, 8] - items[:, 7]) <= 0).all()  # the longest first
     assert sorted(items[items[:, 9] >= 0, 9]) == list(range(slots))
     by_tile = {}
@@ -46,8 +47,8 @@ def test_every_row_tile_s_keys_are_covered_once(seed, rows, keys):
 
 
 def test_long_keys_of_few_rows_are_divided():
-    assert split_size(np.array([512]), 4, 2048) < 32
-    assert split_size(np.full(4096, 256), 8, 512) == 256  # enough row tiles
+    assert split_size(np.array([512]), 4, 256, 5, 128, torch.bfloat16, 32)[0] < 64
+    assert split_size(np.full(4096, 256), 8, 256, 3, 128, torch.bfloat16) == (256, 1)  # enough row tiles
     assert tile_rows([1, 4], 8) == 32 and tile_rows([5], 8) == 128
 
 
@@ -69,7 +70,7 @@ def test_the_cpu():
 
 def _args(**changes):
     a = _native.PromptArgs()
-    a.dtype, a.n_q, a.n_kv, a.head_dim, a.scaling, a.tile_rows, a.n_items = 0, 4, 2, 64, 0.1, 128, 1
+    a.dtype, a.n_q, a.n_kv, a.head_dim, a.scaling, a.tile_rows, a.groups, a.n_items = 0, 4, 2, 64, 0.1, 128, 1, 1
     for name in ("query", "key", "value", "out", "items"):
         setattr(a, name, 4096)
     for name, value in changes.items():
@@ -80,6 +81,8 @@ def _args(**changes):
 @pytest.mark.parametrize("changes,status", [
     ({"dtype": 3}, _native.LF_E_DTYPE), ({"head_dim": 96}, _native.LF_E_UNSUPPORTED), ({"n_q": 3}, _native.LF_E_SHAPE),
     ({"n_kv": 0}, _native.LF_E_SHAPE), ({"n_items": -1}, _native.LF_E_SHAPE), ({"tile_rows": 64}, _native.LF_E_SHAPE),
+    ({"groups": 0}, _native.LF_E_SHAPE), ({"groups": 2, "tile_rows": 32}, _native.LF_E_SHAPE), ({"groups": 2, "dtype": 2}, _native.LF_E_SHAPE),
+    ({"groups": 2, "head_dim": 256}, _native.LF_E_SHAPE),
     ({"n_items": 1 << 30, "n_kv": 2}, _native.LF_E_SHAPE), ({"scaling": float("nan")}, _native.LF_E_SHAPE),
     ({"scaling": float("inf")}, _native.LF_E_SHAPE), ({"n_items": 0}, _native.LF_OK), ({"query": None}, _native.LF_E_NULL),
     ({"out": None}, _native.LF_E_NULL), ({"items": None}, _native.LF_E_NULL), ({"n_merges": 1}, _native.LF_E_NULL),
