@@ -147,6 +147,11 @@ int32_t lf_int4_shared_attention(const lf_int4_layer* layer, const lf_int4_layer
     if (A.n_pages > 0) return LF_E_UNSUPPORTED;
     if (many_rows ? A.dtype != LF_BF16 || layer->head_dim > 128 : shared_split_tokens <= 0 || shared_split_tokens % 32 != 0)
         return many_rows ? LF_E_UNSUPPORTED : LF_E_SHAPE;
+    // (256 threads a workgroup, 2^32 in a grid)
+    const int64_t g = A.n_q / layer->n_kv, rows = g * A.q_len * (layer->batch / prefix->batch), tile = many_rows ? 128 : 16;
+    const int64_t shared = (rows + tile - 1) / tile * layer->n_kv * prefix->batch * shared_splits;
+    const int64_t own = (g * A.q_len + 15) / 16 * layer->n_kv * layer->batch * A.splits;
+    if (shared + own >= 1 << 24) return LF_E_SHAPE;
     return lf::launch_int4_shared(*layer, *prefix, A, shared_splits, shared_split_tokens, many_rows != 0, static_cast<hipStream_t>(stream));
 }
 

@@ -141,7 +141,8 @@ __device__ __forceinline__ void wait_ring() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-// Shared: of a prefix that ``each`` sequences share; the rows are all their queries, and the sums always partial ones.
+// Shared: of prefixes that ``each`` sequences share, whose rows are all their queries (``pre``), and of the sequences' own rows, in
+// one launch; the sums are always partial ones.
 template <int D, int GROUP, int Dt, bool Shared>
 __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(Int4Attention a) {
     using R = Int4Rec<D, GROUP>;
@@ -158,13 +159,26 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     // of sequences of unlike lengths (splits first: 32 ragged contexts of 4K-64K tokens in 4 splits 545 us, against 429: 2 of 8 XCDs
     // had the last, mostly empty split) and the row tiles of a head, which read the same records, few of them; the
     // splits last, so that a long sequence's later ones follow everyone's first.
-    const int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
+    int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
+    const bool pre = Shared && static_cast<int>(blockIdx.x) < a.shared_blocks;
+    const lf_int4_layer L = Shared && !pre ? a.own : a.L;
+    const int splits = Shared && !pre ? a.own_splits : a.splits, split_tokens = Shared && !pre ? a.own_split_tokens : a.split_tokens;
+    if constexpr (Shared) {
+        const int tiles = pre ? a.shared_tiles : a.own_tiles;
+        int id = static_cast<int>(blockIdx.x) - (pre ? 0 : a.shared_blocks);
+        h = id % L.n_kv;
+        id /= L.n_kv;
+        tile = id % tiles;
+        id /= tiles;
+        b = id % L.batch;
+        part = id / L.batch;
+    }
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
     // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
     int i, j;
     SharedRow row_at;
-    if constexpr (Shared) {
+    if (pre) {
         row_at = shared_row(a, b, tile * kTile + col);
         i = row_at.i;
         j = row_at.j;
@@ -176,18 +190,18 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         i = r / a.q_len;
         j = r % a.q_len;
     }
-    const bool real = Shared ? row_at.real : i < a.g;
-    const int seq = Shared ? row_at.b : b;
+    const bool real = pre ? row_at.real : i < a.g;
+    const int seq = pre ? row_at.b : b;
     // The first record is on its way before the sequence's length is: where it lies hangs on neither (with pages or
     // behind a many-row prefix it does).  A wave that finds it has none waits for the load all the same.
-    const uint8_t* base = int4_block(a.L, b, h, 0, R::bytes);
+    const uint8_t* base = int4_block(L, b, h, 0, R::bytes);
     const uint32_t ring = lds_addr(smem) + wave * kRing * R::bytes;
-    const int64_t early = static_cast<int64_t>(part) * (a.split_tokens / kBlock) + wave;
-    const bool ahead = (Shared || (!a.n_pages && !a.prefix)) && early < a.L.cap_tokens / kBlock;
+    const int64_t early = static_cast<int64_t>(part) * (split_tokens / kBlock) + wave;
+    const bool ahead = (Shared || (!a.n_pages && !a.prefix)) && early < L.cap_tokens / kBlock;
     if (ahead) S::load(base + early * R::bytes, ring, lane);
-    const int len = int4_len(a.L, b);
-    const int n = Shared ? 0 : a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-    const int lim = Shared ? shared_limit(a, row_at, len) : real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
+    const int len = int4_len(L, b);
+    const int n = pre ? 0 : a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
+    const int lim = pre ? shared_limit(a, row_at, len) : real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
     int all = real ? lim : 0x7fffffff, top = lim;                 // rows every query of the tile sees, and any
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {
@@ -220,10 +234,10 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         }
         __syncthreads();
     } else {
-        const int blocks = (top + kBlock - 1) / kBlock, per = a.split_tokens / kBlock;
+        const int blocks = (top + kBlock - 1) / kBlock, per = split_tokens / kBlock;
         first = !Shared && a.prefix ? min(prefix_records(a, len, n, tile / (kManyRows / kTile)), blocks)
                                     : static_cast<int>(min(static_cast<int64_t>(part) * per, static_cast<int64_t>(blocks)));
-        last = part + 1 == a.splits ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
+        last = part + 1 == splits ? blocks : static_cast<int>(min(static_cast<int64_t>(first) + per, static_cast<int64_t>(blocks)));
     }
     const int count = last > first + wave ? (last - first - wave + kWaves - 1) / kWaves : 0;  // this wave's records
     // The k-th of them, or -1 for one that is not attended (its place in the ring is filled with another).
@@ -257,7 +271,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     uint32_t most_scale = 0;
     float raise[G];
     if constexpr (NP == 1) {
-        for (int k = lane; k < count; k += kWave) most_scale = max(most_scale, static_cast<uint32_t>(*int4_top(a.L, b, h, block_at(k))));
+        for (int k = lane; k < count; k += kWave) most_scale = max(most_scale, static_cast<uint32_t>(*int4_top(L, b, h, block_at(k))));
 #pragma unroll
         for (int m = 1; m < kWave; m <<= 1) most_scale = max(most_scale, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most_scale), m, kWave)));
     } else {
@@ -480,6 +494,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     }
     if (!real) return;
     const int64_t row = (static_cast<int64_t>(seq) * a.n_q + h * a.g + i) * a.q_len + j;
+    const int part0 = Shared && !pre ? a.splits : a.part0;
     if (!Shared && a.parts == 1) {
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;  // (no row seen: zeros)
 #pragma unroll
@@ -487,10 +502,10 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
         each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<Dt>(a.out, row * D + c, x); });
         return;
     }
-    float* dst = a.part_o + (row * a.parts + a.part0 + part) * D;
+    float* dst = a.part_o + (row * a.parts + part0 + part) * D;
     each_run<D, GROUP>(o, quad, [&](int c, const float (&x)[4]) { store_row<LF_FP32>(dst, c, x); });
     if (quad == 0) {
-        float* ml = a.part_ml + (row * a.parts + a.part0 + part) * 2;
+        float* ml = a.part_ml + (row * a.parts + part0 + part) * 2;
         ml[0] = m_all;
         ml[1] = l_all;
     }
@@ -551,6 +566,12 @@ __global__ __launch_bounds__(256) void int4_merge_kernel(Int4Attention a, int dt
     for (int c = 0; c < C; ++c) store_from_f32(a.out, row * D + lane * C + c, dtype, l == 0.f ? 0.f : o[c] / l);
 }
 
+template <int D>
+void launch_merge(const Int4Attention& a, int batch, int dtype, hipStream_t stream) {
+    const uint32_t rows = static_cast<uint32_t>(batch) * a.n_q * a.q_len;
+    hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.parts > 16 ? 256 : 64), 0, stream, a, dtype);
+}
+
 template <int D, int GROUP, int Dt>
 int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
     const auto fn = int4_attention_kernel<D, GROUP, Dt, false>;
@@ -562,22 +583,24 @@ int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
     Int4Attention rest = a;  // what a many-row launch leaves
     rest.part0 += a.prefix;
     hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, rest);
-    if (a.parts > 1) {
-        const uint32_t rows = static_cast<uint32_t>(a.L.batch) * a.n_q * a.q_len;
-        hipLaunchKernelGGL((int4_merge_kernel<D>), dim3(rows), dim3(a.parts > 16 ? 256 : 64), 0, stream, a, Dt);
-    }
+    if (a.parts > 1) launch_merge<D>(a, a.L.batch, Dt, stream);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }
 
-// The rows of a shared prefix, 16 at a time.
+// The rows of shared prefixes, 16 at a time, and with own_splits the sequences' own and the merge.
 template <int D, int GROUP, int Dt>
-int launch_shared_typed(const Int4Attention& a, hipStream_t stream) {
+int launch_shared_typed(Int4Attention a, hipStream_t stream) {
     const auto fn = int4_attention_kernel<D, GROUP, Dt, true>;
-    const int lds = Ring<D, GROUP>::lds, tiles = (a.g * a.q_len * a.each + kTile - 1) / kTile;
+    const int lds = Ring<D, GROUP>::lds;
     const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
     if (st != LF_OK) return st;
-    hipLaunchKernelGGL(fn, dim3(a.L.n_kv * tiles, a.L.batch, a.splits), dim3(kWaves * kWave), lds, stream, a);
+    a.shared_tiles = (a.g * a.q_len * a.each + kTile - 1) / kTile;
+    a.own_tiles = (a.g * a.q_len + kTile - 1) / kTile;
+    a.shared_blocks = a.L.n_kv * a.shared_tiles * a.L.batch * a.splits;
+    const int own_blocks = a.own.n_kv * a.own_tiles * a.own.batch * a.own_splits;
+    hipLaunchKernelGGL(fn, dim3(a.shared_blocks + own_blocks), dim3(kWaves * kWave), lds, stream, a);
+    if (a.own_splits) launch_merge<D>(a, a.own.batch, Dt, stream);
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? LF_OK : static_cast<int>(err);
 }
@@ -643,15 +666,18 @@ int launch_int4_shared(const lf_int4_layer& L, const lf_int4_layer& P, const lf_
     a.splits = splits;
     a.split_tokens = split_tokens;
     a.each = L.batch / P.batch;
-    a.own_lens = L.lens;
-    a.own_cap = L.cap_tokens;
+    a.own = L;
+    // the sequences' own rows in the same launch, where both are the general kernel's
+    const bool one = !many_rows && A.prefix_splits == 0;
+    a.own_splits = one ? A.splits : 0;
+    a.own_split_tokens = A.split_tokens;
     const int st = many_rows ? launch_int4_shared_rows(a, stream) : int4_dispatch(P, [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
         return A.dtype == LF_BF16 ? launch_shared_typed<D, GROUP, LF_BF16>(a, stream)
                : A.dtype == LF_FP16 ? launch_shared_typed<D, GROUP, LF_FP16>(a, stream)
                                     : launch_shared_typed<D, GROUP, LF_FP32>(a, stream);
     });
-    return st == LF_OK ? launch_own(own, A, stream) : st;
+    return st == LF_OK && !one ? launch_own(own, A, stream) : st;
 }
 
 }  // namespace lf

@@ -124,10 +124,12 @@ struct Int4Attention {
     int prefix;                // splits of the many-row kernel in front of them
     int parts;                 // of every output row
     int part0;                 // the first one of this launch
-    // A shared prefix (the kernels' Shared forms): L holds the prefixes, one for ``each`` sequences in turn.
+    // A shared prefix (the kernels' Shared forms): L holds the prefixes, one for ``each`` sequences in turn, and own the
+    // sequences.  The general kernel's launch holds shared_blocks workgroups of the prefixes, shared_tiles row tiles each,
+    // and behind them those of the sequences' own rows.
+    lf_int4_layer own;
     int each;
-    const int32_t* own_lens;   // [batch] of the sequences behind them
-    int own_cap;
+    int shared_blocks, shared_tiles, own_tiles, own_splits, own_split_tokens;
     float* part_o;             // [batch * n_q * q_len][parts][D]
     float* part_ml;            // [batch * n_q * q_len][parts][2]
 };
@@ -145,7 +147,7 @@ __device__ __forceinline__ SharedRow shared_row(const Int4Attention& a, int pref
 __device__ __forceinline__ int shared_limit(const Int4Attention& a, const SharedRow& row, int len) {
     if (!row.real) return 0;
     const int n = a.q_lens ? min(max(a.q_lens[row.b], 0), a.q_len) : a.q_len;
-    const int own = min(max(a.own_lens[row.b], 0), a.own_cap);
+    const int own = int4_len(a.own, row.b);
     return row.j < n ? min(max(len + own - n + row.j + 1, 0), len) : 0;
 }
 

@@ -677,15 +677,19 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
         a.pages, a.n_pages = pages.data_ptr(), pages.shape[3]
         # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
         tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
+    shared = _shared_plan(manager, layer_idx, q_len, query.dtype, lengths, cus)
     if pages is None and _many_rows(group, q_len, manager.n_kv, D, manager.group_size, query.dtype, tokens):
         a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
                                          many_rows_per_cu(D, manager.group_size), MANY_ROWS_OVERHEAD)
         a.splits = 1
+        if shared:
+            a.prefix_splits = min(a.prefix_splits, MAX_SPLITS // 2)
+    elif shared:
+        a.splits, a.split_tokens = shared[1]
     else:
         a.splits, a.split_tokens = plan_splits(tokens, manager.n_kv * tiles, cus,
                                                workgroups_per_cu(D, manager.group_size))
-    shared = _shared_plan(manager, layer_idx, q_len, query.dtype, lengths, cus)
-    parts = a.splits + a.prefix_splits + (shared[0] if shared else 0)
+    parts = a.splits + a.prefix_splits + (shared[0][0] if shared else 0)
     if parts > 1:
         nbytes = 4 * B * n_q * q_len * parts * (D + 2)  # lf_int4_workspace_bytes
         ws = _workspace(manager, nbytes)
@@ -693,7 +697,7 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
     stream = _native.current_stream_ptr(manager.device)
     if shared:
         prefix = manager.prefix.layers[layer_idx].layer_struct()
-        st = _native.load().lf_int4_shared_attention(layer.layer_struct(), prefix, a, *shared, stream)
+        st = _native.load().lf_int4_shared_attention(layer.layer_struct(), prefix, a, *shared[0], stream)
         _native.check(st, "lf_int4_shared_attention")
         return out
     st = _native.load().lf_int4_attention(layer.layer_struct(), a, stream)
@@ -701,27 +705,62 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
     return out
 
 
-# Query rows per kv head, of all the sequences of a prefix, from which on the many-row kernel takes it.
-SHARED_ROWS = 33
+# From this much work on (products of a row's channel and a token's, over all prefixes) the many-row kernel takes shared
+# prefixes, per group size (bf16, head_dim up to 128, 64 rows): below, the general kernel's launch, which holds the sequences' own
+# rows too, is faster although it unpacks a record for every 16 rows.  us a call with 200 own tokens, general / many-row: 28 /
+# 4 heads of 128, a prefix of 32K, groups of 64, 112 rows 34 / 48, 448 84 / 82, 896 145 / 123; groups of 128, 896 rows 123 /
+# 144; 32 / 8 heads, groups of 32, 64 rows 44 / 55, 128 71 / 61, 512 219 / 156; 14 / 2 heads of 64, 896 rows, groups of 64 and
+# 32, 51 / 56 and 61 / 56; prefixes of 4K, up to 896 rows, 16 to 52 / 19 to 64.
+SHARED_MANY_ROWS = {32: 3e9, 64: 1e10, 128: 3e10}
+SHARED_LEAST_ROWS = 64
+
+
+@functools.lru_cache(maxsize=512)
+def _shared_split(prefixes: tuple, rows: int, batch: int, longest: int, own: int, own_rows: int, slots: int) -> int:
+    """Units that a split takes of shared prefixes (their units, ``rows`` workgroups a split) and of the rows of the ``batch``
+    sequences behind them (``own`` units in all, ``own_rows`` workgroups a split), which run side by side: the size of
+    least estimated time (as ``_plan``)."""
+    total, longest = sum(prefixes) * rows + own * own_rows, max(max(prefixes), longest)
+    least = -(-longest // (MAX_SPLITS // 2))
+
+    def items(size):
+        return rows * sum(-(-u // size) for u in prefixes) + own_rows * (batch + own // size)
+
+    def cost(size):
+        n = items(size)
+        return size + SPLIT_OVERHEAD if n <= slots else (total + SPLIT_OVERHEAD * n) / slots + 0.3 * size
+
+    share = max(1, least, -(-total // slots))
+    sizes = {max(least, total // (slots * k), 1) for k in (2, 3, 4)} | {share, longest}
+    once = next((size for size in range(share, min(longest, 3 * share) + 1) if items(size) <= slots), None)
+    if once:
+        sizes.add(once)
+    return min((min(size, longest) for size in sorted(sizes, reverse=True)), key=cost)
 
 
 def _shared_plan(manager, layer_idx: int, q_len: int, dtype, lengths, cus: int):
-    """``(splits, split_tokens, many_rows)`` of the manager's prefix, or None where there is none."""
+    """``((splits, split_tokens, many_rows)`` of the manager's prefix, ``(splits, split_tokens)`` of the own rows), or None
+    where there is no prefix."""
     prefix = manager.prefix
     if prefix is None:
         return None
     tokens = prefix.layers[layer_idx].lengths
     if not max(tokens):
         return None
-    D, group = manager.head_dim, manager.group_size
-    rows = manager.n_q // manager.n_kv * q_len * (manager.batch_size // prefix.batch_size)
+    D, group, n_kv = manager.head_dim, manager.group_size, manager.n_kv
+    each = manager.n_q // n_kv * q_len
+    rows = each * (manager.batch_size // prefix.batch_size)
     own = manager.layers[layer_idx].lengths
-    behind = all(n >= (q_len if lengths is None else lengths[b]) for b, n in enumerate(own))  # every query sees all of it
-    if rows >= SHARED_ROWS and dtype == torch.bfloat16 and D <= 128 and behind:
-        splits, size = plan_splits(tokens, manager.n_kv * -(-rows // 128), cus, many_rows_per_cu(D, group), MANY_ROWS_OVERHEAD)
-        return min(splits, MAX_SPLITS // 2), size, 1
-    splits, size = plan_splits(tokens, manager.n_kv * -(-rows // 16), cus, workgroups_per_cu(D, group))
-    return splits, size, 0
+    # every query sees all of its prefix
+    behind = min(own) >= q_len or lengths is not None and all(n >= m for n, m in zip(own, lengths))
+    if (rows >= SHARED_LEAST_ROWS and dtype == torch.bfloat16 and D <= 128 and behind
+            and sum(tokens) * rows * n_kv * D >= SHARED_MANY_ROWS[group]):
+        splits, size = plan_splits(tokens, n_kv * -(-rows // 128), cus, many_rows_per_cu(D, group), MANY_ROWS_OVERHEAD)
+        return (min(splits, MAX_SPLITS // 2), size, 1), plan_splits(own, n_kv * -(-each // 16), cus, workgroups_per_cu(D, group))
+    size = _shared_split(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), n_kv * -(-rows // 16),
+                         len(own), max(own) // SPLIT_UNIT + 1, sum(own) // SPLIT_UNIT, n_kv * -(-each // 16),
+                         workgroups_per_cu(D, group) * cus) * SPLIT_UNIT
+    return (-(-max(tokens) // size), size, 0), (-(-max(max(own), 1) // size), size)
 
 
 @_here

@@ -111,6 +111,7 @@ class Rotary:
         with torch.inference_mode(False):
             self._turns = torch.tensor([f / (2 * math.pi) for f in freq], dtype=torch.float64).to(self.device)
         self._stream = _native.current_stream_ptr(self.device)
+        self._args: dict = {}  # argument blocks by the tensors' forms
 
     def _check_rows(self, t: torch.Tensor, name: str) -> torch.Tensor:
         if t.device != self.device:
@@ -139,38 +140,58 @@ class Rotary:
         n_kv = 0 if key is None else key.shape[1]
         if B * T >= 1 << 31 or n_q + n_kv > 4096:
             raise ValueError("at most 2^31 - 1 tokens and 4096 heads a call")
-        a = _native.RotaryArgs()
-        a.dtype = _native.dtype_code(query.dtype)
+        where = None
         if isinstance(positions, torch.Tensor):
             if positions.dtype not in (torch.int32, torch.int64):
                 raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
             if positions.device != self.device:
                 raise ValueError(f"positions are on {positions.device}, the frequencies on {self.device}")
-            shape = tuple(positions.shape)
-            if shape not in ((T,), (1, T), (B, T)):
-                raise ValueError(f"positions must be [{T}], [1, {T}] or [{B}, {T}], got {shape}")
-            a.positions, a.wide = positions.data_ptr(), positions.dtype == torch.int64
-            a.position_strides[0] = positions.stride(0) if len(shape) == 2 and shape[0] > 1 else 0
-            a.position_strides[1] = positions.stride(-1)
+            shape = positions.shape
+            if shape != (T,) and shape != (1, T) and shape != (B, T):
+                raise ValueError(f"positions must be [{T}], [1, {T}] or [{B}, {T}], got {tuple(shape)}")
+            where = (shape, positions.stride(), positions.dtype)
+        code = _native.dtype_code(query.dtype)
+        q_out, k_out = _like(query), None if key is None else _like(key)
+        if query.numel() == 0 and (key is None or key.numel() == 0):
+            return q_out, k_out
+        form = (code, query.shape, query.stride(), None if key is None else (n_kv, key.stride()), where)
+        kept = self._args.get(form)
+        if kept is None:
+            if len(self._args) >= 64:
+                self._args.clear()
+            kept = self._args[form] = self._describe(code, query, key, q_out, k_out, where)
+        a = _native.RotaryArgs.from_buffer_copy(kept)
+        a.query, a.query_out = query.data_ptr(), q_out.data_ptr()
+        if key is not None:
+            a.key, a.key_out = key.data_ptr(), k_out.data_ptr()
+        if where is not None:
+            a.positions = positions.data_ptr()
         else:
             a.start = int(positions)
-        out = _like(query), None if key is None else _like(key)
-        if query.numel() == 0 and (key is None or key.numel() == 0):
-            return out
-        a.batch, a.tokens, a.n_q, a.n_kv = B, T, n_q, n_kv
-        a.head_dim, a.rotary_dim, a.interleaved = D, self.rotary_dim, self.layout == "interleaved"
-        a.turns, a.factor = self._turns.data_ptr(), self.attention_factor
-        a.query, a.query_out = query.data_ptr(), out[0].data_ptr()
-        a.q_strides[:], a.qo_strides[:] = query.stride()[:3], out[0].stride()[:3]
-        if key is not None:
-            a.key, a.key_out = key.data_ptr(), out[1].data_ptr()
-            a.k_strides[:], a.ko_strides[:] = key.stride()[:3], out[1].stride()[:3]
         if torch.cuda.current_device() == self.device.index:
             self._launch(a)
         else:
             with torch.cuda.device(self.device):
                 self._launch(a)
-        return out
+        return q_out, k_out
+
+    def _describe(self, code: int, query, key, q_out, k_out, where):
+        """The argument block of calls of this form, without their addresses."""
+        a = _native.RotaryArgs()
+        a.dtype = code
+        a.batch, a.n_q, a.tokens, a.head_dim = query.shape
+        a.n_kv = 0 if key is None else key.shape[1]
+        a.rotary_dim, a.interleaved = self.rotary_dim, self.layout == "interleaved"
+        a.turns, a.factor = self._turns.data_ptr(), self.attention_factor
+        a.q_strides[:], a.qo_strides[:] = query.stride()[:3], q_out.stride()[:3]
+        if key is not None:
+            a.k_strides[:], a.ko_strides[:] = key.stride()[:3], k_out.stride()[:3]
+        if where is not None:
+            shape, stride, dtype = where
+            a.wide = dtype == torch.int64
+            a.position_strides[0] = stride[0] if len(shape) == 2 and shape[0] > 1 else 0
+            a.position_strides[1] = stride[-1]
+        return a
 
     def _launch(self, a) -> None:
         stream = _native.current_stream_ptr(self.device)

@@ -12,6 +12,15 @@ from tests.int4_helpers import assert_within, attention_bound, many_rows_bound, 
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True, params=["rule", "many"])
+def kernel(request, monkeypatch):
+    """By the rule, which takes these sizes to the general kernel, and by the many-row kernel wherever it serves."""
+    if request.param == "many":
+        monkeypatch.setattr(int4, "SHARED_MANY_ROWS", dict.fromkeys((32, 64, 128), 0))
+        monkeypatch.setattr(int4, "SHARED_LEAST_ROWS", 1)
+    return request.param
+
+
 def pair(gpu, D, group, heads, prefixes, batch, layers=1, **kw):
     n_q, n_kv = heads
     prefix = Int4KVManager(layers, n_q, n_kv, D, 64, group, gpu, batch_size=prefixes)
@@ -122,7 +131,7 @@ def test_without_the_prefix_it_is_the_cache_s_own(gpu):
 
 
 @pytest.mark.parametrize("heads", [(4, 2), (28, 2)])
-def test_rows_taken_back_need_not_be_finite(gpu, heads):
+def test_rows_taken_back_need_not_be_finite(gpu, heads, kernel):
     """What stands behind a prefix's last row: infinities and NaN of rows that were truncated."""
     D, group, common, own = 128, 64, [75], [4, 9, 2]
     before, behind, q, prefix, mgr, out = check(gpu, D, group, heads, "bf16", common, own, seed=14)
@@ -132,7 +141,7 @@ def test_rows_taken_back_need_not_be_finite(gpu, heads):
     prefix.truncate(75)
     again = int4_attention(mgr, 0, q.to(gpu), None, None, D ** -0.5)
     assert_within(again, *want(q, before, behind, common, own, group, D ** -0.5, "bf16", top=65504.0))
-    if heads[0] == 28:  # (the many-row kernel takes its ranges from the rows that are there)
+    if kernel == "many":  # (it takes its ranges from the rows that are there)
         assert torch.equal(again, out)
 
 
