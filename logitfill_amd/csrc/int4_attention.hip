@@ -40,7 +40,7 @@
 
 namespace lf {
 int launch_int4_prefix(const Int4Attention& a, hipStream_t stream);
-int launch_int4_shared_rows(const Int4Attention& a, hipStream_t stream);
+int launch_int4_shared_rows(const Int4Shared& a, hipStream_t stream);
 
 namespace {
 
@@ -141,10 +141,14 @@ __device__ __forceinline__ void wait_ring() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
+// The layer whose rows a workgroup reads.
+__device__ __forceinline__ const lf_int4_layer& layer_of(const Int4Attention& a, bool) { return a.L; }
+__device__ __forceinline__ lf_int4_layer layer_of(const Int4Shared& a, bool pre) { return pre ? a.L : a.own; }
+
 // Shared: of prefixes that ``each`` sequences share, whose rows are all their queries (``pre``), and of the sequences' own rows, in
 // one launch; the sums are always partial ones.
 template <int D, int GROUP, int Dt, bool Shared>
-__global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(Int4Attention a) {
+__global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(typename Int4Call<Shared>::Args a) {
     using R = Int4Rec<D, GROUP>;
     using S = Ring<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, CG = CH / G, VT = D / 16, TG = VT / G;
@@ -160,29 +164,36 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     // had the last, mostly empty split) and the row tiles of a head, which read the same records, few of them; the
     // splits last, so that a long sequence's later ones follow everyone's first.
     int h = blockIdx.x % a.L.n_kv, tile = blockIdx.x / a.L.n_kv, b = blockIdx.y, part = blockIdx.z;
-    const bool pre = Shared && static_cast<int>(blockIdx.x) < a.shared_blocks;
-    const lf_int4_layer L = Shared && !pre ? a.own : a.L;
-    const int splits = Shared && !pre ? a.own_splits : a.splits, split_tokens = Shared && !pre ? a.own_split_tokens : a.split_tokens;
+    bool pre = false;
+    int splits = a.splits, split_tokens = a.split_tokens, part0 = a.part0;
     if constexpr (Shared) {
-        const int tiles = pre ? a.shared_tiles : a.own_tiles;
+        pre = static_cast<int>(blockIdx.x) < a.shared_blocks;
+        const int tiles = pre ? a.shared_tiles : a.own_tiles, batch = pre ? a.L.batch : a.own.batch;
         int id = static_cast<int>(blockIdx.x) - (pre ? 0 : a.shared_blocks);
-        h = id % L.n_kv;
-        id /= L.n_kv;
+        h = id % a.L.n_kv;
+        id /= a.L.n_kv;
         tile = id % tiles;
         id /= tiles;
-        b = id % L.batch;
-        part = id / L.batch;
+        b = id % batch;
+        part = id / batch;
+        if (!pre) {
+            part0 = splits;
+            splits = a.own_splits;
+            split_tokens = a.own_split_tokens;
+        }
     }
+    const auto& L = layer_of(a, pre);
     const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
     const int col = lane & 15, quad = lane >> 4;
     // rows: (head of the group, token), tokens fastest; with pages, the heads of one token
     int i, j;
-    SharedRow row_at;
+    SharedRow row_at = {b, 0, 0, false};
+    if constexpr (Shared)
+        if (pre) row_at = shared_row(a, b, tile * kTile + col);
     if (pre) {
-        row_at = shared_row(a, b, tile * kTile + col);
         i = row_at.i;
         j = row_at.j;
-    } else if (a.n_pages) {
+    } else if (!Shared && a.n_pages) {
         j = tile % a.q_len;
         i = tile / a.q_len * kTile + col;
     } else {
@@ -201,7 +212,9 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     if (ahead) S::load(base + early * R::bytes, ring, lane);
     const int len = int4_len(L, b);
     const int n = pre ? 0 : a.q_lens ? min(max(a.q_lens[b], 0), a.q_len) : a.q_len;
-    const int lim = pre ? shared_limit(a, row_at, len) : real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
+    int lim = real && j < n ? max(len - n + j + 1, 0) : 0;  // rows this query sees
+    if constexpr (Shared)
+        if (pre) lim = shared_limit(a, row_at, len);
     int all = real ? lim : 0x7fffffff, top = lim;                 // rows every query of the tile sees, and any
 #pragma unroll
     for (int m = 1; m < 16; m <<= 1) {
@@ -494,7 +507,6 @@ __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) voi
     }
     if (!real) return;
     const int64_t row = (static_cast<int64_t>(seq) * a.n_q + h * a.g + i) * a.q_len + j;
-    const int part0 = Shared && !pre ? a.splits : a.part0;
     if (!Shared && a.parts == 1) {
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;  // (no row seen: zeros)
 #pragma unroll
@@ -590,7 +602,7 @@ int launch_typed(const Int4Attention& a, int tiles, hipStream_t stream) {
 
 // The rows of shared prefixes, 16 at a time, and with own_splits the sequences' own and the merge.
 template <int D, int GROUP, int Dt>
-int launch_shared_typed(Int4Attention a, hipStream_t stream) {
+int launch_shared_typed(Int4Shared a, hipStream_t stream) {
     const auto fn = int4_attention_kernel<D, GROUP, Dt, true>;
     const int lds = Ring<D, GROUP>::lds;
     const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
@@ -660,7 +672,8 @@ int launch_int4_attention(const lf_int4_layer& L, const lf_int4_args& A, hipStre
 int launch_int4_shared(const lf_int4_layer& L, const lf_int4_layer& P, const lf_int4_args& A, int splits, int split_tokens, bool many_rows,
                        hipStream_t stream) {
     const Int4Attention own = attention_of(L, A, splits);
-    Int4Attention a = own;
+    Int4Shared a{};
+    static_cast<Int4Attention&>(a) = own;
     a.L = P;
     a.part0 = a.prefix = 0;
     a.splits = splits;

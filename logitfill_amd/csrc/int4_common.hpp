@@ -124,14 +124,17 @@ struct Int4Attention {
     int prefix;                // splits of the many-row kernel in front of them
     int parts;                 // of every output row
     int part0;                 // the first one of this launch
-    // A shared prefix (the kernels' Shared forms): L holds the prefixes, one for ``each`` sequences in turn, and own the
-    // sequences.  The general kernel's launch holds shared_blocks workgroups of the prefixes, shared_tiles row tiles each,
-    // and behind them those of the sequences' own rows.
+    float* part_o;             // [batch * n_q * q_len][parts][D]
+    float* part_ml;            // [batch * n_q * q_len][parts][2]
+};
+
+// The same of shared prefixes (the kernels' Shared forms): L holds the prefixes, one for ``each`` sequences in turn, and own the
+// sequences.  The general kernel's launch holds shared_blocks workgroups of the prefixes, shared_tiles row tiles each, and
+// behind them those of the sequences' own rows.
+struct Int4Shared : Int4Attention {
     lf_int4_layer own;
     int each;
     int shared_blocks, shared_tiles, own_tiles, own_splits, own_split_tokens;
-    float* part_o;             // [batch * n_q * q_len][parts][D]
-    float* part_ml;            // [batch * n_q * q_len][parts][2]
 };
 
 // Query row ``r`` of a prefix's (sequence, head of the group, token), tokens fastest.
@@ -139,17 +142,20 @@ struct SharedRow {
     int b, i, j;   // sequence of the whole batch
     bool real;
 };
-__device__ __forceinline__ SharedRow shared_row(const Int4Attention& a, int prefix, int r) {
+__device__ __forceinline__ SharedRow shared_row(const Int4Shared& a, int prefix, int r) {
     const int per = a.g * a.q_len, s = r / per, rest = r - s * per, i = rest / a.q_len;
     return {prefix * a.each + s, i, rest - i * a.q_len, s < a.each};
 }
 // Rows of a prefix of ``len`` that the row's query sees: all of them, unless its sequence is shorter than its queries.
-__device__ __forceinline__ int shared_limit(const Int4Attention& a, const SharedRow& row, int len) {
+__device__ __forceinline__ int shared_limit(const Int4Shared& a, const SharedRow& row, int len) {
     if (!row.real) return 0;
     const int n = a.q_lens ? min(max(a.q_lens[row.b], 0), a.q_len) : a.q_len;
     const int own = int4_len(a.own, row.b);
     return row.j < n ? min(max(len + own - n + row.j + 1, 0), len) : 0;
 }
+
+template <bool Shared> struct Int4Call { using Args = Int4Attention; };
+template <> struct Int4Call<true> { using Args = Int4Shared; };
 
 constexpr int kManyRows = 128;  // query rows of a many-row workgroup
 

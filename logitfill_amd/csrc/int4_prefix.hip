@@ -70,7 +70,7 @@ __device__ __forceinline__ f16x2 halves(uint32_t x) { return __builtin_bit_cast(
 
 // Shared: of a prefix that ``each`` sequences share; the rows are all their queries, and its last record may be a part of one.
 template <int D, int GROUP, bool Shared>
-__global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) void int4_prefix_kernel(Int4Attention a) {
+__global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) void int4_prefix_kernel(typename Int4Call<Shared>::Args a) {
     using R = Int4Rec<D, GROUP>;
     constexpr int G = R::G, CH = R::chunks, VT = D / 16;
     constexpr bool kOne = D == 128 && G == 1;  // the minima's terms by sums
@@ -181,7 +181,8 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
         const int r = tile * kManyRows + (wave * MT + t) * kTile + col;
         SharedRow at = {b, r / a.q_len, r % a.q_len, r / a.q_len < a.g};
         if constexpr (Shared) at = shared_row(a, b, r);
-        lim[t] = Shared ? shared_limit(a, at, len) : 0;
+        lim[t] = 0;
+        if constexpr (Shared) lim[t] = shared_limit(a, at, len);
         float x[CH][8] = {}, most = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -349,7 +350,7 @@ __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) vo
 }
 
 template <bool Shared>
-int launch(const Int4Attention& a, int rows, int splits, hipStream_t stream) {
+int launch(const typename Int4Call<Shared>::Args& a, int rows, int splits, hipStream_t stream) {
     const dim3 grid(a.L.n_kv * ((rows + kManyRows - 1) / kManyRows), a.L.batch, splits);
     const auto of = [&](auto shape) {
         constexpr int D = decltype(shape)::d, GROUP = decltype(shape)::group;
@@ -370,6 +371,6 @@ int launch(const Int4Attention& a, int rows, int splits, hipStream_t stream) {
 }  // namespace
 
 int launch_int4_prefix(const Int4Attention& a, hipStream_t stream) { return launch<false>(a, a.g * a.q_len, a.prefix, stream); }
-int launch_int4_shared_rows(const Int4Attention& a, hipStream_t stream) { return launch<true>(a, a.g * a.q_len * a.each, a.splits, stream); }
+int launch_int4_shared_rows(const Int4Shared& a, hipStream_t stream) { return launch<true>(a, a.g * a.q_len * a.each, a.splits, stream); }
 
 }  // namespace lf

@@ -635,7 +635,7 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     query = _check_query(manager, query, pages is not None or manager.top_pages > 0)
     q_len = query.shape[2]
     B = manager.batch_size
-    if manager.prefix is not None:
+    if manager._prefix is not None:
         if pages is not None:
             raise ValueError("pages are of a sequence's own rows: a manager with a prefix attends them all")
         if manager.prefix.prefix is not None:
@@ -677,7 +677,7 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
         a.pages, a.n_pages = pages.data_ptr(), pages.shape[3]
         # (the list is cut as a whole: a sequence of fewer pages leaves the later splits idle)
         tokens, tiles = ((a.n_pages + 1) * layer.page_size,), -(-group // 16) * q_len * B
-    shared = _shared_plan(manager, layer_idx, q_len, query.dtype, lengths, cus)
+    shared = None if manager._prefix is None else _shared_plan(manager, layer_idx, q_len, query.dtype, lengths, cus)
     if pages is None and _many_rows(group, q_len, manager.n_kv, D, manager.group_size, query.dtype, tokens):
         a.prefix_splits, _ = plan_splits(tokens, manager.n_kv * -(-group * q_len // 128), cus,
                                          many_rows_per_cu(D, manager.group_size), MANY_ROWS_OVERHEAD)
@@ -742,8 +742,6 @@ def _shared_plan(manager, layer_idx: int, q_len: int, dtype, lengths, cus: int):
     """``((splits, split_tokens, many_rows)`` of the manager's prefix, ``(splits, split_tokens)`` of the own rows), or None
     where there is no prefix."""
     prefix = manager.prefix
-    if prefix is None:
-        return None
     tokens = prefix.layers[layer_idx].lengths
     if not max(tokens):
         return None
