@@ -16,14 +16,23 @@ without a transformers cache -- the packed cache holds the history, so callers p
 ``position_ids`` (``PackedDecoder`` does).  ``detach_packed`` restores the original forwards.
 
 With an ``Int4KVManager`` the layers run ``int4_attention`` instead, which caches the new tokens
-before it reads (of a manager with ``top_pages``, over the pages it selects).
+before it reads (of a manager with ``top_pages``, over the pages it selects; of a manager with a
+``prefix``, behind its shared rows).
+
+``prompt_kernels=True`` takes the prompt's own pass to this package, too: positions are turned into
+queries and Keys by ``Rotary``, and a layer without history runs ``prompt_attention`` in place of the
+model's dense attention -- of several prompts at once, packed one behind another
+(``PackedDecoder.prefill`` of a list).
 """
 from __future__ import annotations
 
 import torch
 
+from logitfill_amd import _native
 from logitfill_amd.packed.int4 import Int4KVManager, int4_attention
+from logitfill_amd.packed.prompt import PromptPlan, prompt_attention
 from logitfill_amd.packed.reference import packed_attention, reference_attention
+from logitfill_amd.packed.rotary import Rotary
 
 
 def _dense_attention(attn, query, key, value, attention_mask, kwargs):
@@ -36,7 +45,53 @@ def _dense_attention(attn, query, key, value, attention_mask, kwargs):
     return out  # [B, q_len, n_q, D]
 
 
-def _make_forward(attn, manager, attention_fn):
+class _PromptKernels:
+    """What the layers of a model with ``prompt_kernels`` share: its rotation and, while packed prompts pass through,
+    their plan and the places of their tokens in a padded batch."""
+
+    def __init__(self, model, device):
+        rope, cfg = model.model.rotary_emb, model.config
+        kind = str(getattr(rope, "rope_type", "default"))
+        if "dynamic" in kind or kind == "longrope":
+            raise ValueError(f"prompt_kernels takes frequencies that hang on no length; the model's are {kind!r}")
+        head_dim = model.model.layers[0].self_attn.head_dim
+        if head_dim not in (64, 128, 256):
+            raise ValueError(f"prompt_kernels takes heads of 64, 128 or 256 channels, the model has {head_dim}")
+        freq = rope.inv_freq.tolist()
+        self.rotary = Rotary(head_dim, rotary_dim=2 * len(freq), inv_freq=freq,
+                             attention_factor=float(getattr(rope, "attention_scaling", 1.0)), device=device)
+        self.windows = any(getattr(layer.self_attn, "sliding_window", None) for layer in model.model.layers)
+        self.plan: PromptPlan | None = None
+        self.places: torch.Tensor | None = None
+
+    def pack(self, lengths) -> None:
+        """Prompts of ``lengths`` pass through next, packed."""
+        if self.windows:
+            raise ValueError("packed prompts take a model without sliding windows")
+        self.plan = PromptPlan(lengths, device=self.rotary.device)
+        longest, at, rows = max(lengths), 0, []
+        for n in lengths:
+            rows += [min(at + t, at + n - 1) for t in range(longest)]  # (what stands behind its last token is not read)
+            at += n
+        self.places = _native.upload(rows, torch.int64, self.rotary.device)
+
+    def unpack(self) -> None:
+        self.plan = self.places = None
+
+    def rotate(self, query, key, position_ids):
+        return self.rotary.rotate(query, key, position_ids)
+
+    def commit(self, manager, layer_idx: int, key, value) -> None:
+        """The prompts' rows into the cache, each sequence's its own."""
+        if self.plan is None:
+            manager.commit(layer_idx, key, value)
+            return
+        shape = (key.shape[1], self.plan.batch, -1, key.shape[3])
+        key, value = (t[0].index_select(1, self.places).view(shape).transpose(0, 1) for t in (key, value))
+        manager.commit(layer_idx, key, value, self.plan.lengths)
+
+
+def _make_forward(attn, manager, attention_fn, kernels=None):
     from transformers.models.qwen2.modeling_qwen2 import apply_rotary_pos_emb
 
     layer_idx = attn.layer_idx
@@ -47,10 +102,18 @@ def _make_forward(attn, manager, attention_fn):
         query = attn.q_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         key = attn.k_proj(hidden_states).view(hidden_shape).transpose(1, 2)
         value = attn.v_proj(hidden_states).view(hidden_shape).transpose(1, 2)
-        cos, sin = position_embeddings
-        query, key = apply_rotary_pos_emb(query, key, cos, sin)
+        if kernels is not None and kwargs.get("position_ids") is not None:
+            query, key = kernels.rotate(query, key, kwargs["position_ids"])
+        else:
+            cos, sin = position_embeddings
+            query, key = apply_rotary_pos_emb(query, key, cos, sin)
         past = manager.layer_length(layer_idx)
-        if past == 0:
+        if getattr(manager, "prefix", None) is not None:
+            past += manager.prefix.layer_length(layer_idx)
+        if past == 0 and kernels is not None and not getattr(attn, "sliding_window", None):
+            out = prompt_attention(query, key, value, attn.scaling, kernels.plan).transpose(1, 2)
+            kernels.commit(manager, layer_idx, key, value)
+        elif past == 0:
             out = _dense_attention(attn, query, key, value, attention_mask, kwargs)
             manager.commit(layer_idx, key, value)
         elif getattr(manager, "commits_new_tokens", False):
@@ -69,12 +132,16 @@ def _make_forward(attn, manager, attention_fn):
     return forward
 
 
-def attach_packed(model, manager, attention_fn=packed_attention) -> None:
+def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kernels: bool = False):
     """Route every decoder layer's attention through ``manager`` (a ``PackedKVManager`` whose
     layers match the model's).  ``attention_fn`` is ``packed_attention`` (the HIP path) or
     ``reference_attention`` (dense dequantise-then-attend), same signature.  An ``Int4KVManager``
     takes ``int4_attention`` in place of the default; any other function given for it commits the new
-    tokens itself (``reference_attention``, which reads packed pages, does not: ``ValueError``)."""
+    tokens itself (``reference_attention``, which reads packed pages, does not: ``ValueError``).
+
+    ``prompt_kernels``: queries and Keys are rotated by ``Rotary`` with the model's own frequencies (in float64 angles), and
+    layers without history run ``prompt_attention`` (causal, no attention mask; layers of a sliding window keep the
+    model's).  These give no gradients: call the model under ``torch.no_grad()``."""
     if isinstance(manager, Int4KVManager):
         if attention_fn is reference_attention:
             raise ValueError("reference_attention reads packed pages; an Int4KVManager takes int4_attention")
@@ -86,12 +153,15 @@ def attach_packed(model, manager, attention_fn=packed_attention) -> None:
     if len(manager.layers) != len(layers):
         raise ValueError(f"manager has {len(manager.layers)} layers, the model {len(layers)}")
     for layer in layers:
-        attn = layer.self_attn
-        if manager.n_kv != n_kv or manager.head_dim != attn.head_dim:
+        if manager.n_kv != n_kv or manager.head_dim != layer.self_attn.head_dim:
             raise ValueError("manager shape does not match the model's attention")
+    kernels = _PromptKernels(model, manager.device) if prompt_kernels else None
+    for layer in layers:
+        attn = layer.self_attn
         if not hasattr(attn, "_lf_original_forward"):
             attn._lf_original_forward = attn.forward
-        attn.forward = _make_forward(attn, manager, attention_fn)
+        attn.forward = _make_forward(attn, manager, attention_fn, kernels)
+    return kernels
 
 
 def detach_packed(model) -> None:
@@ -103,8 +173,9 @@ def detach_packed(model) -> None:
 
 
 class PackedDecoder:
-    """Prefill + token-by-token decode of a ``Qwen2ForCausalLM`` over a packed cache (batch 1,
-    as the reference).  ``step`` returns the logits of the last position.
+    """Prefill + token-by-token decode of a ``Qwen2ForCausalLM`` over a packed cache (batch 1, as
+    the reference, or as many sequences as the manager holds).  ``step`` returns the logits of the
+    last position.
 
     ``hf_cache=True`` passes a ``LogitFillCache`` as ``past_key_values`` (the reference adapter's
     ``make_cache``, ``deepseek_qwen.py:141-146``), so the model derives positions and mask sizes
@@ -113,14 +184,17 @@ class PackedDecoder:
     ``defer_flush``: None (default) keeps the manager's own setting; True or False sets it on
     the manager.  A deferring manager leaves every layer's completed page for one
     ``flush_pending`` launch after each forward pass (``step`` calls it) instead of one launch
-    per layer; results are the same either way."""
+    per layer; results are the same either way.
+
+    ``prompt_kernels``: see ``attach_packed``; ``prefill`` then takes a list of prompts, too, one for each of the
+    manager's sequences.  A manager with a ``prefix`` continues it: positions start behind the prefix's tokens."""
 
     def __init__(self, model, manager, attention_fn=packed_attention, *, hf_cache: bool = False,
-                 defer_flush: bool | None = None):
+                 defer_flush: bool | None = None, prompt_kernels: bool = False):
         self.model, self.manager = model, manager
         if defer_flush is not None and hasattr(manager, "defer_flush"):
             manager.defer_flush = bool(defer_flush)
-        attach_packed(model, manager, attention_fn)
+        self.kernels = attach_packed(model, manager, attention_fn, prompt_kernels=prompt_kernels)
         self.cache = None
         if hf_cache:
             from logitfill_amd.packed.cache import LogitFillCache
@@ -133,24 +207,75 @@ class PackedDecoder:
         if flush is not None:
             flush()
 
-    def _forward(self, ids: torch.Tensor, start: int) -> torch.Tensor:
-        if self.cache is not None:
-            out = self.model(input_ids=ids, past_key_values=self.cache, use_cache=True)
-        else:
+    def _prefix_lengths(self) -> list:
+        """Tokens of a shared prefix in front of every sequence."""
+        if getattr(self.manager, "prefix", None) is not None:
+            return self.manager.prefix_lengths(0)
+        return [0] * getattr(self.manager, "batch_size", 1)
+
+    def _lengths(self) -> list:
+        """Every sequence's tokens, those of a shared prefix among them."""
+        own = self.manager.layers[0].lengths
+        return [p + n for p, n in zip(self._prefix_lengths(), own() if callable(own) else own)]
+
+    def _forward(self, ids: torch.Tensor, start) -> torch.Tensor:
+        """``start``: the position of the first token, or of every sequence's."""
+        if isinstance(start, list):
+            if len(set(start)) == 1:
+                start = start[0]
+            else:
+                first = _native.upload(start, torch.int64, ids.device)
+                pos = first[:, None] + torch.arange(ids.shape[-1], device=ids.device)
+        if not isinstance(start, list):
             pos = torch.arange(start, start + ids.shape[-1], device=ids.device)[None]
+        if self.cache is not None:
+            # (the cache's length is sequence 0's: positions of unlike ones are passed, too)
+            more = {"position_ids": pos} if isinstance(start, list) else {}
+            out = self.model(input_ids=ids, past_key_values=self.cache, use_cache=True, **more)
+        else:
             out = self.model(input_ids=ids, position_ids=pos, use_cache=False)
         self._flush()
         return out.logits[:, -1]
 
+    def _prefill_packed(self, prompts) -> torch.Tensor:
+        lengths = [int(p.shape[-1]) for p in prompts]
+        if self.kernels is None:
+            raise ValueError("a list of prompts takes prompt_kernels=True")
+        if any(p.dim() != 1 for p in prompts) or min(lengths, default=0) < 1:
+            raise ValueError("prompts are one-dimensional, of at least one token")
+        if len(prompts) != self.manager.batch_size:
+            raise ValueError(f"{len(prompts)} prompts for a manager of {self.manager.batch_size} sequences")
+        if max(self._prefix_lengths()):
+            raise ValueError("prompts behind a shared prefix are fed as one tensor [batch, tokens]")
+        device = prompts[0].device
+        last = torch.cumsum(torch.tensor(lengths), 0) - 1
+        pos = torch.cat([torch.arange(n, device=device) for n in lengths])[None]
+        self.kernels.pack(lengths)
+        try:
+            # (no mask is made of the packed positions: every layer attends by the plan)
+            out = self.model(input_ids=torch.cat(list(prompts))[None], position_ids=pos, use_cache=False,
+                             attention_mask={"full_attention": None}, logits_to_keep=last.to(device))
+        finally:
+            self.kernels.unpack()
+        self._flush()
+        self.pos = lengths[0]
+        return out.logits[0]
+
     @torch.no_grad()
-    def prefill(self, input_ids: torch.Tensor) -> torch.Tensor:
+    def prefill(self, input_ids) -> torch.Tensor:
+        """Logits of the last position ``[batch, vocab]`` of prompts ``[batch, T]``, or of a list of one-dimensional ones."""
         self.manager.reset()
-        logits = self._forward(input_ids, 0)
-        self.pos = int(input_ids.shape[-1])
+        if isinstance(input_ids, (list, tuple)):
+            return self._prefill_packed(input_ids)
+        start = self._prefix_lengths()
+        logits = self._forward(input_ids, start)
+        self.pos = start[0] + int(input_ids.shape[-1])
         return logits
 
     @torch.no_grad()
     def step(self, token: torch.Tensor) -> torch.Tensor:
-        logits = self._forward(token.view(1, 1), self.pos)
+        """``token``: the next one, or one for each sequence of the manager."""
+        batch = getattr(self.manager, "batch_size", 1)
+        logits = self._forward(token.view(batch, 1), self.pos if batch == 1 else self._lengths())
         self.pos += 1
         return logits
