@@ -64,11 +64,18 @@ def split_size(tiles: np.ndarray, n_kv: int, cus: int, per_cu: int, head_dim: in
         s = -(-longest // parts)
         n = np.maximum(-(-tiles // s), 1)
         sizes = np.sort(np.repeat(-(-tiles // n), n * n_kv))[::-1]
-        # the workgroups of a compute unit's first round, the longest of each rank
-        first = float(sizes[: cus * per_cu : cus].sum()) * shared + ITEM_US
+        slots = cus * per_cu
         even = (float(sizes.sum()) * shared + len(sizes) * 0.25 * ITEM_US) / cus
-        if len(sizes) > cus * per_cu:
-            even += 0.3 * float(sizes[cus * per_cu :].mean()) * shared
+        # the workgroups of the compute unit that has the longest ones of each rank at once
+        first = float(sizes[:slots:cus].sum()) * shared + ITEM_US
+        if per_cu == 1 and len(sizes) > slots:  # one after the other: what is left goes to those that end first
+            load = np.zeros(-(-len(sizes) // slots) * slots)
+            load[: len(sizes)] = sizes * shared + ITEM_US
+            load = load.reshape(-1, slots)
+            load[1::2] = load[1::2, ::-1]
+            first = float(load.sum(0).max())
+        elif len(sizes) > slots:
+            even += 0.3 * float(sizes[slots:].mean()) * shared
         costs = [max(first, even, s * alone + ITEM_US)]
         if pairs and len(sizes) <= cus and s > 1:
             costs.append(-(-s // 2) * max(1.2 * alone, 2.2 * shared) + ITEM_US + PAIR_US)
