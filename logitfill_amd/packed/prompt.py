@@ -10,7 +10,6 @@ Nothing here runs on the CPU.
 """
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
 from typing import NamedTuple, Optional
@@ -148,26 +147,31 @@ class PromptPlan:
         if min(self.lengths + self.key_lengths) < 0 or max(self.lengths + self.key_lengths) > MAX_TOKENS:
             raise ValueError(f"lengths must lie in 0 .. {MAX_TOKENS}")
         self.device = _check_device(device)
+        self._longest = max(self.lengths), max(self.key_lengths)
+        self._total = sum(self.lengths), sum(self.key_lengths)
         self._forms: dict = {}
+        self._args: dict = {}  # argument blocks by the tensors' forms
 
     @property
     def batch(self) -> int:
         return len(self.lengths)
 
-    def _rows(self, shape, lengths, name: str) -> bool:
-        """Whether sequences of ``lengths`` lie packed in ``[B, heads, T, D]``; ``ValueError`` where they do not fit."""
+    def _rows(self, shape, of: int, name: str) -> bool:
+        """Whether the sequences' queries (``of`` 0) or Keys (1) lie packed in ``[B, heads, T, D]``; ``ValueError`` where they do
+        not fit."""
         B, T = shape[0], shape[2]
-        if B == self.batch and max(lengths) <= T:
+        if B == len(self.lengths) and self._longest[of] <= T:
             return False  # (one sequence: both forms are the same)
-        if B == 1 and self.batch > 1 and sum(lengths) <= T:
+        if B == 1 and self._total[of] <= T:
             return True
+        lengths = (self.lengths, self.key_lengths)[of]
         raise ValueError(f"{name} {tuple(shape)} does not hold sequences of {lengths[:8]}{'...' if self.batch > 8 else ''} tokens")
 
     def _form(self, packed_q: bool, packed_k: bool, group: int, n_kv: int, head_dim: int, dtype) -> _Form:
         key = (packed_q, packed_k, group, n_kv, head_dim, dtype)
         form = self._forms.get(key)
-        stream = _native.current_stream_ptr(self.device)
         if form is None:
+            stream = _native.current_stream_ptr(self.device)
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a plan's first call uploads its work: run the step once before the capture")
             rows = tile_rows(self.lengths, group)
@@ -178,11 +182,14 @@ class PromptPlan:
             event = torch.cuda.Event()
             event.record(torch.cuda.current_stream(self.device))
             form = self._forms[key] = _Form(device, len(items), len(merges), slots, rows, groups, stream, event)
-        elif stream != form.stream and not torch.cuda.is_current_stream_capturing():
+        return form
+
+    def _order(self, form: _Form, stream: int) -> None:
+        """The current stream, ``stream``, behind the upload of a form's work (a capture follows a run)."""
+        if stream != form.stream and not torch.cuda.is_current_stream_capturing():
             here = torch.cuda.current_stream(self.device)
             here.wait_event(form.event)
             form.items.record_stream(here)
-        return form
 
 
 def _check_rows(t: torch.Tensor, name: str, query: torch.Tensor) -> torch.Tensor:
@@ -217,6 +224,18 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     Everything is enqueued on the current stream."""
     scaling = float(scaling)
+    if plan is None and query.is_cuda and query.dim() == key.dim() == 4 and query.shape[0] == key.shape[0] > 0:
+        plan = _whole(query.shape[0], query.shape[2], key.shape[2], query.device)
+    if plan is not None:  # (tensors of a form that has been checked)
+        kept = plan._args.get(_form_of(query, key, value, scaling))
+        if kept is not None:
+            q, k, v = query.data_ptr(), key.data_ptr(), value.data_ptr()
+            if not (q | k | v) & 15 and query.device == key.device == value.device == plan.device and not (
+                    torch.is_grad_enabled() and (query.requires_grad or key.requires_grad or value.requires_grad)):
+                if torch.cuda.current_device() == plan.device.index:
+                    return _launch(query, key, value, plan, *kept)
+                with torch.cuda.device(plan.device):
+                    return _launch(query, key, value, plan, *kept)
     if not math.isfinite(scaling):
         raise ValueError(f"scaling must be finite, got {scaling}")
     query, key, value = (_check_rows(t, name, query) for t, name in ((query, "query"), (key, "key"), (value, "value")))
@@ -232,18 +251,26 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if plan is None:
         if key.shape[0] != B:
             raise ValueError(f"query has {B} rows, key {key.shape[0]}")
-        if B == 0:
-            return torch.empty(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
-        plan = _whole(B, T, key.shape[2], query.device)
-    elif plan.device != query.device:
+        return torch.empty(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
+    if plan.device != query.device:
         raise ValueError(f"query is on {query.device}, the plan on {plan.device}")
-    packed_q, packed_k = plan._rows(query.shape, plan.lengths, "query"), plan._rows(key.shape, plan.key_lengths, "key")
-    if max(plan.lengths) * (n_q // n_kv) > 1 << 30:
+    packed_q, packed_k = plan._rows(query.shape, 0, "query"), plan._rows(key.shape, 1, "key")
+    if plan._longest[0] * (n_q // n_kv) > 1 << 30:
         raise ValueError("too many query tokens for one call: feed them in chunks")
-    if torch.cuda.current_device() == query.device.index:
-        return _attend(query, key, value, scaling, plan, packed_q, packed_k, code)
     with torch.cuda.device(query.device):
-        return _attend(query, key, value, scaling, plan, packed_q, packed_k, code)
+        if not plan._longest[0] or not plan._longest[1]:
+            return torch.zeros(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
+        form = plan._form(packed_q, packed_k, n_q // n_kv, n_kv, D, query.dtype)
+        if len(plan._args) >= 64:
+            plan._args.clear()
+        kept = plan._args[_form_of(query, key, value, scaling)] = (_describe(query, key, value, code, scaling, form), form)
+        return _launch(query, key, value, plan, *kept)
+
+
+def _form_of(query, key, value, scaling: float):
+    """What a call's argument block hangs on, but for the tensors' addresses."""
+    return (query.shape, query.stride(), query.dtype, key.shape, key.stride(), key.dtype, value.shape, value.stride(), value.dtype,
+            scaling)
 
 
 @functools.lru_cache(maxsize=64)
@@ -251,28 +278,34 @@ def _whole(B: int, T: int, S: int, device) -> PromptPlan:
     return PromptPlan([T] * B, [S] * B, device=device)
 
 
-def _attend(query, key, value, scaling: float, plan: PromptPlan, packed_q: bool, packed_k: bool, code: int) -> torch.Tensor:
-    """``prompt_attention`` of checked arguments."""
-    B, n_q, T, D = query.shape
-    n_kv = key.shape[1]
-    # (rows that no sequence has are not written by the kernel)
-    make = torch.empty if sum(plan.lengths) == B * T else torch.zeros
-    out = make(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
-    if max(plan.lengths) == 0 or max(plan.key_lengths) == 0:
-        return out.zero_()
-    form = plan._form(packed_q, packed_k, n_q // n_kv, n_kv, D, query.dtype)
+def _describe(query, key, value, code: int, scaling: float, form: _Form):
+    """The argument block of calls of one form, without their tensors' addresses."""
     a = _native.PromptArgs()
-    a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
-    a.dtype, a.n_q, a.n_kv, a.head_dim = code, n_q, n_kv, D
-    a.q_strides[:], a.k_strides[:] = query.stride()[:3], key.stride()[:3]
-    a.v_strides[:], a.out_strides[:] = value.stride()[:3], out.stride()[:3]
+    B, n_q, T, D = query.shape
+    a.dtype, a.n_q, a.n_kv, a.head_dim = code, n_q, key.shape[1], D
+    a.q_strides[:], a.k_strides[:], a.v_strides[:] = query.stride()[:3], key.stride()[:3], value.stride()[:3]
+    a.out_strides[:] = T * n_q * D, D, n_q * D
     a.scaling, a.tile_rows, a.groups = scaling, form.rows, form.groups
     a.items, a.n_items = form.items.data_ptr(), form.n_items
     if form.n_merges:
         a.merges, a.n_merges, a.n_slots = a.items + 48 * form.n_items, form.n_merges, form.n_slots
-        nbytes = 4 * form.n_slots * n_kv * form.rows * (D + 2)  # lf_prompt_workspace_bytes
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=query.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _native.check(_native.load().lf_prompt_attention(ctypes.byref(a), _native.current_stream_ptr(query.device)),
-                  "lf_prompt_attention")
-    return out
+        a.workspace_bytes = 4 * form.n_slots * a.n_kv * form.rows * (D + 2)  # lf_prompt_workspace_bytes
+    return a
+
+
+def _launch(query, key, value, plan: PromptPlan, kept, form: _Form) -> torch.Tensor:
+    """``prompt_attention`` of checked tensors on the current device."""
+    B, n_q, T, D = query.shape
+    stream = _native.current_stream_ptr(plan.device)
+    if stream != form.stream:
+        plan._order(form, stream)
+    # (rows that no sequence has are not written by the kernel)
+    make = torch.empty if plan._total[0] == B * T else torch.zeros
+    out = make((B, T, n_q, D), dtype=query.dtype, device=plan.device)
+    a = _native.PromptArgs.from_buffer_copy(kept)
+    a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
+    if form.n_merges:
+        ws = torch.empty(kept.workspace_bytes, dtype=torch.uint8, device=plan.device)
+        a.workspace = ws.data_ptr()
+    _native.check(_native.load().lf_prompt_attention(a, stream), "lf_prompt_attention")
+    return out.transpose(1, 2)

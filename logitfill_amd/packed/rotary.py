@@ -7,7 +7,6 @@ Nothing here runs on the CPU.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional
 
@@ -129,42 +128,29 @@ class Rotary:
         fp16 or fp32), any strides; new tensors of the inputs' memory order.  ``positions``: every token's, an int32 or
         int64 tensor ``[T]``, ``[1, T]`` or ``[B, T]`` on the device, or the first token's as an int (the others
         follow it).  Enqueued on the current stream."""
-        query = self._check_rows(query, "query")
-        B, n_q, T, D = query.shape
-        if key is not None:
-            key = self._check_rows(key, "key")
-            if key.shape[0] != B or key.shape[2] != T:
-                raise ValueError(f"key must be [{B}, n_kv, {T}, {D}], got {tuple(key.shape)}")
-            if key.dtype != query.dtype:
-                raise TypeError("query and key must share a dtype")
-        n_kv = 0 if key is None else key.shape[1]
-        if B * T >= 1 << 31 or n_q + n_kv > 4096:
-            raise ValueError("at most 2^31 - 1 tokens and 4096 heads a call")
-        where = None
-        if isinstance(positions, torch.Tensor):
-            if positions.dtype not in (torch.int32, torch.int64):
-                raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
-            if positions.device != self.device:
-                raise ValueError(f"positions are on {positions.device}, the frequencies on {self.device}")
-            shape = positions.shape
-            if shape != (T,) and shape != (1, T) and shape != (B, T):
-                raise ValueError(f"positions must be [{T}], [1, {T}] or [{B}, {T}], got {tuple(shape)}")
-            where = (shape, positions.stride(), positions.dtype)
-        code = _native.dtype_code(query.dtype)
+        tensor = isinstance(positions, torch.Tensor)
+        form = (query.shape, query.stride(), query.dtype,
+                None if key is None else (key.shape, key.stride(), key.dtype),
+                (positions.shape, positions.stride(), positions.dtype) if tensor else None)
+        kept = self._args.get(form)
+        if kept is None or query.device != self.device or (key is not None and key.device != self.device) or (
+                tensor and positions.device != self.device) or (
+                torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))):
+            query, key = self._check(query, key, positions)
+            form = (query.shape, query.stride(), query.dtype, None if key is None else (key.shape, key.stride(), key.dtype), form[4])
+            kept = self._args.get(form)
         q_out, k_out = _like(query), None if key is None else _like(key)
         if query.numel() == 0 and (key is None or key.numel() == 0):
             return q_out, k_out
-        form = (code, query.shape, query.stride(), None if key is None else (n_kv, key.stride()), where)
-        kept = self._args.get(form)
         if kept is None:
             if len(self._args) >= 64:
                 self._args.clear()
-            kept = self._args[form] = self._describe(code, query, key, q_out, k_out, where)
+            kept = self._args[form] = self._describe(query, key, q_out, k_out, form[4])
         a = _native.RotaryArgs.from_buffer_copy(kept)
         a.query, a.query_out = query.data_ptr(), q_out.data_ptr()
         if key is not None:
             a.key, a.key_out = key.data_ptr(), k_out.data_ptr()
-        if where is not None:
+        if tensor:
             a.positions = positions.data_ptr()
         else:
             a.start = int(positions)
@@ -175,10 +161,33 @@ class Rotary:
                 self._launch(a)
         return q_out, k_out
 
-    def _describe(self, code: int, query, key, q_out, k_out, where):
+    def _check(self, query, key, positions):
+        """Query and Key as the kernel reads them; errors for what it does not."""
+        query = self._check_rows(query, "query")
+        B, n_q, T, D = query.shape
+        if key is not None:
+            key = self._check_rows(key, "key")
+            if key.shape[0] != B or key.shape[2] != T:
+                raise ValueError(f"key must be [{B}, n_kv, {T}, {D}], got {tuple(key.shape)}")
+            if key.dtype != query.dtype:
+                raise TypeError("query and key must share a dtype")
+        if B * T >= 1 << 31 or n_q + (0 if key is None else key.shape[1]) > 4096:
+            raise ValueError("at most 2^31 - 1 tokens and 4096 heads a call")
+        _native.dtype_code(query.dtype)
+        if isinstance(positions, torch.Tensor):
+            if positions.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+            if positions.device != self.device:
+                raise ValueError(f"positions are on {positions.device}, the frequencies on {self.device}")
+            shape = positions.shape
+            if shape != (T,) and shape != (1, T) and shape != (B, T):
+                raise ValueError(f"positions must be [{T}], [1, {T}] or [{B}, {T}], got {tuple(shape)}")
+        return query, key
+
+    def _describe(self, query, key, q_out, k_out, where):
         """The argument block of calls of this form, without their addresses."""
         a = _native.RotaryArgs()
-        a.dtype = code
+        a.dtype = _native.dtype_code(query.dtype)
         a.batch, a.n_q, a.tokens, a.head_dim = query.shape
         a.n_kv = 0 if key is None else key.shape[1]
         a.rotary_dim, a.interleaved = self.rotary_dim, self.layout == "interleaved"
@@ -197,4 +206,4 @@ class Rotary:
         stream = _native.current_stream_ptr(self.device)
         if stream != self._stream and not torch.cuda.is_current_stream_capturing():
             self._turns.record_stream(torch.cuda.current_stream(self.device))
-        _native.check(_native.load().lf_rotary(ctypes.byref(a), stream), "lf_rotary")
+        _native.check(_native.load().lf_rotary(a, stream), "lf_rotary")

@@ -59,7 +59,7 @@ def test_a_cpu_device():
 
 def _rotary(**kwargs):
     r = Rotary.__new__(Rotary)
-    r.head_dim, r.rotary_dim, r.device = 64, 64, torch.device("cuda", 0)
+    r.head_dim, r.rotary_dim, r.device, r._args = 64, 64, torch.device("cuda", 0), {}
     return r
 
 
