@@ -375,7 +375,8 @@ class Int4KVManager:
         front of ``batch_size / prefix.batch_size`` sequences in turn (all the samples of a prompt, the chats behind a system
         prompt).  ``int4_attention`` then attends a prefix's rows, read once for all its sequences, and the sequence's own
         behind them; commits, ``truncate`` and ``reset`` are of the own rows, and the prefix may be written between calls
-        as any cache.  A captured call holds the prefix's split plan too."""
+        as any cache.  A captured call reads the prefix's arrays and device lengths in its replays, by the split plan of the
+        captured ones: keep it as long as the graph."""
         return self._prefix
 
     @prefix.setter
@@ -743,7 +744,7 @@ def _shared_plan(manager, layer_idx: int, q_len: int, dtype, lengths, cus: int):
     where there is no prefix."""
     prefix = manager.prefix
     tokens = prefix.layers[layer_idx].lengths
-    if not max(tokens):
+    if not max(tokens) and not torch.cuda.is_current_stream_capturing():
         return None
     D, group, n_kv = manager.head_dim, manager.group_size, manager.n_kv
     each = manager.n_q // n_kv * q_len
@@ -758,7 +759,7 @@ def _shared_plan(manager, layer_idx: int, q_len: int, dtype, lengths, cus: int):
     size = _shared_split(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), n_kv * -(-rows // 16),
                          len(own), max(own) // SPLIT_UNIT + 1, sum(own) // SPLIT_UNIT, n_kv * -(-each // 16),
                          workgroups_per_cu(D, group) * cus) * SPLIT_UNIT
-    return (-(-max(tokens) // size), size, 0), (-(-max(max(own), 1) // size), size)
+    return (-(-max(max(tokens), 1) // size), size, 0), (-(-max(max(own), 1) // size), size)
 
 
 @_here

@@ -219,12 +219,14 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
 
     ``plan``: the sequences.  B of them, each from the start of its own row (padded), or, in a batch of one row, all
     behind one another (packed); queries and Keys each in one of the two ways.  None: every row is a sequence of
-    all its tokens.  A sequence's queries are the last of its Keys, and each sees the Keys up to its own.  Rows of
+    all its tokens (not in a capture).  A sequence's queries are the last of its Keys, and each sees the Keys up to its own.  Rows of
     the output behind a sequence's last token, and rows of queries that see no Key, are zeros.
 
     Everything is enqueued on the current stream."""
     scaling = float(scaling)
     if plan is None and query.is_cuda and query.dim() == key.dim() == 4 and query.shape[0] == key.shape[0] > 0:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a captured call takes a plan, which the graph's replays read: make one before the capture")
         plan = _whole(query.shape[0], query.shape[2], key.shape[2], query.device)
     if plan is not None:  # (tensors of a form that has been checked)
         kept = plan._args.get(_form_of(query, key, value, scaling))

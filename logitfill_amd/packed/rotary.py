@@ -80,7 +80,8 @@ class Rotary:
     ``rotary_dim``: the front channels that are rotated (even; default all).  ``layout``: pairs are channel
     j of both halves of those (``"half"``) or neighbours (``"interleaved"``).  ``scaling``: see
     ``frequencies``.  ``inv_freq``: the pairs' angles per position in place of ``base`` and ``scaling``
-    (a model's own), with ``attention_factor`` on the rotated channels."""
+    (a model's own), with ``attention_factor`` on the rotated channels.  A captured graph reads the frequencies: keep the
+    object as long as it."""
 
     def __init__(self, head_dim: int, base: float = 10000.0, *, rotary_dim: Optional[int] = None, layout: str = "half",
                  scaling: Optional[dict] = None, inv_freq=None, attention_factor: Optional[float] = None, device="cuda"):

@@ -208,6 +208,8 @@ def test_a_plan_s_first_call_in_a_capture_is_refused(gpu):
         q.add(1)
         with pytest.raises(RuntimeError, match="before the capture"):
             prompt_attention(q, k, v, 0.1, plan)
+        with pytest.raises(RuntimeError, match="takes a plan"):
+            prompt_attention(q, k, v, 0.1)
     prompt_attention(q, k, v, 0.1, plan)
 
 

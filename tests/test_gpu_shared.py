@@ -205,6 +205,30 @@ def test_streams_and_captured_steps(gpu):
     assert torch.equal(short, again) and not torch.equal(short, out)
 
 
+def test_a_captured_prefix_fills_later(gpu):
+    """What is captured of an empty prefix attends what its device lengths say in a replay."""
+    D = 64
+    prefix, mgr = pair(gpu, D, 32, (4, 2), 1, 2)
+    for m in (prefix, mgr):
+        m.layers[0].reserve(128)
+    before, behind = rows((1, 2, 70, D), "bf16", 1), rows((2, 2, 9, D), "bf16", 2)
+    q = query((2, 4, 1, D), "bf16", 3)
+    qd = q.to(gpu)
+    mgr.commit(0, *(t.to(gpu) for t in behind))
+    int4_attention(mgr, 0, qd, None, None, 0.1)
+    prefix.sync_lengths()
+    mgr.sync_lengths()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = int4_attention(mgr, 0, qd, None, None, 0.1)
+    for common in ([0], [70]):
+        if common[0]:
+            prefix.commit(0, *(t.to(gpu) for t in before))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert_within(out, *want(q, before, behind, common, [9, 9], 32, 0.1, "bf16"))
+
+
 def test_queries_of_any_strides(gpu):
     before, behind, q, prefix, mgr, out = check(gpu, 128, 64, (28, 4), "bf16", [120], [3, 9, 20], q_len=2, seed=16)
     turned = q.transpose(1, 2).contiguous().to(gpu).transpose(1, 2)
