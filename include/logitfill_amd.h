@@ -519,7 +519,7 @@ typedef struct lf_rotary_args {
                                                  all); NULL: token s is at position start + s */
     int64_t position_strides[2];
     int32_t wide;                             /* positions are int64, else int32              */
-    int64_t start;
+    int64_t start;                            /* -2^53 .. 2^53                                */
     const double* turns;                      /* DEVICE [rotary_dim / 2]: frequency / 2 pi    */
     double factor;
 } lf_rotary_args;
@@ -561,7 +561,7 @@ typedef struct lf_prompt_args {
                                                  tile_rows 128, head_dim 64 or 128, bf16 or fp16 (else LF_E_SHAPE) */
     const lf_prompt_item* items;              /* DEVICE                                       */
     const lf_prompt_item* merges;             /* DEVICE (NULL: no row tile is divided)        */
-    int32_t n_items, n_merges, n_slots;
+    int32_t n_items, n_merges, n_slots;       /* n_slots at least 2 n_merges                  */
     void* workspace; int64_t workspace_bytes; /* lf_prompt_workspace_bytes, 16-byte aligned, no initialisation */
 } lf_prompt_args;
 

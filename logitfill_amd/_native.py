@@ -244,6 +244,11 @@ def dtype_code(dtype) -> int:
         raise TypeError(f"unsupported dtype {dtype}; expected bfloat16, float16 or float32") from None
 
 
+def steps(t) -> tuple:
+    """Strides of ``t``'s outer three axes, zero where there is nothing to step over (any number may stand there)."""
+    return tuple([s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)])
+
+
 def current_stream_ptr(device) -> int:
     """The raw hipStream_t of the current stream on ``device`` (torch's C accessor when this
     build has it: no Stream object per call, which the per-layer decode path would pay twice)."""

@@ -31,6 +31,7 @@ int32_t lf_rotary(const lf_rotary_args* args, void* stream) {
     if (static_cast<int64_t>(A.batch) * A.tokens >= 1ll << 31) return LF_E_SHAPE;
     if (static_cast<int64_t>(A.n_q) + A.n_kv > 4096) return LF_E_SHAPE;
     if (!std::isfinite(A.factor)) return LF_E_SHAPE;
+    if (!A.positions && (A.start < -(1ll << 53) || A.start > 1ll << 53)) return LF_E_SHAPE;
     if (A.batch == 0 || A.tokens == 0 || A.n_q + A.n_kv == 0) return LF_OK;
     if (!A.turns || (A.n_q && (!A.query || !A.query_out)) || (A.n_kv && (!A.key || !A.key_out))) return LF_E_NULL;
     return lf::launch_rotary(A, static_cast<hipStream_t>(stream));
@@ -57,6 +58,7 @@ int32_t lf_prompt_attention(const lf_prompt_args* args, void* stream) {
     if (!aligned16(A.query, A.q_strides, esize) || !aligned16(A.key, A.k_strides, esize) || !aligned16(A.value, A.v_strides, esize) ||
         !aligned16(A.out, A.out_strides, esize))
         return LF_E_SHAPE;
+    if (A.n_slots < 2ll * A.n_merges) return LF_E_SHAPE;
     if (A.n_slots) {
         if (!A.workspace) return LF_E_NULL;
         if (!aligned16(A.workspace)) return LF_E_SHAPE;

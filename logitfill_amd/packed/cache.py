@@ -707,7 +707,7 @@ class LogitFillCache(_HFCache):
             raise NotImplementedError("packed pages cannot be cropped")
         keep = int(tokens_to_remove)
         have = self.manager.layers[-1].lengths
-        before = [0] * len(have) if self._prefix() == 0 else self.manager.prefix_lengths(-1)
+        before = [0] * len(have) if getattr(self.manager, "prefix", None) is None else self.manager.prefix_lengths(-1)
         left = [min(keep, p + n) - p if keep >= 0 else max(p + n + keep, 0) - p for n, p in zip(have, before)]
         if min(left) < 0:
             raise ValueError(f"a crop to {keep} would cut the shared prefix of {max(before)} tokens")

@@ -163,6 +163,8 @@ class PromptPlan:
         if B == len(self.lengths) and self._longest[of] <= T:
             return False  # (one sequence: both forms are the same)
         if B == 1 and self._total[of] <= T:
+            if self._total[of] >= 1 << 31:
+                raise ValueError(f"{name}: at most 2^31 - 1 packed tokens")
             return True
         lengths = (self.lengths, self.key_lengths)[of]
         raise ValueError(f"{name} {tuple(shape)} does not hold sequences of {lengths[:8]}{'...' if self.batch > 8 else ''} tokens")
@@ -205,7 +207,7 @@ def _check_rows(t: torch.Tensor, name: str, query: torch.Tensor) -> torch.Tensor
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient, which prompt_attention does not give: call it under torch.no_grad()")
     size = t.element_size()
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in t.stride()[:3]):
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s * size % 16 for s in _native.steps(t)):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -285,7 +287,7 @@ def _describe(query, key, value, code: int, scaling: float, form: _Form):
     a = _native.PromptArgs()
     B, n_q, T, D = query.shape
     a.dtype, a.n_q, a.n_kv, a.head_dim = code, n_q, key.shape[1], D
-    a.q_strides[:], a.k_strides[:], a.v_strides[:] = query.stride()[:3], key.stride()[:3], value.stride()[:3]
+    a.q_strides[:], a.k_strides[:], a.v_strides[:] = _native.steps(query), _native.steps(key), _native.steps(value)
     a.out_strides[:] = T * n_q * D, D, n_q * D
     a.scaling, a.tile_rows, a.groups = scaling, form.rows, form.groups
     a.items, a.n_items = form.items.data_ptr(), form.n_items

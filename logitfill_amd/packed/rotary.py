@@ -8,6 +8,7 @@ Nothing here runs on the CPU.
 from __future__ import annotations
 
 import math
+import operator
 from typing import Optional
 
 import torch
@@ -16,6 +17,7 @@ from logitfill_amd import _native
 from logitfill_amd.packed.cache import _check_device
 
 LAYOUTS = ("half", "interleaved")
+MAX_START = 1 << 53  # what float64 counts exactly
 
 
 def frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[dict] = None) -> tuple[list[float], float]:
@@ -154,7 +156,9 @@ class Rotary:
         if tensor:
             a.positions = positions.data_ptr()
         else:
-            a.start = int(positions)
+            a.start = operator.index(positions)
+            if a.start != positions or not -MAX_START <= a.start <= MAX_START:
+                raise ValueError(f"the first position must lie in -2^53 .. 2^53, got {positions}")
         if torch.cuda.current_device() == self.device.index:
             self._launch(a)
         else:
@@ -193,9 +197,9 @@ class Rotary:
         a.n_kv = 0 if key is None else key.shape[1]
         a.rotary_dim, a.interleaved = self.rotary_dim, self.layout == "interleaved"
         a.turns, a.factor = self._turns.data_ptr(), self.attention_factor
-        a.q_strides[:], a.qo_strides[:] = query.stride()[:3], q_out.stride()[:3]
+        a.q_strides[:], a.qo_strides[:] = _native.steps(query), _native.steps(q_out)
         if key is not None:
-            a.k_strides[:], a.ko_strides[:] = key.stride()[:3], k_out.stride()[:3]
+            a.k_strides[:], a.ko_strides[:] = _native.steps(key), _native.steps(k_out)
         if where is not None:
             shape, stride, dtype = where
             a.wide = dtype == torch.int64

@@ -141,6 +141,16 @@ def test_strides_and_alignment(gpu, dtype):
     assert out.transpose(1, 2).is_contiguous()
 
 
+def test_axes_of_one_have_any_stride(gpu):
+    """What is never stepped over may be off 16 bytes: a batch of one, a head, a token."""
+    D = 64
+    for T, n_q, n_kv in ((9, 1, 1), (1, 2, 1), (1, 1, 1)):
+        q, k, v = inputs((1, n_q, T, D), (1, n_kv, T, D), "bf16", 11)
+        odd = [t.to(gpu).as_strided(t.shape, [s if n > 1 else 8 * T * D + 3 for s, n in zip(t.stride()[:3], t.shape)] + [1]) for t in (q, k, v)]
+        out = prompt_attention(*odd, 0.125)
+        assert_within(out, *expected(q, k, v, [T], [T], 0.125, "bf16", True, True))
+
+
 def test_offsets_past_32_bits(gpu):
     """Rows 2^26 elements apart: the last ones lie past 2^32 elements."""
     T, D, step = 70, 64, 1 << 26

@@ -152,6 +152,8 @@ def test_refused_calls(gpu):
                        (lambda: rot.rotate(q, k, torch.arange(4, device=gpu)), ValueError),
                        (lambda: rot.rotate(q, k, torch.zeros(3, 5, dtype=torch.int32, device=gpu)), ValueError),
                        (lambda: rot.rotate(q, k, torch.arange(5)), ValueError),
+                       (lambda: rot.rotate(q, k, 1.5), TypeError), (lambda: rot.rotate(q, k, 1 << 70), ValueError),
+                       (lambda: rot.rotate(q, k, -(1 << 53) - 1), ValueError),
                        (lambda: rot.rotate(q.clone().requires_grad_(), k, 0), RuntimeError)):
         with pytest.raises(error):
             bad()

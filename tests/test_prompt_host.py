@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from logitfill_amd import _native
-from logitfill_amd.packed import PromptPlan, prompt_attention
+from logitfill_amd.packed import LogitFillCache, PromptPlan, prompt_attention
 from logitfill_amd.packed.prompt import key_tile, split_size, tile_rows, work_items
 
 
@@ -86,6 +86,7 @@ def _args(**changes):
     ({"n_items": 1 << 30, "n_kv": 2}, _native.LF_E_SHAPE), ({"scaling": float("nan")}, _native.LF_E_SHAPE),
     ({"scaling": float("inf")}, _native.LF_E_SHAPE), ({"n_items": 0}, _native.LF_OK), ({"query": None}, _native.LF_E_NULL),
     ({"out": None}, _native.LF_E_NULL), ({"items": None}, _native.LF_E_NULL), ({"n_merges": 1}, _native.LF_E_NULL),
+    ({"n_merges": 1, "merges": 4096}, _native.LF_E_SHAPE), ({"n_merges": 2, "merges": 4096, "n_slots": 3}, _native.LF_E_SHAPE),
     ({"key": 4098}, _native.LF_E_SHAPE), ({"n_slots": 2}, _native.LF_E_NULL),
     ({"n_slots": 2, "workspace": 4100}, _native.LF_E_SHAPE), ({"n_slots": 2, "workspace": 4096, "workspace_bytes": 2 * 2 * 128 * 66 * 4 - 1}, _native.LF_E_WORKSPACE),
 ])
@@ -101,3 +102,40 @@ def test_strides_off_16_bytes_and_null_arguments():
     assert lib.lf_prompt_attention(None, None) == _native.LF_E_NULL
     assert lib.lf_prompt_workspace_bytes(2, 64, 128, 2) == 2 * 2 * 128 * 66 * 4
     assert lib.lf_prompt_workspace_bytes(0, 64, 128, 2) == _native.LF_E_SHAPE
+
+
+class _Layer:
+    def __init__(self, lengths):
+        self.lengths = list(lengths)
+
+
+class _Shared:
+    """What the transformers view sees of an ``Int4KVManager`` behind a prefix."""
+
+    def __init__(self, before, lengths):
+        self.layers, self.before = [_Layer(lengths)], before
+        self.prefix = type("_Prefix", (), {"seq_len": before[0]})()
+
+    seq_len = property(lambda self: self.layers[0].lengths[0])
+
+    def prefix_lengths(self, layer_idx):
+        return list(self.before)
+
+    def truncate(self, lengths):
+        self.layers[0].lengths = list(lengths)
+
+
+@pytest.mark.parametrize("before,lengths,crop,want", [
+    ([0, 5], [4, 4], 7, [4, 2]), ([5, 0], [4, 4], 7, [2, 4]), ([0, 5], [4, 4], -4, [0, 0]), ([0, 0], [4, 3], 2, [2, 2]), ([0, 5], [4, 4], 3, None),
+    ([6, 6], [1, 4], -2, None), ([6, 6], [1, 4], 6, [0, 0]),
+])
+def test_crops_behind_prefixes_of_unlike_lengths(before, lengths, crop, want):
+    mgr = _Shared(before, lengths)
+    cache = LogitFillCache(mgr)
+    assert cache.get_seq_length() == before[0] + lengths[0]
+    if want is None:
+        with pytest.raises(ValueError, match="shared prefix"):
+            cache.crop(crop)
+    else:
+        cache.crop(crop)
+    assert mgr.layers[0].lengths == (lengths if want is None else want)

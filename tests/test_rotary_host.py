@@ -81,6 +81,7 @@ def _args(**changes):
     ({"head_dim": 514}, _native.LF_E_SHAPE), ({"rotary_dim": 66}, _native.LF_E_SHAPE), ({"rotary_dim": 0}, _native.LF_E_SHAPE),
     ({"batch": -1}, _native.LF_E_SHAPE), ({"batch": 1 << 16, "tokens": 1 << 15}, _native.LF_E_SHAPE),
     ({"n_q": 4096}, _native.LF_E_SHAPE), ({"factor": float("inf")}, _native.LF_E_SHAPE), ({"tokens": 0}, _native.LF_OK),
+    ({"start": (1 << 53) + 1}, _native.LF_E_SHAPE), ({"start": -(1 << 53) - 1}, _native.LF_E_SHAPE),
 ])
 def test_the_c_entry_refuses(changes, status):
     assert _native.load().lf_rotary(ctypes.byref(_args(**changes)), None) == status
