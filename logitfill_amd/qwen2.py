@@ -75,6 +75,13 @@ class _PromptKernels:
             at += n
         self.places = _native.upload(rows, torch.int64, self.rotary.device)
 
+    def serves(self, attn, attention_mask) -> bool:
+        """Whether a layer without history is ``prompt_attention``'s: causal, without a mask of its own (an eager model makes the
+        causal one for every layer)."""
+        if getattr(attn, "sliding_window", None):
+            return False
+        return attention_mask is None or getattr(attn.config, "_attn_implementation", None) == "eager"
+
     def unpack(self) -> None:
         self.plan = self.places = None
 
@@ -109,8 +116,8 @@ def _make_forward(attn, manager, attention_fn, kernels=None):
             query, key = apply_rotary_pos_emb(query, key, cos, sin)
         past = manager.layer_length(layer_idx)
         if getattr(manager, "prefix", None) is not None:
-            past += manager.prefix.layer_length(layer_idx)
-        if past == 0 and kernels is not None and not getattr(attn, "sliding_window", None):
+            past += max(manager.prefix_lengths(layer_idx))
+        if past == 0 and kernels is not None and kernels.serves(attn, attention_mask):
             out = prompt_attention(query, key, value, attn.scaling, kernels.plan).transpose(1, 2)
             kernels.commit(manager, layer_idx, key, value)
         elif past == 0:
@@ -140,8 +147,8 @@ def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kerne
     tokens itself (``reference_attention``, which reads packed pages, does not: ``ValueError``).
 
     ``prompt_kernels``: queries and Keys are rotated by ``Rotary`` with the model's own frequencies (in float64 angles), and
-    layers without history run ``prompt_attention`` (causal, no attention mask; layers of a sliding window keep the
-    model's).  These give no gradients: call the model under ``torch.no_grad()``."""
+    layers without history run ``prompt_attention`` (causal; layers of a sliding window keep the model's, and those that get an
+    attention mask, but for an eager model's, which are taken to be causal).  These give no gradients: call the model under ``torch.no_grad()``."""
     if isinstance(manager, Int4KVManager):
         if attention_fn is reference_attention:
             raise ValueError("reference_attention reads packed pages; an Int4KVManager takes int4_attention")

@@ -105,6 +105,44 @@ def test_samples_of_one_prompt_share_it(gpu, kernels):
         assert _rel(more[b], want[1][0]) < 2e-2
 
 
+def test_a_prefix_that_only_some_sequences_have(gpu):
+    """The first pass behind prefixes of which the first is empty attends the others, too."""
+    model = _model(gpu)
+    prompt, tokens = _ids(50, 3, gpu), _ids(6, 4, gpu).view(2, 3)
+    one, got = _int4(gpu), []
+    first = PackedDecoder(model, one, prompt_kernels=True)
+    first.prefill(prompt[None])
+    want = [first.step(t) for t in tokens[1]]
+    detach_packed(model)
+    rows = [[t[:, :, :50].repeat(2, 1, 1, 1) for t in one.layers[i].read(0, 50)] for i in range(2)]
+    for lengths in ([0, 50], [50, 0]):
+        prefix = _int4(gpu, 2)
+        for i in range(2):
+            prefix.commit(i, *rows[i], lengths)
+        dec = PackedDecoder(model, _int4(gpu, 2, prefix=prefix), prompt_kernels=True)
+        got.append(dec.prefill(tokens if lengths[1] else tokens.flip(0)))
+        detach_packed(model)
+    # (rows quantised once more on their way into the prefix; the one without a prefix attends what its cache reads back, too)
+    assert _rel(got[0][1], want[-1][0]) < 2e-2 and _rel(got[1].flip(0), got[0]) < 1e-4
+
+
+def test_a_padded_batch_s_mask_is_the_model_s_own(gpu):
+    """Of a model whose attention makes masks for padding only, a masked batch keeps its result."""
+    model = _model(gpu)
+    model.config._attn_implementation = "sdpa"
+    ids = _ids(40, 6, gpu).view(2, 20)
+    mask = torch.ones(2, 20, dtype=torch.long, device=gpu)
+    mask[1, :7] = 0
+    pos = (mask.cumsum(1) - 1).clamp(min=0)
+    runs = []
+    for kernels in (False, True):
+        attach_packed(model, _int4(gpu, 2), prompt_kernels=kernels)
+        with torch.no_grad():
+            runs.append(model(input_ids=ids, attention_mask=mask, position_ids=pos, use_cache=False).logits[:, -1])
+        detach_packed(model)
+    assert _rel(runs[1], runs[0]) < 1e-4
+
+
 def test_bfloat16_prompts(gpu):
     """The matrix-core kernels of 16-bit rows under the model: close to its own attention in the same type."""
     model = _model(gpu).bfloat16()
