@@ -504,7 +504,7 @@ int64_t lf_int4_select_workspace_bytes(const lf_int4_layer* layer, int32_t q_len
  * ``rotary_dim`` channels -- (j, rotary_dim / 2 + j), or (2 j, 2 j + 1) where ``interleaved`` -- becomes
  * (x cos t - y sin t, y cos t + x sin t) times ``factor``, t = 2 pi * position * turns[j]; the other channels
  * pass through.  Angles are formed in float64, rows rotated in float32 and rounded once.  Outputs do not overlap inputs.
- * head_dim even, 2 .. 512; rotary_dim even, 2 .. head_dim; batch * tokens below 2^31; n_q + n_kv at most 4096 (either
+ * head_dim even, 2 .. 512; rotary_dim even, 2 .. head_dim; batch * tokens below 2^27; n_q + n_kv at most 4096 (either
  * may be 0, its pointers then NULL).
  */
 typedef struct lf_rotary_args {

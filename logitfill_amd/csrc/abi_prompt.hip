@@ -28,7 +28,7 @@ int32_t lf_rotary(const lf_rotary_args* args, void* stream) {
     if (A.batch < 0 || A.tokens < 0 || A.n_q < 0 || A.n_kv < 0) return LF_E_SHAPE;
     if (A.head_dim < 2 || A.head_dim > 512 || A.head_dim % 2 != 0) return LF_E_SHAPE;
     if (A.rotary_dim < 2 || A.rotary_dim > A.head_dim || A.rotary_dim % 2 != 0) return LF_E_SHAPE;
-    if (static_cast<int64_t>(A.batch) * A.tokens >= 1ll << 31) return LF_E_SHAPE;
+    if (static_cast<int64_t>(A.batch) * A.tokens >= 1ll << 27) return LF_E_SHAPE;
     if (static_cast<int64_t>(A.n_q) + A.n_kv > 4096) return LF_E_SHAPE;
     if (!std::isfinite(A.factor)) return LF_E_SHAPE;
     if (!A.positions && (A.start < -(1ll << 53) || A.start > 1ll << 53)) return LF_E_SHAPE;
@@ -50,7 +50,9 @@ int32_t lf_prompt_attention(const lf_prompt_args* args, void* stream) {
     if (A.n_kv <= 0 || A.n_q <= 0 || A.n_q % A.n_kv != 0 || A.n_items < 0 || A.n_merges < 0 || A.n_slots < 0) return LF_E_SHAPE;
     if (A.tile_rows != 32 && A.tile_rows != 128) return LF_E_SHAPE;
     if (A.groups != 1 && (A.groups != 2 || A.tile_rows != 128 || A.head_dim > 128 || A.dtype == LF_FP32)) return LF_E_SHAPE;
-    if (static_cast<int64_t>(A.n_items) * A.n_kv >= 1ll << 31 || static_cast<int64_t>(A.n_merges) * A.n_kv >= 1ll << 31) return LF_E_SHAPE;
+    // (2^32 threads in a grid)
+    const int64_t threads = A.tile_rows == 32 ? 64 : 256 * A.groups;
+    if (static_cast<int64_t>(A.n_items) * A.n_kv * threads >= 1ll << 32 || static_cast<int64_t>(A.n_merges) * A.n_kv * 256 >= 1ll << 32) return LF_E_SHAPE;
     if (!std::isfinite(A.scaling)) return LF_E_SHAPE;
     if (A.n_items == 0) return LF_OK;
     if (!A.query || !A.key || !A.value || !A.out || !A.items || (A.n_merges && !A.merges)) return LF_E_NULL;

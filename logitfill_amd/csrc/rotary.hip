@@ -66,7 +66,7 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryLaunch a) {
     __shared__ int2 where[kMaxTokens];  // (sequence, token) of the workgroup's tokens
     const lf_rotary_args& A = a.A;
     const int pairs = A.rotary_dim / 2, heads = A.n_q + A.n_kv;
-    const uint32_t first = blockIdx.x * static_cast<uint32_t>(a.tokens_per);  // (all tokens are fewer than 2^31)
+    const uint32_t first = blockIdx.x * static_cast<uint32_t>(a.tokens_per);  // (all tokens are fewer than 2^27)
     const int tokens = static_cast<int>(min(static_cast<uint32_t>(a.tokens_per), static_cast<uint32_t>(A.batch) * A.tokens - first));
     if (threadIdx.x < tokens) {
         const uint32_t at = first + threadIdx.x, b = at / A.tokens;
@@ -163,6 +163,8 @@ int launch_rotary(const lf_rotary_args& A, hipStream_t stream) {
     const int64_t tokens = static_cast<int64_t>(A.batch) * A.tokens;
     int64_t per = 2 * kThreads / A.rotary_dim;
     per = per < tokens / 1024 ? per : tokens / 1024;
+    const int64_t least = (tokens + (1 << 23) - 1) >> 23;  // (2^32 threads in a grid)
+    per = per < least ? least : per;
     a.tokens_per = static_cast<int>(per < 1 ? 1 : per > kMaxTokens ? kMaxTokens : per);
     const uint32_t groups = static_cast<uint32_t>((tokens + a.tokens_per - 1) / a.tokens_per);
     const size_t lds = static_cast<size_t>(a.tokens_per) * (A.rotary_dim / 2) * sizeof(float2);

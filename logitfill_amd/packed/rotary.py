@@ -176,8 +176,8 @@ class Rotary:
                 raise ValueError(f"key must be [{B}, n_kv, {T}, {D}], got {tuple(key.shape)}")
             if key.dtype != query.dtype:
                 raise TypeError("query and key must share a dtype")
-        if B * T >= 1 << 31 or n_q + (0 if key is None else key.shape[1]) > 4096:
-            raise ValueError("at most 2^31 - 1 tokens and 4096 heads a call")
+        if B * T >= 1 << 27 or n_q + (0 if key is None else key.shape[1]) > 4096:
+            raise ValueError("at most 2^27 - 1 tokens and 4096 heads a call")
         _native.dtype_code(query.dtype)
         if isinstance(positions, torch.Tensor):
             if positions.dtype not in (torch.int32, torch.int64):

@@ -142,6 +142,16 @@ def test_another_stream_and_a_captured_graph(gpu):
         assert torch.equal(captured[0], again[0]) and torch.equal(captured[1], again[1])
 
 
+def test_more_tokens_than_one_token_workgroups(gpu):
+    """2^24 tokens and more of wide rows: a grid holds 2^32 threads."""
+    T, D = (1 << 24) + 5, 258
+    rot = Rotary(D, device=gpu)
+    x = torch.ones(1, 1, T, D, dtype=torch.bfloat16, device=gpu)
+    out, _ = rot.rotate(x, None, 7)
+    for at in (0, T // 2, T - 3):
+        check(out[:, :, at : at + 3], x[:, :, at : at + 3].cpu(), torch.arange(at + 7, at + 10)[None], rot, "bf16")
+
+
 def test_refused_calls(gpu):
     rot = Rotary(64, device=gpu)
     q, k = torch.zeros(2, 4, 5, 64, device=gpu), torch.zeros(2, 2, 5, 64, device=gpu)

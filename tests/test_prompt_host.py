@@ -83,7 +83,9 @@ def _args(**changes):
     ({"n_kv": 0}, _native.LF_E_SHAPE), ({"n_items": -1}, _native.LF_E_SHAPE), ({"tile_rows": 64}, _native.LF_E_SHAPE),
     ({"groups": 0}, _native.LF_E_SHAPE), ({"groups": 2, "tile_rows": 32}, _native.LF_E_SHAPE), ({"groups": 2, "dtype": 2}, _native.LF_E_SHAPE),
     ({"groups": 2, "head_dim": 256}, _native.LF_E_SHAPE),
-    ({"n_items": 1 << 30, "n_kv": 2}, _native.LF_E_SHAPE), ({"scaling": float("nan")}, _native.LF_E_SHAPE),
+    ({"n_items": 1 << 30, "n_kv": 2}, _native.LF_E_SHAPE), ({"n_items": 1 << 23}, _native.LF_E_SHAPE),
+    ({"n_merges": 1 << 23, "merges": 4096, "n_slots": 1 << 24}, _native.LF_E_SHAPE), ({"n_items": 1 << 25, "tile_rows": 32}, _native.LF_E_SHAPE),
+    ({"n_items": 1 << 22, "groups": 2}, _native.LF_E_SHAPE), ({"scaling": float("nan")}, _native.LF_E_SHAPE),
     ({"scaling": float("inf")}, _native.LF_E_SHAPE), ({"n_items": 0}, _native.LF_OK), ({"query": None}, _native.LF_E_NULL),
     ({"out": None}, _native.LF_E_NULL), ({"items": None}, _native.LF_E_NULL), ({"n_merges": 1}, _native.LF_E_NULL),
     ({"n_merges": 1, "merges": 4096}, _native.LF_E_SHAPE), ({"n_merges": 2, "merges": 4096, "n_slots": 3}, _native.LF_E_SHAPE),

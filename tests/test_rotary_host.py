@@ -79,7 +79,7 @@ def _args(**changes):
 @pytest.mark.parametrize("changes,status", [
     ({}, _native.LF_E_NULL), ({"dtype": 3}, _native.LF_E_DTYPE), ({"head_dim": 63}, _native.LF_E_SHAPE),
     ({"head_dim": 514}, _native.LF_E_SHAPE), ({"rotary_dim": 66}, _native.LF_E_SHAPE), ({"rotary_dim": 0}, _native.LF_E_SHAPE),
-    ({"batch": -1}, _native.LF_E_SHAPE), ({"batch": 1 << 16, "tokens": 1 << 15}, _native.LF_E_SHAPE),
+    ({"batch": -1}, _native.LF_E_SHAPE), ({"batch": 1 << 16, "tokens": 1 << 15}, _native.LF_E_SHAPE), ({"batch": 1 << 13, "tokens": 1 << 14}, _native.LF_E_SHAPE),
     ({"n_q": 4096}, _native.LF_E_SHAPE), ({"factor": float("inf")}, _native.LF_E_SHAPE), ({"tokens": 0}, _native.LF_OK),
     ({"start": (1 << 53) + 1}, _native.LF_E_SHAPE), ({"start": -(1 << 53) - 1}, _native.LF_E_SHAPE),
 ])
