@@ -2,15 +2,30 @@
 // their sequence's Keys.
 //
 // A workgroup takes a tile of query rows of one kv head -- row r is token r / g of the sequence and head r % g of the group, so
-// that a tile's rows see nearly the same Keys -- and walks the Keys in tiles that reach LDS by DMA, one ahead.  Per
-// tile and wave, for 32 rows, on v_mfma_f32_32x32x16:
+// that a tile's rows see nearly the same Keys -- and walks the Keys in tiles.  Per tile and wave, for 32 rows, on
+// v_mfma_f32_32x32x16:
 //     S^T = K . Q^T,   p = 2^(c S - ref),   O^T += V^T . P^T,   l += sum p.
 // A score's lane holds eight of the sixteen Keys that its lane of the second product takes, so P goes from one to the other
 // in registers; the Value operand is read with its Keys in that order by LDS transpose reads.  The reference point of a row
 // moves only when a score passes it by 2^8.
 //
-// Scores and sums are fp32; P is rounded to the rows' type (bf16: 2^-9 of a weight at most, averaged over the Keys, beside the
-// output's own 2^-9; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).
+// Keys and Values of one tile lie in LDS: Values come by DMA while the Keys are multiplied, the next Keys while the Values
+// are.  32 KB of 64 Keys (head_dim 128) and 168 registers let a compute unit hold three workgroups, whose products and
+// exponentials fill each other's waits.
+//
+// Scores and sums are fp32; P is rounded to the rows' type (bf16: 2^-8 of a weight at most, averaged over the Keys, beside the
+// output's own; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).  float32 rows are
+// multiplied as such (32x32x2).
+//
+// Measured: one prompt of 16 384 tokens, 40 / 8 heads of 128, bf16: 2.36 to 2.5 ms, 1 100 to 1 165 TFLOP/s of the products that
+// are not masked (an 8 192^3 bf16 product of the library: 1 220).  Matrix cores 65 % busy, VALU 51 %, LDS 49 %, no bank
+// conflicts, 98 % of the Keys' and Values' reads from L2; the clock falls to 2.0 GHz under that load.  Eight prompts of 300
+// to 8 190 tokens, 28 / 4 heads: 1.36 to 1.4 ms (1 090); 512 tokens behind 16 384: 139 us, 8 of them the merge; 1 061 tokens
+// alone 25 to 26.5; float32, two of 1 500, 8 heads of 256: 191 (half the float32 products' rate).
+// Not faster at 16 384 tokens: Keys buffered twice (two workgroups a CU; the same long, 8 % less of 1 061 tokens alone, where two groups
+// now do more); tiles of 32 Keys (2.5 against 2.45 ms); 64 rows a wave (its sums spill: 9.1); operands read a product
+// ahead; waves' priorities (2.53); float32 as six products of three bf16 parts each, at heads of 256 (more accurate,
+// but 152 registers spill: 250 against 191 us).
 #include "lf_common.hpp"
 #include "decode_common.hpp"
 
@@ -232,7 +247,9 @@ __device__ __attribute__((noinline)) void one_row(const unsigned char* q, const 
     }
 }
 
-// Groups of NW waves of 32 rows each, that take an item's Key tiles in turn and are joined through LDS at its end.
+// Groups of NW waves of 32 rows each, that take an item's Key tiles in turn and are joined through LDS at its end: where there is a
+// workgroup a compute unit at most, two groups do what two workgroups would, without partial sums and the merge's launch (1 061
+// tokens, 28 / 4 heads of 128: 26 us; one group 33, the Keys divided in two and merged 31).
 template <int D, int Dt>
 constexpr int kPerSimd = Dt == LF_FP32 ? (D == 64 ? 3 : D == 128 ? 2 : 1) : (D == 64 ? 4 : D == 128 ? 3 : 2);  // waves, by their registers
 
@@ -287,7 +304,7 @@ __global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, 
 #pragma unroll
         for (int s = 0; s < SQ; ++s) {
             u32x4 w = {0, 0, 0, 0};
-            if (real) w = *reinterpret_cast<const u32x4*>(src + 32 * s);
+            if (real && reach > 0) w = *reinterpret_cast<const u32x4*>(src + 32 * s);
             q[s] = __builtin_bit_cast(x8, w);
         }
     }
@@ -500,7 +517,8 @@ __global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, 
     }
 }
 
-// The splits' sums of a tile's rows at their largest reference point: D / 4 lanes a row, a split after the other.
+// The splits' sums of a tile's rows at their largest reference point: D / 4 lanes a row, eight splits' loads at once.  (8 us for
+// 34 MB of 112 tiles in four parts: HBM and the launch.)
 template <int D, int Dt>
 __global__ __launch_bounds__(256) void prompt_merge_kernel(Prompt a, const lf_prompt_item* items, int tile_rows) {
     constexpr int L = D / 4;

@@ -102,24 +102,33 @@ class _Form(NamedTuple):
     event: torch.cuda.Event
 
 
-def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int, rows: int, head_dim: int, dtype, n_kv: int, cus: int):
-    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``), the merges', the number of partial sums and the groups of a workgroup."""
+def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int, rows: int, head_dim: int, dtype, n_kv: int, cus: int,
+               tokens: int = 0):
+    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``), the merges', the number of partial sums and the groups of a workgroup.
+    What lies behind the sequences in rows of ``tokens`` is queries that see no Key, whose output is zeros."""
     n, m = np.asarray(lengths, dtype=np.int64), np.asarray(key_lengths, dtype=np.int64)
+    q_start, k_start = (np.cumsum(n) - n) * packed_q, (np.cumsum(m) - m) * packed_k
+    q_row, k_row = (np.zeros_like(n) if packed else np.arange(len(n)) for packed in (packed_q, packed_k))
+    ends = n.sum(keepdims=True) if packed_q else n
+    spare = np.flatnonzero(ends < tokens)
+    if len(spare):
+        n, q_start = np.concatenate([n, tokens - ends[spare]]), np.concatenate([q_start, ends[spare]])
+        q_row = np.concatenate([q_row, spare])
+        m, k_row, k_start = (np.concatenate([x, np.zeros(len(spare), dtype=np.int64)]) for x in (m, k_row, k_start))
     per = -(-n * group // rows)  # row tiles of every sequence
     seq = np.repeat(np.arange(len(n)), per)
     tile = np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)
     last_token = np.minimum((tile * rows + rows - 1) // group, n[seq] - 1)
     reach = np.maximum(m[seq] - n[seq] + last_token + 1, 0)
     tiles = -(-reach // key_tile(head_dim, dtype))
-    size, groups = split_size(tiles, n_kv, cus, workgroups_per_cu(rows, head_dim, dtype), head_dim, dtype, rows)
+    size, groups = split_size(tiles[tiles > 0], n_kv, cus, workgroups_per_cu(rows, head_dim, dtype), head_dim, dtype, rows)
     parts = np.maximum(-(-tiles // size), 1)
     each = -(-tiles // parts)
     parts = np.maximum(-(-tiles // np.maximum(each, 1)), 1)  # (no part is empty)
     slot = np.where(parts > 1, np.cumsum(np.where(parts > 1, parts, 0)) - parts, -1)
     base = np.zeros((len(seq), 12), dtype=np.int64)
-    q_start, k_start = np.cumsum(n) - n, np.cumsum(m) - m
-    base[:, 0], base[:, 1] = (0, q_start[seq]) if packed_q else (seq, 0)
-    base[:, 3], base[:, 4] = (0, k_start[seq]) if packed_k else (seq, 0)
+    base[:, 0], base[:, 1] = q_row[seq], q_start[seq]
+    base[:, 3], base[:, 4] = k_row[seq], k_start[seq]
     base[:, 2], base[:, 5], base[:, 6] = n[seq], m[seq], tile
     base[:, 9], base[:, 10] = slot, parts
     merges = base[parts > 1]
@@ -169,8 +178,8 @@ class PromptPlan:
         lengths = (self.lengths, self.key_lengths)[of]
         raise ValueError(f"{name} {tuple(shape)} does not hold sequences of {lengths[:8]}{'...' if self.batch > 8 else ''} tokens")
 
-    def _form(self, packed_q: bool, packed_k: bool, group: int, n_kv: int, head_dim: int, dtype) -> _Form:
-        key = (packed_q, packed_k, group, n_kv, head_dim, dtype)
+    def _form(self, packed_q: bool, packed_k: bool, group: int, n_kv: int, head_dim: int, dtype, tokens: int) -> _Form:
+        key = (packed_q, packed_k, group, n_kv, head_dim, dtype, tokens)
         form = self._forms.get(key)
         if form is None:
             stream = _native.current_stream_ptr(self.device)
@@ -178,7 +187,7 @@ class PromptPlan:
                 raise RuntimeError("a plan's first call uploads its work: run the step once before the capture")
             rows = tile_rows(self.lengths, group)
             items, merges, slots, groups = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, head_dim, dtype, n_kv,
-                                              _cu_count(self.device))
+                                                      _cu_count(self.device), tokens)
             with torch.inference_mode(False):
                 device = _native.upload(np.concatenate([items, merges]).reshape(-1), torch.int32, self.device)
             event = torch.cuda.Event()
@@ -259,12 +268,12 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     if plan.device != query.device:
         raise ValueError(f"query is on {query.device}, the plan on {plan.device}")
     packed_q, packed_k = plan._rows(query.shape, 0, "query"), plan._rows(key.shape, 1, "key")
-    if plan._longest[0] * (n_q // n_kv) > 1 << 30:
+    if T * (n_q // n_kv) > 1 << 30:
         raise ValueError("too many query tokens for one call: feed them in chunks")
     with torch.cuda.device(query.device):
         if not plan._longest[0] or not plan._longest[1]:
             return torch.zeros(B, T, n_q, D, dtype=query.dtype, device=query.device).transpose(1, 2)
-        form = plan._form(packed_q, packed_k, n_q // n_kv, n_kv, D, query.dtype)
+        form = plan._form(packed_q, packed_k, n_q // n_kv, n_kv, D, query.dtype, T)
         if len(plan._args) >= 64:
             plan._args.clear()
         kept = plan._args[_form_of(query, key, value, scaling)] = (_describe(query, key, value, code, scaling, form), form)
@@ -303,9 +312,7 @@ def _launch(query, key, value, plan: PromptPlan, kept, form: _Form) -> torch.Ten
     stream = _native.current_stream_ptr(plan.device)
     if stream != form.stream:
         plan._order(form, stream)
-    # (rows that no sequence has are not written by the kernel)
-    make = torch.empty if plan._total[0] == B * T else torch.zeros
-    out = make((B, T, n_q, D), dtype=query.dtype, device=plan.device)
+    out = torch.empty((B, T, n_q, D), dtype=query.dtype, device=plan.device)
     a = _native.PromptArgs.from_buffer_copy(kept)
     a.query, a.key, a.value, a.out = query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr()
     if form.n_merges:

@@ -46,6 +46,23 @@ def test_every_row_tile_s_keys_are_covered_once(seed, rows, D, dtype):
             assert (divided[b, t][9], divided[b, t][10]) == (parts[0][9], len(parts))
 
 
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("lengths,tokens", [([3, 0, 40], 50), ([7], 7), ([0, 0], 3), ([300, 299], 1000)])
+def test_rows_behind_the_sequences_are_zeros_of_their_own(packed, lengths, tokens):
+    g, rows = 3, 32
+    items, _, _, _ = work_items(lengths, [n + 5 for n in lengths], packed, False, g, rows, 64, torch.bfloat16, 2, 256, tokens)
+    written = np.zeros((1 if packed else len(lengths), tokens), dtype=int)
+    for q_row, start, n, k_row, k_start, m, tile, begin, end, slot, parts, _ in items:
+        if begin:
+            continue
+        for r in range(tile * rows, min((tile + 1) * rows, n * g)):
+            if r % g == 0:
+                written[q_row, start + r // g] += 1
+                inside = start < sum(lengths) if packed else start < lengths[q_row]
+                assert inside == (m > 0) and (inside or (begin, end, slot) == (0, 0, -1))
+    assert (written == 1).all()
+
+
 def test_long_keys_of_few_rows_are_divided():
     assert split_size(np.array([512]), 4, 256, 5, 128, torch.bfloat16, 32)[0] < 64
     assert split_size(np.full(4096, 256), 8, 256, 3, 128, torch.bfloat16) == (256, 1)  # enough row tiles
