@@ -19,9 +19,10 @@
 //
 // Measured: one prompt of 16 384 tokens, 40 / 8 heads of 128, bf16: 2.36 to 2.5 ms, 1 100 to 1 165 TFLOP/s of the products that
 // are not masked (an 8 192^3 bf16 product of the library: 1 220).  Matrix cores 65 % busy, VALU 51 %, LDS 49 %, no bank
-// conflicts, 98 % of the Keys' and Values' reads from L2; the clock falls to 2.0 GHz under that load.  Eight prompts of 300
-// to 8 190 tokens, 28 / 4 heads: 1.36 to 1.4 ms (1 090); 512 tokens behind 16 384: 139 us, 8 of them the merge; 1 061 tokens
-// alone 25 to 26.5; float32, two of 1 500, 8 heads of 256: 191 (half the float32 products' rate).
+// conflicts, 97 % of the Keys' and Values' reads from L2; the clock falls to 2.0 GHz under that load.  Eight prompts of 300
+// to 8 190 tokens, 28 / 4 heads: 1.35 to 1.4 ms (1 090); 512 tokens behind 16 384: 138 us, 8 of them the merge; 1 061 tokens
+// alone 25; float32, two of 1 500, 8 heads of 256: 191 (half the float32 products' rate).  At head_dim 64 the exponentials bound a
+// tile: sixteen of 1 to 1 500 tokens, 14 / 2 heads, fp16: 45 us, 0.69 a Key tile and compute unit, 0.43 of them VALU work.
 // Not faster at 16 384 tokens: Keys buffered twice (two workgroups a CU; the same long, 8 % less of 1 061 tokens alone, where two groups
 // now do more); tiles of 32 Keys (2.5 against 2.45 ms); 64 rows a wave (its sums spill: 9.1); operands read a product
 // ahead; waves' priorities (2.53); float32 as six products of three bf16 parts each, at heads of 256 (more accurate,
@@ -249,7 +250,7 @@ __device__ __attribute__((noinline)) void one_row(const unsigned char* q, const 
 
 // Groups of NW waves of 32 rows each, that take an item's Key tiles in turn and are joined through LDS at its end: where there is a
 // workgroup a compute unit at most, two groups do what two workgroups would, without partial sums and the merge's launch (1 061
-// tokens, 28 / 4 heads of 128: 26 us; one group 33, the Keys divided in two and merged 31).
+// tokens, 28 / 4 heads of 128: 25 us; one group 32, the Keys divided in two or three and merged 31 and 30).
 template <int D, int Dt>
 constexpr int kPerSimd = Dt == LF_FP32 ? (D == 64 ? 3 : D == 128 ? 2 : 1) : (D == 64 ? 4 : D == 128 ? 3 : 2);  // waves, by their registers
 

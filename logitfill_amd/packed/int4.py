@@ -10,7 +10,8 @@ graph and replayed until the capacity is reached.
 * ``Int4KVManager``  -- the cache of a model's layers (``commit``, ``truncate``, ``reset``; a layer's
   ``read`` / ``dequantize``).
 * ``int4_attention`` -- commits the new tokens, then attends over the cached rows; with ``pages``
-  over those pages and the query's own one only.
+  over those pages and the query's own one only; of a manager with a ``prefix``, behind the rows of another
+  manager that several of its sequences share.
 * ``select_pages``   -- the pages whose Keys' bounds admit the largest ``q . k``, per query token and
   kv head.
 
