@@ -14,8 +14,8 @@
 // exponentials fill each other's waits.
 //
 // Scores and sums are fp32; P is rounded to the rows' type (bf16: 2^-8 of a weight at most, averaged over the Keys, beside the
-// output's own; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).  float32 rows are
-// multiplied as such (32x32x2).
+// output's own; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).  float32 rows: see
+// prompt_split_kernel, or, of heads of 256 and single waves, multiplied as such (32x32x2).
 //
 // Measured: one prompt of 16 384 tokens, 40 / 8 heads of 128, bf16: 2.36 to 2.5 ms, 1 100 to 1 165 TFLOP/s of the products that
 // are not masked (an 8 192^3 bf16 product of the library: 1 220).  Matrix cores 65 % busy, VALU 51 %, LDS 49 %, no bank
@@ -25,8 +25,7 @@
 // tile: sixteen of 1 to 1 500 tokens, 14 / 2 heads, fp16: 45 us, 0.69 a Key tile and compute unit, 0.43 of them VALU work.
 // Not faster at 16 384 tokens: Keys buffered twice (two workgroups a CU; the same long, 8 % less of 1 061 tokens alone, where two groups
 // now do more); tiles of 32 Keys (2.5 against 2.45 ms); 64 rows a wave (its sums spill: 9.1); operands read a product
-// ahead; waves' priorities (2.53); float32 as six products of three bf16 parts each, at heads of 256 (more accurate,
-// but 152 registers spill: 250 against 191 us).
+// ahead; waves' priorities (2.53).
 #include "lf_common.hpp"
 #include "decode_common.hpp"
 
@@ -248,6 +247,55 @@ __device__ __attribute__((noinline)) void one_row(const unsigned char* q, const 
     }
 }
 
+// The end of an item for the pair of lanes (col, hi) that holds a row: its output, or a split's sums; rows of a tile with Values
+// that are not finite are formed anew over Keys begin .. end - 1.
+template <int D, int Dt, int NW>
+__device__ __forceinline__ void finish(const Prompt& a, const lf_prompt_item& item, int h, int wave, int col, int hi, int i, int j, bool real,
+                                       int lim, int begin, int end, bool odd, float l, float ref, const f32x16 (&o)[D / 32]) {
+    using E = Element<Dt>;
+    constexpr bool kWide = Dt == LF_FP32;
+    constexpr int ES = kWide ? 4 : 2, CB = D / 32, kRows = 32 * NW;
+    if (odd) {
+        if (!real) return;
+        const unsigned char* src = static_cast<const unsigned char*>(a.q) +
+            ES * (item.q_row * a.qs[0] + static_cast<int64_t>(h * a.g + i) * a.qs[1] + static_cast<int64_t>(item.q_start + j) * a.qs[2]);
+        const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2];
+        const int64_t at = (static_cast<int64_t>(item.slot) * a.n_kv + h) * kRows + wave * 32 + col;
+        const int64_t k = item.k_row * a.ks[0] + h * a.ks[1] + static_cast<int64_t>(item.k_start) * a.ks[2];
+        const int64_t v = item.k_row * a.vs[0] + h * a.vs[1] + static_cast<int64_t>(item.k_start) * a.vs[2];
+        const unsigned char *kbase = static_cast<const unsigned char*>(a.k) + ES * k, *vbase = static_cast<const unsigned char*>(a.v) + ES * v;
+        one_row<D, Dt>(src, kbase, vbase, ES * a.ks[2], ES * a.vs[2], begin, min(end, lim), hi, a.qscale,
+                       item.slot < 0 ? static_cast<unsigned char*>(a.out) + ES * to : nullptr, a.part_o + at * D, a.part_ml + 2 * at);
+        return;
+    }
+    if (!real) return;
+    // channels 32 c + 8 n + 4 hi .. + 3
+    if (item.slot < 0) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;  // (no Key seen: zeros)
+        const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2] + 4 * hi;
+#pragma unroll
+        for (int c = 0; c < CB; ++c)
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const f32x4 x = {o[c][4 * n] * inv, o[c][4 * n + 1] * inv, o[c][4 * n + 2] * inv, o[c][4 * n + 3] * inv};
+                if constexpr (kWide) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to + 32 * c + 8 * n) = x;
+                else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to + 32 * c + 8 * n) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+            }
+        return;
+    }
+    const int64_t at = (static_cast<int64_t>(item.slot) * a.n_kv + h) * kRows + wave * 32 + col;
+    float* dst = a.part_o + at * D + 4 * hi;
+#pragma unroll
+    for (int c = 0; c < CB; ++c)
+#pragma unroll
+        for (int n = 0; n < 4; ++n)
+            *reinterpret_cast<f32x4*>(dst + 32 * c + 8 * n) = f32x4{o[c][4 * n], o[c][4 * n + 1], o[c][4 * n + 2], o[c][4 * n + 3]};
+    if (hi == 0) {
+        a.part_ml[2 * at] = l == 0.f ? -__builtin_inff() : ref;
+        a.part_ml[2 * at + 1] = l;
+    }
+}
+
 // Groups of NW waves of 32 rows each, that take an item's Key tiles in turn and are joined through LDS at its end: where there is a
 // workgroup a compute unit at most, two groups do what two workgroups would, without partial sums and the merge's launch (1 061
 // tokens, 28 / 4 heads of 128: 25 us; one group 32, the Keys divided in two or three and merged 31 and 30).
@@ -294,7 +342,6 @@ __global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, 
     const int first = item.begin, last = min(item.end, (reach + KT - 1) / KT);
 
     const Loader<D, Dt, NW> loader(a, item, h, wave, lane, reach);
-    const unsigned char *kbase = loader.keys.base, *vbase = loader.values.base;
     if (first + turn < last) loader.fill(loader.keys, first + turn, lds);
 
     x8 q[SQ];
@@ -480,42 +527,229 @@ __global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, 
         }
     }
 
-    if (odd) {
-        if (!real) return;
-        const unsigned char* src = static_cast<const unsigned char*>(a.q) +
-            ES * (item.q_row * a.qs[0] + static_cast<int64_t>(h * a.g + i) * a.qs[1] + static_cast<int64_t>(item.q_start + j) * a.qs[2]);
-        const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2];
-        const int64_t at = (static_cast<int64_t>(item.slot) * a.n_kv + h) * kRows + wave * 32 + col;
-        one_row<D, Dt>(src, kbase, vbase, ES * a.ks[2], ES * a.vs[2], first * KT, min(last * KT, lim), hi, a.qscale,
-                       item.slot < 0 ? static_cast<unsigned char*>(a.out) + ES * to : nullptr, a.part_o + at * D, a.part_ml + 2 * at);
-        return;
+    finish<D, Dt, NW>(a, item, h, wave, col, hi, i, j, real, lim, first * KT, last * KT, odd, l, ref, o);
+}
+
+// float32 rows of 64 and 128 channels, 128 query rows a workgroup, on the bf16 matrix cores: a number is the sum of three bf16
+// parts of eight bits each, and of the nine products of two numbers' parts the six largest are formed, that of the first parts
+// apart from the others; those left out are 2^-21 of |x y| or less.  Six products at sixteen times the float32 products' rate.
+// Keys and Values are taken apart once, on their way from registers to LDS (32 of each a tile, three planes of bf16 rows);
+// the next tile's loads run beside the products.
+//
+// Four prompts of 2 000 to 4 096 tokens, 16 / 8 heads of 128: 1 060 us (1 060 TFLOP/s of bf16 products), of 64: 625; by float32
+// products 1 460 and 830, and the largest error among 700 tokens falls from 1.2e-6 to 5.6e-7 and from 9.5e-7 to 7.1e-7.  Two
+// waves a SIMD at both sizes (at 128 29 registers are spilled; three waves at 64 spilled 48: 750 us).  At head_dim 256 query
+// parts and sums pass the registers (152 spilled, 4 250 us against 3 240), and a single wave's 32 rows would share the parting
+// of their Keys with nobody: those are multiplied as they are.
+template <int D>
+struct Planes {
+    using T = Tile<D, LF_BF16>;
+    static constexpr int keys = 32, plane = keys * T::row;
+    static constexpr int units = keys * D / 8 / 256;  // eight channels of a row, of Keys and of Values each, per thread
+    static constexpr int lds = 6 * plane;
+};
+// x's and y's parts, a word of each: eight bits of what is left, so that the three are the number, cut rather than rounded (the
+// largest numbers stay finite).
+__device__ __forceinline__ void three_parts(float x, float y, uint32_t (&w)[3]) {
+#pragma unroll
+    for (int n = 0; n < 3; ++n) {
+        const uint32_t u = __float_as_uint(x), v = __float_as_uint(y);
+        w[n] = __builtin_amdgcn_perm(v, u, 0x07060302);
+        x -= __uint_as_float(u & 0xffff0000u);
+        y -= __uint_as_float(v & 0xffff0000u);
     }
-    if (!real) return;
-    // channels 32 c + 8 n + 4 hi .. + 3
-    if (item.slot < 0) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;  // (no Key seen: zeros)
-        const int64_t to = item.q_row * a.os[0] + static_cast<int64_t>(h * a.g + i) * a.os[1] + static_cast<int64_t>(item.q_start + j) * a.os[2] + 4 * hi;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+template <int D>
+__global__ __launch_bounds__(4 * kWave, 2) void prompt_split_kernel(Prompt a) {
+    using P = Planes<D>;
+    using T = typename P::T;
+    using E = Element<LF_BF16>;
+    constexpr int NW = 4, KT = P::keys, SQ = D / 16, CB = D / 32, KK = 2, U = P::units;
+    constexpr int kRows = 32 * NW;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];  // three planes of Keys, three of Values
+    __shared__ int odd_rows;  // whether Keys or Values were not finite: parts of infinity are not
+    if (threadIdx.x == 0) odd_rows = 0;
+    __syncthreads();
+    const int h = blockIdx.x % a.n_kv;
+    const lf_prompt_item item = load_item(a);
+    const int lane = threadIdx.x % kWave, wave = in_sgpr(static_cast<int>(threadIdx.x / kWave));
+    const int col = lane & 31, hi = lane >> 5;
+    const uint32_t lds = lds_addr(smem);
+
+    const int row = item.tile * kRows + wave * 32 + col;
+    const int j = row / a.g, i = row - j * a.g;
+    const bool real = j < item.n_q;
+    const int lim = real ? max(item.n_k - item.n_q + j + 1, 0) : 0;
+    int all = real ? lim : 0x7fffffff;
 #pragma unroll
-        for (int c = 0; c < CB; ++c)
+    for (int m = 1; m < 32; m <<= 1) all = min(all, __shfl_xor(all, m, kWave));
+    all = in_sgpr(all);
+    const int last_token = min((item.tile * kRows + kRows - 1) / a.g, item.n_q - 1);
+    const int reach = max(item.n_k - item.n_q + last_token + 1, 0);
+    const int first = item.begin, last = min(item.end, (reach + KT - 1) / KT);
+
+    const unsigned char* kbase = in_sgpr(static_cast<const unsigned char*>(a.k) + 4 * (item.k_row * a.ks[0] + h * a.ks[1] + static_cast<int64_t>(item.k_start) * a.ks[2]));
+    const unsigned char* vbase = in_sgpr(static_cast<const unsigned char*>(a.v) + 4 * (item.k_row * a.vs[0] + h * a.vs[1] + static_cast<int64_t>(item.k_start) * a.vs[2]));
+    const int64_t kstride = 4 * a.ks[2], vstride = 4 * a.vs[2];
+    f32x4 next[2][U][2];  // the next tile's eight channels of Keys, of Values
+    const auto load = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const f32x4 x = {o[c][4 * n] * inv, o[c][4 * n + 1] * inv, o[c][4 * n + 2] * inv, o[c][4 * n + 3] * inv};
-                if constexpr (kWide) *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + to + 32 * c + 8 * n) = x;
-                else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to + 32 * c + 8 * n) = u32x2{E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+        for (int u = 0; u < U; ++u) {
+            const int unit = u * 256 + threadIdx.x, r = unit / (D / 8), c = unit % (D / 8);
+            const int64_t at = min(t * KT + r, reach - 1);  // (in place of Keys past the last one that is seen, that one)
+            const f32x4* k = reinterpret_cast<const f32x4*>(kbase + at * kstride + 32 * c);
+            const f32x4* v = reinterpret_cast<const f32x4*>(vbase + at * vstride + 32 * c);
+            next[0][u][0] = k[0];
+            next[0][u][1] = k[1];
+            next[1][u][0] = v[0];
+            next[1][u][1] = v[1];
+        }
+    };
+    const auto stage = [&]() __attribute__((always_inline)) {
+        bool fine = true;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int unit = u * 256 + threadIdx.x, r = unit / (D / 8), c = unit % (D / 8);
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                u32x4 w[3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t parts[3];
+                    const f32x4& x = next[side][u][e / 2];
+                    fine = fine && finite(x[2 * (e % 2)]) && finite(x[2 * (e % 2) + 1]);
+                    three_parts(x[2 * (e % 2)], x[2 * (e % 2) + 1], parts);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) w[n][e] = parts[n];
+                }
+                unsigned char* to = smem + (side ? 3 * P::plane : 0) + r * T::row + 16 * (c ^ (side ? T::value_swap(r) : T::key_swap(r)));
+#pragma unroll
+                for (int n = 0; n < 3; ++n) *reinterpret_cast<u32x4*>(to + n * P::plane) = w[n];
             }
-        return;
-    }
-    const int64_t at = (static_cast<int64_t>(item.slot) * a.n_kv + h) * kRows + wave * 32 + col;
-    float* dst = a.part_o + at * D + 4 * hi;
+        }
+        if (!fine) odd_rows = 1;
+    };
+    if (first < last) load(first);
+
+    bool odd = false;
+    bf16x8 q[SQ][3];
+    {
+        const float* src = static_cast<const float*>(a.q) + item.q_row * a.qs[0] + static_cast<int64_t>(h * a.g + i) * a.qs[1] +
+                           static_cast<int64_t>(item.q_start + j) * a.qs[2] + 8 * hi;
 #pragma unroll
-    for (int c = 0; c < CB; ++c)
+        for (int n = 0; n < SQ; ++n) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f}, y = x;
+            if (real && reach > 0) {
+                x = *reinterpret_cast<const f32x4*>(src + 16 * n);
+                y = *reinterpret_cast<const f32x4*>(src + 16 * n + 4);
+            }
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-            *reinterpret_cast<f32x4*>(dst + 32 * c + 8 * n) = f32x4{o[c][4 * n], o[c][4 * n + 1], o[c][4 * n + 2], o[c][4 * n + 3]};
-    if (hi == 0) {
-        a.part_ml[2 * at] = l == 0.f ? -__builtin_inff() : ref;
-        a.part_ml[2 * at + 1] = l;
+            for (int e = 0; e < 4; ++e) odd = odd || !finite(x[e]) || !finite(y[e]);
+            if (a.qscale < 0.f) {
+                x = -x;
+                y = -y;
+            }
+            u32x4 w[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t parts[3];
+                three_parts(e < 2 ? x[2 * e] : y[2 * e - 4], e < 2 ? x[2 * e + 1] : y[2 * e - 3], parts);
+#pragma unroll
+                for (int m = 0; m < 3; ++m) w[m][e] = parts[m];
+            }
+#pragma unroll
+            for (int m = 0; m < 3; ++m) q[n][m] = __builtin_bit_cast(bf16x8, w[m]);
+        }
     }
+    const float scale = fmaxf(fabsf(a.qscale), 1e-37f);
+
+    f32x16 o[CB];
+#pragma unroll
+    for (int c = 0; c < CB; ++c) o[c] = f32x16{};
+    float l = 0.f, ref = 0.f, limit = -__builtin_inff();
+    const uint32_t keys = lds + col * T::row + 16 * (hi ^ T::key_swap(col));
+    const int group = lane >> 4, in16 = lane & 15;
+    const int vrow = 4 * (group >> 1) + (in16 >> 2), vcol = 16 * (group & 1) + 4 * (in16 & 3);
+    const uint32_t values = lds + 3 * P::plane + vrow * T::row + 16 * ((vcol / 8) ^ T::value_swap(vrow)) + 2 * (vcol & 7);
+
+    for (int t = first; t < last; ++t) {
+        __syncthreads();  // nobody reads the last tile any more
+        stage();
+        __syncthreads();
+        if (t + 1 < last) load(t + 1);
+        const int k0 = t * KT;
+        f32x16 s = f32x16{}, rest = f32x16{};
+#pragma unroll
+        for (int n = 0; n < SQ; ++n) {
+            bf16x8 k[3];
+#pragma unroll
+            for (int m = 0; m < 3; ++m) k[m] = __builtin_bit_cast(bf16x8, read16((keys ^ (32 * n)) + m * P::plane));
+#pragma unroll
+            for (int sum = 2; sum > 0; --sum)
+#pragma unroll
+                for (int m = 0; m <= sum; ++m) rest = E::mfma(k[m], q[n][sum - m], rest);
+            s = E::mfma(k[0], q[n][0], s);
+            if (n % 2 == 1) phase();
+        }
+        s += rest;
+        const bool masked = k0 + KT > all;
+        if (masked) {
+            phase();  // (a branch, not selects in every tile)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = k0 + 8 * (r / 4) + 4 * hi + r % 4 < lim ? s[r] : -__builtin_inff();
+        }
+        float most = -__builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = fmaxf(most, s[r]);
+        most *= scale;
+        if (__any(most > limit)) {
+            most = halves_max(most);
+            const bool moves = most > limit;
+            const float down = !moves ? 1.f : limit == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - most);
+            if (moves) { ref = most; limit = most + 8.f; }
+            l *= down;
+#pragma unroll
+            for (int c = 0; c < CB; ++c) o[c] *= down;
+        }
+        bf16x8 p[KK][3];
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            u32x4 w[3];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[8 * kk + 2 * e], scale, -ref));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[8 * kk + 2 * e + 1], scale, -ref));
+                l += x + y;
+                uint32_t parts[3];
+                three_parts(x, y, parts);
+#pragma unroll
+                for (int m = 0; m < 3; ++m) w[m][e] = parts[m];
+            }
+#pragma unroll
+            for (int m = 0; m < 3; ++m) p[kk][m] = __builtin_bit_cast(bf16x8, w[m]);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int c = 0; c < CB; ++c) {
+                bf16x8 v[3];
+#pragma unroll
+                for (int m = 0; m < 3; ++m) {
+                    const uint32_t at = (values ^ (64 * c)) + m * P::plane + 16 * kk * T::row;
+                    const u32x2 x = read_tr(at), y = read_tr(at + 8 * T::row);
+                    v[m] = __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], y[0], y[1]});
+                }
+#pragma unroll
+                for (int sum = 2; sum >= 0; --sum)
+#pragma unroll
+                    for (int m = 0; m <= sum; ++m) o[c] = E::mfma(v[m], p[kk][sum - m], o[c]);
+                if (c % 2 == 1) phase();
+            }
+    }
+    // (the last barrier is behind every tile's Keys and Values)
+    finish<D, LF_FP32, NW>(a, item, h, wave, col, hi, i, j, real, lim, first * KT, last * KT, __any(odd) || odd_rows != 0, halves_sum(l), ref, o);
 }
 
 // The splits' sums of a tile's rows at their largest reference point: D / 4 lanes a row, eight splits' loads at once.  (8 us for
@@ -562,15 +796,13 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(Prompt a, const lf_pr
     else *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(a.out) + to) = u32x2{Element<Dt>::pack(o[0], o[1]), Element<Dt>::pack(o[2], o[3])};
 }
 
-template <int D, int Dt, int NW, int Groups>
-int launch_rows(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
-    const auto fn = prompt_kernel<D, Dt, NW, Groups>;
-    constexpr int lds = Shape<D, Dt, NW, Groups>::lds;
+template <int D, int Dt>
+int launch_rows(void (*fn)(Prompt), int waves, int lds, const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
     const int st = allow_dynamic_lds(reinterpret_cast<const void*>(fn), lds);
     if (st != LF_OK) return st;
-    hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(A.n_items) * A.n_kv), dim3(Groups * NW * kWave), lds, stream, a);
+    hipLaunchKernelGGL(fn, dim3(static_cast<uint32_t>(A.n_items) * A.n_kv), dim3(waves * kWave), lds, stream, a);
     if (A.n_merges) {
-        const int rows = 32 * NW, per = 256 / (D / 4);
+        const int rows = A.tile_rows, per = 256 / (D / 4);
         hipLaunchKernelGGL((prompt_merge_kernel<D, Dt>), dim3(static_cast<uint32_t>(A.n_merges) * A.n_kv, (rows + per - 1) / per), dim3(256), 0,
                            stream, a, A.merges, rows);
     }
@@ -580,9 +812,14 @@ int launch_rows(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
 
 template <int D, int Dt>
 int launch_typed(const Prompt& a, const lf_prompt_args& A, hipStream_t stream) {
-    if constexpr (D <= 128 && Dt != LF_FP32)
-        if (A.groups == 2) return launch_rows<D, Dt, 4, 2>(a, A, stream);
-    return A.tile_rows == 32 ? launch_rows<D, Dt, 1, 1>(a, A, stream) : launch_rows<D, Dt, 4, 1>(a, A, stream);
+    if (A.tile_rows == 32) return launch_rows<D, Dt>(prompt_kernel<D, Dt, 1, 1>, 1, Shape<D, Dt, 1, 1>::lds, a, A, stream);
+    if constexpr (D <= 128 && Dt == LF_FP32) {
+        return launch_rows<D, Dt>(prompt_split_kernel<D>, 4, Planes<D>::lds, a, A, stream);
+    } else {
+        if constexpr (D <= 128)
+            if (A.groups == 2) return launch_rows<D, Dt>(prompt_kernel<D, Dt, 4, 2>, 8, Shape<D, Dt, 4, 2>::lds, a, A, stream);
+        return launch_rows<D, Dt>(prompt_kernel<D, Dt, 4, 1>, 4, Shape<D, Dt, 4, 1>::lds, a, A, stream);
+    }
 }
 
 template <int D>

@@ -26,7 +26,7 @@ MAX_TOKENS = 1 << 24  # of a sequence
 # holds as many as it can (four waves; of the model's head_dim, float32 or not); of a workgroup's start and end; of the
 # launch that merges divided row tiles; of joining a workgroup's two groups.
 TILE_US = {(64, False): (0.9, 0.69), (128, False): (1.5, 0.95), (256, False): (1.5, 1.25),
-           (64, True): (2.2, 2.0), (128, True): (4.1, 3.9), (256, True): (8.4, 8.4)}
+           (64, True): (1.95, 1.5), (128, True): (3.5, 2.7), (256, True): (8.4, 8.4)}
 ITEM_US, MERGE_US, PAIR_US = 3.0, 5.0, 1.5
 
 
@@ -45,7 +45,7 @@ def workgroups_per_cu(rows: int, head_dim: int, dtype) -> int:
     wide = dtype == torch.float32
     if rows == 32:
         return (163840 // 2) // (key_tile(head_dim, dtype) * head_dim * (4 if wide else 2))
-    return {64: 3 if wide else 4, 128: 2 if wide else 3, 256: 1 if wide else 2}[head_dim]
+    return {64: 2 if wide else 4, 128: 2 if wide else 3, 256: 1 if wide else 2}[head_dim]
 
 
 def split_size(tiles: np.ndarray, n_kv: int, cus: int, per_cu: int, head_dim: int, dtype, rows: int = 128) -> tuple[int, int]:

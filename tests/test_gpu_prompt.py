@@ -119,6 +119,30 @@ def test_what_is_masked_need_not_be_finite(gpu, D, dtype):
     assert torch.isinf(out[0, :2, late[1] : 100, 3]).all() and torch.isfinite(out[0, :2, : late[1]]).all()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("late", [False, True])
+def test_float32_s_ends(gpu, D, late):
+    """Keys whose scores are -inf (of rows that see them in whole tiles or in masked ones), Values of a quarter of the largest
+    number and of 2^-100: as float64 has them."""
+    T, at = 300, 290 if late else 40
+    q, k, v = inputs((1, 2, T, D), (1, 2, T, D), "fp32", 12)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    v[0, 1, 41, 7] = torch.finfo(torch.float32).max / 4
+    v[0, 0, :, 9] = 2.0 ** -100
+    hidden = k.clone()
+    k[0, 0, at, 3] = -float("inf")
+    hidden[0, 0, at] = 0
+    out = prompt_attention(q.to(gpu), k.to(gpu), v.to(gpu), D ** -0.5).cpu()
+    want, tol = expected(q, hidden, v, [T], [T], D ** -0.5, "fp32", True, True)
+    # rows that see it: without it
+    qn, kn, vn = (f32(t).astype(np.float64) for t in (q, hidden, v))
+    seen = np.tril(np.ones((T, T), dtype=bool))
+    seen[:, at] = False
+    want[0, 0], tol[0, 0] = attend(qn[0, 0], kn[0, 0], vn[0, 0], D ** -0.5, seen, "fp32")
+    assert_within(out, want, tol)
+    assert float(out[0, 0, :, 9].min()) > 0.9 * 2.0 ** -100 and torch.isfinite(out).all()
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 def test_strides_and_alignment(gpu, dtype):
     """Views of one fused projection, rows off 16 bytes, broadcast kv heads, channels not innermost."""
