@@ -21,7 +21,7 @@
 // are not masked (an 8 192^3 bf16 product of the library: 1 220).  Matrix cores 65 % busy, VALU 51 %, LDS 49 %, no bank
 // conflicts, 97 % of the Keys' and Values' reads from L2; the clock falls to 2.0 GHz under that load.  Eight prompts of 300
 // to 8 190 tokens, 28 / 4 heads: 1.35 to 1.4 ms (1 090); 512 tokens behind 16 384: 138 us, 8 of them the merge; 1 061 tokens
-// alone 25; float32, two of 1 500, 8 heads of 256: 191 (half the float32 products' rate).  At head_dim 64 the exponentials bound a
+// alone 25; float32, two of 1 500, 8 heads of 256: 177 (8.4 a Key tile, 6.8 of them float32 products).  At head_dim 64 the exponentials bound a
 // tile: sixteen of 1 to 1 500 tokens, 14 / 2 heads, fp16: 45 us, 0.69 a Key tile and compute unit, 0.43 of them VALU work.
 // Not faster at 16 384 tokens: Keys buffered twice (two workgroups a CU; the same long, 8 % less of 1 061 tokens alone, where two groups
 // now do more); tiles of 32 Keys (2.5 against 2.45 ms); 64 rows a wave (its sums spill: 9.1); operands read a product

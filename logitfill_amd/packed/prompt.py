@@ -57,10 +57,11 @@ def split_size(tiles: np.ndarray, n_kv: int, cus: int, per_cu: int, head_dim: in
     alone, shared = TILE_US[head_dim, dtype == torch.float32]
     best, choice = None, (longest, 1)
     pairs = rows == 128 and head_dim <= 128 and dtype != torch.float32
-    for parts in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256):
-        if parts > longest:
-            break
-        s = -(-longest // parts)
+    at_most = {-(-longest // parts) for parts in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256) if parts <= longest}
+    if per_cu == 1:  # (whose ends, all of one compute unit in turn, hang on a tile more or less)
+        at_most |= {s - 1 for s in at_most if s > 1}
+    for s in sorted(at_most, reverse=True):
+        whole = s >= longest
         n = np.maximum(-(-tiles // s), 1)
         sizes = np.sort(np.repeat(-(-tiles // n), n * n_kv))[::-1]
         slots = cus * per_cu
@@ -68,21 +69,22 @@ def split_size(tiles: np.ndarray, n_kv: int, cus: int, per_cu: int, head_dim: in
         # the workgroups of the compute unit that has the longest ones of each rank at once
         first = float(sizes[:slots:cus].sum()) * shared + ITEM_US
         if per_cu == 1 and len(sizes) > slots:  # one after the other: what is left goes to those that end first
-            load = np.zeros(-(-len(sizes) // slots) * slots)
-            load[: len(sizes)] = sizes * shared + ITEM_US
-            load = load.reshape(-1, slots)
-            load[1::2] = load[1::2, ::-1]
-            first = float(load.sum(0).max())
+            load = np.zeros(slots)
+            for at in range(0, len(sizes), slots):
+                turn = sizes[at : at + slots]
+                load.sort()
+                load[: len(turn)] += turn * shared + ITEM_US
+            first = float(load.max())
         elif len(sizes) > slots:
             even += 0.3 * float(sizes[slots:].mean()) * shared
         costs = [max(first, even, s * alone + ITEM_US)]
         if pairs and len(sizes) <= cus and s > 1:
             costs.append(-(-s // 2) * max(1.2 * alone, 2.2 * shared) + ITEM_US + PAIR_US)
-        more = MERGE_US + 8e-6 * float(n[n > 1].sum()) * n_kv * rows * (head_dim + 2) / 4 if parts > 1 else 0.0
+        more = MERGE_US + 8e-6 * float(n[n > 1].sum()) * n_kv * rows * (head_dim + 2) / 4 if not whole else 0.0
         for groups, cost in enumerate(costs, 1):
             if best is None or cost + more < 0.97 * best:
                 best, choice = cost + more, (s, groups)
-        if parts == 1 and len(sizes) >= 4 * cus * per_cu:
+        if whole and len(sizes) >= 4 * cus * per_cu:
             break  # (as many row tiles keep every compute unit at work)
         if min(costs) + more > 1.5 * best:
             break
