@@ -566,6 +566,27 @@ typedef struct lf_prompt_args {
 } lf_prompt_args;
 
 int32_t lf_prompt_attention(const lf_prompt_args* args, void* stream);
+
+/*
+ * The work of such a call, planned on the host.  lf_prompt_split writes split[2], the Key tiles that an item takes at most and
+ * the groups, of least estimated time.  lf_prompt_items writes the items, and behind them the merges, where ``cap`` holds both;
+ * else LF_E_WORKSPACE.  counts[3] (n_items, n_merges, n_slots) are set either way.  What lies behind the sequences in rows of
+ * ``tokens`` becomes queries that see no Key, whose output is zeros (0: nothing does).
+ */
+#define LF_PROMPT_TOKENS (1 << 24)            /* of a sequence at most                        */
+
+typedef struct lf_prompt_batch {
+    const int32_t *lengths, *key_lengths;     /* HOST [batch]: queries and Keys of every sequence */
+    int32_t batch;
+    int32_t packed_q, packed_k;               /* sequences one behind another in row 0, or each in its own row */
+    int32_t tokens;
+    int32_t group, n_kv, head_dim, dtype;     /* group: query heads per kv head; group * tokens (and lengths) at most 2^30 */
+    int32_t tile_rows;                        /* 32 or 128                                    */
+    int32_t compute_units;
+} lf_prompt_batch;
+
+int32_t lf_prompt_split(const lf_prompt_batch* batch, int32_t* split);
+int32_t lf_prompt_items(const lf_prompt_batch* batch, int32_t split_size, lf_prompt_item* items, int32_t cap, int32_t* counts);
 int64_t lf_prompt_workspace_bytes(int32_t n_kv, int32_t head_dim, int32_t tile_rows, int32_t n_slots);
 
 #ifdef __cplusplus

@@ -155,6 +155,17 @@ class PromptArgs(ctypes.Structure):
     ]
 
 
+class PromptBatch(ctypes.Structure):
+    """``lf_prompt_batch``."""
+
+    _fields_ = [
+        ("lengths", c_void_p), ("key_lengths", c_void_p),
+        ("batch", c_int32), ("packed_q", c_int32), ("packed_k", c_int32), ("tokens", c_int32),
+        ("group", c_int32), ("n_kv", c_int32), ("head_dim", c_int32), ("dtype", c_int32),
+        ("tile_rows", c_int32), ("compute_units", c_int32),
+    ]
+
+
 _SIGNATURES = {
     "lf_abi_version": (c_int32, []),
     "lf_build_info": (c_char_p, []),
@@ -195,6 +206,8 @@ _SIGNATURES = {
     "lf_int4_select_workspace_bytes": (c_int64, [POINTER(Int4Layer), c_int32]),
     "lf_rotary": (c_int32, [POINTER(RotaryArgs), c_void_p]),
     "lf_prompt_attention": (c_int32, [POINTER(PromptArgs), c_void_p]),
+    "lf_prompt_split": (c_int32, [POINTER(PromptBatch), c_void_p]),
+    "lf_prompt_items": (c_int32, [POINTER(PromptBatch), c_int32, c_void_p, c_int32, c_void_p]),
     "lf_prompt_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
 }
 

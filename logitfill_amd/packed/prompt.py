@@ -10,6 +10,7 @@ Nothing here runs on the CPU.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import NamedTuple, Optional
@@ -21,13 +22,7 @@ from logitfill_amd import _native
 from logitfill_amd.packed.cache import _check_device
 from logitfill_amd.packed.reference import _cu_count
 
-MAX_TOKENS = 1 << 24  # of a sequence
-# Microseconds of a Key tile for a workgroup that has its compute unit to itself, and a compute unit's share of one where it
-# holds as many as it can (four waves; of the model's head_dim, float32 or not); of a workgroup's start and end; of the
-# launch that merges divided row tiles; of joining a workgroup's two groups.
-TILE_US = {(64, False): (0.9, 0.69), (128, False): (1.5, 0.95), (256, False): (1.5, 1.25),
-           (64, True): (1.95, 1.5), (128, True): (3.5, 2.7), (256, True): (8.4, 8.4)}
-ITEM_US, MERGE_US, PAIR_US = 3.0, 5.0, 1.5
+MAX_TOKENS = 1 << 24  # of a sequence (LF_PROMPT_TOKENS)
 
 
 def key_tile(head_dim: int, dtype) -> int:
@@ -40,55 +35,11 @@ def tile_rows(lengths, group: int) -> int:
     return 32 if max(lengths) * group <= 32 else 128
 
 
-def workgroups_per_cu(rows: int, head_dim: int, dtype) -> int:
-    """Workgroups that a CU holds: of four waves by their registers, of one by the LDS of its tiles."""
-    wide = dtype == torch.float32
-    if rows == 32:
-        return (163840 // 2) // (key_tile(head_dim, dtype) * head_dim * (4 if wide else 2))
-    return {64: 2 if wide else 4, 128: 2 if wide else 3, 256: 1 if wide else 2}[head_dim]
-
-
-def split_size(tiles: np.ndarray, n_kv: int, cus: int, per_cu: int, head_dim: int, dtype, rows: int = 128) -> tuple[int, int]:
-    """``(Key tiles that a workgroup takes at most, its groups)`` of row tiles that see ``tiles`` each: of least estimated time
-    on ``cus`` compute units of ``per_cu`` workgroups.  A division's gain is the compute units that it sets to work, its price
-    the partial sums, written and read once, and the launch that merges them.  Two groups share a workgroup's tiles
-    without either, where a compute unit has one workgroup at most."""
-    longest = int(tiles.max(initial=1))
-    alone, shared = TILE_US[head_dim, dtype == torch.float32]
-    best, choice = None, (longest, 1)
-    pairs = rows == 128 and head_dim <= 128 and dtype != torch.float32
-    at_most = {-(-longest // parts) for parts in (1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256) if parts <= longest}
-    if per_cu == 1:  # (whose ends, all of one compute unit in turn, hang on a tile more or less)
-        at_most |= {s - 1 for s in at_most if s > 1}
-    for s in sorted(at_most, reverse=True):
-        whole = s >= longest
-        n = np.maximum(-(-tiles // s), 1)
-        sizes = np.sort(np.repeat(-(-tiles // n), n * n_kv))[::-1]
-        slots = cus * per_cu
-        even = (float(sizes.sum()) * shared + len(sizes) * 0.25 * ITEM_US) / cus
-        # the workgroups of the compute unit that has the longest ones of each rank at once
-        first = float(sizes[:slots:cus].sum()) * shared + ITEM_US
-        if per_cu == 1 and len(sizes) > slots:  # one after the other: what is left goes to those that end first
-            load = np.zeros(slots)
-            for at in range(0, len(sizes), slots):
-                turn = sizes[at : at + slots]
-                load.sort()
-                load[: len(turn)] += turn * shared + ITEM_US
-            first = float(load.max())
-        elif len(sizes) > slots:
-            even += 0.3 * float(sizes[slots:].mean()) * shared
-        costs = [max(first, even, s * alone + ITEM_US)]
-        if pairs and len(sizes) <= cus and s > 1:
-            costs.append(-(-s // 2) * max(1.2 * alone, 2.2 * shared) + ITEM_US + PAIR_US)
-        more = MERGE_US + 8e-6 * float(n[n > 1].sum()) * n_kv * rows * (head_dim + 2) / 4 if not whole else 0.0
-        for groups, cost in enumerate(costs, 1):
-            if best is None or cost + more < 0.97 * best:
-                best, choice = cost + more, (s, groups)
-        if whole and len(sizes) >= 4 * cus * per_cu:
-            break  # (as many row tiles keep every compute unit at work)
-        if min(costs) + more > 1.5 * best:
-            break
-    return choice
+def split_size(batch: _native.PromptBatch) -> tuple[int, int]:
+    """``(Key tiles that a workgroup takes at most, its groups)``: ``lf_prompt_split``."""
+    split = (ctypes.c_int32 * 2)()
+    _native.check(_native.load().lf_prompt_split(batch, split), "lf_prompt_split")
+    return split[0], split[1]
 
 
 class _Form(NamedTuple):
@@ -106,43 +57,24 @@ class _Form(NamedTuple):
 
 def work_items(lengths, key_lengths, packed_q: bool, packed_k: bool, group: int, rows: int, head_dim: int, dtype, n_kv: int, cus: int,
                tokens: int = 0):
-    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``), the merges', the number of partial sums and the groups of a workgroup.
-    What lies behind the sequences in rows of ``tokens`` is queries that see no Key, whose output is zeros."""
-    n, m = np.asarray(lengths, dtype=np.int64), np.asarray(key_lengths, dtype=np.int64)
-    q_start, k_start = (np.cumsum(n) - n) * packed_q, (np.cumsum(m) - m) * packed_k
-    q_row, k_row = (np.zeros_like(n) if packed else np.arange(len(n)) for packed in (packed_q, packed_k))
-    ends = n.sum(keepdims=True) if packed_q else n
-    spare = np.flatnonzero(ends < tokens)
-    if len(spare):
-        n, q_start = np.concatenate([n, tokens - ends[spare]]), np.concatenate([q_start, ends[spare]])
-        q_row = np.concatenate([q_row, spare])
-        m, k_row, k_start = (np.concatenate([x, np.zeros(len(spare), dtype=np.int64)]) for x in (m, k_row, k_start))
-    per = -(-n * group // rows)  # row tiles of every sequence
-    seq = np.repeat(np.arange(len(n)), per)
-    tile = np.arange(len(seq)) - np.repeat(np.cumsum(per) - per, per)
-    last_token = np.minimum((tile * rows + rows - 1) // group, n[seq] - 1)
-    reach = np.maximum(m[seq] - n[seq] + last_token + 1, 0)
-    tiles = -(-reach // key_tile(head_dim, dtype))
-    size, groups = split_size(tiles[tiles > 0], n_kv, cus, workgroups_per_cu(rows, head_dim, dtype), head_dim, dtype, rows)
-    parts = np.maximum(-(-tiles // size), 1)
-    each = -(-tiles // parts)
-    parts = np.maximum(-(-tiles // np.maximum(each, 1)), 1)  # (no part is empty)
-    slot = np.where(parts > 1, np.cumsum(np.where(parts > 1, parts, 0)) - parts, -1)
-    base = np.zeros((len(seq), 12), dtype=np.int64)
-    base[:, 0], base[:, 1] = q_row[seq], q_start[seq]
-    base[:, 3], base[:, 4] = k_row[seq], k_start[seq]
-    base[:, 2], base[:, 5], base[:, 6] = n[seq], m[seq], tile
-    base[:, 9], base[:, 10] = slot, parts
-    merges = base[parts > 1]
-    at = np.repeat(np.arange(len(seq)), parts)
-    part = np.arange(len(at)) - np.repeat(np.cumsum(parts) - parts, parts)
-    items = base[at]
-    items[:, 7] = part * each[at]
-    items[:, 8] = np.minimum(items[:, 7] + each[at], tiles[at])
-    items[:, 9] = np.where(items[:, 9] < 0, -1, items[:, 9] + part)
-    # the longest first: the short ones fill what is left
-    items = items[np.argsort(items[:, 7] - items[:, 8], kind="stable")]
-    return items.astype(np.int32), merges.astype(np.int32), int(np.where(parts > 1, parts, 0).sum()), groups
+    """The ``lf_prompt_item`` rows of a call (int32 ``[n, 12]``) and, behind them, of its merges; ``(n_items, n_merges, n_slots)`` and
+    the groups of a workgroup.  What lies behind the sequences in rows of ``tokens`` is queries that see no Key, whose output is
+    zeros."""
+    n, m = np.asarray(lengths, dtype=np.int32), np.asarray(key_lengths, dtype=np.int32)
+    batch = _native.PromptBatch(n.ctypes.data, m.ctypes.data, len(n), packed_q, packed_k, tokens, group, n_kv, head_dim,
+                                _native.dtype_code(dtype), rows, cus)
+    size, groups = split_size(batch)
+    counts = (ctypes.c_int32 * 3)()
+    lib = _native.load()
+    cap = 0
+    while True:  # (asks for the counts first)
+        items = np.zeros((cap, 12), dtype=np.int32)
+        status = lib.lf_prompt_items(batch, size, items.ctypes.data, cap, counts)
+        if status != _native.LF_E_WORKSPACE or cap:
+            break
+        cap = counts[0] + counts[1]
+    _native.check(status, "lf_prompt_items")
+    return items, tuple(counts), groups
 
 
 class PromptPlan:
@@ -188,13 +120,13 @@ class PromptPlan:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a plan's first call uploads its work: run the step once before the capture")
             rows = tile_rows(self.lengths, group)
-            items, merges, slots, groups = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, head_dim, dtype, n_kv,
+            items, counts, groups = work_items(self.lengths, self.key_lengths, packed_q, packed_k, group, rows, head_dim, dtype, n_kv,
                                                       _cu_count(self.device), tokens)
             with torch.inference_mode(False):
-                device = _native.upload(np.concatenate([items, merges]).reshape(-1), torch.int32, self.device)
+                device = _native.upload(items.reshape(-1), torch.int32, self.device)
             event = torch.cuda.Event()
             event.record(torch.cuda.current_stream(self.device))
-            form = self._forms[key] = _Form(device, len(items), len(merges), slots, rows, groups, stream, event)
+            form = self._forms[key] = _Form(device, *counts, rows, groups, stream, event)
         return form
 
     def _order(self, form: _Form, stream: int) -> None:

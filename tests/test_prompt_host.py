@@ -7,7 +7,7 @@ import torch
 
 from logitfill_amd import _native
 from logitfill_amd.packed import LogitFillCache, PromptPlan, prompt_attention
-from logitfill_amd.packed.prompt import key_tile, split_size, tile_rows, work_items
+from logitfill_amd.packed.prompt import key_tile, tile_rows, work_items
 
 
 @pytest.mark.parametrize("seed", range(12))
@@ -19,7 +19,9 @@ def test_every_row_tile_s_keys_are_covered_once(seed, rows, D, dtype):
     n = rng.integers(0, 700, B)
     m = np.maximum(0, n + rng.integers(-20, 4000, B))
     packed = bool(seed % 2)
-    items, merges, slots, groups = work_items(n, m, packed, not packed, g, rows, D, dtype, n_kv, 256)
+    items, (n_items, n_merges, slots), groups = work_items(n, m, packed, not packed, g, rows, D, dtype, n_kv, 256)
+    items, merges = items[:n_items], items[n_items:]
+    assert len(merges) == n_merges and groups in (1, 2)
     assert (np.diff(items[:, 8] - items[:, 7]) <= 0).all()  # the longest first
     assert sorted(items[items[:, 9] >= 0, 9]) == list(range(slots))
     by_tile = {}
@@ -50,7 +52,8 @@ def test_every_row_tile_s_keys_are_covered_once(seed, rows, D, dtype):
 @pytest.mark.parametrize("lengths,tokens", [([3, 0, 40], 50), ([7], 7), ([0, 0], 3), ([300, 299], 1000)])
 def test_rows_behind_the_sequences_are_zeros_of_their_own(packed, lengths, tokens):
     g, rows = 3, 32
-    items, _, _, _ = work_items(lengths, [n + 5 for n in lengths], packed, False, g, rows, 64, torch.bfloat16, 2, 256, tokens)
+    items, (n_items, _, _), _ = work_items(lengths, [n + 5 for n in lengths], packed, False, g, rows, 64, torch.bfloat16, 2, 256, tokens)
+    items = items[:n_items]
     written = np.zeros((1 if packed else len(lengths), tokens), dtype=int)
     for q_row, start, n, k_row, k_start, m, tile, begin, end, slot, parts, _ in items:
         if begin:
@@ -64,8 +67,10 @@ def test_rows_behind_the_sequences_are_zeros_of_their_own(packed, lengths, token
 
 
 def test_long_keys_of_few_rows_are_divided():
-    assert split_size(np.array([512]), 4, 256, 5, 128, torch.bfloat16, 32)[0] < 64
-    assert split_size(np.full(4096, 256), 8, 256, 3, 128, torch.bfloat16) == (256, 1)  # enough row tiles
+    items, counts, groups = work_items([1], [32768], True, True, 4, 32, 128, torch.bfloat16, 4, 256)
+    assert max(items[:, 8] - items[:, 7]) < 64 and counts == (len(items) - 1, 1, len(items) - 1) and groups == 1
+    items, counts, groups = work_items([4096] * 64, [16384] * 64, True, True, 8, 128, 128, torch.bfloat16, 8, 256)
+    assert counts == (64 * 256, 0, 0) and groups == 1  # enough row tiles
     assert tile_rows([1, 4], 8) == 32 and tile_rows([5], 8) == 128
 
 
@@ -158,3 +163,44 @@ def test_crops_behind_prefixes_of_unlike_lengths(before, lengths, crop, want):
     else:
         cache.crop(crop)
     assert mgr.layers[0].lengths == (lengths if want is None else want)
+
+
+def _batch(lengths=(5, 7), key_lengths=(9, 7), **changes):
+    n, m = np.array(lengths, dtype=np.int32), np.array(key_lengths, dtype=np.int32)
+    b = _native.PromptBatch(n.ctypes.data, m.ctypes.data, len(n), 1, 1, 0, 4, 2, 64, 0, 128, 256)
+    for name, value in changes.items():
+        setattr(b, name, value)
+    return b, (n, m)
+
+
+@pytest.mark.parametrize("changes,status", [
+    ({"lengths": None}, _native.LF_E_NULL), ({"key_lengths": None}, _native.LF_E_NULL), ({"dtype": 3}, _native.LF_E_DTYPE),
+    ({"head_dim": 96}, _native.LF_E_UNSUPPORTED), ({"batch": 0}, _native.LF_E_SHAPE), ({"tokens": -1}, _native.LF_E_SHAPE),
+    ({"group": 0}, _native.LF_E_SHAPE), ({"n_kv": 0}, _native.LF_E_SHAPE), ({"compute_units": 0}, _native.LF_E_SHAPE),
+    ({"tile_rows": 64}, _native.LF_E_SHAPE), ({"group": 1 << 29}, _native.LF_E_SHAPE), ({"tokens": 1 << 30}, _native.LF_E_SHAPE),
+])
+def test_the_planner_refuses(changes, status):
+    b, kept = _batch(**{k: v for k, v in changes.items() if v is not None})
+    for name in (k for k, v in changes.items() if v is None):
+        setattr(b, name, None)
+    lib, split, counts = _native.load(), (ctypes.c_int32 * 2)(), (ctypes.c_int32 * 3)()
+    assert lib.lf_prompt_split(b, split) == status and lib.lf_prompt_items(b, 4, None, 0, counts) == status
+    for lengths in ((-1, 4), ((1 << 24) + 1, 4)):
+        b, kept = _batch(lengths)
+        assert lib.lf_prompt_split(b, split) == _native.LF_E_SHAPE
+    b, kept = _batch()
+    assert lib.lf_prompt_split(b, None) == lib.lf_prompt_items(b, 4, None, 9, counts) == _native.LF_E_NULL
+    assert lib.lf_prompt_split(None, split) == lib.lf_prompt_items(b, 4, None, 0, None) == _native.LF_E_NULL
+    assert lib.lf_prompt_items(b, 0, None, 0, counts) == _native.LF_E_SHAPE
+
+
+def test_the_planner_writes_what_fits_only():
+    b, kept = _batch((300, 7), (900, 7))
+    lib, counts = _native.load(), (ctypes.c_int32 * 3)()
+    assert lib.lf_prompt_items(b, 4, None, 0, counts) == _native.LF_E_WORKSPACE
+    n = counts[0] + counts[1]
+    assert counts[1] > 0 and counts[2] >= 2 * counts[1]
+    items = np.full((n + 1, 12), -7, dtype=np.int32)
+    assert lib.lf_prompt_items(b, 4, items.ctypes.data, n - 1, counts) == _native.LF_E_WORKSPACE and (items == -7).all()
+    assert lib.lf_prompt_items(b, 4, items.ctypes.data, n, counts) == _native.LF_OK
+    assert (items[n] == -7).all() and (items[:n, 2] > 0).all()
