@@ -710,10 +710,11 @@ def _attend(manager, layer_idx: int, layer, query: torch.Tensor, new, scaling: f
 # From this much work on (products of a row's channel and a token's, over all prefixes) the many-row kernel takes shared
 # prefixes, per group size (bf16, head_dim up to 128, 64 rows): below, the general kernel's launch, which holds the sequences' own
 # rows too, is faster although it unpacks a record for every 16 rows.  us a call with 200 own tokens, general / many-row: 28 /
-# 4 heads of 128, a prefix of 32K, groups of 64, 112 rows 34 / 48, 448 84 / 82, 896 145 / 123; groups of 128, 896 rows 123 /
-# 144; 32 / 8 heads, groups of 32, 64 rows 44 / 55, 128 71 / 61, 512 219 / 156; 14 / 2 heads of 64, 896 rows, groups of 64 and
-# 32, 51 / 56 and 61 / 56; prefixes of 4K, up to 896 rows, 16 to 52 / 19 to 64.
-SHARED_MANY_ROWS = {32: 3e9, 64: 1e10, 128: 3e10}
+# 4 heads of 128, a prefix of 32K, groups of 64, 224 rows 53 / 59, 448 86 / 81, 896 155 / 121; groups of 128, 896 rows 134 /
+# 141, 1 792 243 / 233; 32 / 8 heads, groups of 32, 64 rows 44 / 54, 128 73 / 60, 512 216 / 155; 14 / 2 heads of 64, 896 rows,
+# groups of 64 and 32, 49 / 55 and 58 / 55, 1 792, groups of 64, 104 / 84; prefixes of 4K and 8K, 896 rows, groups of 64, 33 / 52 and
+# 53 / 63.
+SHARED_MANY_ROWS = {32: 3e9, 64: 6e9, 128: 3e10}
 SHARED_LEAST_ROWS = 64
 
 
