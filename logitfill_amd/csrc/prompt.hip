@@ -25,7 +25,8 @@
 // tile: sixteen of 1 to 1 500 tokens, 14 / 2 heads, fp16: 45 us, 0.69 a Key tile and compute unit, 0.43 of them VALU work.
 // Not faster at 16 384 tokens: Keys buffered twice (two workgroups a CU; the same long, 8 % less of 1 061 tokens alone, where two groups
 // now do more); tiles of 32 Keys (2.5 against 2.45 ms); 64 rows a wave (its sums spill: 9.1); operands read a product
-// ahead; waves' priorities (2.53).
+// ahead; waves' priorities (2.53); sums of the rounded weights by dot products (the same; at head_dim 64 46.5 us for 45, the error
+// 2.3e-4 for 2.6e-4).
 #include "lf_common.hpp"
 #include "decode_common.hpp"
 
