@@ -549,12 +549,12 @@ def many_rows_per_cu(head_dim: int, group: int) -> int:
 
 
 @functools.lru_cache(maxsize=512)
-def _plan(units: tuple, rows: int, slots: int, overhead: float) -> int:
+def _plan(units: tuple, rows: int, slots: int, overhead: float, most: int) -> int:
     """Units a split takes, of sequences of ``units`` (their work, ``rows`` workgroups a split): the size of least
     estimated time -- all work and every split's fixed cost over the slots, and part of a split's for the last round,
-    or one split's where all are there at once."""
+    or one split's where all are there at once.  No sequence is in more than ``most``."""
     total, longest = sum(units) * rows, max(units)
-    least = -(-longest // MAX_SPLITS)
+    least = -(-longest // most)
 
     def items(size):
         return rows * sum(-(-u // size) for u in units)
@@ -577,12 +577,13 @@ def _plan(units: tuple, rows: int, slots: int, overhead: float) -> int:
     return min((min(size, longest) for size in sorted(sizes, reverse=True)), key=cost)
 
 
-def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3, overhead: float = SPLIT_OVERHEAD) -> tuple[int, int]:
+def plan_splits(tokens, rows: int, cus: int, per_cu: int = 3, overhead: float = SPLIT_OVERHEAD,
+                most: int = MAX_SPLITS) -> tuple[int, int]:
     """``(splits, tokens of each)`` for sequences of ``tokens`` rows (an int, or one per sequence), ``rows``
-    workgroups per sequence and split."""
+    workgroups per sequence and split; at most ``most`` splits."""
     tokens = (tokens,) if isinstance(tokens, int) else tokens
     size = _plan(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), rows, per_cu * cus,
-                 overhead) * SPLIT_UNIT
+                 overhead, most) * SPLIT_UNIT
     return -(-max(max(tokens), 1) // size), size
 
 
@@ -766,7 +767,9 @@ def _shared_plan(manager, layer_idx: int, q_len: int, dtype, lengths, cus: int):
     if (rows >= SHARED_LEAST_ROWS and dtype == torch.bfloat16 and D <= 128 and behind
             and sum(tokens) * rows * n_kv * D >= SHARED_MANY_ROWS[group]):
         splits, size = plan_splits(tokens, n_kv * -(-rows // 128), cus, many_rows_per_cu(D, group), MANY_ROWS_OVERHEAD)
-        return (min(splits, MAX_SPLITS // 2), size, 1), plan_splits(own, n_kv * -(-each // 16), cus, workgroups_per_cu(D, group))
+        splits = min(splits, MAX_SPLITS // 2)
+        # (a row's parts are at most MAX_SPLITS + 1; one long sequence among short ones asks for many)
+        return (splits, size, 1), plan_splits(own, n_kv * -(-each // 16), cus, workgroups_per_cu(D, group), most=MAX_SPLITS + 1 - splits)
     size = _shared_split(tuple([(n + SPLIT_UNIT - 1) // SPLIT_UNIT or 1 for n in tokens]), n_kv * -(-rows // 16),
                          len(own), max(own) // SPLIT_UNIT + 1, sum(own) // SPLIT_UNIT, n_kv * -(-each // 16),
                          cus, workgroups_per_cu(D, group), SHARED_ITEM * max(D, 128) / 128) * SPLIT_UNIT
