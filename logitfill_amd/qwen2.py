@@ -45,9 +45,25 @@ def _dense_attention(attn, query, key, value, attention_mask, kwargs):
     return out  # [B, q_len, n_q, D]
 
 
+def _is_causal(mask, tokens: int) -> bool:
+    """Whether an attention mask (additive, or truth values) is the causal one of ``tokens``, for every sequence (a host
+    synchronisation; not in a capture)."""
+    if not isinstance(mask, torch.Tensor) or mask.dim() != 4 or tuple(mask.shape[2:]) != (tokens, tokens):
+        return False
+    if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+        return False
+    if mask.dtype == torch.bool:
+        seen, hidden = mask, ~mask
+    elif mask.is_floating_point():
+        seen, hidden = mask == 0, mask <= torch.finfo(mask.dtype).min
+    else:
+        return False
+    return bool(torch.where(torch.ones(tokens, tokens, dtype=torch.bool, device=mask.device).tril(), seen, hidden).all())
+
+
 class _PromptKernels:
-    """What the layers of a model with ``prompt_kernels`` share: its rotation and, while packed prompts pass through,
-    their plan and the places of their tokens in a padded batch."""
+    """What the layers of a model with ``prompt_kernels`` share: its rotation, what is known of the masks of the pass that is
+    under way, and, while packed prompts pass through, their plan and the places of their tokens in a padded batch."""
 
     def __init__(self, model, device):
         rope, cfg = model.model.rotary_emb, model.config
@@ -63,6 +79,19 @@ class _PromptKernels:
         self.windows = any(getattr(layer.self_attn, "sliding_window", None) for layer in model.model.layers)
         self.plan: PromptPlan | None = None
         self.places: torch.Tensor | None = None
+        self.masks: list | None = None  # of the pass under way: (mask, whether it is the causal one)
+        self._hooks = [model.model.register_forward_pre_hook(self._begin),
+                       model.model.register_forward_hook(self._end, always_call=True)]
+
+    def detach(self) -> None:
+        for hook in self._hooks:
+            hook.remove()
+
+    def _begin(self, module, args) -> None:
+        self.masks = []
+
+    def _end(self, module, args, output) -> None:
+        self.masks = None
 
     def pack(self, lengths) -> None:
         """Prompts of ``lengths`` pass through next, packed."""
@@ -75,12 +104,31 @@ class _PromptKernels:
             at += n
         self.places = _native.upload(rows, torch.int64, self.rotary.device)
 
-    def serves(self, attn, attention_mask) -> bool:
-        """Whether a layer without history is ``prompt_attention``'s: causal, without a mask of its own (an eager model makes the
-        causal one for every layer)."""
+    def serves(self, attn, attention_mask, tokens: int, is_causal=None) -> bool:
+        """Whether a layer without history is ``prompt_attention``'s: where the model's own attention of ``tokens`` would be
+        causal over every whole sequence.  Packed prompts are (they come without a mask); so is sdpa without a mask (it gets
+        one for padding and for sequences in one row), and an eager model, which gets one for every call, where that is the causal
+        one.  Other implementations tell padding and packed rows in ways of their own."""
         if getattr(attn, "sliding_window", None):
             return False
-        return attention_mask is None or getattr(attn.config, "_attn_implementation", None) == "eager"
+        if self.plan is not None:
+            return True
+        if is_causal is False or not getattr(attn, "is_causal", True) or not getattr(attn.config, "is_causal", True):
+            return False
+        kind = getattr(attn.config, "_attn_implementation", None)
+        if kind == "sdpa":
+            return attention_mask is None
+        return kind == "eager" and self._is_causal(attention_mask, tokens)
+
+    def _is_causal(self, mask, tokens: int) -> bool:
+        """``_is_causal``, looked up once a pass (its layers get one mask)."""
+        for seen, answer in self.masks or ():
+            if seen is mask:
+                return answer
+        answer = _is_causal(mask, tokens)
+        if self.masks is not None:
+            self.masks.append((mask, answer))
+        return answer
 
     def unpack(self) -> None:
         self.plan = self.places = None
@@ -117,7 +165,7 @@ def _make_forward(attn, manager, attention_fn, kernels=None):
         past = manager.layer_length(layer_idx)
         if getattr(manager, "prefix", None) is not None:
             past += max(manager.prefix_lengths(layer_idx))
-        if past == 0 and kernels is not None and kernels.serves(attn, attention_mask):
+        if past == 0 and kernels is not None and kernels.serves(attn, attention_mask, query.shape[2], kwargs.get("is_causal")):
             out = prompt_attention(query, key, value, attn.scaling, kernels.plan).transpose(1, 2)
             kernels.commit(manager, layer_idx, key, value)
         elif past == 0:
@@ -147,8 +195,10 @@ def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kerne
     tokens itself (``reference_attention``, which reads packed pages, does not: ``ValueError``).
 
     ``prompt_kernels``: queries and Keys are rotated by ``Rotary`` with the model's own frequencies (in float64 angles), and
-    layers without history run ``prompt_attention`` (causal; layers of a sliding window keep the model's, and those that get an
-    attention mask, but for an eager model's, which are taken to be causal).  These give no gradients: call the model under ``torch.no_grad()``."""
+    layers without history run ``prompt_attention`` where the model's own attention (eager or sdpa) would be causal over every
+    whole sequence: those of a sliding window keep the model's, and so do calls whose mask hides more (padding, sequences in one
+    row, a mask of the caller's; an eager model's mask is looked at once a pass, which waits for the device).  These give no
+    gradients: call the model under ``torch.no_grad()``."""
     if isinstance(manager, Int4KVManager):
         if attention_fn is reference_attention:
             raise ValueError("reference_attention reads packed pages; an Int4KVManager takes int4_attention")
@@ -163,6 +213,8 @@ def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kerne
         if manager.n_kv != n_kv or manager.head_dim != layer.self_attn.head_dim:
             raise ValueError("manager shape does not match the model's attention")
     kernels = _PromptKernels(model, manager.device) if prompt_kernels else None
+    _drop_kernels(model)
+    model._lf_prompt_kernels = kernels
     for layer in layers:
         attn = layer.self_attn
         if not hasattr(attn, "_lf_original_forward"):
@@ -171,7 +223,14 @@ def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kerne
     return kernels
 
 
+def _drop_kernels(model) -> None:
+    kernels = model.__dict__.pop("_lf_prompt_kernels", None)
+    if kernels is not None:
+        kernels.detach()
+
+
 def detach_packed(model) -> None:
+    _drop_kernels(model)
     for layer in model.model.layers:
         attn = layer.self_attn
         if hasattr(attn, "_lf_original_forward"):
