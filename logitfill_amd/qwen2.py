@@ -342,6 +342,8 @@ class PackedDecoder:
     def step(self, token: torch.Tensor) -> torch.Tensor:
         """``token``: the next one, or one for each sequence of the manager."""
         batch = getattr(self.manager, "batch_size", 1)
-        logits = self._forward(token.view(batch, 1), self.pos if batch == 1 else self._lengths())
+        # (one sequence behind a prefix may begin with a step; a cache that tells no lengths counts here)
+        own = batch == 1 and getattr(self.manager, "prefix", None) is None
+        logits = self._forward(token.view(batch, 1), self.pos if own else self._lengths())
         self.pos += 1
         return logits
