@@ -146,6 +146,15 @@ class _PromptKernels:
         manager.commit(layer_idx, key, value, self.plan.lengths)
 
 
+def _history(manager, layer_idx: int) -> int:
+    """Tokens in front of a call's own: of the longest sequence, its prefix's among them."""
+    lengths = getattr(manager.layers[layer_idx], "lengths", None)
+    if lengths is None:  # (a cache of one sequence)
+        return manager.layer_length(layer_idx)
+    own = max(lengths() if callable(lengths) else lengths)
+    return own if getattr(manager, "prefix", None) is None else own + max(manager.prefix_lengths(layer_idx))
+
+
 def _make_forward(attn, manager, attention_fn, kernels=None):
     from transformers.models.qwen2.modeling_qwen2 import apply_rotary_pos_emb
 
@@ -162,9 +171,7 @@ def _make_forward(attn, manager, attention_fn, kernels=None):
         else:
             cos, sin = position_embeddings
             query, key = apply_rotary_pos_emb(query, key, cos, sin)
-        past = manager.layer_length(layer_idx)
-        if getattr(manager, "prefix", None) is not None:
-            past += max(manager.prefix_lengths(layer_idx))
+        past = _history(manager, layer_idx)
         if past == 0 and kernels is not None and kernels.serves(attn, attention_mask, query.shape[2], kwargs.get("is_causal")):
             out = prompt_attention(query, key, value, attn.scaling, kernels.plan).transpose(1, 2)
             kernels.commit(manager, layer_idx, key, value)
