@@ -225,8 +225,8 @@ __device__ __attribute__((noinline)) void one_row(const unsigned char* q, const 
 #pragma unroll
             for (int c = 0; c < H; ++c) o[c] *= down;
         }
+        // (a weight of zero counts, too: times a Value that is not finite it is NaN, as in the products)
         const float w = s == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(s - (m == -__builtin_inff() ? 0.f : m));
-        if (w == 0.f) continue;  // (as a masked one)
         l += w;
 #pragma unroll
         for (int c = 0; c < H; c += 8) {
@@ -785,8 +785,9 @@ __global__ __launch_bounds__(256) void prompt_merge_kernel(Prompt a, const lf_pr
         o *= down;
 #pragma unroll
         for (int k = 0; k < kTake; ++k) {
-            if (s0 + k >= item.parts || ms[k] == -__builtin_inff()) continue;
-            const float w = __builtin_amdgcn_exp2f(ms[k] - m);
+            if (s0 + k >= item.parts) continue;
+            // (of a split without a weight above zero the sums are zeros, or NaN from a Value that is not finite)
+            const float w = ms[k] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ms[k] - m);
             l = fmaf(w, ls[k], l);
             o += w * x[k];
         }
