@@ -329,14 +329,10 @@ __global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, 
     const int j = row / a.g, i = row - j * a.g;
     const bool real = j < item.n_q;
     const int lim = real ? max(item.n_k - item.n_q + j + 1, 0) : 0;  // Keys this row sees
-    int all = real ? lim : 0x7fffffff, top = lim;                    // that every row of the wave sees, and any
+    int all = real ? lim : 0x7fffffff;                               // that every row of the wave sees
 #pragma unroll
-    for (int m = 1; m < 32; m <<= 1) {
-        all = min(all, __shfl_xor(all, m, kWave));
-        top = max(top, __shfl_xor(top, m, kWave));
-    }
+    for (int m = 1; m < 32; m <<= 1) all = min(all, __shfl_xor(all, m, kWave));
     all = in_sgpr(all);
-    top = in_sgpr(top);
     // the workgroup's last row that is real sees the most
     const int last_token = min((item.tile * kRows + kRows - 1) / a.g, item.n_q - 1);
     const int reach = max(item.n_k - item.n_q + last_token + 1, 0);

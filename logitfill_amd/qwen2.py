@@ -66,7 +66,7 @@ class _PromptKernels:
     under way, and, while packed prompts pass through, their plan and the places of their tokens in a padded batch."""
 
     def __init__(self, model, device):
-        rope, cfg = model.model.rotary_emb, model.config
+        rope = model.model.rotary_emb
         kind = str(getattr(rope, "rope_type", "default"))
         if "dynamic" in kind or kind == "longrope":
             raise ValueError(f"prompt_kernels takes frequencies that hang on no length; the model's are {kind!r}")
