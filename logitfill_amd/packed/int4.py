@@ -639,7 +639,7 @@ def int4_attention(manager: Int4KVManager, layer_idx: int, query: torch.Tensor, 
     q_len = query.shape[2]
     B = manager.batch_size
     if manager._prefix is not None:
-        if pages is not None:
+        if pages is not None or manager.top_pages:  # (the attribute may be set behind the prefix)
             raise ValueError("pages are of a sequence's own rows: a manager with a prefix attends them all")
         if manager.prefix.prefix is not None:
             raise ValueError("the manager's prefix has a prefix of its own")

@@ -35,3 +35,19 @@ def test_one_long_sequence_among_short_ones_behind_a_long_prefix(gpu, monkeypatc
     assert_within(out[:1], *ref, "the long one")
     some = want(q[1:], before, tuple(t[1:] for t in behind), common, own[1:], group, D ** -0.5, "bf16")
     assert_within(out[1:], *some, "the short ones")
+
+
+def test_top_pages_set_behind_a_prefix(gpu):
+    """Refused before the new tokens are committed."""
+    prefix = Int4KVManager(1, 4, 2, 64, 64, 32, gpu)
+    mgr = Int4KVManager(1, 4, 2, 64, 64, 32, gpu, batch_size=2, prefix=prefix)
+    k = torch.ones(2, 2, 200, 64, device=gpu)
+    prefix.commit(0, k[:1], k[:1])
+    mgr.commit(0, k, k)
+    q = torch.ones(2, 4, 1, 64, device=gpu)
+    mgr.top_pages = 2
+    with pytest.raises(ValueError, match="pages"):
+        int4_attention(mgr, 0, q, k[:, :, :1], k[:, :, :1], 0.1)
+    assert mgr.layers[0].lengths == [200, 200]
+    mgr.top_pages = 0
+    assert torch.isfinite(int4_attention(mgr, 0, q, k[:, :, :1], k[:, :, :1], 0.1)).all()
