@@ -146,12 +146,13 @@ __device__ __forceinline__ const lf_int4_layer& layer_of(const Int4Attention& a,
 __device__ __forceinline__ lf_int4_layer layer_of(const Int4Shared& a, bool pre) { return pre ? a.L : a.own; }
 
 // Shared: of prefixes that ``each`` sequences share, whose rows are all their queries (``pre``), and of the sequences' own rows, in
-// one launch; the sums are always partial ones.  A prefix's records are read once from HBM, but unpacked for every 16 rows: that
-// bounds it.  16 sequences of up to 600 tokens behind a prefix of 32 768 (28 / 4 heads of 128, groups of 64, bf16, one query each,
-// 112 rows a kv head): a call of 31 to 33 us, 22 MB (4 us of a copy), VALU 47 % busy; sequences with as many rows of their own each
-// take 57.  32 sequences behind four of 4 000 to 16 300 (40 / 8 heads, groups of 128, fp16, three queries
-// each): 77 us, VALU 61 %.  (Two row tiles a wave, which share the unpacking: 34 and 79 where this took 32 and 79; its registers
-// leave two waves a SIMD in place of three.)
+// one launch; the sums are always partial ones.  A prefix's records are read once from HBM, but unpacked for every 16 rows, and
+// a wave's unpacking, products and waits follow one another: nothing is busy throughout.  16 sequences of up to 600 tokens behind
+// a prefix of 32 768 (28 / 4 heads of 128, groups of 64, bf16, one query each, 112 rows a kv head): a call of 30 to 33 us, 22 MB
+// (4 us of a copy), VALU 47 % busy, matrix cores 10 %; sequences with as many rows of their own each take 57.  32 sequences behind
+// four of 4 000 to 16 300 (40 / 8 heads, groups of 128, fp16, three queries each): 77 us, VALU 61 %, matrix cores 26 %.  (Two row
+// tiles a wave, which share the unpacking: 34 and 79 where this took 32 and 79; its registers leave two waves a SIMD in place of
+// three.)
 template <int D, int GROUP, int Dt, bool Shared>
 __global__ __launch_bounds__(kWaves * kWave, D == 64 ? 4 : D == 128 ? 3 : 2) void int4_attention_kernel(typename Int4Call<Shared>::Args a) {
     using R = Int4Rec<D, GROUP>;

@@ -69,7 +69,8 @@ __device__ __forceinline__ void phase() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ f16x2 halves(uint32_t x) { return __builtin_bit_cast(f16x2, x); }
 
 // Shared: of a prefix that ``each`` sequences share; the rows are all their queries, and its last record may be a part of one.
-// (448 rows a kv head behind 32 768 tokens, 4 kv heads of 128, groups of 64: a call of 81 us, the general kernel's 86; 896: 121, 155.)
+// (448 rows a kv head behind 32 768 tokens, 4 kv heads of 128, groups of 64: a call of 81 to 84 us, the general kernel's 86; 896: 121, 155;
+// 1 792: 214; of groups of 128 236.)
 template <int D, int GROUP, bool Shared>
 __global__ __launch_bounds__(kWaves * kWave, D == 128 && GROUP < 128 ? 2 : 3) void int4_prefix_kernel(typename Int4Call<Shared>::Args a) {
     using R = Int4Rec<D, GROUP>;

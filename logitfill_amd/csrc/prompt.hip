@@ -14,15 +14,21 @@
 // exponentials fill each other's waits.
 //
 // Scores and sums are fp32; P is rounded to the rows' type (bf16: 2^-8 of a weight at most, averaged over the Keys, beside the
-// output's own; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).  float32 rows: see
-// prompt_split_kernel, or, of heads of 256 and single waves, multiplied as such (32x32x2).
+// output's own; fp16: formed as up to 2^15, so that it keeps weights down to 2^-31 of their row's largest).  Its lower part would
+// be a third product beside two, in a kernel that the matrix cores bound at long prompts.  float32 rows: see prompt_split_kernel,
+// or, of heads of 256 and single waves, multiplied as such (32x32x2).  Weights reach 2^8 (fp16: 2^15) before they are divided by
+// their sum: Values past 2^119 over the tokens (bf16, fp32) may overflow the sums.
 //
 // Measured: one prompt of 16 384 tokens, 40 / 8 heads of 128, bf16: 2.36 to 2.5 ms, 1 100 to 1 165 TFLOP/s of the products that
 // are not masked (an 8 192^3 bf16 product of the library: 1 220).  Matrix cores 65 % busy, VALU 51 %, LDS 49 %, no bank
 // conflicts, 97 % of the Keys' and Values' reads from L2; the clock falls to 2.0 GHz under that load.  Eight prompts of 300
 // to 8 190 tokens, 28 / 4 heads: 1.35 to 1.4 ms (1 090); 512 tokens behind 16 384: 138 us, 8 of them the merge; 1 061 tokens
-// alone 25; float32, two of 1 500, 8 heads of 256: 177 (8.4 a Key tile, 6.8 of them float32 products).  At head_dim 64 the exponentials bound a
-// tile: sixteen of 1 to 1 500 tokens, 14 / 2 heads, fp16: 45 us, 0.69 a Key tile and compute unit, 0.43 of them VALU work.
+// alone 26.6; float32, two of 1 500, 8 heads of 256: 181 (8.4 a Key tile, 6.8 of them float32 products).  16-bit heads of 256, 8 192
+// tokens, 16 / 8 heads: 530 to 590 (1 010).  Single tokens, 28 / 4 heads of 128: sixteen behind 32 768 each 201 us, 5.3 TB/s (float32
+// 669, 3.2), one 34, four behind 1 000 15.  At head_dim 64 a wave's exponentials and products follow
+// one another, and four waves a SIMD do not fill all of it.  Sixteen of 1 to 1 500 tokens, 14 / 2 heads, fp16: 43 us, 0.69 a Key
+// tile and compute unit, 0.43 of them VALU work (VALU 46 % busy, matrix cores 21 %); 8 192 tokens, 16 / 8 heads, bf16: 169, 815
+// TFLOP/s (61 %, 42 %).
 // Not faster at 16 384 tokens: Keys buffered twice (two workgroups a CU; the same long, 8 % less of 1 061 tokens alone, where two groups
 // now do more); tiles of 32 Keys (2.5 against 2.45 ms); 64 rows a wave (its sums spill: 9.1); operands read a product
 // ahead; waves' priorities (2.53); sums of the rounded weights by dot products (the same; at head_dim 64 46.5 us for 45, the error
@@ -299,7 +305,7 @@ __device__ __forceinline__ void finish(const Prompt& a, const lf_prompt_item& it
 
 // Groups of NW waves of 32 rows each, that take an item's Key tiles in turn and are joined through LDS at its end: where there is a
 // workgroup a compute unit at most, two groups do what two workgroups would, without partial sums and the merge's launch (1 061
-// tokens, 28 / 4 heads of 128: 25 us; one group 32, the Keys divided in two or three and merged 31 and 30).
+// tokens, 28 / 4 heads of 128: 26.6 us; one group 32, the Keys divided in two or three and merged 31 and 30).
 template <int D, int Dt>
 constexpr int kPerSimd = Dt == LF_FP32 ? (D == 64 ? 3 : D == 128 ? 2 : 1) : (D == 64 ? 4 : D == 128 ? 3 : 2);  // waves, by their registers
 
@@ -533,8 +539,13 @@ __global__ __launch_bounds__(Groups * NW * kWave, (Groups > 1 ? 2 : kPerSimd<D, 
 // Keys and Values are taken apart once, on their way from registers to LDS (32 of each a tile, three planes of bf16 rows);
 // the next tile's loads run beside the products.
 //
-// Four prompts of 2 000 to 4 096 tokens, 16 / 8 heads of 128: 1 060 us (1 060 TFLOP/s of bf16 products), of 64: 625; by float32
-// products 1 460 and 830, and the largest error among 700 tokens falls from 1.2e-6 to 5.6e-7 and from 9.5e-7 to 7.1e-7.  Two
+// A part below 2^-133, bf16's least, is lost: numbers below 2^-110 are off by up to that (Values of 1e-34: 5e-7 of them, of 1e-38
+// 5e-3).  Parts of what is not finite are not it: one Key or Value that is not, in any tile that a workgroup walks, seen by its rows or
+// not, has all its rows formed anew one Key at a time (a NaN at token 10 of one prompt, the four prompts below, heads of 128: 32 ms for
+// 1.06, of 64 16; prompt_kernel, which looks at masked tiles only, 3.4 ms for 3.2 at 256).
+//
+// Four prompts of 2 000 to 4 096 tokens, 16 / 8 heads of 128: 1 040 to 1 080 us (1 060 TFLOP/s of bf16 products), of 64: 520 to 650; by
+// float32 products 1 450 and 840, and the largest error among 700 tokens falls from 1.2e-6 to 5.6e-7 and from 9.5e-7 to 7.1e-7.  Two
 // waves a SIMD at both sizes (at 128 29 registers are spilled; three waves at 64 spilled 48: 750 us).  At head_dim 256 query
 // parts and sums pass the registers (152 spilled, 4 250 us against 3 240), and a single wave's 32 rows would share the parting
 // of their Keys with nobody: those are multiplied as they are.

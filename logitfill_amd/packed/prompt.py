@@ -165,7 +165,9 @@ def prompt_attention(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor
     ``plan``: the sequences.  B of them, each from the start of its own row (padded), or, in a batch of one row, all
     behind one another (packed); queries and Keys each in one of the two ways.  None: every row is a sequence of
     all its tokens (not in a capture).  A sequence's queries are the last of its Keys, and each sees the Keys up to its own.  Rows of
-    the output behind a sequence's last token, and rows of queries that see no Key, are zeros.
+    the output behind a sequence's last token, and rows of queries that see no Key, are zeros.  What a row does not see need
+    not be finite; a Value that it sees and that is not counts whatever its weight.  Finite ones in bf16 and fp32 may overflow
+    the sums past 2^119 over the tokens.
 
     Everything is enqueued on the current stream."""
     scaling = float(scaling)
