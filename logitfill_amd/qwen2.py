@@ -80,12 +80,13 @@ class _PromptKernels:
         self.plan: PromptPlan | None = None
         self.places: torch.Tensor | None = None
         self.masks: list | None = None  # of the pass under way: (mask, whether it is the causal one)
-        self._hooks = [model.model.register_forward_pre_hook(self._begin),
-                       model.model.register_forward_hook(self._end, always_call=True)]
 
-    def detach(self) -> None:
-        for hook in self._hooks:
-            hook.remove()
+    def watch(self, model) -> None:
+        """Learn of the model's passes, until ``_drop_kernels``."""
+        # (functions, not methods: a copy of the model does not copy what is behind them)
+        hooks = (model.model.register_forward_pre_hook(lambda *args: self._begin(*args)),
+                 model.model.register_forward_hook(lambda *args: self._end(*args), always_call=True))
+        model._lf_drop_kernels = lambda: [hook.remove() for hook in hooks]
 
     def _begin(self, module, args) -> None:
         self.masks = []
@@ -221,7 +222,8 @@ def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kerne
             raise ValueError("manager shape does not match the model's attention")
     kernels = _PromptKernels(model, manager.device) if prompt_kernels else None
     _drop_kernels(model)
-    model._lf_prompt_kernels = kernels
+    if kernels is not None:
+        kernels.watch(model)
     for layer in layers:
         attn = layer.self_attn
         if not hasattr(attn, "_lf_original_forward"):
@@ -231,9 +233,7 @@ def attach_packed(model, manager, attention_fn=packed_attention, *, prompt_kerne
 
 
 def _drop_kernels(model) -> None:
-    kernels = model.__dict__.pop("_lf_prompt_kernels", None)
-    if kernels is not None:
-        kernels.detach()
+    model.__dict__.pop("_lf_drop_kernels", lambda: None)()
 
 
 def detach_packed(model) -> None:

@@ -1,5 +1,7 @@
 """Calls of a model with ``prompt_kernels`` whose masks hide more than later tokens: the model's own result, whichever way its
 attention is made; calls without such a mask run the prompt attention."""
+import copy
+
 import pytest
 import torch
 
@@ -102,3 +104,13 @@ def test_attaching_anew_and_passes_that_fail(gpu, calls):
     attach_packed(model, mgr)
     assert not model.model._forward_pre_hooks and not model.model._forward_hooks
     detach_packed(model)
+
+
+def test_a_model_with_the_kernels_can_be_copied(gpu):
+    model = _model(gpu)
+    ids = torch.arange(9, device=gpu)[None]
+    want = PackedDecoder(model, Int4KVManager(2, 4, 2, 128, 64, 32, gpu), prompt_kernels=True).prefill(ids)
+    other = copy.deepcopy(model)
+    detach_packed(model)
+    got = PackedDecoder(other, Int4KVManager(2, 4, 2, 128, 64, 32, gpu), prompt_kernels=True).prefill(ids)
+    assert torch.equal(got, want)
