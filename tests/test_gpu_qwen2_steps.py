@@ -98,3 +98,25 @@ def test_rows_of_some_sequences_only(gpu, kernels):
         for i in range(2):
             assert _rel(got[i][b], alone.step(tokens[i, b])[0]) < 2e-2, (b, i)
         detach_packed(model)
+
+
+@pytest.mark.parametrize("kind", ["eager", "sdpa"])
+@pytest.mark.parametrize("hf_cache", [False, True])
+def test_prefixes_of_unlike_lengths(gpu, kind, hf_cache):
+    """Two sequences behind each of two prefixes: a pass of three tokens, then steps, as sequences on their own."""
+    model = _model(gpu)
+    model.config._attn_implementation = kind
+    prompts, tokens = [_ids(n, n, gpu) for n in (60, 35)], _ids(20, 4, gpu).view(4, 5)
+    prefix = _int4(gpu, 2)
+    PackedDecoder(model, prefix, prompt_kernels=True).prefill(prompts)
+    mgr = _int4(gpu, 4, prefix=prefix)
+    dec = PackedDecoder(model, mgr, hf_cache=hf_cache, prompt_kernels=True)
+    got = [dec.prefill(tokens[:, :3])] + [dec.step(tokens[:, i]) for i in (3, 4)]
+    detach_packed(model)
+    assert mgr.prefix_lengths(1) == [60, 60, 35, 35] and mgr.layers[1].lengths == [5] * 4
+    for b in range(4):
+        alone = PackedDecoder(model, _int4(gpu), prompt_kernels=True)
+        alone.prefill(prompts[b // 2][None])
+        want = [alone.step(t) for t in tokens[b]][2:]
+        detach_packed(model)
+        assert all(_rel(x[b], w[0]) < 2e-2 for x, w in zip(got, want)), b
